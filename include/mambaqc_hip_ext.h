@@ -1,7 +1,8 @@
 /* Entry points of libmambaqc_hip.so beside the drop-in boundary of mambaqc_hip.h: products
  * and fused steps that the Python layers choose by size, each computing what operators of
- * mambaqc_hip.h or torch compute otherwise. Conventions, status codes and dtype codes are
- * that header's. */
+ * mambaqc_hip.h or torch compute otherwise, and the operators of a recurrent stack (the gated
+ * scan, the gate with norms and residual, the AdamW step). Conventions, status codes and dtype
+ * codes are that header's. */
 #ifndef MAMBAQC_HIP_EXT_H
 #define MAMBAQC_HIP_EXT_H
 
@@ -108,6 +109,35 @@ int mqc_step_norm_out_gate(const void* Y, int64_t M, int64_t d_inner, const floa
                            void* out, int dtype, void* stream);
 /* 1 where mqc_step_norm_out_gate takes M rows of d_inner quaternions, else 0. */
 int mqc_step_norm_out_gate_fits(int64_t M, int64_t d_inner);
+
+/* The gated scan over [batch, seq_len, width]: D = softplus(dt), a = exp(-D exp(log_rate)),
+ *   h_t = a_t h_{t-1} + (1 - a_t) sigmoid(g_t) x_t,  y_t = h_t
+ * from h0 (fp32 [batch, width]; NULL: zeros). reset (bytes [batch, seq_len], or NULL): where it is
+ * not 0, h_{t-1} is taken as 0. Tokens of dt, g and x are *_row elements apart (all batch x seq_len
+ * of them), y is dense. h_last (fp32, or NULL) may be h0. carries (fp32 [batch,
+ * ceil(seq_len / mqc_gated_scan_chunk()), width], or NULL): the states that the backward starts
+ * from, each chunk's before its first token.
+ * workspace of mqc_gated_scan_workspace_bytes. width and seq_len at most 2^31, batch at most 65535.
+ *
+ * Backward: gradients of dt, g, x (dense), log_rate [width], and of h0 (or NULL) from dy and
+ * dh_last (or NULL); every size at least 1.
+ * The step: one token of each sequence, h (fp32 [batch, width]) updated in place. */
+int mqc_gated_scan_chunk(void);
+int64_t mqc_gated_scan_workspace_bytes(int64_t batch, int64_t seq_len, int64_t width);
+int mqc_gated_scan_fwd(const void* dt, int64_t dt_row, const void* g, int64_t g_row, const void* x,
+                       int64_t x_row, const float* log_rate, const float* h0, const void* reset,
+                       void* y, float* h_last, float* carries, int64_t batch, int64_t seq_len,
+                       int64_t width, int dtype, void* workspace, int64_t workspace_bytes,
+                       void* stream);
+int mqc_gated_scan_bwd(const void* dt, int64_t dt_row, const void* g, int64_t g_row, const void* x,
+                       int64_t x_row, const float* log_rate, const void* reset,
+                       const float* carries, const void* dy, const float* dh_last, void* ddt,
+                       void* dg, void* dx, float* dlog_rate, float* dh0, int64_t batch,
+                       int64_t seq_len, int64_t width, int dtype, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+int mqc_gated_scan_step(const void* dt, int64_t dt_row, const void* g, int64_t g_row, const void* x,
+                        int64_t x_row, const float* log_rate, float* h, void* y, int64_t batch,
+                        int64_t width, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -107,8 +107,13 @@ SIGNATURES_EXT = {
     "mqc_step_norm_out_gate_fits": [_i64, _i64],
     "mqc_step_ssm": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f32,
                      _int, _vp],
+    "mqc_gated_scan_chunk": [],
+    "mqc_gated_scan_fwd": [_vp, _i64] * 3 + [_vp] * 6 + [_i64] * 3 + [_int, _vp, _i64, _vp],
+    "mqc_gated_scan_bwd": [_vp, _i64] * 3 + [_vp] * 10 + [_i64] * 3 + [_int, _vp, _i64, _vp],
+    "mqc_gated_scan_step": [_vp, _i64] * 3 + [_vp] * 3 + [_i64] * 2 + [_int, _vp],
 }
 SIGNATURES_EXT_I64 = {
+    "mqc_gated_scan_workspace_bytes": [_i64, _i64, _i64],
     "mqc_qln_bwd_sums_workspace_bytes": [_i64, _i64],
     "mqc_q_chunked_workspace_bytes": [_i64, _i64, _i64, _i64, _int],
     "mqc_ssm_fused_bc_short_workspace_bytes": [_i64, _i64, _i64, _i64],

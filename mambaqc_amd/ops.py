@@ -25,7 +25,7 @@ from torch.library import custom_op, register_autograd
 
 from . import _native as nat
 from .block import _gate_operands, _out_gate_backward
-from .kernels import cayley_transform, parallel_scan, quaternion_ops
+from .kernels import cayley_transform, gated, parallel_scan, quaternion_ops
 from .kernels import ssm_fused as sf
 from .kernels.quaternion_norm import _qln_backward, _qln_forward
 from .layers.causal_conv1d import _conv_silu_backward, _ConvSiLU, _rows_view
@@ -493,3 +493,73 @@ OPS = (
     "quaternion_layer_norm", "quaternion_layer_norm_backward", "causal_conv1d_silu",
     "causal_conv1d_silu_backward", "out_gate", "out_gate_backward",
 )
+
+
+# --- the gated scan -------------------------------------------------------------
+
+@custom_op(f"{NS}::gated_scan", mutates_args=())
+def gated_scan(dt_raw: Tensor, g_raw: Tensor, x: Tensor, log_rate: Tensor,
+               h0: Optional[Tensor] = None,
+               reset: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+    """Inference: (y in the promoted dtype, h_last fp32 [B, W])."""
+    return gated._scan_forward(dt_raw, g_raw, x, log_rate, h0, reset, False)[:2]
+
+
+@gated_scan.register_fake
+def _(dt_raw, g_raw, x, log_rate, h0=None, reset=None):
+    b, t, d = x.shape
+    return (x.new_empty(b, t, d, dtype=gated._scan_dtype(dt_raw, g_raw, x)),
+            x.new_empty(b, d, dtype=torch.float32))
+
+
+@custom_op(f"{NS}::gated_scan_train", mutates_args=())
+def gated_scan_train(dt_raw: Tensor, g_raw: Tensor, x: Tensor, log_rate: Tensor,
+                     h0: Optional[Tensor] = None,
+                     reset: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
+    """(y, h_last, the chunks' entry states for the backward)."""
+    return gated._scan_forward(dt_raw, g_raw, x, log_rate, h0, reset, True)[:3]
+
+
+@gated_scan_train.register_fake
+def _(dt_raw, g_raw, x, log_rate, h0=None, reset=None):
+    b, t, d = x.shape
+    every = gated.scan_chunk()
+    return (x.new_empty(b, t, d, dtype=gated._scan_dtype(dt_raw, g_raw, x)),
+            x.new_empty(b, d, dtype=torch.float32),
+            x.new_empty(b, (t + every - 1) // every, d, dtype=torch.float32))
+
+
+@custom_op(f"{NS}::gated_scan_backward", mutates_args=())
+def gated_scan_backward(dt_raw: Tensor, g_raw: Tensor, x: Tensor, log_rate: Tensor,
+                        reset: Optional[Tensor], carries: Tensor, dy: Tensor,
+                        dh_last: Tensor) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """(ddt, dg, dx in the promoted dtype, dlog_rate and dh0 in fp32)."""
+    ct = gated._scan_dtype(dt_raw, g_raw, x)
+    operands = (dt_raw.to(ct), g_raw.to(ct), x.to(ct), nat.param_f32(log_rate),
+                None if reset is None else reset.contiguous())
+    return gated._scan_backward(operands, carries, dy, dh_last, True)
+
+
+@gated_scan_backward.register_fake
+def _(dt_raw, g_raw, x, log_rate, reset, carries, dy, dh_last):
+    ct = gated._scan_dtype(dt_raw, g_raw, x)
+    b, _, d = x.shape
+    grads = [x.new_empty(x.shape, dtype=ct) for _ in range(3)]
+    return (*grads, x.new_empty(d, dtype=torch.float32), x.new_empty(b, d, dtype=torch.float32))
+
+
+def _gated_scan_setup(ctx, inputs, output):
+    dt_raw, g_raw, x, log_rate, h0, reset = inputs
+    ctx.save_for_backward(dt_raw, g_raw, x, log_rate, reset, output[2])
+    ctx.h0_dtype = None if h0 is None else h0.dtype
+
+
+def _gated_scan_bwd(ctx, dy, dh_last, _gcarries):
+    dt_raw, g_raw, x, log_rate, reset, carries = ctx.saved_tensors
+    ddt, dg, dx, drate, dh0 = gated_scan_backward(dt_raw, g_raw, x, log_rate, reset, carries, dy,
+                                                  dh_last)
+    return (ddt.to(dt_raw.dtype), dg.to(g_raw.dtype), dx.to(x.dtype), drate.to(log_rate.dtype),
+            None if ctx.h0_dtype is None else dh0.to(ctx.h0_dtype), None)
+
+
+register_autograd(f"{NS}::gated_scan_train", _gated_scan_bwd, setup_context=_gated_scan_setup)

@@ -1,0 +1,94 @@
+"""The gated scan's refusals and shape rules, without a GPU."""
+import ctypes
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+import mambaqc_amd  # noqa: F401  (registers torch.ops.mambaqc.*)
+from mambaqc_amd import _native as nat
+from mambaqc_amd.kernels import gated_scan, gated_scan_step_
+from mambaqc_amd.kernels.gated import _rows
+
+FAKE = ctypes.c_void_p(4096)  # never dereferenced: validation fails first
+
+
+def z(*shape, **kw):
+    return torch.zeros(*shape, **kw)
+
+
+def test_refuses_shapes_types_and_devices():
+    x, lam = z(2, 3, 4), z(4)
+    with pytest.raises(ValueError, match="one shape"):
+        gated_scan(z(2, 3, 5), x, x, lam)
+    with pytest.raises(ValueError, match="one shape"):
+        gated_scan(z(3, 4), z(3, 4), z(3, 4), lam)
+    with pytest.raises(ValueError, match="log_rate"):
+        gated_scan(x, x, x, z(3))
+    with pytest.raises(ValueError, match="state"):
+        gated_scan(x, x, x, lam, h0=z(2, 3, 4))
+    with pytest.raises(ValueError, match="reset"):
+        gated_scan(x, x, x, lam, reset=z(2, 3))
+    with pytest.raises(ValueError, match="reset"):
+        gated_scan(x, x, x, lam, reset=z(2, 4, dtype=torch.bool))
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        gated_scan(x, x, x, lam)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        gated_scan(x.requires_grad_(), x, x, lam)
+    with pytest.raises(ValueError, match="one token"):
+        gated_scan_step_(x, x, x, lam, z(2, 4))
+    one = z(2, 1, 4)
+    with pytest.raises(ValueError, match="contiguous float32"):
+        gated_scan_step_(one, one, one, lam, z(2, 4, dtype=torch.float16))
+    with pytest.raises(ValueError, match="contiguous float32"):
+        gated_scan_step_(one, one, one, lam, z(4, 2).T)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        gated_scan_step_(one, one, one, lam, z(2, 4))
+
+
+def test_validation_codes():
+    lib = nat.load()
+    fwd = lambda b, t, d, row=None, dtype=0, ptr=FAKE, ws=1 << 40: lib.mqc_gated_scan_fwd(
+        ptr, d if row is None else row, FAKE, d, FAKE, d, FAKE, None, None, FAKE, FAKE, None, b, t, d,
+        dtype, FAKE, ws, None)
+    assert fwd(-1, 3, 4) == -2 and fwd(1, -3, 4) == -2 and fwd(1, 3, -4) == -2
+    assert fwd(2, 3, 4, row=3) == -2
+    assert fwd(2, 3, 4, dtype=5) == -3
+    assert fwd(2, 3, 4, ptr=None) == -1
+    assert fwd(1 << 20, 3, 4) == -5
+    assert fwd(2, 3, 4, ws=3) == -6
+    assert fwd(0, 3, 4, ptr=None) == 0 and fwd(2, 3, 0, ptr=None) == 0
+    bwd = lambda b, t, d, ws=1 << 40, ptr=FAKE: lib.mqc_gated_scan_bwd(
+        FAKE, d, FAKE, d, FAKE, d, FAKE, None, ptr, FAKE, None, FAKE, FAKE, FAKE, FAKE, None, b, t, d,
+        0, FAKE, ws, None)
+    assert bwd(0, 3, 4) == -2 and bwd(2, 0, 4) == -2 and bwd(2, 3, 0) == -2
+    assert bwd(2, 3, 4, ws=3) == -6 and bwd(2, 3, 4, ptr=None) == -1
+    step = lambda b, d, ptr=FAKE, dtype=0: lib.mqc_gated_scan_step(
+        FAKE, d, FAKE, d, FAKE, d, FAKE, ptr, FAKE, b, d, dtype, None)
+    assert step(2, 4, ptr=None) == -1 and step(2, 4, dtype=3) == -3 and step(-2, 4) == -2
+    assert step(0, 4) == 0
+    assert lib.mqc_gated_scan_workspace_bytes(-1, 1, 1) == -2
+
+
+def test_rows_read_in_place():
+    wide = z(3, 5, 24)
+    for part in (wide[..., :8], wide[..., 8:], wide[:, :1, 4:9], wide[:1, 2:4, 4:9]):
+        view, row = _rows(part, torch.float32)
+        assert view.data_ptr() == part.data_ptr()
+        assert row >= part.shape[2]
+    assert _rows(wide[:, 1:2, :8], torch.float32)[1] == 5 * 24  # one token a sequence
+    for part in (wide[:, 1:3, :8], wide.transpose(0, 1), wide[..., ::2], wide[:1].expand(3, -1, -1)):
+        view, row = _rows(part, torch.float32)
+        assert view.is_contiguous() and row == part.shape[2]
+
+
+def test_fake_kernels():
+    with FakeTensorMode():
+        x = torch.empty(2, 70, 6, device="cuda", dtype=torch.bfloat16)
+        lam, h0 = torch.empty(6, device="cuda"), torch.empty(2, 6, device="cuda")
+        y, h = torch.ops.mambaqc.gated_scan(x, x, x.float(), lam, h0, None)
+        assert y.shape == (2, 70, 6) and y.dtype == torch.float32 and h.shape == (2, 6)
+        y, h, carries = torch.ops.mambaqc.gated_scan_train(x, x, x, lam, None, None)
+        assert y.dtype == torch.bfloat16 and carries.dtype == torch.float32
+        every = nat.load().mqc_gated_scan_chunk()
+        assert carries.shape == (2, -(-70 // every), 6)
