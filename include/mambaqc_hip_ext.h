@@ -139,6 +139,32 @@ int mqc_gated_scan_step(const void* dt, int64_t dt_row, const void* g, int64_t g
                         int64_t x_row, const float* log_rate, float* h, void* y, int64_t batch,
                         int64_t width, int dtype, void* stream);
 
+/* One AdamW step over `count` tensors, each element in fp32:
+ *   g = grad * (*clip);  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   p = p decay - m / (sqrt(v) root_scale + eps) step_size
+ * (decay = 1 - lr weight_decay, step_size = lr / (1 - beta1^t), root_scale = 1 / sqrt(1 - beta2^t);
+ * clip, a device float, may be NULL). Elements of p and grad are of the row's dtype.
+ * mqc_adamw_step: rows of six values: p, grad, m, v, element count, dtype (pointers as integers);
+ * m and v fp32.
+ * mqc_adamw8_step: rows of nine: p, grad, m, r, m_scale, r_scale, element count, dtype, seed; m and
+ * r = sqrt(v) e4m3 bytes, with a power-of-two scale (fp32) for each 256 elements. Rounded up or down
+ * by seed, place and `step`, such that m's and v's means are kept.
+ * Pointers are aligned to their elements; the rows are read before the call returns.
+ *
+ * mqc_grad_norm: rows of three values: grad, element count, dtype. *norm = the 2-norm of all their
+ * elements (summed in 64 bits, in a fixed order), *clip = min(1, max_norm / (norm + 1e-6)); workspace
+ * (8-byte aligned) of mqc_grad_norm_workspace_bytes. */
+int mqc_adamw_step(const int64_t* tensors, int64_t count, float decay, float step_size,
+                   float root_scale, float beta1, float one_minus_beta1, float beta2,
+                   float one_minus_beta2, float eps, const float* clip, void* stream);
+int mqc_adamw8_step(const int64_t* tensors, int64_t count, float decay, float step_size,
+                    float root_scale, float beta1, float one_minus_beta1, float beta2,
+                    float one_minus_beta2, float eps, const float* clip, uint32_t step,
+                    void* stream);
+int64_t mqc_grad_norm_workspace_bytes(const int64_t* tensors, int64_t count);
+int mqc_grad_norm(const int64_t* tensors, int64_t count, double max_norm, float* norm, float* clip,
+                  void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

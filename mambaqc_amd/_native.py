@@ -28,6 +28,8 @@ _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
+_u32 = ctypes.c_uint32
 
 # name -> argtypes (all return int status)
 SIGNATURES = {
@@ -107,12 +109,16 @@ SIGNATURES_EXT = {
     "mqc_step_norm_out_gate_fits": [_i64, _i64],
     "mqc_step_ssm": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f32,
                      _int, _vp],
+    "mqc_adamw_step": [_vp, _i64] + [_f32] * 8 + [_vp, _vp],
+    "mqc_adamw8_step": [_vp, _i64] + [_f32] * 8 + [_vp, _u32, _vp],
+    "mqc_grad_norm": [_vp, _i64, _f64, _vp, _vp, _vp, _i64, _vp],
     "mqc_gated_scan_chunk": [],
     "mqc_gated_scan_fwd": [_vp, _i64] * 3 + [_vp] * 6 + [_i64] * 3 + [_int, _vp, _i64, _vp],
     "mqc_gated_scan_bwd": [_vp, _i64] * 3 + [_vp] * 10 + [_i64] * 3 + [_int, _vp, _i64, _vp],
     "mqc_gated_scan_step": [_vp, _i64] * 3 + [_vp] * 3 + [_i64] * 2 + [_int, _vp],
 }
 SIGNATURES_EXT_I64 = {
+    "mqc_grad_norm_workspace_bytes": [_vp, _i64],
     "mqc_gated_scan_workspace_bytes": [_i64, _i64, _i64],
     "mqc_qln_bwd_sums_workspace_bytes": [_i64, _i64],
     "mqc_q_chunked_workspace_bytes": [_i64, _i64, _i64, _i64, _int],

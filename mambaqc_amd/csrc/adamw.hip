@@ -1,0 +1,481 @@
+// One AdamW step over many tensors, its states in 32 or in 8 bits, and the gradients' norm that clips
+// it. For each element, in fp32 and in this order (no contraction, so that the states do not depend
+// on the compiler):
+//   g = grad clip;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+//   p = p decay - m / (sqrt(v) root_scale + eps) step_size
+// with decay = 1 - lr weight_decay, step_size = lr / (1 - beta1^t), root_scale = 1 / sqrt(1 - beta2^t).
+// p is rounded to its type once.
+//
+// 8-bit states: m and r = sqrt(v) are held as e4m3 numbers times a power of two for each 256 elements,
+// the least one that brings the largest of them under 448. Two choices make such a coarse state
+// follow its average (a step of e4m3 is 6 to 12 % of the value, an update of v moves it by 5 or by
+// 0.1 %, and rounding to nearest would never move it):
+//   - a value goes up or down to one of its two neighbours by a number made from its place, the seed
+//     and the step t, such that the mean is kept: of m for m, of r^2 = v for r. Over the steps the
+//     numbers of one element are a golden-ratio sequence, evenly spread, so the errors of successive
+//     steps mostly cancel;
+//   - the scale is a power of two, so a value that does not change stays on its code when the scale
+//     does not change, and what is rounded is the update alone. (Under a scale that moved with the
+//     largest element every element would be rounded anew at each step.)
+// r is never rounded to 0 unless it is 0: m / (0 + eps) would be any size. Values that are not finite
+// become NaN (code 0x7f), and do not set the scale.
+//
+// The tensors come as a table in the kernel's arguments (no copy to the device, kTableMax to a launch);
+// a workgroup finds its tensor by its place in the running count of workgroups.
+#include "common.hpp"
+
+namespace mqc {
+
+constexpr int kTableMax = 48;
+constexpr int kAdamThreads = 256;
+constexpr int kAdamVec = 4;                                  // elements a lane takes at once
+constexpr int kAdamIters = 4;
+constexpr int kAdamChunk = kAdamThreads * kAdamVec * kAdamIters;  // elements of a workgroup
+constexpr int kStateBlock = 64 * kAdamVec;                   // elements that share a scale
+
+struct AdamTable {
+  void* p[kTableMax];
+  const void* grad[kTableMax];
+  void* m[kTableMax];
+  void* v[kTableMax];
+  int64_t n[kTableMax];
+  uint32_t first[kTableMax];  // workgroups before this tensor's
+  int count;
+};
+struct Adam8Table {
+  AdamTable t;
+  float* m_scale[kTableMax];
+  float* v_scale[kTableMax];
+  uint32_t seed[kTableMax];
+};
+struct AdamScalars {
+  float decay, step_size, root_scale, beta1, one_beta1, beta2, one_beta2, eps;
+  const float* clip;
+  uint32_t step;
+};
+static_assert(sizeof(Adam8Table) + sizeof(AdamScalars) <= 4096, "kernel arguments");
+
+// The tensor of this workgroup: the last that starts at or before it.
+__device__ inline int table_find(const uint32_t* first, int count) {
+  int lo = 0, hi = count;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (first[mid] <= blockIdx.x) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// n <= 4 elements from p, as a vector where that is allowed.
+template <typename T>
+__device__ inline void load4(const T* p, int n, bool vec, float (&out)[4]) {
+  if (vec) {
+    load_vec<T, 4>(p, out);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = i < n ? load_scalar(p + i) : 0.f;
+  }
+}
+template <typename T>
+__device__ inline void store4(T* p, int n, bool vec, const float (&in)[4]) {
+  if (vec) {
+    store_vec<T, 4>(p, in);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) store_scalar(p + i, in[i]);
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamTable tab, AdamScalars k) {
+#pragma clang fp contract(off)
+  const int i = table_find(tab.first, tab.count);
+  T* p = (T*)tab.p[i];
+  const T* grad = (const T*)tab.grad[i];
+  float *m = (float*)tab.m[i], *v = (float*)tab.v[i];
+  const int64_t n = tab.n[i];
+  const int64_t base = (int64_t)(blockIdx.x - tab.first[i]) * kAdamChunk + threadIdx.x * kAdamVec;
+  const bool fits = (((uintptr_t)p | (uintptr_t)grad) % (4 * sizeof(T)) | ((uintptr_t)m | (uintptr_t)v) % 16) == 0;
+  const float clip = k.clip ? *k.clip : 1.f;
+  float pv[kAdamIters][4], gv[kAdamIters][4], mv[kAdamIters][4], vv[kAdamIters][4];
+#pragma unroll
+  for (int j = 0; j < kAdamIters; ++j) {
+    const int64_t at = base + j * kAdamThreads * kAdamVec;
+    const int left = n - at < 4 ? (int)(n - at) : 4;
+    const bool vec = fits && left == 4;
+    if (left <= 0) continue;
+    load4<T>(p + at, left, vec, pv[j]);
+    load4<T>(grad + at, left, vec, gv[j]);
+    load4<float>(m + at, left, vec, mv[j]);
+    load4<float>(v + at, left, vec, vv[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < kAdamIters; ++j) {
+    const int64_t at = base + j * kAdamThreads * kAdamVec;
+    const int left = n - at < 4 ? (int)(n - at) : 4;
+    const bool vec = fits && left == 4;
+    if (left <= 0) continue;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float g = k.clip ? gv[j][c] * clip : gv[j][c];
+      mv[j][c] = mv[j][c] * k.beta1 + g * k.one_beta1;
+      vv[j][c] = vv[j][c] * k.beta2 + g * g * k.one_beta2;
+      pv[j][c] = pv[j][c] * k.decay - mv[j][c] / (sqrtf(vv[j][c]) * k.root_scale + k.eps) * k.step_size;
+    }
+    store4<T>(p + at, left, vec, pv[j]);
+    store4<float>(m + at, left, vec, mv[j]);
+    store4<float>(v + at, left, vec, vv[j]);
+  }
+}
+
+// The largest of a wave's values, the same in every lane: within rows of 16 lanes by DPP, then the
+// four rows' lanes through scalar registers. Bits of floats >= 0 order as the floats do.
+__device__ inline uint32_t wave_max_bits(uint32_t v) {
+#define MQC_MAX(MOVE)                                                   \
+  {                                                                     \
+    const uint32_t o = __float_as_uint(MOVE(__uint_as_float(v)));       \
+    v = v > o ? v : o;                                                  \
+  }
+  MQC_MAX(lane_xor1) MQC_MAX(lane_xor2) MQC_MAX(row_rot4) MQC_MAX(row_rot8)
+#undef MQC_MAX
+  const uint32_t a = __builtin_amdgcn_readlane(v, 0), b = __builtin_amdgcn_readlane(v, 16);
+  const uint32_t c = __builtin_amdgcn_readlane(v, 32), d = __builtin_amdgcn_readlane(v, 48);
+  const uint32_t x = a > b ? a : b, y = c > d ? c : d;
+  return x > y ? x : y;
+}
+
+// The exponent field of the block's power of two, from its largest value's bits.
+__device__ inline int scale_field(uint32_t top) {
+  const int e = (int)(top >> 23) + ((top & 0x7fffff) > 0x600000) - 8;
+  return e < 1 ? 1 : e;
+}
+
+constexpr uint32_t kMulA = 0x6a09e667u, kMulB = 0xbb67ae85u, kGolden = 0x9e3779b9u;
+// An even 32-bit value for an element: sums and products with the fractional parts of sqrt 2, sqrt 3
+// and the golden ratio, shifted together.
+__device__ inline uint32_t place_bits(uint32_t x) {
+  x = (x ^ (x >> 16)) * kMulA;
+  x = (x ^ (x >> 15)) * kMulB;
+  return x ^ (x >> 16);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kAdamThreads) void adamw8_kernel(Adam8Table tab, AdamScalars k) {
+#pragma clang fp contract(off)
+  const int i = table_find(tab.t.first, tab.t.count);
+  T* p = (T*)tab.t.p[i];
+  const T* grad = (const T*)tab.t.grad[i];
+  uint8_t *m = (uint8_t*)tab.t.m[i], *v = (uint8_t*)tab.t.v[i];
+  const int64_t n = tab.t.n[i];
+  const bool fits = (((uintptr_t)p | (uintptr_t)grad) % (4 * sizeof(T)) | ((uintptr_t)m | (uintptr_t)v) % 4) == 0;
+  const float clip = k.clip ? *k.clip : 1.f;
+  const int lane = threadIdx.x & 63;
+  // A wave takes kAdamIters blocks of 256 elements, four elements a lane.
+  const int64_t block0 = (int64_t)(blockIdx.x - tab.t.first[i]) * (kAdamChunk / kStateBlock) +
+                         __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kAdamIters;
+#pragma unroll
+  for (int j = 0; j < kAdamIters; ++j) {
+    const int64_t block = block0 + j, at = block * kStateBlock + lane * 4;
+    if (block * kStateBlock >= n) return;
+    const int left = n - at < 0 ? 0 : n - at < 4 ? (int)(n - at) : 4;
+    const bool vec = fits && left == 4;
+    float pv[4], gv[4], r[4], mm[4];
+    load4<T>(p + at, left, vec, pv);
+    load4<T>(grad + at, left, vec, gv);
+    uint32_t mc = 0, vc = 0;
+    if (vec) {
+      mc = *(const uint32_t*)(m + at);
+      vc = *(const uint32_t*)(v + at);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (c < left) mc |= (uint32_t)m[at + c] << (8 * c), vc |= (uint32_t)v[at + c] << (8 * c);
+    }
+    const float ms = tab.m_scale[i][block], vs = tab.v_scale[i][block];
+    uint32_t mtop = 0, vtop = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float g = k.clip ? gv[c] * clip : gv[c];
+      const float m0 = (c == 0   ? __builtin_amdgcn_cvt_f32_fp8(mc, 0)
+                        : c == 1 ? __builtin_amdgcn_cvt_f32_fp8(mc, 1)
+                        : c == 2 ? __builtin_amdgcn_cvt_f32_fp8(mc, 2)
+                                 : __builtin_amdgcn_cvt_f32_fp8(mc, 3)) * ms;
+      const float r0 = (c == 0   ? __builtin_amdgcn_cvt_f32_fp8(vc, 0)
+                        : c == 1 ? __builtin_amdgcn_cvt_f32_fp8(vc, 1)
+                        : c == 2 ? __builtin_amdgcn_cvt_f32_fp8(vc, 2)
+                                 : __builtin_amdgcn_cvt_f32_fp8(vc, 3)) * vs;
+      mm[c] = m0 * k.beta1 + g * k.one_beta1;
+      r[c] = sqrtf(r0 * r0 * k.beta2 + g * g * k.one_beta2);
+      pv[c] = pv[c] * k.decay - mm[c] / (r[c] * k.root_scale + k.eps) * k.step_size;
+      const uint32_t ma = __float_as_uint(mm[c]) & 0x7fffffffu, ra = __float_as_uint(r[c]);
+      if (ma < 0x7f800000u && ma > mtop) mtop = ma;
+      if (ra < 0x7f800000u && ra > vtop) vtop = ra;
+    }
+    store4<T>(p + at, left, vec, pv);
+    const int mf = scale_field(wave_max_bits(mtop)), vf = scale_field(wave_max_bits(vtop));
+    if (lane == 0) {
+      tab.m_scale[i][block] = __uint_as_float((uint32_t)mf << 23);
+      tab.v_scale[i][block] = __uint_as_float((uint32_t)vf << 23);
+    }
+    const float mi = __uint_as_float((uint32_t)(254 - mf) << 23);
+    const float vi = __uint_as_float((uint32_t)(254 - vf) << 23);
+    uint32_t mo = 0, vo = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint64_t place = (uint64_t)(at + c);
+      const uint32_t bits = place_bits((uint32_t)place + (uint32_t)(place >> 32) * kMulB + tab.seed[i] * kGolden);
+      const float um = (float)((bits + k.step * kGolden) >> 8) * 0x1p-24f;
+      const float uv = (float)((((bits << 16) | (bits >> 16)) + k.step * kMulB) >> 8) * 0x1p-24f;
+      {  // m: q in steps of its binade (the lowest is 2^-6 on), up with probability q - floor(q)
+        const float x = fabsf(mm[c]) * mi;
+        int f = (int)(__float_as_uint(x) >> 23);
+        f = f < 121 ? 121 : f;
+        const float q = x * __uint_as_float((uint32_t)(257 - f) << 23);
+        uint32_t code = ((uint32_t)(f - 121) << 3) + (uint32_t)floorf(q + um);
+        code = code > 0x7eu ? 0x7eu : code;  // q + um may round up to the step past 448
+        if (!(x < 512.f)) code = 0x7f;
+        mo |= (code | (mm[c] < 0.f ? 0x80u : 0u)) << (8 * c);
+      }
+      {  // r: up with probability (q^2 - k^2) / ((k + 1)^2 - k^2)
+        const float x = r[c] * vi;
+        int f = (int)(__float_as_uint(x) >> 23);
+        f = f < 121 ? 121 : f;
+        const float q = x * __uint_as_float((uint32_t)(257 - f) << 23);
+        const float lo = floorf(q);
+        uint32_t code = ((uint32_t)(f - 121) << 3) + (uint32_t)lo +
+                        (uv * (2.f * lo + 1.f) < (q - lo) * (q + lo) ? 1u : 0u);
+        code = x > 0.f && code == 0 ? 1u : code;
+        if (!(x < 512.f)) code = 0x7f;
+        vo |= code << (8 * c);
+      }
+    }
+    if (vec) {
+      *(uint32_t*)(m + at) = mo;
+      *(uint32_t*)(v + at) = vo;
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (c < left) m[at + c] = (uint8_t)(mo >> (8 * c)), v[at + c] = (uint8_t)(vo >> (8 * c));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The norm: each workgroup's sum of squares in 64 bits (fp32 squares of fp32 gradients neither
+// overflow nor lose digits there), then one workgroup's sum of those in a fixed order.
+// ---------------------------------------------------------------------------
+constexpr int kNormChunk = 256 * 4 * 8;
+struct NormTable {
+  const void* grad[kTableMax];
+  int64_t n[kTableMax];
+  uint32_t first[kTableMax];
+  int count;
+};
+
+__device__ inline double wave_sum_f64(double v) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+  return v;
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void grad_norm_kernel(NormTable tab, double* partial) {
+  __shared__ double red[4];
+  const int i = table_find(tab.first, tab.count);
+  const T* grad = (const T*)tab.grad[i];
+  const int64_t n = tab.n[i];
+  const int64_t base = (int64_t)(blockIdx.x - tab.first[i]) * kNormChunk + threadIdx.x * 4;
+  const bool fits = (uintptr_t)grad % (4 * sizeof(T)) == 0;
+  float gv[8][4];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int64_t at = base + j * 1024;
+    const int left = n - at < 0 ? 0 : n - at < 4 ? (int)(n - at) : 4;
+    load4<T>(grad + at, left, fits && left == 4, gv[j]);
+  }
+  double s = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) s += (double)gv[j][c] * (double)gv[j][c];
+  s = wave_sum_f64(s);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) partial[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+
+__global__ __launch_bounds__(1024) void grad_norm_end_kernel(const double* partial, int64_t count,
+                                                             double max_norm, float* norm, float* clip) {
+  __shared__ double red[16];
+  double s = 0;
+  for (int64_t i = threadIdx.x; i < count; i += 1024) s += partial[i];
+  s = wave_sum_f64(s);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0;
+    for (int i = 0; i < 16; ++i) s += red[i];
+    s = sqrt(s);
+    *norm = (float)s;
+    const double c = max_norm / (s + 1e-6);
+    *clip = (float)(c > 1.0 ? 1.0 : c);  // a NaN stays one
+  }
+}
+
+inline bool known_dtype(int64_t d) { return d == MQC_F32 || d == MQC_BF16 || d == MQC_F16; }
+
+template <typename T>
+void launch_adamw(const AdamTable& t, const AdamScalars& k, uint32_t blocks, hipStream_t s) {
+  adamw_kernel<T><<<dim3(blocks), dim3(kAdamThreads), 0, s>>>(t, k);
+}
+template <typename T>
+void launch_adamw(const Adam8Table& t, const AdamScalars& k, uint32_t blocks, hipStream_t s) {
+  adamw8_kernel<T><<<dim3(blocks), dim3(kAdamThreads), 0, s>>>(t, k);
+}
+template <typename T>
+void launch_norm(const NormTable& t, double* partial, uint32_t blocks, hipStream_t s) {
+  grad_norm_kernel<T><<<dim3(blocks), dim3(256), 0, s>>>(t, partial);
+}
+#define MQC_LAUNCH(F, dtype, ...)                     \
+  switch (dtype) {                                    \
+    case MQC_F32: F<float>(__VA_ARGS__); break;       \
+    case MQC_BF16: F<bf16_t>(__VA_ARGS__); break;     \
+    default: F<f16_t>(__VA_ARGS__); break;            \
+  }
+
+// Workgroups of a tensor; a launch holds at most 2^31 - 1 of them.
+inline int64_t chunks_of(int64_t n, int64_t chunk) { return (n + chunk - 1) / chunk; }
+
+// Fills tables with the tensors of one dtype after another and calls launch(table, blocks, dtype) for
+// each full one. rows: `width` values a tensor, its element count at `n_at` and dtype code at `d_at`.
+template <typename Table, typename Put, typename Launch>
+int by_tables(const int64_t* rows, int64_t count, int width, int n_at, int d_at, int64_t chunk,
+              Put put, Launch launch) {
+  for (int dtype : {MQC_F32, MQC_BF16, MQC_F16}) {
+    Table t{};
+    int used = 0;
+    int64_t blocks = 0;
+    for (int64_t i = 0; i <= count; ++i) {
+      const int64_t* row = rows + i * width;
+      const bool mine = i < count && row[d_at] == dtype && row[n_at] > 0;
+      const int64_t more = mine ? chunks_of(row[n_at], chunk) : 0;
+      if (used > 0 && (i == count || (mine && (used == kTableMax || blocks + more > 0x7fffffffLL)))) {
+        launch(t, used, (uint32_t)blocks, dtype);
+        const int st = launch_status();
+        if (st != MQC_OK) return st;
+        used = 0, blocks = 0;
+      }
+      if (mine) put(t, used++, row, (uint32_t)blocks), blocks += more;
+    }
+  }
+  return MQC_OK;
+}
+
+inline int check_rows(const int64_t* rows, int64_t count, int width, int pointers, int n_at, int d_at,
+                      int64_t chunk) {
+  if (count < 0) return MQC_E_SHAPE;
+  if (count > 0 && !rows) return MQC_E_NULL;
+  for (int64_t i = 0; i < count; ++i) {
+    const int64_t* row = rows + i * width;
+    if (row[n_at] < 0) return MQC_E_SHAPE;
+    if (!known_dtype(row[d_at])) return MQC_E_DTYPE;
+    if (chunks_of(row[n_at], chunk) > 0x7fffffffLL) return MQC_E_LIMIT;
+    const uintptr_t size = row[d_at] == MQC_F32 ? 4 : 2;
+    for (int c = 0; c < pointers; ++c) {
+      if (row[n_at] > 0 && !row[c]) return MQC_E_NULL;
+      if (c < 2 && (uintptr_t)row[c] % size) return MQC_E_ALIGN;
+    }
+  }
+  return MQC_OK;
+}
+
+inline void put_adam(AdamTable& t, int at, const int64_t* row, int64_t n, uint32_t first) {
+  t.p[at] = (void*)row[0];
+  t.grad[at] = (const void*)row[1];
+  t.m[at] = (void*)row[2];
+  t.v[at] = (void*)row[3];
+  t.n[at] = n;
+  t.first[at] = first;
+}
+
+}  // namespace mqc
+
+using namespace mqc;
+
+extern "C" int mqc_adamw_step(const int64_t* tensors, int64_t count, float decay, float step_size,
+                              float root_scale, float beta1, float one_minus_beta1, float beta2,
+                              float one_minus_beta2, float eps, const float* clip, void* stream) {
+  const int st = check_rows(tensors, count, 6, 4, 4, 5, kAdamChunk);
+  if (st != MQC_OK) return st;
+  for (int64_t i = 0; i < count; ++i)
+    if ((tensors[6 * i + 2] | tensors[6 * i + 3]) % 4) return MQC_E_ALIGN;
+  const AdamScalars k{decay, step_size, root_scale, beta1, one_minus_beta1, beta2, one_minus_beta2,
+                      eps, clip, 0};
+  return by_tables<AdamTable>(
+      tensors, count, 6, 4, 5, kAdamChunk,
+      [](AdamTable& t, int at, const int64_t* row, uint32_t first) { put_adam(t, at, row, row[4], first); },
+      [&](AdamTable& t, int used, uint32_t blocks, int dtype) {
+        t.count = used;
+        MQC_LAUNCH(launch_adamw, dtype, t, k, blocks, (hipStream_t)stream)
+      });
+}
+
+extern "C" int mqc_adamw8_step(const int64_t* tensors, int64_t count, float decay, float step_size,
+                               float root_scale, float beta1, float one_minus_beta1, float beta2,
+                               float one_minus_beta2, float eps, const float* clip, uint32_t step,
+                               void* stream) {
+  const int st = check_rows(tensors, count, 9, 6, 6, 7, kAdamChunk);
+  if (st != MQC_OK) return st;
+  for (int64_t i = 0; i < count; ++i)
+    if ((tensors[9 * i + 4] | tensors[9 * i + 5]) % 4) return MQC_E_ALIGN;
+  const AdamScalars k{decay, step_size, root_scale, beta1, one_minus_beta1, beta2, one_minus_beta2,
+                      eps, clip, step};
+  return by_tables<Adam8Table>(
+      tensors, count, 9, 6, 7, kAdamChunk,
+      [](Adam8Table& t, int at, const int64_t* row, uint32_t first) {
+        put_adam(t.t, at, row, row[6], first);
+        t.m_scale[at] = (float*)row[4];
+        t.v_scale[at] = (float*)row[5];
+        t.seed[at] = (uint32_t)row[8];
+      },
+      [&](Adam8Table& t, int used, uint32_t blocks, int dtype) {
+        t.t.count = used;
+        MQC_LAUNCH(launch_adamw, dtype, t, k, blocks, (hipStream_t)stream)
+      });
+}
+
+extern "C" int64_t mqc_grad_norm_workspace_bytes(const int64_t* tensors, int64_t count) {
+  const int st = check_rows(tensors, count, 3, 1, 1, 2, kNormChunk);
+  if (st != MQC_OK) return st;
+  int64_t blocks = 0;
+  for (int64_t i = 0; i < count; ++i) blocks += chunks_of(tensors[3 * i + 1], kNormChunk);
+  return blocks * (int64_t)sizeof(double);
+}
+
+extern "C" int mqc_grad_norm(const int64_t* tensors, int64_t count, double max_norm, float* norm,
+                             float* clip, void* workspace, int64_t workspace_bytes, void* stream) {
+  const int64_t need = mqc_grad_norm_workspace_bytes(tensors, count);
+  if (need < 0) return (int)need;
+  if (!norm || !clip) return MQC_E_NULL;
+  if (workspace_bytes < need) return MQC_E_SPACE;
+  if (need > 0 && !workspace) return MQC_E_NULL;
+  if (!aligned(workspace, 8)) return MQC_E_ALIGN;
+  double* partial = (double*)workspace;
+  hipStream_t s = (hipStream_t)stream;
+  const int st = by_tables<NormTable>(
+      tensors, count, 3, 1, 2, kNormChunk,
+      [](NormTable& t, int at, const int64_t* row, uint32_t first) {
+        t.grad[at] = (const void*)row[0];
+        t.n[at] = row[1];
+        t.first[at] = first;
+      },
+      [&](NormTable& t, int used, uint32_t blocks, int dtype) {
+        t.count = used;
+        MQC_LAUNCH(launch_norm, dtype, t, partial, blocks, s)
+        partial += blocks;
+      });
+  if (st != MQC_OK) return st;
+  grad_norm_end_kernel<<<dim3(1), dim3(1024), 0, s>>>((const double*)workspace,
+                                                      need / (int64_t)sizeof(double), max_norm, norm, clip);
+  return launch_status();
+}

@@ -1,0 +1,254 @@
+"""AdamW on the GPU: one launch for up to 48 tensors of a dtype, states in 32 or in 8 bits, the
+gradients' norm and its clipping on the device.
+
+    p <- p (1 - lr weight_decay) - lr m^ / (sqrt(v^) + eps),  m^ = m / (1 - beta1^t),  v^ = v / (1 - beta2^t)
+
+computed in fp32 from p and its gradient in their own dtype (fp32, bf16 or fp16), and rounded to p's
+dtype once. `AdamW` is the torch.optim.Optimizer (the reference's trainer uses torch's, train.py:182-206:
+clip to 1.0, then the step); `adamw_step_`, `adamw8_step_` and `grad_norm` are the operators under it.
+
+8-bit states hold m and sqrt(v) as torch.float8_e4m3fn with a power-of-two scale for each 256 elements
+of a tensor: 2.03 bytes a parameter instead of 8 (a 14.66 B parameter model: 30 GB instead of 117).
+Their rounding keeps the means of m and of v (csrc/adamw.hip); it needs a seed, and the same seed and
+step give the same bits.
+"""
+from __future__ import annotations
+
+import ctypes
+import itertools
+import math
+
+import torch
+
+from . import _native as nat
+
+STATE_BLOCK = 256  # elements that share a scale
+
+
+def state_blocks(numel: int) -> int:
+    """Scales of an 8-bit state of numel elements."""
+    return -(-numel // STATE_BLOCK)
+
+
+def _rows(values) -> ctypes.Array:
+    return (ctypes.c_int64 * max(1, len(values)))(*values)
+
+
+def _check_tensors(name, params, grads, *states):
+    """params and grads of one device, dtypes and shapes that match, all dense."""
+    if not all(len(s) == len(params) for s in (grads, *states)):
+        raise ValueError(f"{name}: lists of different lengths "
+                         f"{[len(s) for s in (params, grads, *states)]}")
+    for p, g in zip(params, grads):
+        if p.shape != g.shape or p.dtype != g.dtype:
+            raise ValueError(f"{name}: a gradient is {g.dtype} {tuple(g.shape)}, its parameter "
+                             f"{p.dtype} {tuple(p.shape)}")
+        if g.layout != torch.strided or not p.is_contiguous() or not g.is_contiguous():
+            raise ValueError(f"{name}: parameters and gradients must be contiguous")
+        nat.dtype_code(p)
+    flat = list(itertools.chain(params, grads, *states))
+    if flat:
+        nat.require_device(name, *flat)
+
+
+def _check_state(name, what, params, states, dtype, count=None):
+    for p, s in zip(params, states):
+        numel = p.numel() if count is None else count(p.numel())
+        if s.dtype != dtype or s.numel() != numel or not s.is_contiguous():
+            raise ValueError(f"{name}: {what} must be contiguous {dtype} of {numel} elements, got "
+                             f"{s.dtype} of {s.numel()}")
+
+
+def _scalars(step, lr, betas, eps, weight_decay):
+    if step < 1:
+        raise ValueError(f"adamw: steps count from 1, got {step}")
+    (b1, b2), lr = betas, float(lr)
+    return (1 - lr * weight_decay, lr / (1 - b1 ** step), 1 / math.sqrt(1 - b2 ** step), b1, 1 - b1,
+            b2, 1 - b2, eps)
+
+
+def _norm_and_clip(grads, max_norm):
+    """(norm, clip) as fp32 scalars on the gradients' device."""
+    dev = grads[0].device
+    rows = _rows([v for g in grads for v in (g.data_ptr(), g.numel(), nat.dtype_code(g))])
+    nbytes = nat.load().mqc_grad_norm_workspace_bytes(rows, len(grads))
+    if nbytes < 0:
+        nat.check(nbytes, "mqc_grad_norm")
+    out = torch.empty(2, device=dev, dtype=torch.float32)
+    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
+    nat.call("mqc_grad_norm", out, rows, len(grads), float(max_norm), out.data_ptr(),
+             out.data_ptr() + 4, ws.data_ptr(), nbytes, nat.stream_of(out))
+    return out[0], out[1]
+
+
+def grad_norm(grads: list[torch.Tensor]) -> torch.Tensor:
+    """The 2-norm of all elements of the tensors together (fp32 scalar on their device; summed in 64
+    bits, in a fixed order)."""
+    grads = [g.detach() for g in grads]
+    if not grads:
+        raise ValueError("grad_norm: no tensors")
+    _check_tensors("grad_norm", grads, grads)
+    return _norm_and_clip(grads, math.inf)[0]
+
+
+def _updated(*lists):
+    """The kernels write through pointers: tell autograd (and whatever keeps copies of parameters by
+    their version, as param_f32 does) that these tensors changed."""
+    for tensors in lists:
+        torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+
+
+def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float = 1e-3,
+                betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
+                max_norm: float | None = None) -> torch.Tensor | None:
+    """One AdamW step in place over lists of tensors: contiguous parameters and gradients of one
+    dtype each (fp32, bf16 or fp16), fp32 states. step counts from 1. With max_norm the gradients
+    are scaled by min(1, max_norm / (norm + 1e-6)) as they are read (they stay as they are), norm
+    over all of them, which is returned (fp32 scalar on the device)."""
+    params, grads = [p.detach() for p in params], [g.detach() for g in grads]
+    how = _scalars(step, lr, betas, eps, weight_decay)
+    _check_state("adamw_step_", "states", params, exp_avgs, torch.float32)
+    _check_state("adamw_step_", "states", params, exp_avg_sqs, torch.float32)
+    _check_tensors("adamw_step_", params, grads, exp_avgs, exp_avg_sqs)
+    if not params:
+        return None
+    norm, clip = (None, None) if max_norm is None else _norm_and_clip(grads, max_norm)
+    _launch32(params, grads, exp_avgs, exp_avg_sqs, how, clip)
+    return norm
+
+
+def _launch32(params, grads, ms, vs, how, clip):
+    rows = _rows([x for p, g, m, v in zip(params, grads, ms, vs)
+                  for x in (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(),
+                            nat.dtype_code(p))])
+    nat.call("mqc_adamw_step", params[0], rows, len(params), *how, nat.ptr(clip),
+             nat.stream_of(params[0]))
+    _updated(params, ms, vs)
+
+
+def adamw8_step_(params, grads, exp_avgs, exp_avg_scales, root_avg_sqs, root_avg_sq_scales, *,
+                 step: int, seed: int = 0, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, max_norm: float | None = None) -> torch.Tensor | None:
+    """adamw_step_ with states in 8 bits: exp_avgs and root_avg_sqs (sqrt(v)) torch.float8_e4m3fn
+    tensors of the parameters' sizes, their scales fp32 of state_blocks(numel) elements. What a state
+    stands for is its value times its block's scale. Tensor i of the lists rounds by seed + i."""
+    params, grads = [p.detach() for p in params], [g.detach() for g in grads]
+    how = _scalars(step, lr, betas, eps, weight_decay)
+    for what, states in (("states", exp_avgs), ("states", root_avg_sqs)):
+        _check_state("adamw8_step_", what, params, states, torch.float8_e4m3fn)
+    for what, states in (("scales", exp_avg_scales), ("scales", root_avg_sq_scales)):
+        _check_state("adamw8_step_", what, params, states, torch.float32, state_blocks)
+    _check_tensors("adamw8_step_", params, grads, exp_avgs, exp_avg_scales, root_avg_sqs,
+                   root_avg_sq_scales)
+    if not params:
+        return None
+    norm, clip = (None, None) if max_norm is None else _norm_and_clip(grads, max_norm)
+    _launch8(params, grads, exp_avgs, exp_avg_scales, root_avg_sqs, root_avg_sq_scales, how, clip,
+             step, range(seed, seed + len(params)))
+    return norm
+
+
+def _launch8(params, grads, ms, mscales, rs, rscales, how, clip, step, seeds):
+    rows = _rows([x for p, g, m, a, r, b, s in zip(params, grads, ms, mscales, rs, rscales, seeds)
+                  for x in (p.data_ptr(), g.data_ptr(), m.data_ptr(), r.data_ptr(), a.data_ptr(),
+                            b.data_ptr(), p.numel(), nat.dtype_code(p), s & 0xFFFFFFFF)])
+    nat.call("mqc_adamw8_step", params[0], rows, len(params), *how, nat.ptr(clip),
+             step & 0xFFFFFFFF, nat.stream_of(params[0]))
+    _updated(params, ms, mscales, rs, rscales)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW with decoupled weight decay over the kernels of this module.
+
+    state_bits: 32, or 8 for e4m3 states of the parameters with at least min_8bit_size elements
+    (smaller ones keep 32: they are no memory, and norms and gains are the ones that matter).
+    max_norm: the gradients' norm, over all groups together, is clipped to it as they are read;
+    `grad_norm` holds the last step's norm (a device scalar, not clipped). seed: of the 8-bit states'
+    rounding. Steps and learning rates are the host's: a step is not captured into a graph."""
+
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+                 weight_decay: float = 1e-2, state_bits: int = 32, min_8bit_size: int = 4096,
+                 max_norm: float | None = None, seed: int = 0):
+        if lr < 0 or eps < 0 or weight_decay < 0:
+            raise ValueError(f"AdamW: lr {lr}, eps {eps} and weight_decay {weight_decay} are not "
+                             "negative")
+        if not all(0 <= b < 1 for b in betas):
+            raise ValueError(f"AdamW: betas are in [0, 1), got {betas}")
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: state_bits is 8 or 32, got {state_bits}")
+        super().__init__(params, {"lr": lr, "betas": tuple(betas), "eps": eps,
+                                  "weight_decay": weight_decay, "state_bits": state_bits})
+        self.min_8bit_size, self.max_norm, self.seed = min_8bit_size, max_norm, seed
+        self.grad_norm = None
+
+    def _state_of(self, p, bits):
+        s = self.state[p]
+        if not s:
+            s["step"] = 0
+            if bits == 8 and p.numel() >= self.min_8bit_size:
+                for k in ("exp_avg", "root_avg_sq"):
+                    s[k] = torch.zeros(p.shape, device=p.device, dtype=torch.uint8).view(
+                        torch.float8_e4m3fn)
+                    s[k + "_scale"] = torch.ones(state_blocks(p.numel()), device=p.device)
+            else:
+                s["exp_avg"] = torch.zeros(p.shape, device=p.device, dtype=torch.float32)
+                s["exp_avg_sq"] = torch.zeros(p.shape, device=p.device, dtype=torch.float32)
+        return s
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: a step counts on the host and is not captured into a graph")
+        todo, grads, place = {}, [], 0
+        for index, group in enumerate(self.param_groups):
+            for p in group["params"]:
+                place += 1
+                if p.grad is None:
+                    continue
+                if p.grad.layout != torch.strided:
+                    raise ValueError("AdamW: sparse gradients are not supported")
+                g = p.grad.detach().contiguous()
+                if g.dtype != p.dtype:
+                    g = g.to(p.dtype)
+                s = self._state_of(p, group["state_bits"])
+                grads.append(g)
+                todo.setdefault((index, s["step"], "root_avg_sq" in s), []).append(
+                    (p.detach(), g, s, self.seed + place))
+        if not grads:
+            return loss
+        _check_tensors("AdamW", [p for t in todo.values() for p, *_ in t],
+                       [g for t in todo.values() for _, g, *_ in t])
+        clip = None
+        if self.max_norm is not None:
+            self.grad_norm, clip = _norm_and_clip(grads, self.max_norm)
+        for (index, step, eight), entries in todo.items():
+            group = self.param_groups[index]
+            how = _scalars(step + 1, group["lr"], group["betas"], group["eps"],
+                           group["weight_decay"])
+            params, gs, states, seeds = zip(*entries)
+            if eight:
+                _launch8(params, gs, *([s[k] for s in states] for k in (
+                    "exp_avg", "exp_avg_scale", "root_avg_sq", "root_avg_sq_scale")), how, clip,
+                    step + 1, seeds)
+            else:
+                _launch32(params, gs, *([s[k] for s in states] for k in ("exp_avg", "exp_avg_sq")),
+                          how, clip)
+            for s in states:
+                s["step"] = step + 1
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """torch's loading casts floating states to the parameter's dtype: the states' own are
+        put back from what was saved."""
+        super().load_state_dict(state_dict)
+        ids = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
+        params = itertools.chain.from_iterable(g["params"] for g in self.param_groups)
+        for i, p in zip(ids, params):
+            saved = state_dict["state"].get(i)
+            if saved is not None:
+                self.state[p] = {k: v.detach().to(p.device, copy=True).contiguous()
+                                 if isinstance(v, torch.Tensor) else v for k, v in saved.items()}

@@ -1,0 +1,90 @@
+"""The AdamW step's refusals and argument checks, without a GPU."""
+import ctypes
+
+import pytest
+import torch
+
+from mambaqc_amd import _native as nat
+from mambaqc_amd.optim import AdamW, adamw8_step_, adamw_step_, grad_norm, state_blocks
+
+E4M3 = torch.float8_e4m3fn
+
+
+def rows(*values):
+    return (ctypes.c_int64 * max(1, len(values)))(*values)
+
+
+def test_refuses_lists_that_do_not_match():
+    t = [torch.ones(6)]
+    with pytest.raises(ValueError, match="lengths"):
+        adamw_step_(t, [], [], [], step=1)
+    with pytest.raises(ValueError, match="states"):
+        adamw_step_(t, t, [torch.ones(5)], t, step=1)
+    with pytest.raises(ValueError, match="states"):
+        adamw_step_(t, t, t, [torch.ones(6, dtype=torch.float16)], step=1)
+    with pytest.raises(ValueError, match="gradient"):
+        adamw_step_(t, [torch.ones(6, dtype=torch.float16)], t, t, step=1)
+    with pytest.raises(ValueError, match="gradient"):
+        adamw_step_(t, [torch.ones(2, 3)], t, t, step=1)
+    with pytest.raises(ValueError, match="contiguous"):
+        adamw_step_([torch.ones(12)[::2]], t, t, t, step=1)
+    with pytest.raises(TypeError, match="unsupported dtype"):
+        d = [torch.ones(6, dtype=torch.float64)]
+        adamw_step_(d, d, t, t, step=1)
+    with pytest.raises(ValueError, match="count from 1"):
+        adamw_step_(t, t, t, t, step=0)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        adamw_step_(t, t, t, t, step=1)
+    assert adamw_step_([], [], [], [], step=1) is None
+
+
+def test_refuses_8_bit_states_that_do_not_match():
+    t, s = [torch.ones(300)], [torch.ones(2)]
+    c = [torch.zeros(300, dtype=torch.uint8).view(E4M3)]
+    assert state_blocks(300) == 2 and state_blocks(0) == 0 and state_blocks(256) == 1
+    with pytest.raises(ValueError, match="states"):
+        adamw8_step_(t, t, t, s, c, s, step=1)
+    with pytest.raises(ValueError, match="scales"):
+        adamw8_step_(t, t, c, [torch.ones(1)], c, s, step=1)
+    with pytest.raises(ValueError, match="scales"):
+        adamw8_step_(t, t, c, s, c, [torch.ones(3)], step=1)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        adamw8_step_(t, t, c, s, c, s, step=1)
+
+
+def test_optimizer_arguments():
+    p = torch.nn.Parameter(torch.ones(3))
+    for bad in ({"lr": -1.0}, {"betas": (1.0, 0.9)}, {"state_bits": 16}, {"eps": -1e-8},
+                {"weight_decay": -0.1}):
+        with pytest.raises(ValueError):
+            AdamW([p], **bad)
+    opt = AdamW([p])
+    assert opt.step() is None  # nothing has a gradient
+    p.grad = torch.ones(3)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        opt.step()
+    with pytest.raises(ValueError, match="no tensors"):
+        grad_norm([])
+
+
+def test_validation_codes():
+    lib, how = nat.load(), [1.0] * 8
+    step = lambda *v, count=1: lib.mqc_adamw_step(rows(*v), count, *how, None, None)
+    assert step(0, 64, 64, 64, 5, 0) == -1
+    assert step(64, 64, 64, 64, -5, 0) == -2
+    assert step(64, 64, 64, 64, 5, 9) == -3
+    assert step(66, 64, 64, 64, 5, 0) == -4 and step(64, 64, 66, 64, 5, 0) == -4
+    assert step(64, 65, 64, 64, 5, 1) == -4
+    assert step(64, 64, 64, 64, 1 << 62, 0) == -5
+    assert step(count=-1) == -2 and step(count=0) == 0
+    assert step(0, 0, 0, 0, 0, 0) == 0  # nothing to do
+    assert lib.mqc_adamw_step(None, 1, *how, None, None) == -1
+    step8 = lambda *v: lib.mqc_adamw8_step(rows(*v), 1, *how, None, 1, None)
+    assert step8(64, 64, 64, 64, 64, 0, 5, 0, 0) == -1
+    assert step8(64, 64, 64, 64, 66, 64, 5, 0, 0) == -4
+    assert step8(64, 64, 64, 64, 64, 64, 5, 4, 0) == -3
+    assert lib.mqc_grad_norm_workspace_bytes(rows(64, 8193, 0, 64, 1, 1), 2) == 24
+    assert lib.mqc_grad_norm_workspace_bytes(rows(64, -1, 0), 1) == -2
+    fake = ctypes.c_void_p(4096)
+    assert lib.mqc_grad_norm(rows(64, 10, 0), 1, 1.0, None, fake, fake, 64, None) == -1
+    assert lib.mqc_grad_norm(rows(64, 10, 0), 1, 1.0, fake, fake, fake, 4, None) == -6
