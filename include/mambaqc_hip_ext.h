@@ -139,6 +139,26 @@ int mqc_gated_scan_step(const void* dt, int64_t dt_row, const void* g, int64_t g
                         int64_t x_row, const float* log_rate, float* h, void* y, int64_t batch,
                         int64_t width, int dtype, void* stream);
 
+/* Between two blocks, for each of `rows` rows of d (1 to mqc_gate_norm_max_width()) elements:
+ *   v = sigmoid(z) y,  r = v / sqrt(mean v^2 + eps) post,  out = x + scale r,
+ *   n = out / sqrt(mean out^2 + eps) pre
+ * x, y, out and n dense, rows of z z_row elements apart; z NULL: v = y; post NULL: r = v. post, scale
+ * and pre are [d]. stats (fp32 [rows, 2], or NULL) takes the two inverse norms for the backward. out
+ * may be x or y, n may be y.
+ * Backward, from dout and dn (dense; either may be NULL, zeros): dx, dy and dz dense, dpost (with
+ * post), dscale and dpre [d] summed over the rows in a fixed order; rows at least 1, workspace of
+ * mqc_gate_norm_workspace_bytes. */
+int64_t mqc_gate_norm_max_width(void);
+int64_t mqc_gate_norm_workspace_bytes(int64_t rows, int64_t d);
+int mqc_gate_norm_fwd(const void* x, const void* y, const void* z, int64_t z_row, const float* post,
+                      const float* scale, const float* pre, void* out, void* n, float* stats,
+                      int64_t rows, int64_t d, float eps, int dtype, void* stream);
+int mqc_gate_norm_bwd(const void* x, const void* y, const void* z, int64_t z_row, const float* post,
+                      const float* scale, const float* pre, const float* stats, const void* dout,
+                      const void* dn, void* dx, void* dy, void* dz, float* dpost, float* dscale,
+                      float* dpre, int64_t rows, int64_t d, int dtype, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
 /* One AdamW step over `count` tensors, each element in fp32:
  *   g = grad * (*clip);  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *   p = p decay - m / (sqrt(v) root_scale + eps) step_size

@@ -109,6 +109,8 @@ SIGNATURES_EXT = {
     "mqc_step_norm_out_gate_fits": [_i64, _i64],
     "mqc_step_ssm": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _f32,
                      _int, _vp],
+    "mqc_gate_norm_fwd": [_vp] * 3 + [_i64] + [_vp] * 6 + [_i64] * 2 + [_f32, _int, _vp],
+    "mqc_gate_norm_bwd": [_vp] * 3 + [_i64] + [_vp] * 12 + [_i64] * 2 + [_int, _vp, _i64, _vp],
     "mqc_adamw_step": [_vp, _i64] + [_f32] * 8 + [_vp, _vp],
     "mqc_adamw8_step": [_vp, _i64] + [_f32] * 8 + [_vp, _u32, _vp],
     "mqc_grad_norm": [_vp, _i64, _f64, _vp, _vp, _vp, _i64, _vp],
@@ -118,6 +120,8 @@ SIGNATURES_EXT = {
     "mqc_gated_scan_step": [_vp, _i64] * 3 + [_vp] * 3 + [_i64] * 2 + [_int, _vp],
 }
 SIGNATURES_EXT_I64 = {
+    "mqc_gate_norm_max_width": [],
+    "mqc_gate_norm_workspace_bytes": [_i64, _i64],
     "mqc_grad_norm_workspace_bytes": [_vp, _i64],
     "mqc_gated_scan_workspace_bytes": [_i64, _i64, _i64],
     "mqc_qln_bwd_sums_workspace_bytes": [_i64, _i64],

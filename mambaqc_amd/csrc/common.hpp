@@ -232,6 +232,20 @@ __device__ inline float sum_halves_to_low(float v) {
   return a + b;
 }
 
+// Sum over the wave, the same in every lane: within rows of 16 lanes by DPP, then the four rows'
+// through scalar registers.
+__device__ inline float wave_sum_all(float v) {
+  v += lane_xor1(v);
+  v += lane_xor2(v);
+  v += row_rot4(v);
+  v += row_rot8(v);
+  const int b = __builtin_bit_cast(int, v);
+  const auto row = [&](int lane) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, lane));
+  };
+  return (row(0) + row(16)) + (row(32) + row(48));
+}
+
 // ---------------------------------------------------------------------------
 // The SSM's front (elementwise.hip; the decode step): delta = softplus(dt_raw) and the gate's
 // sigmoid.
@@ -249,6 +263,14 @@ __device__ inline float front_softplus(float v) {
   return fmaxf(v, 0.f) + l;
 }
 __device__ inline float front_sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
+
+// sigmoid(v) and 1 - sigmoid(v), neither by subtraction.
+__device__ inline void sigmoid_pair(float v, float& s, float& c) {
+  const float e = __expf(-fabsf(v));
+  const float r = __builtin_amdgcn_rcpf(1.f + e);
+  s = v < 0.f ? e * r : r;
+  c = v < 0.f ? r : e * r;
+}
 
 // ---------------------------------------------------------------------------
 // XCD-aware block order. MI355X dispatches the workgroups of a launch to its 8

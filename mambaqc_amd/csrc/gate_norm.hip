@@ -1,0 +1,413 @@
+// What stands between two blocks of a pre-norm and post-norm stack, in one pass over the row:
+//   v = sigmoid(z) y,  rho = 1 / sqrt(mean v^2 + eps),  r = v rho post
+//   o = x + scale r,   tau = 1 / sqrt(mean o^2 + eps),  n = o tau pre
+// o is the residual stream, n what the next block reads; without z the gate is 1, without post r = v.
+// Backward, from do and dn (means over the row, w = scale post, u = dn pre):
+//   O = do + tau u - o tau^3 mean(u o)                                (the gradient of o, dx = O)
+//   dv = rho w O - v rho^3 mean(w O v)   (without post dv = scale O)  dy = dv sigmoid(z)
+//   dz = dv v (1 - sigmoid(z)),  dscale = sum over rows of O r,  dpost = sum of scale O v rho,
+//   dpre = sum of dn o tau
+// mean(w O v) splits into mean(w v (do + tau u)) - tau^3 mean(u o) mean(w v o), so that a row takes
+// one reduction (of three sums) and not two, the second waiting for the first.
+// Everything between the loads and the stores is fp32; n comes from o before o is rounded.
+#include "common.hpp"
+
+namespace mqc {
+
+template <typename T>
+struct GateNormArgs {
+  const T *x, *y, *z;
+  int64_t z_row;  // elements between rows of z
+  const float *post, *scale, *pre;
+  int64_t rows, d;
+  float eps;
+  // forward
+  T *out, *n;
+  float* stats;  // [rows, 2]: rho and tau, or NULL
+  // backward
+  const T *dout, *dn;
+  T *dx, *dy, *dz;
+  float* part;  // [3, workgroups, d]: sums of O r, dn o tau, and scale O v rho
+};
+
+// Four consecutive elements from wherever they start (rows of odd widths do not start at multiples
+// of a vector; gfx950 loads and stores those as it does aligned ones), `left` of them.
+template <typename T>
+__device__ inline void load_part(const T* row, uint32_t i, int left, float (&out)[4]) {
+  const T* p = row + i;
+  if (left >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      typedef float any4 __attribute__((ext_vector_type(4), aligned(4)));
+      const any4 v = *reinterpret_cast<const any4*>(p);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) out[c] = v[c];
+    } else {
+      typedef uint32_t any2 __attribute__((ext_vector_type(2), aligned(2)));
+      const any2 v = *reinterpret_cast<const any2*>(p);
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        out[c] = io<T>::bits_to_f32(c & 1 ? v[c / 2] >> 16 : v[c / 2] & 0xffffu);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) out[c] = c < left ? load_scalar(p + c) : 0.f;
+  }
+}
+template <typename T>
+__device__ inline void store_part(T* row, uint32_t i, int left, const float (&in)[4]) {
+  T* p = row + i;
+  if (left >= 4) {
+    if constexpr (sizeof(T) == 4) {
+      typedef float any4 __attribute__((ext_vector_type(4), aligned(4)));
+      *reinterpret_cast<any4*>(p) = any4{in[0], in[1], in[2], in[3]};
+    } else {
+      typedef uint32_t any2 __attribute__((ext_vector_type(2), aligned(2)));
+      *reinterpret_cast<any2*>(p) = any2{pack2<T>(in[0], in[1]), pack2<T>(in[2], in[3])};
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (c < left) store_scalar(p + c, in[c]);
+  }
+}
+
+// A row belongs to a team: one wave (ONE), or all waves of the workgroup. Its sums, the same in every
+// lane; `red` holds 16 floats a sum.
+template <bool ONE, int N>
+__device__ inline void team_sum(float (&v)[N], float* red) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = wave_sum_all(v[i]);
+  if constexpr (!ONE) {
+    const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) red[16 * i + wave] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = 0.f;
+#pragma unroll 2
+    for (int w = 0; w < waves; ++w) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += red[16 * i + w];
+    }
+  }
+}
+
+constexpr int kOneRows = 4;  // rows (waves) of a workgroup whose teams are single waves
+
+// A lane holds elements 4 (lane + team m) + 0..3 of its row for m < NV.
+template <typename T, int NV, bool ONE>
+__global__ __launch_bounds__(ONE ? 64 * kOneRows : 1024) void gate_norm_fwd_kernel(GateNormArgs<T> k) {
+  __shared__ float red[ONE ? 1 : 32];
+  const int team = ONE ? 64 : blockDim.x, t = ONE ? threadIdx.x & 63 : threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = (int)k.d;
+  const int64_t row = ONE ? (int64_t)blockIdx.x * kOneRows + wave : blockIdx.x;
+  if (row >= k.rows) return;  // whole teams; a team of several waves has its row
+  const int64_t base = row * k.d;
+  float x[NV][4], v[NV][4];
+  float s[1] = {0.f};
+#pragma unroll
+  for (int m = 0; m < NV; ++m) {
+    const uint32_t i = 4 * (t + m * team);
+    const int left = d - (int)i;
+    load_part(k.x + base, i, left, x[m]);
+    load_part(k.y + base, i, left, v[m]);
+    if (k.z) {
+      float z[4];
+      load_part(k.z + row * k.z_row, i, left, z);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float sg, cg;
+        sigmoid_pair(z[c], sg, cg);
+        v[m][c] *= sg;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) s[0] = fmaf(v[m][c], v[m][c], s[0]);
+  }
+  const float inv = 1.f / (float)k.d;
+  float rho = 1.f;
+  if (k.post) {
+    team_sum<ONE>(s, red);
+    rho = 1.f / sqrtf(s[0] * inv + k.eps);
+  }
+  s[0] = 0.f;
+#pragma unroll
+  for (int m = 0; m < NV; ++m) {
+    const uint32_t i = 4 * (t + m * team);
+    const int left = d - (int)i;
+    float sc[4], po[4];
+    load_part(k.scale, i, left, sc);
+    if (k.post) load_part(k.post, i, left, po);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float r = k.post ? v[m][c] * rho * po[c] : v[m][c];
+      x[m][c] = fmaf(sc[c], r, x[m][c]);
+      s[0] = fmaf(x[m][c], x[m][c], s[0]);
+    }
+    store_part(k.out + base, i, left, x[m]);
+  }
+  team_sum<ONE>(s, red + (ONE ? 0 : 16));
+  const float tau = 1.f / sqrtf(s[0] * inv + k.eps);
+#pragma unroll
+  for (int m = 0; m < NV; ++m) {
+    const uint32_t i = 4 * (t + m * team);
+    const int left = d - (int)i;
+    float pre[4];
+    load_part(k.pre, i, left, pre);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) x[m][c] *= tau * pre[c];
+    store_part(k.n + base, i, left, x[m]);
+  }
+  if (k.stats && t == 0) {
+    k.stats[2 * row] = rho;
+    k.stats[2 * row + 1] = tau;
+  }
+}
+
+// Teams walk rows (their number, + teams, ..) and keep the weights' sums in registers.
+template <typename T, int NV, bool ONE>
+__global__ __launch_bounds__(ONE ? 64 * kOneRows : 1024) void gate_norm_bwd_kernel(GateNormArgs<T> k) {
+  __shared__ float red[2][ONE ? 1 : 48];
+  __shared__ float fold[ONE ? kOneRows - 1 : 1][ONE ? 3 * NV * 256 : 1];
+  const int team = ONE ? 64 : blockDim.x, t = ONE ? threadIdx.x & 63 : threadIdx.x;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = (int)k.d;
+  const float inv = 1.f / (float)k.d;
+  float sum[3][NV][4], sc[NV][4], po[NV][4], pre[NV][4];
+  const auto weights = [&] {
+#pragma unroll
+    for (int m = 0; m < NV; ++m) {
+      const uint32_t i = 4 * (t + m * team);
+      const int left = d - (int)i;
+      load_part(k.scale, i, left, sc[m]);
+      load_part(k.pre, i, left, pre[m]);
+      if (k.post) load_part(k.post, i, left, po[m]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) po[m][c] = k.post ? po[m][c] : 1.f;
+    }
+  };
+  if constexpr (NV == 1) weights();
+#pragma unroll
+  for (int m = 0; m < NV; ++m)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) sum[0][m][c] = sum[1][m][c] = sum[2][m][c] = 0.f;
+  const int64_t first = ONE ? (int64_t)blockIdx.x * kOneRows + wave : blockIdx.x;
+  const int64_t step = ONE ? (int64_t)gridDim.x * kOneRows : gridDim.x;
+  int flip = 0;  // two sets of sums: one barrier a row is enough
+  for (int64_t row = first; row < k.rows; row += step, flip ^= 1) {
+    const int64_t base = row * k.d;
+    const float rho = k.stats[2 * row], tau = k.stats[2 * row + 1];
+    float o[NV][4], v[NV][4], sg[NV][4], cg[NV][4], dn[NV][4], g[NV][4];
+    float s[3] = {0.f, 0.f, 0.f};
+    if constexpr (NV > 1) weights();
+#pragma unroll
+    for (int m = 0; m < NV; ++m) {
+      const uint32_t i = 4 * (t + m * team);
+      const int left = d - (int)i;
+      load_part(k.x + base, i, left, o[m]);
+      load_part(k.y + base, i, left, v[m]);
+      if (k.z) load_part(k.z + row * k.z_row, i, left, sg[m]);
+      if (k.dout) load_part(k.dout + base, i, left, g[m]);
+      if (k.dn) load_part(k.dn + base, i, left, dn[m]);
+    }
+#pragma unroll
+    for (int m = 0; m < NV; ++m)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if (!k.dout) g[m][c] = 0.f;
+        if (!k.dn) dn[m][c] = 0.f;
+        if (k.z) {
+          sigmoid_pair(sg[m][c], sg[m][c], cg[m][c]);
+          v[m][c] *= sg[m][c];
+        }
+        o[m][c] = fmaf(sc[m][c], v[m][c] * rho * po[m][c], o[m][c]);
+        const float u = dn[m][c] * pre[m][c], wv = sc[m][c] * po[m][c] * v[m][c];
+        g[m][c] = fmaf(tau, u, g[m][c]);
+        sum[1][m][c] = fmaf(dn[m][c] * tau, o[m][c], sum[1][m][c]);
+        s[0] = fmaf(u, o[m][c], s[0]);
+        s[1] = fmaf(wv, g[m][c], s[1]);
+        s[2] = fmaf(wv, o[m][c], s[2]);
+      }
+    team_sum<ONE>(s, red[flip]);
+    if constexpr (NV > 1) weights();  // not held meanwhile, nor z's gates: a lane has 128 registers
+    const float back = tau * tau * tau * s[0] * inv;
+    const float side = k.post ? rho * rho * rho * inv * (s[1] - back * s[2]) : 0.f;
+#pragma unroll
+    for (int m = 0; m < NV; ++m) {
+      const uint32_t i = 4 * (t + m * team);
+      const int left = d - (int)i;
+      float dy[4], dz[4];
+      if constexpr (NV > 1) {
+        if (k.z) {
+          load_part(k.z + row * k.z_row, i, left, sg[m]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sigmoid_pair(sg[m][c], sg[m][c], cg[m][c]);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float O = fmaf(-back, o[m][c], g[m][c]), vr = v[m][c] * rho;
+        sum[0][m][c] = fmaf(O, vr * po[m][c], sum[0][m][c]);
+        sum[2][m][c] = fmaf(sc[m][c] * O, vr, sum[2][m][c]);
+        g[m][c] = O;
+        const float dv = fmaf(rho * sc[m][c] * po[m][c], O, -side * v[m][c]);
+        dy[c] = k.z ? dv * sg[m][c] : dv;
+        dz[c] = k.z ? dv * v[m][c] * cg[m][c] : 0.f;
+      }
+      store_part(k.dx + base, i, left, g[m]);
+      store_part(k.dy + base, i, left, dy);
+      if (k.z) store_part(k.dz + base, i, left, dz);
+    }
+  }
+  if constexpr (ONE) {  // the workgroup's waves into its first
+    if (wave > 0) {
+#pragma unroll
+      for (int j = 0; j < 3; ++j)
+#pragma unroll
+        for (int m = 0; m < NV; ++m)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) fold[wave - 1][((j * NV + m) * 4 + c) * 64 + t] = sum[j][m][c];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+#pragma unroll
+    for (int w = 0; w < kOneRows - 1; ++w)
+#pragma unroll
+      for (int j = 0; j < 3; ++j)
+#pragma unroll
+        for (int m = 0; m < NV; ++m)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sum[j][m][c] += fold[w][((j * NV + m) * 4 + c) * 64 + t];
+  }
+#pragma unroll
+  for (int j = 0; j < 3; ++j)
+#pragma unroll
+    for (int m = 0; m < NV; ++m) {
+      const uint32_t i = 4 * (t + m * team);
+      store_part(k.part + ((int64_t)j * gridDim.x + blockIdx.x) * k.d, i, d - (int)i, sum[j][m]);
+    }
+}
+
+constexpr int64_t kGateNormMaxWidth = 8192;
+
+inline int64_t gate_norm_bwd_blocks(int64_t rows, int64_t d) {
+  const int64_t need = d <= 256 ? (rows + kOneRows - 1) / kOneRows : rows;
+  return need < 512 ? need : 512;
+}
+
+template <typename T>
+int launch_gate_norm_fwd(const GateNormArgs<T>& k, hipStream_t s) {
+#define MQC_GN(NV, ONE, BLOCKS, WAVES)                                                           \
+  gate_norm_fwd_kernel<T, NV, ONE><<<dim3((unsigned)(BLOCKS)), dim3(64 * (WAVES)), 0, s>>>(k);   \
+  return launch_status();
+  const int64_t four = (k.rows + kOneRows - 1) / kOneRows;
+  if (k.d <= 256) { MQC_GN(1, true, four, kOneRows) }
+  if (k.d <= 512) { MQC_GN(2, true, four, kOneRows) }
+  if (k.d <= 768) { MQC_GN(3, true, four, kOneRows) }
+  if (k.d <= 1024) { MQC_GN(4, true, four, kOneRows) }
+  MQC_GN(4, false, k.rows, (k.d + 1023) / 1024)
+#undef MQC_GN
+}
+
+template <typename T>
+int launch_gate_norm_bwd(const GateNormArgs<T>& k, float* dscale, float* dpre, float* dpost,
+                         hipStream_t s) {
+  const int64_t blocks = gate_norm_bwd_blocks(k.rows, k.d);
+#define MQC_GN(NV, ONE, WAVES) \
+  gate_norm_bwd_kernel<T, NV, ONE><<<dim3((unsigned)blocks), dim3(64 * (WAVES)), 0, s>>>(k);
+  if (k.d <= 256) {
+    MQC_GN(1, true, kOneRows)
+  } else if (k.d <= 4096) {
+    MQC_GN(1, false, (k.d + 255) / 256)
+  } else {
+    MQC_GN(2, false, (k.d + 511) / 512)
+  }
+#undef MQC_GN
+  const int st = launch_status();
+  if (st != MQC_OK) return st;
+  const int64_t each = blocks * k.d;
+  return mqc_sum_rows(k.part, dscale, k.d, k.part + each, dpre, k.d, k.part + 2 * each, dpost,
+                      dpost ? k.d : 0, blocks, s);
+}
+
+inline int gate_norm_shape(int64_t rows, int64_t d, const void* z, int64_t z_row, int dtype) {
+  if (rows < 0 || d < 1) return MQC_E_SHAPE;
+  if (dtype != MQC_F32 && dtype != MQC_BF16 && dtype != MQC_F16) return MQC_E_DTYPE;
+  if (z && rows > 1 && z_row < d) return MQC_E_SHAPE;
+  if (d > kGateNormMaxWidth || rows > 0x7fffffffLL) return MQC_E_LIMIT;
+  return MQC_OK;
+}
+
+template <typename T>
+GateNormArgs<T> gate_norm_args(const void* x, const void* y, const void* z, int64_t z_row,
+                               const float* post, const float* scale, const float* pre,
+                               int64_t rows, int64_t d, float eps) {
+  GateNormArgs<T> k{};
+  k.x = (const T*)x; k.y = (const T*)y; k.z = (const T*)z; k.z_row = z_row;
+  k.post = post; k.scale = scale; k.pre = pre;
+  k.rows = rows; k.d = d; k.eps = eps;
+  return k;
+}
+
+}  // namespace mqc
+
+using namespace mqc;
+
+#define MQC_BY_DTYPE(F)                    \
+  switch (dtype) {                         \
+    case MQC_F32: return F(float);         \
+    case MQC_BF16: return F(bf16_t);       \
+    default: return F(f16_t);              \
+  }
+
+extern "C" int64_t mqc_gate_norm_max_width(void) { return kGateNormMaxWidth; }
+
+extern "C" int64_t mqc_gate_norm_workspace_bytes(int64_t rows, int64_t d) {
+  if (rows < 1 || d < 1) return MQC_E_SHAPE;
+  if (d > kGateNormMaxWidth) return MQC_E_LIMIT;
+  return gate_norm_bwd_blocks(rows, d) * 3 * d * (int64_t)sizeof(float);
+}
+
+extern "C" int mqc_gate_norm_fwd(const void* x, const void* y, const void* z, int64_t z_row,
+                                 const float* post, const float* scale, const float* pre, void* out,
+                                 void* n, float* stats, int64_t rows, int64_t d, float eps,
+                                 int dtype, void* stream) {
+  const int st = gate_norm_shape(rows, d, z, z_row, dtype);
+  if (st != MQC_OK) return st;
+  if (rows == 0) return MQC_OK;
+  if (!x || !y || !scale || !pre || !out || !n) return MQC_E_NULL;
+#define MQC_F(T)                                                                        \
+  [&] {                                                                                 \
+    GateNormArgs<T> k = gate_norm_args<T>(x, y, z, z_row, post, scale, pre, rows, d, eps); \
+    k.out = (T*)out; k.n = (T*)n; k.stats = stats;                                      \
+    return launch_gate_norm_fwd<T>(k, (hipStream_t)stream);                             \
+  }()
+  MQC_BY_DTYPE(MQC_F)
+#undef MQC_F
+}
+
+extern "C" int mqc_gate_norm_bwd(const void* x, const void* y, const void* z, int64_t z_row,
+                                 const float* post, const float* scale, const float* pre,
+                                 const float* stats, const void* dout, const void* dn, void* dx,
+                                 void* dy, void* dz, float* dpost, float* dscale, float* dpre,
+                                 int64_t rows, int64_t d, int dtype, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
+  const int st = gate_norm_shape(rows, d, z, z_row, dtype);
+  if (st != MQC_OK) return st;
+  if (rows < 1) return MQC_E_SHAPE;
+  if (!x || !y || !scale || !pre || !stats || !dx || !dy || (z && !dz) || (post && !dpost) ||
+      !dscale || !dpre || !workspace)
+    return MQC_E_NULL;
+  if (workspace_bytes < mqc_gate_norm_workspace_bytes(rows, d)) return MQC_E_SPACE;
+#define MQC_F(T)                                                                       \
+  [&] {                                                                                \
+    GateNormArgs<T> k = gate_norm_args<T>(x, y, z, z_row, post, scale, pre, rows, d, 0.f); \
+    k.stats = const_cast<float*>(stats);                                               \
+    k.dout = (const T*)dout; k.dn = (const T*)dn;                                      \
+    k.dx = (T*)dx; k.dy = (T*)dy; k.dz = (T*)dz; k.part = (float*)workspace;           \
+    return launch_gate_norm_bwd<T>(k, dscale, dpre, post ? dpost : nullptr, (hipStream_t)stream); \
+  }()
+  MQC_BY_DTYPE(MQC_F)
+#undef MQC_F
+}

@@ -60,14 +60,6 @@ struct ScanSpan {
 __device__ inline float scan_step(float c, float s, float h) {
   return fmaf(c, s - h, scan_fast(c) ? s : h);
 }
-// sigmoid(v) and 1 - sigmoid(v), neither by subtraction.
-__device__ inline void scan_sigmoid(float v, float& s, float& c) {
-  const float e = __expf(-fabsf(v));
-  const float r = __builtin_amdgcn_rcpf(1.f + e);
-  s = v < 0.f ? e * r : r;
-  c = v < 0.f ? r : e * r;
-}
-
 template <typename T>
 struct ScanArgs {
   const T *dt, *g, *x;
@@ -106,7 +98,7 @@ __global__ __launch_bounds__(64) void gated_scan_fwd_kernel(ScanArgs<T> k) {
     }
     float p, sg, cg;
     const float c = scan_decay(load_scalar(k.dt + row * k.dt_row + d), rate, p);
-    scan_sigmoid(load_scalar(k.g + row * k.g_row + d), sg, cg);
+    sigmoid_pair(load_scalar(k.g + row * k.g_row + d), sg, cg);
     if (k.reset && k.reset[row]) u = left = 0.f, span.cut(), cut = true;
     u = scan_step(c, sg * load_scalar(k.x + row * k.x_row + d), u);
     left = scan_fade(c, left);
@@ -135,7 +127,7 @@ __global__ __launch_bounds__(64) void gated_scan_bwd_kernel(ScanArgs<T> k) {
       const int64_t row = b * k.seq + t0 + i;
       float p, sg, cg;
       const float c = scan_decay(load_scalar(k.dt + row * k.dt_row + d), rate, p);
-      scan_sigmoid(load_scalar(k.g + row * k.g_row + d), sg, cg);
+      sigmoid_pair(load_scalar(k.g + row * k.g_row + d), sg, cg);
       if (k.reset && k.reset[row]) u = left = 0.f;
       states[i][threadIdx.x] = u + left;
       u = scan_step(c, sg * load_scalar(k.x + row * k.x_row + d), u);
@@ -146,8 +138,8 @@ __global__ __launch_bounds__(64) void gated_scan_bwd_kernel(ScanArgs<T> k) {
       const float dtv = load_scalar(k.dt + row * k.dt_row + d);
       float p, sg, cg, sd, cd;
       const float c = scan_decay(dtv, rate, p);
-      scan_sigmoid(load_scalar(k.g + row * k.g_row + d), sg, cg);
-      scan_sigmoid(dtv, sd, cd);
+      sigmoid_pair(load_scalar(k.g + row * k.g_row + d), sg, cg);
+      sigmoid_pair(dtv, sd, cd);
       const float s = sg * load_scalar(k.x + row * k.x_row + d);
       G += load_scalar(k.dy + row * k.width + d);
       const float dp = scan_a(c) * G * (s - states[i][threadIdx.x]);
@@ -170,7 +162,7 @@ __global__ __launch_bounds__(256) void gated_scan_step_kernel(ScanArgs<T> k, flo
   if (d >= k.width) return;
   float p, sg, cg;
   const float c = scan_decay(load_scalar(k.dt + b * k.dt_row + d), scan_rate(k.log_rate[d]), p);
-  scan_sigmoid(load_scalar(k.g + b * k.g_row + d), sg, cg);
+  sigmoid_pair(load_scalar(k.g + b * k.g_row + d), sg, cg);
   const float v = scan_step(c, sg * load_scalar(k.x + b * k.x_row + d), h[b * k.width + d]);
   h[b * k.width + d] = v;
   store_scalar(k.y + b * k.width + d, v);

@@ -25,7 +25,7 @@ from torch.library import custom_op, register_autograd
 
 from . import _native as nat
 from .block import _gate_operands, _out_gate_backward
-from .kernels import cayley_transform, gated, parallel_scan, quaternion_ops
+from .kernels import cayley_transform, gate_norm, gated, parallel_scan, quaternion_ops
 from .kernels import ssm_fused as sf
 from .kernels.quaternion_norm import _qln_backward, _qln_forward
 from .layers.causal_conv1d import _conv_silu_backward, _ConvSiLU, _rows_view
@@ -486,15 +486,6 @@ def _gate_bwd(ctx, dout):
 register_autograd(f"{NS}::out_gate", _gate_bwd, setup_context=_gate_setup)
 
 
-OPS = (
-    "quaternion_multiply", "quaternion_conjugate", "quaternion_inverse", "quaternion_norm",
-    "cayley_discretization", "cumprod_scan", "ssm_forward_q", "ssm_step_q", "ssm_forward_dl",
-    "ssm_forward_dl_train", "ssm_backward_dl", "ssm_front", "ssm_front_backward",
-    "quaternion_layer_norm", "quaternion_layer_norm_backward", "causal_conv1d_silu",
-    "causal_conv1d_silu_backward", "out_gate", "out_gate_backward",
-)
-
-
 # --- the gated scan -------------------------------------------------------------
 
 @custom_op(f"{NS}::gated_scan", mutates_args=())
@@ -563,3 +554,67 @@ def _gated_scan_bwd(ctx, dy, dh_last, _gcarries):
 
 
 register_autograd(f"{NS}::gated_scan_train", _gated_scan_bwd, setup_context=_gated_scan_setup)
+
+
+# --- gate, norms and residual between blocks --------------------------------------
+
+@custom_op(f"{NS}::gate_norm_residual", mutates_args=())
+def gate_norm_residual(x: Tensor, y: Tensor, z: Optional[Tensor], post_weight: Optional[Tensor],
+                       scale: Tensor, pre_weight: Tensor,
+                       eps: float = 1e-6) -> Tuple[Tensor, Tensor, Tensor]:
+    """(out, n in the promoted dtype, the rows' inverse norms fp32 [rows, 2])."""
+    return gate_norm._forward(gate_norm._operands(x, y, z, post_weight, scale, pre_weight), eps, True)
+
+
+@gate_norm_residual.register_fake
+def _(x, y, z, post_weight, scale, pre_weight, eps=1e-6):
+    out = x.new_empty(x.shape, dtype=gate_norm._dtype(x, y, z))
+    rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
+    return out, torch.empty_like(out), x.new_empty(rows, 2, dtype=torch.float32)
+
+
+@custom_op(f"{NS}::gate_norm_residual_backward", mutates_args=())
+def gate_norm_residual_backward(
+        x: Tensor, y: Tensor, z: Optional[Tensor], post_weight: Optional[Tensor], scale: Tensor,
+        pre_weight: Tensor, stats: Tensor, dout: Tensor,
+        dn: Tensor) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """(dx, dy, dz in the promoted dtype, dpost, dscale, dpre in fp32); dz and dpost are empty where
+    they do not apply."""
+    ops = gate_norm._operands(x, y, z, post_weight, scale, pre_weight)
+    dx, dy, dz, dpost, dscale, dpre = gate_norm._backward(ops, stats, dout, dn)
+    return (dx, dy, x.new_empty(0, dtype=dx.dtype) if dz is None else dz,
+            dscale.new_empty(0) if dpost is None else dpost, dscale, dpre)
+
+
+@gate_norm_residual_backward.register_fake
+def _(x, y, z, post_weight, scale, pre_weight, stats, dout, dn):
+    dx = x.new_empty(x.shape, dtype=gate_norm._dtype(x, y, z))
+    d = scale.new_empty(scale.shape, dtype=torch.float32)
+    return (dx, torch.empty_like(dx), dx.new_empty(0) if z is None else torch.empty_like(dx),
+            d.new_empty(0) if post_weight is None else torch.empty_like(d), torch.empty_like(d), d)
+
+
+def _gate_norm_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:6], output[2])
+
+
+def _gate_norm_bwd(ctx, dout, dn, _gstats):
+    *ops, stats = ctx.saved_tensors
+    dx, dy, dz, dpost, dscale, dpre = gate_norm_residual_backward(*ops, stats, dout, dn)
+    x, y, z, post, scale, pre = ops
+    return (dx.to(x.dtype), dy.to(y.dtype), None if z is None else dz.to(z.dtype),
+            None if post is None else dpost.to(post.dtype), dscale.to(scale.dtype),
+            dpre.to(pre.dtype), None)
+
+
+register_autograd(f"{NS}::gate_norm_residual", _gate_norm_bwd, setup_context=_gate_norm_setup)
+
+
+OPS = (
+    "quaternion_multiply", "quaternion_conjugate", "quaternion_inverse", "quaternion_norm",
+    "cayley_discretization", "cumprod_scan", "ssm_forward_q", "ssm_step_q", "ssm_forward_dl",
+    "ssm_forward_dl_train", "ssm_backward_dl", "ssm_front", "ssm_front_backward",
+    "quaternion_layer_norm", "quaternion_layer_norm_backward", "causal_conv1d_silu",
+    "causal_conv1d_silu_backward", "out_gate", "out_gate_backward", "gated_scan", "gated_scan_train",
+    "gated_scan_backward", "gate_norm_residual", "gate_norm_residual_backward",
+)
