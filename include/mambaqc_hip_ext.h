@@ -117,7 +117,7 @@ int mqc_step_norm_out_gate_fits(int64_t M, int64_t d_inner);
  * of them), y is dense. h_last (fp32, or NULL) may be h0. carries (fp32 [batch,
  * ceil(seq_len / mqc_gated_scan_chunk()), width], or NULL): the states that the backward starts
  * from, each chunk's before its first token.
- * workspace of mqc_gated_scan_workspace_bytes. width and seq_len at most 2^31, batch at most 65535.
+ * workspace (16-byte aligned) of mqc_gated_scan_workspace_bytes. width and seq_len at most 2^31, batch at most 65535.
  *
  * Backward: gradients of dt, g, x (dense), log_rate [width], and of h0 (or NULL) from dy and
  * dh_last (or NULL); every size at least 1.

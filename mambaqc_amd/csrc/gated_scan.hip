@@ -12,54 +12,68 @@
 
 namespace mqc {
 
-// Steps of a chunk, which is walked from zero: y_t = u_t + d_t, u the chunk's own part and d what is
-// left of the state before it, and the state goes from chunk to chunk by the chunk's whole decay and
-// its last u. A state that grows slowly over many tokens is so rounded once a chunk, not once a
-// token. A training forward stores the states between chunks.
-constexpr int kScanChunk = 128;
+// The exponents are held in base 2: p_t = log2(e) D_t exp(log_rate), a_t = 2^-p_t.
+//
+// Time is cut into chunks, a chunk into one span of steps for each of its waves, and a lane walks one
+// channel of its wave's span: first from zero (u, its last state, and the sum of p, which give what the
+// span makes of any state before it), then, once the state before the span is known, through the
+// states themselves. The spans of a chunk join in LDS. Between chunks the state goes through memory
+// within the launch: see scan_entry.
 
-// log(1 + e) by its series below 3/32 (the first left-out term is under 2^-24 of the sum there),
-// where rounding 1 + e would lose digits.
-__device__ inline float scan_softplus(float v) {
-  const float e = __expf(-fabsf(v));
-  const float series =
-      e * (1.f - e * (0.5f - e * (1.f / 3 - e * (0.25f - e * (0.2f - e * (1.f / 6 - e * (1.f / 7)))))));
-  return fmaxf(v, 0.f) + (e < 0.09375f ? series : __logf(1.f + e));
+constexpr int kScanLanes = 64;    // channels of a workgroup
+constexpr int kScanWaves = 8;     // spans of a chunk
+constexpr int kScanSteps = 16;    // steps of a span, forward
+constexpr int kScanBack = 8;      // and backward (whose steps take twice the registers)
+constexpr int kScanChunk = kScanWaves * kScanBack;  // steps between the states that training stores
+constexpr int kScanGroup = 16;    // chunks that are joined one by one (scan_entry)
+
+// log2(1 + 2^v): what rounding 1 + e leaves of e is added to first order.
+__device__ inline float scan_softplus2(float v) {
+  const float e = __builtin_amdgcn_exp2f(-fabsf(v));
+  const float u = 1.f + e;
+  return fmaf(e - (u - 1.f), 1.44269504f, fmaxf(v, 0.f) + __builtin_amdgcn_logf(u));
 }
 
 // A step's decay as one number c. A slow channel has a near 1 and forgets by 1 - a a token: rounding
 // a to fp32 would shift its rate, and with it the gain at rest, by 2^-25 / (1 - a). So c is 1 - a
-// (from its own series) while that is under a half, and -a after that; the sign bit tells.
-struct ScanRate { float log_rate, rate; };
-__device__ inline ScanRate scan_rate(float log_rate) { return {log_rate, expf(log_rate)}; }
-__device__ inline float scan_decay(float dt, ScanRate r, float& p) {
-  p = scan_softplus(dt) * r.rate;
-  if (__builtin_expect(dt < -80.f, 0)) p = __expf(dt + r.log_rate);  // exp(dt) alone underflows
-  p = p > 3e38f ? 3e38f : p;  // p a stays 0 there, not inf * 0; a NaN stays one
-  const float a = __expf(-p);
-  const float series =
-      p * (1.f - p * (0.5f - p * (1.f / 6 - p * (1.f / 24 - p * (1.f / 120 - p * (1.f / 720))))));
-  const float w = p < 0.25f ? series : 1.f - a;
-  return w < 0.5f ? w : -a;
+// while p < 1 (a minimax fit of (1 - 2^-p) / p on [0, 1], off by 2^-26.6, rounded by 2^-23), and -a
+// after that; the sign bit tells.
+__device__ inline float scan_code(float p) {
+  float w = fmaf(p, -1.14580565e-4f, 1.29078003e-3f);
+  w = fmaf(p, w, -9.5962761e-3f);
+  w = fmaf(p, w, 5.5498954e-2f);
+  w = fmaf(p, w, -2.40226060e-1f);
+  w = fmaf(p, w, 6.93147182e-1f);
+  return p < 1.f ? p * w : -__builtin_amdgcn_exp2f(-p);
 }
 __device__ inline bool scan_fast(float c) { return __float_as_int(c) < 0; }  // c is -a
 __device__ inline float scan_a(float c) { return scan_fast(c) ? -c : 1.f - c; }
 __device__ inline float scan_w(float c) { return scan_fast(c) ? 1.f + c : c; }
 // a v, and a h + (1 - a) s.
 __device__ inline float scan_fade(float c, float v) { return scan_fast(c) ? -c * v : fmaf(-c, v, v); }
-// The decay of two steps: 1 - a from its own sum, a from its own product.
-struct ScanSpan {
-  float a = 1.f, w = 0.f;
-  __device__ void then(float c) {
-    a *= scan_a(c);
-    w = fmaf(scan_w(c), 1.f - w, w);
-  }
-  __device__ void cut() { a = 0.f, w = 1.f; }
-  __device__ float c() const { return w < 0.5f ? w : -a; }
-};
 __device__ inline float scan_step(float c, float s, float h) {
   return fmaf(c, s - h, scan_fast(c) ? s : h);
 }
+
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
+struct ScanRate { float log2_rate, rate; };
+__device__ inline ScanRate scan_rate(float log_rate) {
+  const float r = expf(log_rate);
+  return {log_rate * kLog2e, r > 3e38f ? 3e38f : r};  // (a gradient times the rate is then 0, not NaN)
+}
+// p of a step. Below dt = -80, where exp(dt) alone would underflow, from the sum of the logarithms.
+__device__ inline float scan_p(float dt, ScanRate r) { return scan_softplus2(dt * kLog2e) * r.rate; }
+__device__ inline float scan_p_low(float dt, ScanRate r) {
+  return __builtin_amdgcn_exp2f(fmaf(dt, kLog2e, r.log2_rate)) * kLog2e;
+}
+
+// What a span (or a chunk) makes of the state h before it: u + 2^-p h, and u alone behind a reset.
+// c is scan_code(p), or kScanCut.
+constexpr float kScanCut = 2.f;
+__device__ inline float scan_join(float c, float u, float h) {
+  return c == kScanCut ? u : u + scan_fade(c, h);
+}
+
 template <typename T>
 struct ScanArgs {
   const T *dt, *g, *x;
@@ -76,83 +90,329 @@ struct ScanArgs {
   const T* dy;
   const float* dh_last;
   T *ddt, *dg, *dx;
-  float *drate, *dh0;
+  float *drate, *dh0;  // drate: [batch, chunks, width]
+  // the states between chunks (several of them)
+  uint32_t* ticket;
+  uint32_t* ends;   // [batch, groups, width]
+  uint64_t* spans;  // [batch, chunks, width]
 };
 
-// A lane walks one channel of one sequence.
-template <typename T>
-__global__ __launch_bounds__(64) void gated_scan_fwd_kernel(ScanArgs<T> k) {
-  const int64_t d = (int64_t)blockIdx.x * 64 + threadIdx.x, b = blockIdx.y;
-  if (d >= k.width) return;
-  const ScanRate rate = scan_rate(k.log_rate[d]);
-  float h = k.h0 ? k.h0[b * k.width + d] : 0.f, u = 0.f, left = h;
-  const int64_t chunks = (k.seq + kScanChunk - 1) / kScanChunk;
-  ScanSpan span;
-  bool cut = false;
-  for (int64_t t = 0; t < k.seq; ++t) {
-    const int64_t row = b * k.seq + t;
-    if (t % kScanChunk == 0) {
-      if (t > 0) h = cut ? u : u + scan_fade(span.c(), h);
-      if (k.carries) k.carries[(b * chunks + t / kScanChunk) * k.width + d] = h;
-      u = 0.f, left = h, span = ScanSpan(), cut = false;
-    }
-    float p, sg, cg;
-    const float c = scan_decay(load_scalar(k.dt + row * k.dt_row + d), rate, p);
-    sigmoid_pair(load_scalar(k.g + row * k.g_row + d), sg, cg);
-    if (k.reset && k.reset[row]) u = left = 0.f, span.cut(), cut = true;
-    u = scan_step(c, sg * load_scalar(k.x + row * k.x_row + d), u);
-    left = scan_fade(c, left);
-    span.then(c);
-    store_scalar(k.y + row * k.width + d, u + left);
+// ---------------------------------------------------------------------------
+// The state before a chunk. Each chunk posts its span (c, u) as one 64-bit word, the last one of each
+// group of kScanGroup chunks posts the state after it as one 32-bit word, and a chunk joins its
+// group's earlier spans, in order, to the state that the group before it posted: always the same sums,
+// whoever comes first. A word is data and flag in one: all bits set (a NaN that is never posted) is
+// "not yet", and the clearing launch sets that. Workgroups take their chunk from a counter, in order
+// of time, so whatever one waits for is already running; a wait that does not end in about a second
+// all the same posts NaN and goes on.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kNoWord = 0xffffffffu;
+constexpr uint32_t kNanBits = 0x7fc00000u;
+__device__ inline uint32_t word_of(float v) { return v == v ? __float_as_uint(v) : kNanBits; }
+template <typename W>
+__device__ inline void post(W* at, W v) {
+  __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <typename W>
+__device__ inline W peek(const W* at) {
+  return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ inline uint64_t span_word(float c, float u) {
+  return ((uint64_t)word_of(c) << 32) | word_of(u);
+}
+// Reads again until the word is there (the same number of times in every lane of the wave).
+template <typename W>
+__device__ inline W await(const W* at, W v, bool on, int& patience) {
+  while (__any(on && v == (W)~(W)0) && --patience > 0) {
+    __builtin_amdgcn_s_sleep(2);
+    if (on) v = peek(at);
   }
-  if (k.seq > 0) h = cut ? u : u + scan_fade(span.c(), h);
-  if (k.h_last) k.h_last[b * k.width + d] = h;
+  return v;
 }
 
-// Backward: the chunks from the last to the first, each walked forward from its stored entry state
-// with its states kept in LDS, then back.
-template <typename T>
-__global__ __launch_bounds__(64) void gated_scan_bwd_kernel(ScanArgs<T> k) {
-  __shared__ float states[kScanChunk][64];
-  const int64_t d = (int64_t)blockIdx.x * 64 + threadIdx.x, b = blockIdx.y;
-  if (d >= k.width) return;
-  const int64_t chunks = (k.seq + kScanChunk - 1) / kScanChunk;
-  const ScanRate rate = scan_rate(k.log_rate[d]);
-  float G = k.dh_last ? k.dh_last[b * k.width + d] : 0.f, drate = 0.f;
-  for (int64_t j = chunks - 1; j >= 0; --j) {
-    const int64_t t0 = j * kScanChunk;
-    const int n = (int)(k.seq - t0 < kScanChunk ? k.seq - t0 : kScanChunk);
-    float left = k.carries[(b * chunks + j) * k.width + d], u = 0.f;
-    for (int i = 0; i < n; ++i) {
-      const int64_t row = b * k.seq + t0 + i;
-      float p, sg, cg;
-      const float c = scan_decay(load_scalar(k.dt + row * k.dt_row + d), rate, p);
-      sigmoid_pair(load_scalar(k.g + row * k.g_row + d), sg, cg);
-      if (k.reset && k.reset[row]) u = left = 0.f;
-      states[i][threadIdx.x] = u + left;
-      u = scan_step(c, sg * load_scalar(k.x + row * k.x_row + d), u);
-      left = scan_fade(c, left);
-    }
-    for (int i = n - 1; i >= 0; --i) {
-      const int64_t row = b * k.seq + t0 + i;
-      const float dtv = load_scalar(k.dt + row * k.dt_row + d);
-      float p, sg, cg, sd, cd;
-      const float c = scan_decay(dtv, rate, p);
-      sigmoid_pair(load_scalar(k.g + row * k.g_row + d), sg, cg);
-      sigmoid_pair(dtv, sd, cd);
-      const float s = sg * load_scalar(k.x + row * k.x_row + d);
-      G += load_scalar(k.dy + row * k.width + d);
-      const float dp = scan_a(c) * G * (s - states[i][threadIdx.x]);
-      const float ds = scan_w(c) * G;
-      store_scalar(k.ddt + row * k.width + d, dp * rate.rate * sd);
-      store_scalar(k.dg + row * k.width + d, ds * s * cg);
-      store_scalar(k.dx + row * k.width + d, ds * sg);
-      drate = fmaf(dp, p, drate);
-      G = k.reset && k.reset[row] ? 0.f : scan_fade(c, G);
-    }
+// BACK: chunks run from the last to the first, and n counts chunks from that end.
+template <bool BACK>
+__device__ inline float scan_entry(const uint64_t* spans, const uint32_t* ends, int64_t chunks,
+                                   int64_t n, int64_t width, float first, bool on) {
+  const int64_t group = n / kScanGroup;
+  const int member = (int)(n % kScanGroup);
+  const auto span_at = [&](int m) {
+    const int64_t i = group * kScanGroup + m;
+    return spans + (BACK ? chunks - 1 - i : i) * width;
+  };
+  int patience = 1 << 20;
+  uint64_t w[kScanGroup - 1];
+#pragma unroll
+  for (int m = 0; m < kScanGroup - 1; ++m) w[m] = m < member && on ? peek(span_at(m)) : 0;
+  float h = first;
+  if (group > 0) {
+    const uint32_t* at = ends + (group - 1) * width;
+    h = __uint_as_float(await(at, on ? peek(at) : 0u, on, patience));
   }
-  k.drate[b * k.width + d] = drate;
-  if (k.dh0) k.dh0[b * k.width + d] = G;
+#pragma unroll
+  for (int m = 0; m < kScanGroup - 1; ++m)
+    if (m < member) {
+      const uint64_t v = await(span_at(m), w[m], on, patience);
+      h = scan_join(__uint_as_float((uint32_t)(v >> 32)), __uint_as_float((uint32_t)v), h);
+    }
+  return h;
+}
+
+__global__ __launch_bounds__(256) void scan_clear_kernel(uint4* words, int64_t count) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < count) words[i] = i == 0 ? uint4{0, 0, 0, 0} : uint4{kNoWord, kNoWord, kNoWord, kNoWord};
+}
+
+// Which chunk (from the end where the walk starts) of which 64 channels of which sequence.
+struct ScanPlace { int64_t n, b, d0; };
+template <bool CHAIN>
+__device__ inline ScanPlace scan_place(uint32_t* ticket, int64_t width, int64_t tiles, uint32_t* lds) {
+  uint32_t i = blockIdx.x;
+  if constexpr (CHAIN) {
+    if (threadIdx.x == 0)
+      *lds = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    i = __builtin_amdgcn_readfirstlane(*lds);
+  }
+  const int64_t across = (width + kScanLanes - 1) / kScanLanes;
+  const int64_t tile = i % (uint32_t)tiles;
+  return {(int64_t)(i / (uint32_t)tiles), tile / across, tile % across * kScanLanes};
+}
+
+// The resets of a span's steps as bits (bit i: step i).
+__device__ inline uint32_t scan_resets(const uint8_t* reset, int64_t row, int n) {
+  const int lane = threadIdx.x & 63;
+  const bool cut = reset && lane < n && reset[row + lane];
+  return __builtin_amdgcn_readfirstlane((uint32_t)__ballot(cut));
+}
+
+// Forward: a workgroup takes one chunk of 64 channels.
+template <typename T, bool CHAIN>
+__global__ __launch_bounds__(64 * kScanWaves) void gated_scan_fwd_kernel(ScanArgs<T> k, int64_t tiles) {
+  __shared__ float part[3][kScanWaves][64];  // p (-1 behind a reset), c, u of each span
+  __shared__ float entry[64];
+  __shared__ uint32_t place;
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const ScanPlace at = scan_place<CHAIN>(k.ticket, k.width, tiles, &place);
+  const int64_t d = at.d0 + lane, b = at.b;
+  const bool on = d < k.width;
+  const int64_t dc = on ? d : k.width - 1;  // lanes past the end read the last channel
+  const int64_t chunk = (int64_t)waves * kScanSteps, chunks = CHAIN ? (k.seq + chunk - 1) / chunk : 1;
+  const int64_t t0 = at.n * chunk + wave * kScanSteps, row0 = b * k.seq + t0;
+  const int n = k.seq - t0 < kScanSteps ? (k.seq > t0 ? (int)(k.seq - t0) : 0) : kScanSteps;
+  const ScanRate rate = scan_rate(k.log_rate[dc]);
+  float c[kScanSteps], s[kScanSteps];
+  uint32_t cuts = 0;
+  float p = 0.f, u = 0.f;
+  if (n > 0) {
+    cuts = scan_resets(k.reset, row0, n);
+    float low = 0.f;
+#pragma unroll
+    for (int i = 0; i < kScanSteps; ++i) {
+      const int64_t row = row0 + (i < n ? i : n - 1);
+      const float dt = load_scalar(k.dt + row * k.dt_row + dc);
+      const float g = load_scalar(k.g + row * k.g_row + dc), x = load_scalar(k.x + row * k.x_row + dc);
+      low = fminf(low, dt);
+      c[i] = scan_p(dt, rate);
+      s[i] = x * __builtin_amdgcn_rcpf(1.f + __expf(-g));
+    }
+    if (__builtin_expect(__any(low < -80.f), 0)) {
+#pragma unroll
+      for (int i = 0; i < kScanSteps; ++i) {
+        const int64_t row = row0 + (i < n ? i : n - 1);
+        const float dt = load_scalar(k.dt + row * k.dt_row + dc);
+        if (dt < -80.f) c[i] = scan_p_low(dt, rate);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kScanSteps; ++i)
+      if (i < n) {
+        if (cuts >> i & 1) u = 0.f, p = 0.f;
+        p += c[i];
+        c[i] = scan_code(c[i]);
+        u = scan_step(c[i], s[i], u);
+      }
+  }
+  part[0][wave][lane] = cuts ? -1.f : p;
+  part[1][wave][lane] = cuts ? kScanCut : scan_code(p);
+  part[2][wave][lane] = u;
+  float h = 0.f;
+  if (wave == 0 && at.n == 0) {
+    h = k.h0 ? k.h0[b * k.width + dc] : 0.f;
+    entry[lane] = h;
+  }
+  __syncthreads();
+  if constexpr (CHAIN) {
+    if (wave == 0) {
+      const int64_t groups = (chunks + kScanGroup - 1) / kScanGroup;
+      uint64_t* spans = k.spans + b * chunks * k.width + d;
+      uint32_t* ends = k.ends + b * groups * k.width + d;
+      const bool last = at.n % kScanGroup == kScanGroup - 1;
+      float cu = h, cp = 0.f;
+      bool cut = at.n == 0;  // the first chunk posts its state (h0 is not read again: h_last may be h0)
+#pragma unroll
+      for (int w = 0; w < kScanWaves; ++w) {
+        const float wp = part[0][w][lane];
+        cut |= wp < 0.f;
+        cp += wp;
+        cu = scan_join(part[1][w][lane], part[2][w][lane], cu);
+      }
+      const float cc = cut ? kScanCut : scan_code(cp);
+      if (!last && on) post(spans + at.n * k.width, span_word(cc, cu));
+      if (at.n > 0) entry[lane] = h = scan_entry<false>(spans, ends, chunks, at.n, k.width, 0.f, on);
+      if (last && on) post(ends + at.n / kScanGroup * k.width, word_of(scan_join(cc, cu, h)));
+    }
+    __syncthreads();
+  }
+  h = entry[lane];
+  if (n == 0) {
+    if (k.seq == 0 && k.h_last && on && wave == 0) k.h_last[b * k.width + d] = h;
+    return;
+  }
+  for (int w = 0; w < wave; ++w) h = scan_join(part[1][w][lane], part[2][w][lane], h);
+  if (k.carries && t0 % kScanChunk == 0 && on) {
+    const int64_t every = (k.seq + kScanChunk - 1) / kScanChunk;
+    k.carries[(b * every + t0 / kScanChunk) * k.width + d] = h;
+  }
+#pragma unroll
+  for (int i = 0; i < kScanSteps; ++i)
+    if (i < n) {
+      if (cuts >> i & 1) h = 0.f;
+      h = scan_step(c[i], s[i], h);
+      if (on) store_scalar(k.y + (row0 + i) * k.width + d, h);
+    }
+  if (k.h_last && on && t0 + n == k.seq) k.h_last[b * k.width + d] = h;
+}
+
+// Backward: the chunks from the last to the first, each from its stored entry state. What a span makes
+// of the adjoint A behind it (A = a G of the step after) is v + 2^-p A.
+template <typename T, bool CHAIN>
+__global__ __launch_bounds__(64 * kScanWaves) void gated_scan_bwd_kernel(ScanArgs<T> k, int64_t tiles) {
+  __shared__ float part[4][kScanWaves][64];  // p (-1 behind a reset), c, u, v of each span
+  __shared__ float entry[64];
+  __shared__ uint32_t place;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const ScanPlace at = scan_place<CHAIN>(k.ticket, k.width, tiles, &place);
+  const int64_t d = at.d0 + lane, b = at.b;
+  const bool on = d < k.width;
+  const int64_t dc = on ? d : k.width - 1;
+  const int64_t chunks = CHAIN ? (k.seq + kScanChunk - 1) / kScanChunk : 1, j = chunks - 1 - at.n;
+  const int64_t t0 = j * kScanChunk + wave * kScanBack, row0 = b * k.seq + t0;
+  const int n = k.seq - t0 < kScanBack ? (k.seq > t0 ? (int)(k.seq - t0) : 0) : kScanBack;
+  const ScanRate rate = scan_rate(k.log_rate[dc]);
+  // c; s, later s - h; dy; sigmoid(g); s (1 - sigmoid(g)); dp/ddt = rate sigmoid(dt); p
+  float c[kScanBack], e[kScanBack], dy[kScanBack], sg[kScanBack], q[kScanBack], sd[kScanBack],
+      ps[kScanBack];
+  uint32_t cuts = 0;
+  float p = 0.f, u = 0.f, v = 0.f;
+  if (n > 0) {
+    cuts = scan_resets(k.reset, row0, n);
+    float low = 0.f;
+#pragma unroll
+    for (int i = 0; i < kScanBack; ++i) {
+      const int64_t row = row0 + (i < n ? i : n - 1);
+      const float dt = load_scalar(k.dt + row * k.dt_row + dc);
+      const float g = load_scalar(k.g + row * k.g_row + dc), x = load_scalar(k.x + row * k.x_row + dc);
+      dy[i] = load_scalar(k.dy + row * k.width + dc);
+      low = fminf(low, dt);
+      float cg, cd;
+      sigmoid_pair(g, sg[i], cg);
+      sigmoid_pair(dt, sd[i], cd);
+      e[i] = x * sg[i];
+      q[i] = e[i] * cg;
+      sd[i] *= rate.rate;
+      ps[i] = scan_p(dt, rate);
+    }
+    if (__builtin_expect(__any(low < -80.f), 0)) {
+#pragma unroll
+      for (int i = 0; i < kScanBack; ++i) {
+        const int64_t row = row0 + (i < n ? i : n - 1);
+        const float dt = load_scalar(k.dt + row * k.dt_row + dc);
+        if (dt < -80.f) ps[i] = scan_p_low(dt, rate), sd[i] = ps[i] * kLn2;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kScanBack; ++i)
+      if (i < n) {
+        if (cuts >> i & 1) u = 0.f, p = 0.f;
+        p += ps[i];
+        c[i] = scan_code(ps[i]);
+        u = scan_step(c[i], e[i], u);
+      }
+#pragma unroll
+    for (int i = kScanBack - 1; i >= 0; --i)
+      if (i < n) v = cuts >> i & 1 ? 0.f : scan_fade(c[i], dy[i] + v);
+  }
+  part[0][wave][lane] = cuts ? -1.f : p;
+  part[1][wave][lane] = cuts ? kScanCut : scan_code(p);
+  part[2][wave][lane] = u;
+  part[3][wave][lane] = v;
+  __syncthreads();
+  const float behind = k.dh_last ? k.dh_last[b * k.width + dc] : 0.f;
+  if constexpr (CHAIN) {
+    if (wave == 0) {
+      const int64_t groups = (chunks + kScanGroup - 1) / kScanGroup;
+      uint64_t* spans = k.spans + b * chunks * k.width + d;
+      uint32_t* ends = k.ends + b * groups * k.width + d;
+      const bool last = at.n % kScanGroup == kScanGroup - 1;
+      float cv = 0.f, cp = 0.f;
+      bool cut = false;
+#pragma unroll
+      for (int w = kScanWaves - 1; w >= 0; --w) {
+        const float wp = part[0][w][lane];
+        cut |= wp < 0.f;
+        cp += wp;
+        cv = scan_join(part[1][w][lane], part[3][w][lane], cv);
+      }
+      const float cc = cut ? kScanCut : scan_code(cp);
+      if (!last && on) post(spans + j * k.width, span_word(cc, cv));
+      const float A = scan_entry<true>(spans, ends, chunks, at.n, k.width, behind, on);
+      if (last && on) post(ends + at.n / kScanGroup * k.width, word_of(scan_join(cc, cv, A)));
+      entry[lane] = A;
+    }
+    __syncthreads();
+  }
+  float A = CHAIN ? entry[lane] : behind, drate = 0.f;
+  if (n > 0) {
+    float h = k.carries[(b * chunks + j) * k.width + dc];
+    for (int w = 0; w < wave; ++w) h = scan_join(part[1][w][lane], part[2][w][lane], h);
+    for (int w = kScanWaves - 1; w > wave; --w) A = scan_join(part[1][w][lane], part[3][w][lane], A);
+#pragma unroll
+    for (int i = 0; i < kScanBack; ++i)
+      if (i < n) {
+        if (cuts >> i & 1) h = 0.f;
+        const float s = e[i];
+        e[i] = s - h;
+        h = scan_step(c[i], s, h);
+      }
+#pragma unroll
+    for (int i = kScanBack - 1; i >= 0; --i)
+      if (i < n) {
+        const float G = dy[i] + A, aG = scan_fade(c[i], G);
+        const float dp = aG * e[i], ds = scan_w(c[i]) * G;
+        const int64_t to = (row0 + i) * k.width + d;
+        if (on) {
+          store_scalar(k.ddt + to, dp * sd[i]);
+          store_scalar(k.dg + to, ds * q[i]);
+          store_scalar(k.dx + to, ds * sg[i]);
+        }
+        // (2^-p is 0 long before p = 300: no 0 times infinity)
+        drate = fmaf(dp, fminf(ps[i], 300.f), drate);
+        A = cuts >> i & 1 ? 0.f : aG;
+      }
+    if (k.dh0 && on && t0 == 0) k.dh0[b * k.width + d] = A;
+  }
+  __syncthreads();
+  part[0][wave][lane] = drate;
+  __syncthreads();
+  if (wave == 0 && on) {
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kScanWaves; ++w) sum += part[0][w][lane];
+    k.drate[(b * chunks + j) * k.width + d] = sum * kLn2;
+  }
 }
 
 // One token for each sequence, the state in place.
@@ -160,26 +420,69 @@ template <typename T>
 __global__ __launch_bounds__(256) void gated_scan_step_kernel(ScanArgs<T> k, float* h) {
   const int64_t d = (int64_t)blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
   if (d >= k.width) return;
-  float p, sg, cg;
-  const float c = scan_decay(load_scalar(k.dt + b * k.dt_row + d), scan_rate(k.log_rate[d]), p);
-  sigmoid_pair(load_scalar(k.g + b * k.g_row + d), sg, cg);
-  const float v = scan_step(c, sg * load_scalar(k.x + b * k.x_row + d), h[b * k.width + d]);
+  const float dt = load_scalar(k.dt + b * k.dt_row + d), g = load_scalar(k.g + b * k.g_row + d);
+  const float s = load_scalar(k.x + b * k.x_row + d) * __builtin_amdgcn_rcpf(1.f + __expf(-g));
+  const ScanRate rate = scan_rate(k.log_rate[d]);
+  const float c = scan_code(dt < -80.f ? scan_p_low(dt, rate) : scan_p(dt, rate));
+  const float v = scan_step(c, s, h[b * k.width + d]);
   h[b * k.width + d] = v;
   store_scalar(k.y + b * k.width + d, v);
 }
 
+// The workspace of a launch over several chunks: the ticket's 16 bytes, the spans, the ends; and of the
+// backward the partial sums of dlog_rate behind them.
+struct ScanSpace { int64_t chunks, words, bytes; };
+inline ScanSpace scan_space(int64_t batch, int64_t seq, int64_t width, int64_t chunk) {
+  const int64_t chunks = (seq + chunk - 1) / chunk, groups = (chunks + kScanGroup - 1) / kScanGroup;
+  const int64_t words = chunks > 1 ? batch * width * (8 * chunks + 4 * groups) : 0;
+  return {chunks, words, words > 0 ? (words + 31) / 16 * 16 : 0};
+}
+
 template <typename T>
-int launch_gated_scan_fwd(const ScanArgs<T>& k, int64_t batch, hipStream_t s) {
-  gated_scan_fwd_kernel<T><<<dim3((unsigned)((k.width + 63) / 64), (unsigned)batch), dim3(64), 0, s>>>(k);
+int scan_chain(ScanArgs<T>& k, const ScanSpace& w, int64_t batch, char* ws, hipStream_t s) {
+  k.ticket = (uint32_t*)ws;
+  k.spans = (uint64_t*)(ws + 16);
+  k.ends = (uint32_t*)(k.spans + batch * w.chunks * k.width);
+  const int64_t quads = w.bytes / 16;
+  scan_clear_kernel<<<dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s>>>((uint4*)ws, quads);
   return launch_status();
 }
 
 template <typename T>
-int launch_gated_scan_bwd(ScanArgs<T> k, int64_t batch, float* drate, hipStream_t s) {
-  gated_scan_bwd_kernel<T><<<dim3((unsigned)((k.width + 63) / 64), (unsigned)batch), dim3(64), 0, s>>>(k);
+int launch_gated_scan_fwd(ScanArgs<T> k, int64_t batch, char* ws, hipStream_t s) {
+  const int64_t tiles = batch * ((k.width + kScanLanes - 1) / kScanLanes);
+  const ScanSpace w = scan_space(batch, k.seq, k.width, kScanWaves * kScanSteps);
+  if (w.chunks > 1) {
+    const int st = scan_chain(k, w, batch, ws, s);
+    if (st != MQC_OK) return st;
+    gated_scan_fwd_kernel<T, true>
+        <<<dim3((unsigned)(tiles * w.chunks)), dim3(64 * kScanWaves), 0, s>>>(k, tiles);
+  } else {
+    const int64_t waves = k.seq > 0 ? (k.seq + kScanSteps - 1) / kScanSteps : 1;
+    gated_scan_fwd_kernel<T, false>
+        <<<dim3((unsigned)tiles), dim3((unsigned)(64 * waves)), 0, s>>>(k, tiles);
+  }
+  return launch_status();
+}
+
+template <typename T>
+int launch_gated_scan_bwd(ScanArgs<T> k, int64_t batch, float* drate, char* ws, hipStream_t s) {
+  const int64_t tiles = batch * ((k.width + kScanLanes - 1) / kScanLanes);
+  const ScanSpace w = scan_space(batch, k.seq, k.width, kScanChunk);
+  k.drate = (float*)(ws + w.bytes);
+  if (w.chunks > 1) {
+    const int st = scan_chain(k, w, batch, ws, s);
+    if (st != MQC_OK) return st;
+    gated_scan_bwd_kernel<T, true>
+        <<<dim3((unsigned)(tiles * w.chunks)), dim3(64 * kScanWaves), 0, s>>>(k, tiles);
+  } else {
+    gated_scan_bwd_kernel<T, false>
+        <<<dim3((unsigned)tiles), dim3(64 * kScanWaves), 0, s>>>(k, tiles);
+  }
   const int st = launch_status();
   if (st != MQC_OK) return st;
-  return mqc_sum_rows(k.drate, drate, k.width, nullptr, nullptr, 0, nullptr, nullptr, 0, batch, s);
+  return mqc_sum_rows(k.drate, drate, k.width, nullptr, nullptr, 0, nullptr, nullptr, 0,
+                      batch * w.chunks, s);
 }
 
 template <typename T>
@@ -196,6 +499,9 @@ inline int scan_shape(int64_t batch, int64_t seq, int64_t width, int64_t dt_row,
   if (dtype != MQC_F32 && dtype != MQC_BF16 && dtype != MQC_F16) return MQC_E_DTYPE;
   if (batch * seq > 1 && (dt_row < width || g_row < width || x_row < width)) return MQC_E_SHAPE;
   if (batch > 65535 || seq > (1LL << 31) || width > (1LL << 31)) return MQC_E_LIMIT;
+  // Workgroups are counted in 31 bits (2^43 elements).
+  if (batch * ((width + kScanLanes - 1) / kScanLanes) > 0x7fffffffLL / (seq / kScanChunk + 1))
+    return MQC_E_LIMIT;
   return MQC_OK;
 }
 
@@ -226,7 +532,8 @@ extern "C" int mqc_gated_scan_chunk(void) { return kScanChunk; }
 
 extern "C" int64_t mqc_gated_scan_workspace_bytes(int64_t batch, int64_t seq_len, int64_t width) {
   if (batch < 0 || seq_len < 0 || width < 0) return MQC_E_SHAPE;
-  return batch * width * (int64_t)sizeof(float);
+  const ScanSpace w = scan_space(batch, seq_len, width, kScanChunk);
+  return w.bytes + batch * w.chunks * width * (int64_t)sizeof(float);
 }
 
 extern "C" int mqc_gated_scan_fwd(const void* dt, int64_t dt_row, const void* g, int64_t g_row,
@@ -242,11 +549,12 @@ extern "C" int mqc_gated_scan_fwd(const void* dt, int64_t dt_row, const void* g,
   if (seq_len == 0 && !h_last) return MQC_OK;
   if (workspace_bytes < mqc_gated_scan_workspace_bytes(batch, seq_len, width)) return MQC_E_SPACE;
   if (workspace_bytes > 0 && !workspace) return MQC_E_NULL;
+  if (!aligned(workspace, 16)) return MQC_E_ALIGN;
 #define MQC_F(T)                                                                               \
   [&] {                                                                                        \
     ScanArgs<T> k = scan_args<T>(dt, dt_row, g, g_row, x, x_row, log_rate, reset, seq_len, width); \
     k.h0 = h0; k.y = (T*)y; k.h_last = h_last; k.carries = carries;                            \
-    return launch_gated_scan_fwd<T>(k, batch, (hipStream_t)stream);                            \
+    return launch_gated_scan_fwd<T>(k, batch, (char*)workspace, (hipStream_t)stream);                            \
   }()
   MQC_BY_DTYPE(MQC_F)
 #undef MQC_F
@@ -266,13 +574,14 @@ extern "C" int mqc_gated_scan_bwd(const void* dt, int64_t dt_row, const void* g,
       !workspace)
     return MQC_E_NULL;
   if (workspace_bytes < mqc_gated_scan_workspace_bytes(batch, seq_len, width)) return MQC_E_SPACE;
+  if (!aligned(workspace, 16)) return MQC_E_ALIGN;
 #define MQC_F(T)                                                                               \
   [&] {                                                                                        \
     ScanArgs<T> k = scan_args<T>(dt, dt_row, g, g_row, x, x_row, log_rate, reset, seq_len, width); \
     k.carries = const_cast<float*>(carries);                                                   \
     k.dy = (const T*)dy; k.dh_last = dh_last; k.ddt = (T*)ddt; k.dg = (T*)dg; k.dx = (T*)dx;    \
-    k.drate = (float*)workspace; k.dh0 = dh0;                                                  \
-    return launch_gated_scan_bwd<T>(k, batch, dlog_rate, (hipStream_t)stream);                 \
+    k.dh0 = dh0;                                                                               \
+    return launch_gated_scan_bwd<T>(k, batch, dlog_rate, (char*)workspace, (hipStream_t)stream); \
   }()
   MQC_BY_DTYPE(MQC_F)
 #undef MQC_F
