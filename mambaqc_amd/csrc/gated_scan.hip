@@ -20,12 +20,14 @@ namespace mqc {
 // states themselves. The spans of a chunk join in LDS. Between chunks the state goes through memory
 // within the launch: see scan_entry.
 
-constexpr int kScanLanes = 64;    // channels of a workgroup
-constexpr int kScanWaves = 8;     // spans of a chunk
-constexpr int kScanSteps = 16;    // steps of a span, forward
-constexpr int kScanBack = 8;      // and backward (whose steps take twice the registers)
-constexpr int kScanChunk = kScanWaves * kScanBack;  // steps between the states that training stores
-constexpr int kScanGroup = 16;    // chunks that are joined one by one (scan_entry)
+constexpr int kScanLanes = 64;   // channels of a workgroup
+constexpr int kScanWaves = 8;    // spans of a chunk, forward
+constexpr int kScanSteps = 16;   // steps of a span
+constexpr int kBackWaves = 4;    // and backward (whose steps take three times the registers)
+constexpr int kBackSteps = 16;
+constexpr int kScanChunk = kBackWaves * kBackSteps;  // steps between the states that training stores
+constexpr int kScanGroup = 16;   // chunks that are joined one by one (scan_entry)
+static_assert(kScanWaves * kScanSteps % kScanChunk == 0 && kScanChunk % kScanSteps == 0, "stored states");
 
 // log2(1 + 2^v): what rounding 1 + e leaves of e is added to first order.
 __device__ inline float scan_softplus2(float v) {
@@ -36,15 +38,19 @@ __device__ inline float scan_softplus2(float v) {
 
 // A step's decay as one number c. A slow channel has a near 1 and forgets by 1 - a a token: rounding
 // a to fp32 would shift its rate, and with it the gain at rest, by 2^-25 / (1 - a). So c is 1 - a
-// while p < 1 (a minimax fit of (1 - 2^-p) / p on [0, 1], off by 2^-26.6, rounded by 2^-23), and -a
+// while p < 1 (scan_slow: a minimax fit of (1 - 2^-p) / p on [0, 1], off by 2^-26.6, rounded by 2^-23), and -a
 // after that; the sign bit tells.
-__device__ inline float scan_code(float p) {
+__device__ inline float scan_slow(float p) {
   float w = fmaf(p, -1.14580565e-4f, 1.29078003e-3f);
   w = fmaf(p, w, -9.5962761e-3f);
   w = fmaf(p, w, 5.5498954e-2f);
   w = fmaf(p, w, -2.40226060e-1f);
   w = fmaf(p, w, 6.93147182e-1f);
-  return p < 1.f ? p * w : -__builtin_amdgcn_exp2f(-p);
+  return p * w;
+}
+__device__ inline float scan_code(float p, float& a) {
+  a = __builtin_amdgcn_exp2f(-p);
+  return p < 1.f ? scan_slow(p) : -a;
 }
 __device__ inline bool scan_fast(float c) { return __float_as_int(c) < 0; }  // c is -a
 __device__ inline float scan_a(float c) { return scan_fast(c) ? -c : 1.f - c; }
@@ -67,12 +73,29 @@ __device__ inline float scan_p_low(float dt, ScanRate r) {
   return __builtin_amdgcn_exp2f(fmaf(dt, kLog2e, r.log2_rate)) * kLog2e;
 }
 
-// What a span (or a chunk) makes of the state h before it: u + 2^-p h, and u alone behind a reset.
-// c is scan_code(p), or kScanCut.
+// What steps, spans or a chunk make of the state h before them: u + a h, as u and the code c of their
+// decay; u alone behind a reset (kScanCut). Over a span's steps the decay is the product of theirs, or
+// where that is over a half, of the sum of theirs: 1 - a would be lost in the product, and the product
+// in the sum (2^-p is off by p 2^-25 of itself).
 constexpr float kScanCut = 2.f;
 __device__ inline float scan_join(float c, float u, float h) {
   return c == kScanCut ? u : u + scan_fade(c, h);
 }
+struct ScanDecay {
+  float p = 0.f, a = 1.f;
+  __device__ float code() const { return p < 1.f ? scan_slow(p) : -a; }
+};
+// The same of joined codes.
+struct ScanJoint {
+  float a = 1.f, w = 0.f;
+  bool cut = false;
+  __device__ void then(float c) {
+    cut |= c == kScanCut;
+    a *= scan_a(c);
+    w = fmaf(scan_w(c), 1.f - w, w);
+  }
+  __device__ float code() const { return cut ? kScanCut : w < 0.5f ? w : -a; }
+};
 
 template <typename T>
 struct ScanArgs {
@@ -92,7 +115,7 @@ struct ScanArgs {
   T *ddt, *dg, *dx;
   float *drate, *dh0;  // drate: [batch, chunks, width]
   // the states between chunks (several of them)
-  uint32_t* ticket;
+  uint32_t* tickets;  // [batch, tiles of the width]
   uint32_t* ends;   // [batch, groups, width]
   uint64_t* spans;  // [batch, chunks, width]
 };
@@ -117,67 +140,99 @@ template <typename W>
 __device__ inline W peek(const W* at) {
   return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ inline uint64_t span_word(float c, float u) {
-  return ((uint64_t)word_of(c) << 32) | word_of(u);
-}
-// Reads again until the word is there (the same number of times in every lane of the wave).
-template <typename W>
-__device__ inline W await(const W* at, W v, bool on, int& patience) {
-  while (__any(on && v == (W)~(W)0) && --patience > 0) {
-    __builtin_amdgcn_s_sleep(2);
-    if (on) v = peek(at);
-  }
-  return v;
+__global__ __launch_bounds__(256) void scan_clear_kernel(uint4* words, int64_t zeros, int64_t count) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const uint32_t v = i < zeros ? 0 : kNoWord;
+  if (i < count) words[i] = uint4{v, v, v, v};
 }
 
-// BACK: chunks run from the last to the first, and n counts chunks from that end.
-template <bool BACK>
-__device__ inline float scan_entry(const uint64_t* spans, const uint32_t* ends, int64_t chunks,
-                                   int64_t n, int64_t width, float first, bool on) {
-  const int64_t group = n / kScanGroup;
-  const int member = (int)(n % kScanGroup);
-  const auto span_at = [&](int m) {
-    const int64_t i = group * kScanGroup + m;
-    return spans + (BACK ? chunks - 1 - i : i) * width;
-  };
-  int patience = 1 << 20;
-  uint64_t w[kScanGroup - 1];
-#pragma unroll
-  for (int m = 0; m < kScanGroup - 1; ++m) w[m] = m < member && on ? peek(span_at(m)) : 0;
-  float h = first;
-  if (group > 0) {
-    const uint32_t* at = ends + (group - 1) * width;
-    h = __uint_as_float(await(at, on ? peek(at) : 0u, on, patience));
+// Which chunk (from the end where the walk starts) of which 64 channels of which sequence. Each of
+// these `tiles` has a counter of its own: one for all cost 8 ns a workgroup.
+struct ScanPlace { int64_t n, b, d0; };
+template <bool CHAIN>
+__device__ inline ScanPlace scan_place(uint32_t* tickets, int64_t width, uint32_t tiles, uint32_t* lds) {
+  const uint32_t across = (uint32_t)((width + kScanLanes - 1) / kScanLanes), tile = __builtin_amdgcn_readfirstlane(blockIdx.x % tiles);
+  uint32_t n = 0;
+  if constexpr (CHAIN) {
+    if (threadIdx.x == 0)
+      *lds = __hip_atomic_fetch_add(tickets + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    n = __builtin_amdgcn_readfirstlane(*lds);
   }
+  const uint32_t b = __builtin_amdgcn_readfirstlane(tile / across);
+  return {n, b, (int64_t)(tile - b * across) * kScanLanes};
+}
+
+// Posts the chunk's span (c, u; wave 0's) and returns the state before it to wave 0, `first` at the
+// start. The waves wait for the words side by side, and wave 0 joins them. BACK: chunks run from the
+// last to the first, and place.n counts from that end.
+template <int WAVES, bool BACK, typename T>
+__device__ inline float scan_entry(const ScanArgs<T>& k, const ScanPlace& at, int64_t chunks,
+                                   uint32_t in, bool on, int wave, float c, float u, float first,
+                                   float (*words)[kScanGroup][64]) {
+  constexpr int EACH = kScanGroup / WAVES;  // words of a wave: its number, + WAVES, ..
+  const int lane = threadIdx.x & 63;
+  const int64_t groups = (chunks + kScanGroup - 1) / kScanGroup, group = (uint32_t)at.n / kScanGroup;
+  const int member = (uint32_t)at.n % kScanGroup;
+  uint64_t* spans = k.spans + at.b * chunks * k.width + at.d0;
+  uint32_t* ends = k.ends + at.b * groups * k.width + at.d0;
+  const auto span_at = [&](int64_t n) { return spans + (BACK ? chunks - 1 - n : n) * k.width; };
+  if (wave == 0 && member < kScanGroup - 1 && on)
+    post(span_at(at.n) + in, ((uint64_t)word_of(c) << 32) | word_of(u));
+  // The last wave has one span less (a group's last is not posted) and the end before the group.
+  const bool end = wave == WAVES - 1 && group > 0;
+  if (on && (wave < member || end)) {
+    uint64_t w[EACH] = {};
+    uint32_t e = 0;
+    bool wait;
+    int patience = 1 << 20;
+    do {
 #pragma unroll
-  for (int m = 0; m < kScanGroup - 1; ++m)
-    if (m < member) {
-      const uint64_t v = await(span_at(m), w[m], on, patience);
-      h = scan_join(__uint_as_float((uint32_t)(v >> 32)), __uint_as_float((uint32_t)v), h);
+      for (int i = 0; i < EACH; ++i)
+        if (wave + i * WAVES < member) w[i] = peek(span_at(group * kScanGroup + wave + i * WAVES) + in);
+      if (end) e = peek(ends + (group - 1) * k.width + in);
+      wait = e == kNoWord;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) wait |= w[i] == ~(uint64_t)0;
+    } while (wait && --patience > 0);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      words[0][wave + i * WAVES][lane] = __uint_as_float((uint32_t)(w[i] >> 32));
+      words[1][wave + i * WAVES][lane] = __uint_as_float((uint32_t)w[i]);
     }
+    if (end) words[0][kScanGroup - 1][lane] = __uint_as_float(e);
+  }
+  __syncthreads();
+  float h = first;
+  if (wave == 0) {
+    if (group > 0) h = words[0][kScanGroup - 1][lane];
+    for (int m = 0; m < member; ++m) h = scan_join(words[0][m][lane], words[1][m][lane], h);
+    if (member == kScanGroup - 1 && on) post(ends + group * k.width + in, word_of(scan_join(c, u, h)));
+  }
   return h;
 }
 
-__global__ __launch_bounds__(256) void scan_clear_kernel(uint4* words, int64_t count) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < count) words[i] = i == 0 ? uint4{0, 0, 0, 0} : uint4{kNoWord, kNoWord, kNoWord, kNoWord};
-}
-
-// Which chunk (from the end where the walk starts) of which 64 channels of which sequence.
-struct ScanPlace { int64_t n, b, d0; };
-template <bool CHAIN>
-__device__ inline ScanPlace scan_place(uint32_t* ticket, int64_t width, int64_t tiles, uint32_t* lds) {
-  uint32_t i = blockIdx.x;
-  if constexpr (CHAIN) {
-    if (threadIdx.x == 0)
-      *lds = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    i = __builtin_amdgcn_readfirstlane(*lds);
+// A row that all lanes share, in two scalar registers, from which a lane reads or writes at its byte
+// offset. next() keeps it a running pointer: left alone, the compiler computes all rows' addresses
+// ahead and spills them.
+template <typename T>
+struct ScanRow {
+  using Raw = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
+  using Global = __attribute__((address_space(1))) char*;
+  Global at;
+  int64_t by;
+  __device__ ScanRow(const T* p, int64_t step) : at((Global)(char*)p), by(step * (int64_t)sizeof(T)) {}
+  __device__ T load(uint32_t off) const {
+    return __builtin_bit_cast(T, *(__attribute__((address_space(1))) Raw*)(at + off));
   }
-  const int64_t across = (width + kScanLanes - 1) / kScanLanes;
-  const int64_t tile = i % (uint32_t)tiles;
-  return {(int64_t)(i / (uint32_t)tiles), tile / across, tile % across * kScanLanes};
-}
+  __device__ void store(uint32_t off, float v) const {
+    *(__attribute__((address_space(1))) Raw*)(at + off) = __builtin_bit_cast(Raw, io<T>::from_f32(v));
+  }
+  __device__ void next() {
+    at += by;
+    asm volatile("" : "+s"(at));
+  }
+};
 
 // The resets of a span's steps as bits (bit i: step i).
 __device__ inline uint32_t scan_resets(const uint8_t* reset, int64_t row, int n) {
@@ -188,55 +243,72 @@ __device__ inline uint32_t scan_resets(const uint8_t* reset, int64_t row, int n)
 
 // Forward: a workgroup takes one chunk of 64 channels.
 template <typename T, bool CHAIN>
-__global__ __launch_bounds__(64 * kScanWaves) void gated_scan_fwd_kernel(ScanArgs<T> k, int64_t tiles) {
-  __shared__ float part[3][kScanWaves][64];  // p (-1 behind a reset), c, u of each span
-  __shared__ float entry[64];
+__global__ __launch_bounds__(64 * kScanWaves) void gated_scan_fwd_kernel(ScanArgs<T> k, uint32_t tiles) {
+  __shared__ float part[2][kScanWaves][64];  // c and u of each span
+  __shared__ float words[CHAIN ? 2 : 1][kScanGroup][64], entry[64];
   __shared__ uint32_t place;
   const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const ScanPlace at = scan_place<CHAIN>(k.ticket, k.width, tiles, &place);
+  const ScanPlace at = scan_place<CHAIN>(k.tickets, k.width, tiles, &place);
   const int64_t d = at.d0 + lane, b = at.b;
   const bool on = d < k.width;
-  const int64_t dc = on ? d : k.width - 1;  // lanes past the end read the last channel
+  const uint32_t in = on ? lane : (uint32_t)(k.width - 1 - at.d0);  // lanes past the end read the last
+  const int64_t dc = at.d0 + in;
+  const uint32_t off = in * (uint32_t)sizeof(T);
   const int64_t chunk = (int64_t)waves * kScanSteps, chunks = CHAIN ? (k.seq + chunk - 1) / chunk : 1;
   const int64_t t0 = at.n * chunk + wave * kScanSteps, row0 = b * k.seq + t0;
   const int n = k.seq - t0 < kScanSteps ? (k.seq > t0 ? (int)(k.seq - t0) : 0) : kScanSteps;
   const ScanRate rate = scan_rate(k.log_rate[dc]);
   float c[kScanSteps], s[kScanSteps];
-  uint32_t cuts = 0;
-  float p = 0.f, u = 0.f;
-  if (n > 0) {
-    cuts = scan_resets(k.reset, row0, n);
+  const uint32_t cuts = scan_resets(k.reset, row0, n);
+  ScanDecay span;
+  float u = 0.f;
+  // PLAIN: all steps are there and none is a reset.
+  const auto walk = [&](auto plain) {
+    constexpr bool PLAIN = decltype(plain)::value;
+    ScanRow<T> dts(k.dt + row0 * k.dt_row + at.d0, k.dt_row);
+    ScanRow<T> gs(k.g + row0 * k.g_row + at.d0, k.g_row), xs(k.x + row0 * k.x_row + at.d0, k.x_row);
+    T raw[3][kScanSteps];
+#pragma unroll
+    for (int i = 0; i < kScanSteps; ++i) {
+      raw[0][i] = dts.load(off), raw[1][i] = gs.load(off), raw[2][i] = xs.load(off);
+      if (PLAIN || i + 1 < n) dts.next(), gs.next(), xs.next();
+    }
+    __builtin_amdgcn_sched_barrier(0);  // all loads first
     float low = 0.f;
 #pragma unroll
     for (int i = 0; i < kScanSteps; ++i) {
-      const int64_t row = row0 + (i < n ? i : n - 1);
-      const float dt = load_scalar(k.dt + row * k.dt_row + dc);
-      const float g = load_scalar(k.g + row * k.g_row + dc), x = load_scalar(k.x + row * k.x_row + dc);
+      const float dt = io<T>::to_f32(raw[0][i]), g = io<T>::to_f32(raw[1][i]);
+      const float x = io<T>::to_f32(raw[2][i]);
       low = fminf(low, dt);
       c[i] = scan_p(dt, rate);
       s[i] = x * __builtin_amdgcn_rcpf(1.f + __expf(-g));
     }
     if (__builtin_expect(__any(low < -80.f), 0)) {
+      ScanRow<T> again(k.dt + row0 * k.dt_row + at.d0, k.dt_row);
 #pragma unroll
       for (int i = 0; i < kScanSteps; ++i) {
-        const int64_t row = row0 + (i < n ? i : n - 1);
-        const float dt = load_scalar(k.dt + row * k.dt_row + dc);
+        const float dt = io<T>::to_f32(again.load(off));
+        if (PLAIN || i + 1 < n) again.next();
         if (dt < -80.f) c[i] = scan_p_low(dt, rate);
       }
     }
 #pragma unroll
     for (int i = 0; i < kScanSteps; ++i)
-      if (i < n) {
-        if (cuts >> i & 1) u = 0.f, p = 0.f;
-        p += c[i];
-        c[i] = scan_code(c[i]);
+      if (PLAIN || i < n) {
+        if (!PLAIN && (cuts >> i & 1)) u = 0.f;
+        float a;
+        span.p += c[i];
+        c[i] = scan_code(c[i], a);
+        span.a *= a;
         u = scan_step(c[i], s[i], u);
       }
-  }
-  part[0][wave][lane] = cuts ? -1.f : p;
-  part[1][wave][lane] = cuts ? kScanCut : scan_code(p);
-  part[2][wave][lane] = u;
+  };
+  const bool plain = n == kScanSteps && cuts == 0;
+  if (plain) walk(std::true_type());
+  else if (n > 0) walk(std::false_type());
+  part[0][wave][lane] = cuts ? kScanCut : span.code();
+  part[1][wave][lane] = u;
   float h = 0.f;
   if (wave == 0 && at.n == 0) {
     h = k.h0 ? k.h0[b * k.width + dc] : 0.f;
@@ -244,25 +316,19 @@ __global__ __launch_bounds__(64 * kScanWaves) void gated_scan_fwd_kernel(ScanArg
   }
   __syncthreads();
   if constexpr (CHAIN) {
+    float cu = h, cc = 0.f;
     if (wave == 0) {
-      const int64_t groups = (chunks + kScanGroup - 1) / kScanGroup;
-      uint64_t* spans = k.spans + b * chunks * k.width + d;
-      uint32_t* ends = k.ends + b * groups * k.width + d;
-      const bool last = at.n % kScanGroup == kScanGroup - 1;
-      float cu = h, cp = 0.f;
-      bool cut = at.n == 0;  // the first chunk posts its state (h0 is not read again: h_last may be h0)
+      ScanJoint all;
+      all.cut = at.n == 0;  // the first chunk posts its state (h0 is not read again: h_last may be h0)
 #pragma unroll
       for (int w = 0; w < kScanWaves; ++w) {
-        const float wp = part[0][w][lane];
-        cut |= wp < 0.f;
-        cp += wp;
-        cu = scan_join(part[1][w][lane], part[2][w][lane], cu);
+        all.then(part[0][w][lane]);
+        cu = scan_join(part[0][w][lane], part[1][w][lane], cu);
       }
-      const float cc = cut ? kScanCut : scan_code(cp);
-      if (!last && on) post(spans + at.n * k.width, span_word(cc, cu));
-      if (at.n > 0) entry[lane] = h = scan_entry<false>(spans, ends, chunks, at.n, k.width, 0.f, on);
-      if (last && on) post(ends + at.n / kScanGroup * k.width, word_of(scan_join(cc, cu, h)));
+      cc = all.code();
     }
+    h = scan_entry<kScanWaves, false>(k, at, chunks, in, on, wave, cc, cu, h, words);
+    if (wave == 0) entry[lane] = h;
     __syncthreads();
   }
   h = entry[lane];
@@ -270,52 +336,78 @@ __global__ __launch_bounds__(64 * kScanWaves) void gated_scan_fwd_kernel(ScanArg
     if (k.seq == 0 && k.h_last && on && wave == 0) k.h_last[b * k.width + d] = h;
     return;
   }
-  for (int w = 0; w < wave; ++w) h = scan_join(part[1][w][lane], part[2][w][lane], h);
+  for (int w = 0; w < wave; ++w) h = scan_join(part[0][w][lane], part[1][w][lane], h);
   if (k.carries && t0 % kScanChunk == 0 && on) {
     const int64_t every = (k.seq + kScanChunk - 1) / kScanChunk;
     k.carries[(b * every + t0 / kScanChunk) * k.width + d] = h;
   }
+  if (!on) return;
+  ScanRow<T> y(k.y + row0 * k.width + at.d0, k.width);
+  if (plain) {
 #pragma unroll
-  for (int i = 0; i < kScanSteps; ++i)
-    if (i < n) {
-      if (cuts >> i & 1) h = 0.f;
+    for (int i = 0; i < kScanSteps; ++i) {
       h = scan_step(c[i], s[i], h);
-      if (on) store_scalar(k.y + (row0 + i) * k.width + d, h);
+      y.store(off, h);
+      y.next();
     }
-  if (k.h_last && on && t0 + n == k.seq) k.h_last[b * k.width + d] = h;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kScanSteps; ++i)
+      if (i < n) {
+        if (cuts >> i & 1) h = 0.f;
+        h = scan_step(c[i], s[i], h);
+        y.store(off, h);
+        y.next();
+      }
+  }
+  if (k.h_last && t0 + n == k.seq) k.h_last[b * k.width + d] = h;
 }
 
 // Backward: the chunks from the last to the first, each from its stored entry state. What a span makes
 // of the adjoint A behind it (A = a G of the step after) is v + 2^-p A.
 template <typename T, bool CHAIN>
-__global__ __launch_bounds__(64 * kScanWaves) void gated_scan_bwd_kernel(ScanArgs<T> k, int64_t tiles) {
-  __shared__ float part[4][kScanWaves][64];  // p (-1 behind a reset), c, u, v of each span
-  __shared__ float entry[64];
+__global__ __launch_bounds__(64 * kBackWaves) void gated_scan_bwd_kernel(ScanArgs<T> k, uint32_t tiles) {
+  __shared__ float part[3][kBackWaves][64];  // c, u and v of each span
+  __shared__ float words[CHAIN ? 2 : 1][kScanGroup][64], entry[64];
   __shared__ uint32_t place;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const ScanPlace at = scan_place<CHAIN>(k.ticket, k.width, tiles, &place);
+  const ScanPlace at = scan_place<CHAIN>(k.tickets, k.width, tiles, &place);
   const int64_t d = at.d0 + lane, b = at.b;
   const bool on = d < k.width;
-  const int64_t dc = on ? d : k.width - 1;
+  const uint32_t in = on ? lane : (uint32_t)(k.width - 1 - at.d0);  // lanes past the end read the last
+  const int64_t dc = at.d0 + in;
+  const uint32_t off = in * (uint32_t)sizeof(T);
   const int64_t chunks = CHAIN ? (k.seq + kScanChunk - 1) / kScanChunk : 1, j = chunks - 1 - at.n;
-  const int64_t t0 = j * kScanChunk + wave * kScanBack, row0 = b * k.seq + t0;
-  const int n = k.seq - t0 < kScanBack ? (k.seq > t0 ? (int)(k.seq - t0) : 0) : kScanBack;
+  const int64_t t0 = j * kScanChunk + wave * kBackSteps, row0 = b * k.seq + t0;
+  const int n = k.seq - t0 < kBackSteps ? (k.seq > t0 ? (int)(k.seq - t0) : 0) : kBackSteps;
   const ScanRate rate = scan_rate(k.log_rate[dc]);
   // c; s, later s - h; dy; sigmoid(g); s (1 - sigmoid(g)); dp/ddt = rate sigmoid(dt); p
-  float c[kScanBack], e[kScanBack], dy[kScanBack], sg[kScanBack], q[kScanBack], sd[kScanBack],
-      ps[kScanBack];
-  uint32_t cuts = 0;
-  float p = 0.f, u = 0.f, v = 0.f;
-  if (n > 0) {
-    cuts = scan_resets(k.reset, row0, n);
+  float c[kBackSteps], e[kBackSteps], dy[kBackSteps], sg[kBackSteps], q[kBackSteps], sd[kBackSteps],
+      ps[kBackSteps];
+  const uint32_t cuts = scan_resets(k.reset, row0, n);
+  ScanDecay span;
+  float u = 0.f, v = 0.f;
+  // PLAIN: all steps are there and none is a reset.
+  const auto walk = [&](auto plain) {
+    constexpr bool PLAIN = decltype(plain)::value;
+    ScanRow<T> dts(k.dt + row0 * k.dt_row + at.d0, k.dt_row);
+    ScanRow<T> gs(k.g + row0 * k.g_row + at.d0, k.g_row), xs(k.x + row0 * k.x_row + at.d0, k.x_row);
+    ScanRow<T> dys(k.dy + row0 * k.width + at.d0, k.width);
+    T raw[4][kBackSteps];
+#pragma unroll
+    for (int i = 0; i < kBackSteps; ++i) {
+      raw[0][i] = dts.load(off), raw[1][i] = gs.load(off), raw[2][i] = xs.load(off);
+      raw[3][i] = dys.load(off);
+      if (PLAIN || i + 1 < n) dts.next(), gs.next(), xs.next(), dys.next();
+    }
+    __builtin_amdgcn_sched_barrier(0);  // all loads first
     float low = 0.f;
 #pragma unroll
-    for (int i = 0; i < kScanBack; ++i) {
-      const int64_t row = row0 + (i < n ? i : n - 1);
-      const float dt = load_scalar(k.dt + row * k.dt_row + dc);
-      const float g = load_scalar(k.g + row * k.g_row + dc), x = load_scalar(k.x + row * k.x_row + dc);
-      dy[i] = load_scalar(k.dy + row * k.width + dc);
+    for (int i = 0; i < kBackSteps; ++i) {
+      const float dt = io<T>::to_f32(raw[0][i]), g = io<T>::to_f32(raw[1][i]);
+      const float x = io<T>::to_f32(raw[2][i]);
+      dy[i] = io<T>::to_f32(raw[3][i]);
       low = fminf(low, dt);
       float cg, cd;
       sigmoid_pair(g, sg[i], cg);
@@ -326,82 +418,87 @@ __global__ __launch_bounds__(64 * kScanWaves) void gated_scan_bwd_kernel(ScanArg
       ps[i] = scan_p(dt, rate);
     }
     if (__builtin_expect(__any(low < -80.f), 0)) {
+      ScanRow<T> again(k.dt + row0 * k.dt_row + at.d0, k.dt_row);
 #pragma unroll
-      for (int i = 0; i < kScanBack; ++i) {
-        const int64_t row = row0 + (i < n ? i : n - 1);
-        const float dt = load_scalar(k.dt + row * k.dt_row + dc);
+      for (int i = 0; i < kBackSteps; ++i) {
+        const float dt = io<T>::to_f32(again.load(off));
+        if (PLAIN || i + 1 < n) again.next();
         if (dt < -80.f) ps[i] = scan_p_low(dt, rate), sd[i] = ps[i] * kLn2;
       }
     }
 #pragma unroll
-    for (int i = 0; i < kScanBack; ++i)
-      if (i < n) {
-        if (cuts >> i & 1) u = 0.f, p = 0.f;
-        p += ps[i];
-        c[i] = scan_code(ps[i]);
+    for (int i = 0; i < kBackSteps; ++i)
+      if (PLAIN || i < n) {
+        if (!PLAIN && (cuts >> i & 1)) u = 0.f;
+        float a;
+        span.p += ps[i];
+        c[i] = scan_code(ps[i], a);
+        span.a *= a;
         u = scan_step(c[i], e[i], u);
       }
 #pragma unroll
-    for (int i = kScanBack - 1; i >= 0; --i)
-      if (i < n) v = cuts >> i & 1 ? 0.f : scan_fade(c[i], dy[i] + v);
-  }
-  part[0][wave][lane] = cuts ? -1.f : p;
-  part[1][wave][lane] = cuts ? kScanCut : scan_code(p);
-  part[2][wave][lane] = u;
-  part[3][wave][lane] = v;
+    for (int i = kBackSteps - 1; i >= 0; --i)
+      if (PLAIN || i < n) v = !PLAIN && (cuts >> i & 1) ? 0.f : scan_fade(c[i], dy[i] + v);
+  };
+  const bool all = n == kBackSteps && cuts == 0;
+  if (all) walk(std::true_type());
+  else if (n > 0) walk(std::false_type());
+  part[0][wave][lane] = cuts ? kScanCut : span.code();
+  part[1][wave][lane] = u;
+  part[2][wave][lane] = v;
   __syncthreads();
-  const float behind = k.dh_last ? k.dh_last[b * k.width + dc] : 0.f;
+  float A = k.dh_last ? k.dh_last[b * k.width + dc] : 0.f;
   if constexpr (CHAIN) {
+    float cv = 0.f, cc = 0.f;
     if (wave == 0) {
-      const int64_t groups = (chunks + kScanGroup - 1) / kScanGroup;
-      uint64_t* spans = k.spans + b * chunks * k.width + d;
-      uint32_t* ends = k.ends + b * groups * k.width + d;
-      const bool last = at.n % kScanGroup == kScanGroup - 1;
-      float cv = 0.f, cp = 0.f;
-      bool cut = false;
+      ScanJoint all;
 #pragma unroll
-      for (int w = kScanWaves - 1; w >= 0; --w) {
-        const float wp = part[0][w][lane];
-        cut |= wp < 0.f;
-        cp += wp;
-        cv = scan_join(part[1][w][lane], part[3][w][lane], cv);
+      for (int w = kBackWaves - 1; w >= 0; --w) {
+        all.then(part[0][w][lane]);
+        cv = scan_join(part[0][w][lane], part[2][w][lane], cv);
       }
-      const float cc = cut ? kScanCut : scan_code(cp);
-      if (!last && on) post(spans + j * k.width, span_word(cc, cv));
-      const float A = scan_entry<true>(spans, ends, chunks, at.n, k.width, behind, on);
-      if (last && on) post(ends + at.n / kScanGroup * k.width, word_of(scan_join(cc, cv, A)));
-      entry[lane] = A;
+      cc = all.code();
     }
+    A = scan_entry<kBackWaves, true>(k, at, chunks, in, on, wave, cc, cv, A, words);
+    if (wave == 0) entry[lane] = A;
     __syncthreads();
+    A = entry[lane];
   }
-  float A = CHAIN ? entry[lane] : behind, drate = 0.f;
+  float drate = 0.f;
   if (n > 0) {
     float h = k.carries[(b * chunks + j) * k.width + dc];
-    for (int w = 0; w < wave; ++w) h = scan_join(part[1][w][lane], part[2][w][lane], h);
-    for (int w = kScanWaves - 1; w > wave; --w) A = scan_join(part[1][w][lane], part[3][w][lane], A);
+    for (int w = 0; w < wave; ++w) h = scan_join(part[0][w][lane], part[1][w][lane], h);
+    for (int w = kBackWaves - 1; w > wave; --w) A = scan_join(part[0][w][lane], part[2][w][lane], A);
+    const auto back = [&](auto plain) {
+      constexpr bool PLAIN = decltype(plain)::value;
 #pragma unroll
-    for (int i = 0; i < kScanBack; ++i)
-      if (i < n) {
-        if (cuts >> i & 1) h = 0.f;
-        const float s = e[i];
-        e[i] = s - h;
-        h = scan_step(c[i], s, h);
-      }
-#pragma unroll
-    for (int i = kScanBack - 1; i >= 0; --i)
-      if (i < n) {
-        const float G = dy[i] + A, aG = scan_fade(c[i], G);
-        const float dp = aG * e[i], ds = scan_w(c[i]) * G;
-        const int64_t to = (row0 + i) * k.width + d;
-        if (on) {
-          store_scalar(k.ddt + to, dp * sd[i]);
-          store_scalar(k.dg + to, ds * q[i]);
-          store_scalar(k.dx + to, ds * sg[i]);
+      for (int i = 0; i < kBackSteps; ++i)
+        if (PLAIN || i < n) {
+          if (!PLAIN && (cuts >> i & 1)) h = 0.f;
+          const float s = e[i];
+          e[i] = s - h;
+          h = scan_step(c[i], s, h);
         }
-        // (2^-p is 0 long before p = 300: no 0 times infinity)
-        drate = fmaf(dp, fminf(ps[i], 300.f), drate);
-        A = cuts >> i & 1 ? 0.f : aG;
-      }
+      const int64_t to = (row0 + (PLAIN ? kBackSteps : n) - 1) * k.width + at.d0;
+      ScanRow<T> ddt(k.ddt + to, -k.width), dg(k.dg + to, -k.width), dx(k.dx + to, -k.width);
+#pragma unroll
+      for (int i = kBackSteps - 1; i >= 0; --i)
+        if (PLAIN || i < n) {
+          const float G = dy[i] + A, aG = scan_fade(c[i], G);
+          const float dp = aG * e[i], ds = scan_w(c[i]) * G;
+          ddt.store(off, dp * sd[i]);
+          dg.store(off, ds * q[i]);
+          dx.store(off, ds * sg[i]);
+          ddt.next(), dg.next(), dx.next();
+          // (2^-p is 0 long before p = 300: no 0 times infinity)
+          drate = fmaf(dp, fminf(ps[i], 300.f), drate);
+          A = !PLAIN && (cuts >> i & 1) ? 0.f : aG;
+        }
+    };
+    if (on) {
+      if (all) back(std::true_type());
+      else back(std::false_type());
+    }
     if (k.dh0 && on && t0 == 0) k.dh0[b * k.width + d] = A;
   }
   __syncthreads();
@@ -410,7 +507,7 @@ __global__ __launch_bounds__(64 * kScanWaves) void gated_scan_bwd_kernel(ScanArg
   if (wave == 0 && on) {
     float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kScanWaves; ++w) sum += part[0][w][lane];
+    for (int w = 0; w < kBackWaves; ++w) sum += part[0][w][lane];
     k.drate[(b * chunks + j) * k.width + d] = sum * kLn2;
   }
 }
@@ -423,28 +520,33 @@ __global__ __launch_bounds__(256) void gated_scan_step_kernel(ScanArgs<T> k, flo
   const float dt = load_scalar(k.dt + b * k.dt_row + d), g = load_scalar(k.g + b * k.g_row + d);
   const float s = load_scalar(k.x + b * k.x_row + d) * __builtin_amdgcn_rcpf(1.f + __expf(-g));
   const ScanRate rate = scan_rate(k.log_rate[d]);
-  const float c = scan_code(dt < -80.f ? scan_p_low(dt, rate) : scan_p(dt, rate));
+  float a;
+  const float c = scan_code(dt < -80.f ? scan_p_low(dt, rate) : scan_p(dt, rate), a);
   const float v = scan_step(c, s, h[b * k.width + d]);
   h[b * k.width + d] = v;
   store_scalar(k.y + b * k.width + d, v);
 }
 
-// The workspace of a launch over several chunks: the ticket's 16 bytes, the spans, the ends; and of the
-// backward the partial sums of dlog_rate behind them.
-struct ScanSpace { int64_t chunks, words, bytes; };
+// The workspace of a launch over several chunks: the tiles' counters, the spans, the ends (each from a
+// multiple of 16 bytes); and of the backward the partial sums of dlog_rate behind them.
+struct ScanSpace { int64_t chunks, counters, spans, bytes; };
 inline ScanSpace scan_space(int64_t batch, int64_t seq, int64_t width, int64_t chunk) {
   const int64_t chunks = (seq + chunk - 1) / chunk, groups = (chunks + kScanGroup - 1) / kScanGroup;
-  const int64_t words = chunks > 1 ? batch * width * (8 * chunks + 4 * groups) : 0;
-  return {chunks, words, words > 0 ? (words + 31) / 16 * 16 : 0};
+  if (chunks <= 1) return {chunks, 0, 0, 0};
+  const auto whole = [](int64_t bytes) { return (bytes + 15) / 16 * 16; };
+  const int64_t counters = whole(4 * batch * ((width + kScanLanes - 1) / kScanLanes));
+  const int64_t spans = whole(8 * batch * chunks * width);
+  return {chunks, counters, spans, counters + spans + whole(4 * batch * groups * width)};
 }
 
 template <typename T>
-int scan_chain(ScanArgs<T>& k, const ScanSpace& w, int64_t batch, char* ws, hipStream_t s) {
-  k.ticket = (uint32_t*)ws;
-  k.spans = (uint64_t*)(ws + 16);
-  k.ends = (uint32_t*)(k.spans + batch * w.chunks * k.width);
+int scan_chain(ScanArgs<T>& k, const ScanSpace& w, char* ws, hipStream_t s) {
+  k.tickets = (uint32_t*)ws;
+  k.spans = (uint64_t*)(ws + w.counters);
+  k.ends = (uint32_t*)(ws + w.counters + w.spans);
   const int64_t quads = w.bytes / 16;
-  scan_clear_kernel<<<dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s>>>((uint4*)ws, quads);
+  scan_clear_kernel<<<dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s>>>(
+      (uint4*)ws, w.counters / 16, quads);
   return launch_status();
 }
 
@@ -453,14 +555,14 @@ int launch_gated_scan_fwd(ScanArgs<T> k, int64_t batch, char* ws, hipStream_t s)
   const int64_t tiles = batch * ((k.width + kScanLanes - 1) / kScanLanes);
   const ScanSpace w = scan_space(batch, k.seq, k.width, kScanWaves * kScanSteps);
   if (w.chunks > 1) {
-    const int st = scan_chain(k, w, batch, ws, s);
+    const int st = scan_chain(k, w, ws, s);
     if (st != MQC_OK) return st;
     gated_scan_fwd_kernel<T, true>
-        <<<dim3((unsigned)(tiles * w.chunks)), dim3(64 * kScanWaves), 0, s>>>(k, tiles);
+        <<<dim3((unsigned)(tiles * w.chunks)), dim3(64 * kScanWaves), 0, s>>>(k, (uint32_t)tiles);
   } else {
     const int64_t waves = k.seq > 0 ? (k.seq + kScanSteps - 1) / kScanSteps : 1;
     gated_scan_fwd_kernel<T, false>
-        <<<dim3((unsigned)tiles), dim3((unsigned)(64 * waves)), 0, s>>>(k, tiles);
+        <<<dim3((unsigned)tiles), dim3((unsigned)(64 * waves)), 0, s>>>(k, (uint32_t)tiles);
   }
   return launch_status();
 }
@@ -471,13 +573,13 @@ int launch_gated_scan_bwd(ScanArgs<T> k, int64_t batch, float* drate, char* ws, 
   const ScanSpace w = scan_space(batch, k.seq, k.width, kScanChunk);
   k.drate = (float*)(ws + w.bytes);
   if (w.chunks > 1) {
-    const int st = scan_chain(k, w, batch, ws, s);
+    const int st = scan_chain(k, w, ws, s);
     if (st != MQC_OK) return st;
     gated_scan_bwd_kernel<T, true>
-        <<<dim3((unsigned)(tiles * w.chunks)), dim3(64 * kScanWaves), 0, s>>>(k, tiles);
+        <<<dim3((unsigned)(tiles * w.chunks)), dim3(64 * kBackWaves), 0, s>>>(k, (uint32_t)tiles);
   } else {
     gated_scan_bwd_kernel<T, false>
-        <<<dim3((unsigned)tiles), dim3(64 * kScanWaves), 0, s>>>(k, tiles);
+        <<<dim3((unsigned)tiles), dim3(64 * kBackWaves), 0, s>>>(k, (uint32_t)tiles);
   }
   const int st = launch_status();
   if (st != MQC_OK) return st;
