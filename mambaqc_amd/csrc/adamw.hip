@@ -20,40 +20,46 @@
 // r is never rounded to 0 unless it is 0: m / (0 + eps) would be any size. Values that are not finite
 // become NaN (code 0x7f), and do not set the scale.
 //
-// The tensors come as a table in the kernel's arguments (no copy to the device, kTableMax to a launch);
+// The tensors come as a table in the kernel's arguments (no copy to the device; as many to a launch as
+// fit 4 KiB);
 // a workgroup finds its tensor by its place in the running count of workgroups.
 #include "common.hpp"
 
 namespace mqc {
 
-constexpr int kTableMax = 48;
 constexpr int kAdamThreads = 256;
 constexpr int kAdamVec = 4;                                  // elements a lane takes at once
 constexpr int kAdamIters = 4;
 constexpr int kAdamChunk = kAdamThreads * kAdamVec * kAdamIters;  // elements of a workgroup
-constexpr int kStateBlock = 64 * kAdamVec;                   // elements that share a scale
+constexpr int kStateBlock = 256;                             // elements that share a scale
 
-struct AdamTable {
-  void* p[kTableMax];
-  const void* grad[kTableMax];
-  void* m[kTableMax];
-  void* v[kTableMax];
-  int64_t n[kTableMax];
-  uint32_t first[kTableMax];  // workgroups before this tensor's
+template <int MAX>
+struct AdamTableOf {
+  static constexpr int kMax = MAX;
+  void* p[MAX];
+  const void* grad[MAX];
+  void* m[MAX];
+  void* v[MAX];
+  int64_t n[MAX];
+  uint32_t first[MAX];  // workgroups before this tensor's
   int count;
 };
+using AdamTable = AdamTableOf<88>;
 struct Adam8Table {
-  AdamTable t;
-  float* m_scale[kTableMax];
-  float* v_scale[kTableMax];
-  uint32_t seed[kTableMax];
+  static constexpr int kMax = 60;
+  AdamTableOf<kMax> t;
+  float* m_scale[kMax];
+  float* v_scale[kMax];
+  uint32_t seed[kMax];
 };
 struct AdamScalars {
   float decay, step_size, root_scale, beta1, one_beta1, beta2, one_beta2, eps;
   const float* clip;
   uint32_t step;
 };
-static_assert(sizeof(Adam8Table) + sizeof(AdamScalars) <= 4096, "kernel arguments");
+static_assert(sizeof(Adam8Table) + sizeof(AdamScalars) <= 4096 &&
+                  sizeof(AdamTable) + sizeof(AdamScalars) <= 4096,
+              "kernel arguments");
 
 // The tensor of this workgroup: the last that starts at or before it.
 __device__ inline int table_find(const uint32_t* first, int count) {
@@ -128,9 +134,8 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamTable tab, Adam
   }
 }
 
-// The largest of a wave's values, the same in every lane: within rows of 16 lanes by DPP, then the
-// four rows' lanes through scalar registers. Bits of floats >= 0 order as the floats do.
-__device__ inline uint32_t wave_max_bits(uint32_t v) {
+// The largest of a row of 16 lanes, the same in each. Bits of floats >= 0 order as the floats do.
+__device__ inline uint32_t row_max_bits(uint32_t v) {
 #define MQC_MAX(MOVE)                                                   \
   {                                                                     \
     const uint32_t o = __float_as_uint(MOVE(__uint_as_float(v)));       \
@@ -138,10 +143,7 @@ __device__ inline uint32_t wave_max_bits(uint32_t v) {
   }
   MQC_MAX(lane_xor1) MQC_MAX(lane_xor2) MQC_MAX(row_rot4) MQC_MAX(row_rot8)
 #undef MQC_MAX
-  const uint32_t a = __builtin_amdgcn_readlane(v, 0), b = __builtin_amdgcn_readlane(v, 16);
-  const uint32_t c = __builtin_amdgcn_readlane(v, 32), d = __builtin_amdgcn_readlane(v, 48);
-  const uint32_t x = a > b ? a : b, y = c > d ? c : d;
-  return x > y ? x : y;
+  return v;
 }
 
 // The exponent field of the block's power of two, from its largest value's bits.
@@ -159,6 +161,102 @@ __device__ inline uint32_t place_bits(uint32_t x) {
   return x ^ (x >> 16);
 }
 
+// 16 consecutive elements from wherever they start.
+template <typename T>
+__device__ inline void load16(const T* p, int left, float (&out)[16]) {
+  typedef uint32_t words4 __attribute__((ext_vector_type(4), aligned(2)));
+  constexpr int EACH = 16 / sizeof(T);
+  if (left == 16) {
+#pragma unroll
+    for (int i = 0; i < 16 / EACH; ++i) {
+      const words4 v = reinterpret_cast<const words4*>(p)[i];
+#pragma unroll
+      for (int c = 0; c < EACH; ++c)
+        if constexpr (sizeof(T) == 4) out[EACH * i + c] = __uint_as_float(v[c]);
+        else out[EACH * i + c] = io<T>::bits_to_f32(c & 1 ? v[c / 2] >> 16 : v[c / 2] & 0xffffu);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 16; ++c) out[c] = c < left ? load_scalar(p + c) : 0.f;
+  }
+}
+template <typename T>
+__device__ inline void store16(T* p, int left, const float (&in)[16]) {
+  typedef uint32_t words4 __attribute__((ext_vector_type(4), aligned(2)));
+  if (left == 16) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T); ++i) {
+      words4 v;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if constexpr (sizeof(T) == 4) v[c] = __float_as_uint(in[4 * i + c]);
+        else v[c] = pack2<T>(in[8 * i + 2 * c], in[8 * i + 2 * c + 1]);
+      reinterpret_cast<words4*>(p)[i] = v;
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < 16; ++c)
+      if (c < left) store_scalar(p + c, in[c]);
+  }
+}
+typedef uint32_t codes16 __attribute__((ext_vector_type(4), aligned(1)));
+__device__ inline codes16 load_codes(const uint8_t* p, int left) {
+  codes16 v = {0, 0, 0, 0};
+  if (left == 16) return *reinterpret_cast<const codes16*>(p);
+#pragma unroll
+  for (int c = 0; c < 16; ++c)
+    if (c < left) v[c / 4] |= (uint32_t)p[c] << (8 * (c % 4));
+  return v;
+}
+__device__ inline void store_codes(uint8_t* p, int left, codes16 v) {
+  if (left == 16) {
+    *reinterpret_cast<codes16*>(p) = v;
+  } else {
+#pragma unroll
+    for (int c = 0; c < 16; ++c)
+      if (c < left) p[c] = (uint8_t)(v[c / 4] >> (8 * (c % 4)));
+  }
+}
+__device__ inline void decode16(codes16 v, float scale, float (&out)[16]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(v[i], false);
+    const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(v[i], true);
+    out[4 * i] = lo[0] * scale, out[4 * i + 1] = lo[1] * scale;
+    out[4 * i + 2] = hi[0] * scale, out[4 * i + 3] = hi[1] * scale;
+  }
+}
+
+// The codes of one element's |m| and r under scales of exponent fields mf and vf, rounded by `bits`.
+// In steps of its binade (the lowest is 2^-6 on) a value is q; |m| goes up with probability q - floor(q),
+// r with (q^2 - k^2) / ((k + 1)^2 - k^2), k = floor(q).
+struct AdamCodes { uint32_t m, r; };
+__device__ inline AdamCodes adam_codes(float am, float r, int mf, int vf, uint32_t bits, uint32_t step) {
+#pragma clang fp contract(off)
+  const float um = (float)((bits + step * kGolden) >> 8);  // 2^24 times a number below 1
+  const float uv = (float)((((bits << 16) | (bits >> 16)) + step * kMulB) >> 8);
+  AdamCodes out;
+  {
+    const int e = (int)(__float_as_uint(am) >> 23), t = e > mf - 6 ? e : mf - 6;
+    const float q = __builtin_ldexpf(am, 130 - t);
+    const uint32_t code = ((uint32_t)(t + 6 - mf) << 3) + (uint32_t)fmaf(um, 0x1p-24f, q);
+    out.m = code > 0x7eu ? 0x7eu : code;  // q + um may round up to the step past 448
+  }
+  {
+    const int e = (int)(__float_as_uint(r) >> 23), t = e > vf - 6 ? e : vf - 6;
+    const float q = __builtin_ldexpf(r, 130 - t), k = floorf(q);
+    const bool up = uv * fmaf(k, 0x1p-23f, 0x1p-24f) < (q - k) * (q + k);
+    const uint32_t code = ((uint32_t)(t + 6 - vf) << 3) + (uint32_t)k + (up ? 1u : 0u);
+    out.r = code > 0 ? code : 1u;
+  }
+  return out;
+}
+
+// A lane takes 16 elements and a row of 16 lanes a block, so the block's largest come from four moves
+// within the row. What bounds it is arithmetic more than memory (10 bytes an element with bf16
+// parameters): square root and reciprocal are the hardware's with one correction (the root's makes it
+// the rounded one), good from 2^-96 to 2^126. Blocks that hold anything else (v of 0, overflow, NaN, a
+// scale at the end of its range) take the library's, and tests.
 template <typename T>
 __global__ __launch_bounds__(kAdamThreads) void adamw8_kernel(Adam8Table tab, AdamScalars k) {
 #pragma clang fp contract(off)
@@ -167,97 +265,92 @@ __global__ __launch_bounds__(kAdamThreads) void adamw8_kernel(Adam8Table tab, Ad
   const T* grad = (const T*)tab.t.grad[i];
   uint8_t *m = (uint8_t*)tab.t.m[i], *v = (uint8_t*)tab.t.v[i];
   const int64_t n = tab.t.n[i];
-  const bool fits = (((uintptr_t)p | (uintptr_t)grad) % (4 * sizeof(T)) | ((uintptr_t)m | (uintptr_t)v) % 4) == 0;
   const float clip = k.clip ? *k.clip : 1.f;
-  const int lane = threadIdx.x & 63;
-  // A wave takes kAdamIters blocks of 256 elements, four elements a lane.
-  const int64_t block0 = (int64_t)(blockIdx.x - tab.t.first[i]) * (kAdamChunk / kStateBlock) +
-                         __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * kAdamIters;
-#pragma unroll
-  for (int j = 0; j < kAdamIters; ++j) {
-    const int64_t block = block0 + j, at = block * kStateBlock + lane * 4;
-    if (block * kStateBlock >= n) return;
-    const int left = n - at < 0 ? 0 : n - at < 4 ? (int)(n - at) : 4;
-    const bool vec = fits && left == 4;
-    float pv[4], gv[4], r[4], mm[4];
-    load4<T>(p + at, left, vec, pv);
-    load4<T>(grad + at, left, vec, gv);
-    uint32_t mc = 0, vc = 0;
-    if (vec) {
-      mc = *(const uint32_t*)(m + at);
-      vc = *(const uint32_t*)(v + at);
-    } else {
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (c < left) mc |= (uint32_t)m[at + c] << (8 * c), vc |= (uint32_t)v[at + c] << (8 * c);
-    }
+  const int64_t block = (int64_t)(blockIdx.x - tab.t.first[i]) * (kAdamChunk / kStateBlock) + (threadIdx.x >> 4);
+  const int64_t at = block * kStateBlock + (threadIdx.x & 15) * 16;
+  if (block * kStateBlock >= n) return;  // whole rows of lanes
+  const int left = n - at >= 16 ? 16 : n > at ? (int)(n - at) : 0;
+  float pv[16], mm[16], x[16];
+  {
+    float gv[16];
+    load16<T>(grad + at, left, gv);
+    const codes16 mc = load_codes(m + at, left), vc = load_codes(v + at, left);
     const float ms = tab.m_scale[i][block], vs = tab.v_scale[i][block];
-    uint32_t mtop = 0, vtop = 0;
+    load16<T>(p + at, left, pv);
+    decode16(mc, ms, mm);
+    decode16(vc, vs, x);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < 16; ++c) {
       const float g = k.clip ? gv[c] * clip : gv[c];
-      const float m0 = (c == 0   ? __builtin_amdgcn_cvt_f32_fp8(mc, 0)
-                        : c == 1 ? __builtin_amdgcn_cvt_f32_fp8(mc, 1)
-                        : c == 2 ? __builtin_amdgcn_cvt_f32_fp8(mc, 2)
-                                 : __builtin_amdgcn_cvt_f32_fp8(mc, 3)) * ms;
-      const float r0 = (c == 0   ? __builtin_amdgcn_cvt_f32_fp8(vc, 0)
-                        : c == 1 ? __builtin_amdgcn_cvt_f32_fp8(vc, 1)
-                        : c == 2 ? __builtin_amdgcn_cvt_f32_fp8(vc, 2)
-                                 : __builtin_amdgcn_cvt_f32_fp8(vc, 3)) * vs;
-      mm[c] = m0 * k.beta1 + g * k.one_beta1;
-      r[c] = sqrtf(r0 * r0 * k.beta2 + g * g * k.one_beta2);
-      pv[c] = pv[c] * k.decay - mm[c] / (r[c] * k.root_scale + k.eps) * k.step_size;
-      const uint32_t ma = __float_as_uint(mm[c]) & 0x7fffffffu, ra = __float_as_uint(r[c]);
-      if (ma < 0x7f800000u && ma > mtop) mtop = ma;
-      if (ra < 0x7f800000u && ra > vtop) vtop = ra;
-    }
-    store4<T>(p + at, left, vec, pv);
-    const int mf = scale_field(wave_max_bits(mtop)), vf = scale_field(wave_max_bits(vtop));
-    if (lane == 0) {
-      tab.m_scale[i][block] = __uint_as_float((uint32_t)mf << 23);
-      tab.v_scale[i][block] = __uint_as_float((uint32_t)vf << 23);
-    }
-    const float mi = __uint_as_float((uint32_t)(254 - mf) << 23);
-    const float vi = __uint_as_float((uint32_t)(254 - vf) << 23);
-    uint32_t mo = 0, vo = 0;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const uint64_t place = (uint64_t)(at + c);
-      const uint32_t bits = place_bits((uint32_t)place + (uint32_t)(place >> 32) * kMulB + tab.seed[i] * kGolden);
-      const float um = (float)((bits + k.step * kGolden) >> 8) * 0x1p-24f;
-      const float uv = (float)((((bits << 16) | (bits >> 16)) + k.step * kMulB) >> 8) * 0x1p-24f;
-      {  // m: q in steps of its binade (the lowest is 2^-6 on), up with probability q - floor(q)
-        const float x = fabsf(mm[c]) * mi;
-        int f = (int)(__float_as_uint(x) >> 23);
-        f = f < 121 ? 121 : f;
-        const float q = x * __uint_as_float((uint32_t)(257 - f) << 23);
-        uint32_t code = ((uint32_t)(f - 121) << 3) + (uint32_t)floorf(q + um);
-        code = code > 0x7eu ? 0x7eu : code;  // q + um may round up to the step past 448
-        if (!(x < 512.f)) code = 0x7f;
-        mo |= (code | (mm[c] < 0.f ? 0x80u : 0u)) << (8 * c);
-      }
-      {  // r: up with probability (q^2 - k^2) / ((k + 1)^2 - k^2)
-        const float x = r[c] * vi;
-        int f = (int)(__float_as_uint(x) >> 23);
-        f = f < 121 ? 121 : f;
-        const float q = x * __uint_as_float((uint32_t)(257 - f) << 23);
-        const float lo = floorf(q);
-        uint32_t code = ((uint32_t)(f - 121) << 3) + (uint32_t)lo +
-                        (uv * (2.f * lo + 1.f) < (q - lo) * (q + lo) ? 1u : 0u);
-        code = x > 0.f && code == 0 ? 1u : code;
-        if (!(x < 512.f)) code = 0x7f;
-        vo |= code << (8 * c);
-      }
-    }
-    if (vec) {
-      *(uint32_t*)(m + at) = mo;
-      *(uint32_t*)(v + at) = vo;
-    } else {
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (c < left) m[at + c] = (uint8_t)(mo >> (8 * c)), v[at + c] = (uint8_t)(vo >> (8 * c));
+      mm[c] = mm[c] * k.beta1 + g * k.one_beta1;
+      x[c] = x[c] * x[c] * k.beta2 + g * g * k.one_beta2;
     }
   }
+  uint32_t mtop = 0, xtop = 0, low = 0xffffffffu;
+#pragma unroll
+  for (int c = 0; c < 16; ++c) {
+    const uint32_t ma = __float_as_uint(mm[c]) & 0x7fffffffu, xb = __float_as_uint(x[c]);
+    mtop = ma > mtop ? ma : mtop;
+    xtop = xb > xtop ? xb : xtop;
+    low = xb < low ? xb : low;
+  }
+  mtop = row_max_bits(mtop);
+  xtop = row_max_bits(xtop);
+  const bool plain = low >= 0x0f800000u && xtop < 0x7e800000u && mtop < 0x7f800000u && mtop >= 0x08000000u;
+  const auto root = [](float a) {
+    const float y = __builtin_amdgcn_rsqf(a), s = a * y;
+    return fmaf(fmaf(-s, s, a), 0.5f * y, s);
+  };
+  const uint32_t at_bits = (uint32_t)at + (uint32_t)((uint64_t)at >> 32) * kMulB + tab.seed[i] * kGolden;
+  codes16 mo = {0, 0, 0, 0}, vo = {0, 0, 0, 0};
+  int mf, vf;
+  if (__all(plain)) {
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+      x[c] = root(x[c]);
+      const float by = __builtin_amdgcn_rcpf(fmaf(x[c], k.root_scale, k.eps));
+      pv[c] = fmaf(pv[c], k.decay, -(mm[c] * k.step_size * by));
+    }
+    store16<T>(p + at, left, pv);
+    mf = scale_field(mtop), vf = scale_field(__float_as_uint(root(__uint_as_float(xtop))));
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+      const AdamCodes code = adam_codes(fabsf(mm[c]), x[c], mf, vf, place_bits(at_bits + c), k.step);
+      mo[c / 4] |= (code.m | (__float_as_uint(mm[c]) >> 24 & 0x80u)) << (8 * (c % 4));
+      vo[c / 4] |= code.r << (8 * (c % 4));
+    }
+  } else {
+    mtop = xtop = 0;
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+      x[c] = sqrtf(x[c]);
+      pv[c] = pv[c] * k.decay - mm[c] / (x[c] * k.root_scale + k.eps) * k.step_size;
+      const uint32_t ma = __float_as_uint(mm[c]) & 0x7fffffffu, xb = __float_as_uint(x[c]);
+      if (ma < 0x7f800000u && ma > mtop) mtop = ma;
+      if (xb < 0x7f800000u && xb > xtop) xtop = xb;
+    }
+    store16<T>(p + at, left, pv);
+    mf = scale_field(row_max_bits(mtop)), vf = scale_field(row_max_bits(xtop));
+    const float mi = __uint_as_float((uint32_t)(254 - mf) << 23);
+    const float vi = __uint_as_float((uint32_t)(254 - vf) << 23);
+#pragma unroll
+    for (int c = 0; c < 16; ++c) {
+      const bool m_ok = fabsf(mm[c]) < __builtin_inff(), r_ok = x[c] < __builtin_inff();
+      const float am = m_ok ? fabsf(mm[c]) * mi : 0.f, r = r_ok ? x[c] * vi : 0.f;
+      AdamCodes code = adam_codes(am, r, 127, 127, place_bits(at_bits + c), k.step);
+      if (!(r > 0.f)) code.r = 0;
+      if (!m_ok) code.m = 0x7f;
+      if (!r_ok) code.r = 0x7f;
+      mo[c / 4] |= (code.m | (mm[c] < 0.f ? 0x80u : 0u)) << (8 * (c % 4));
+      vo[c / 4] |= code.r << (8 * (c % 4));
+    }
+  }
+  if ((threadIdx.x & 15) == 0) {
+    tab.m_scale[i][block] = __uint_as_float((uint32_t)mf << 23);
+    tab.v_scale[i][block] = __uint_as_float((uint32_t)vf << 23);
+  }
+  store_codes(m + at, left, mo);
+  store_codes(v + at, left, vo);
 }
 
 // ---------------------------------------------------------------------------
@@ -266,9 +359,10 @@ __global__ __launch_bounds__(kAdamThreads) void adamw8_kernel(Adam8Table tab, Ad
 // ---------------------------------------------------------------------------
 constexpr int kNormChunk = 256 * 4 * 8;
 struct NormTable {
-  const void* grad[kTableMax];
-  int64_t n[kTableMax];
-  uint32_t first[kTableMax];
+  static constexpr int kMax = 160;
+  const void* grad[kMax];
+  int64_t n[kMax];
+  uint32_t first[kMax];
   int count;
 };
 
@@ -359,7 +453,7 @@ int by_tables(const int64_t* rows, int64_t count, int width, int n_at, int d_at,
       const int64_t* row = rows + i * width;
       const bool mine = i < count && row[d_at] == dtype && row[n_at] > 0;
       const int64_t more = mine ? chunks_of(row[n_at], chunk) : 0;
-      if (used > 0 && (i == count || (mine && (used == kTableMax || blocks + more > 0x7fffffffLL)))) {
+      if (used > 0 && (i == count || (mine && (used == Table::kMax || blocks + more > 0x7fffffffLL)))) {
         launch(t, used, (uint32_t)blocks, dtype);
         const int st = launch_status();
         if (st != MQC_OK) return st;
@@ -389,7 +483,8 @@ inline int check_rows(const int64_t* rows, int64_t count, int width, int pointer
   return MQC_OK;
 }
 
-inline void put_adam(AdamTable& t, int at, const int64_t* row, int64_t n, uint32_t first) {
+template <typename Table>
+inline void put_adam(Table& t, int at, const int64_t* row, int64_t n, uint32_t first) {
   t.p[at] = (void*)row[0];
   t.grad[at] = (const void*)row[1];
   t.m[at] = (void*)row[2];

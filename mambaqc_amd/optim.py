@@ -1,5 +1,5 @@
-"""AdamW on the GPU: one launch for up to 48 tensors of a dtype, states in 32 or in 8 bits, the
-gradients' norm and its clipping on the device.
+"""AdamW on the GPU: one launch for 88 tensors of a dtype (60 with 8-bit states), states in 32 or in 8
+bits, the gradients' norm and its clipping on the device.
 
     p <- p (1 - lr weight_decay) - lr m^ / (sqrt(v^) + eps),  m^ = m / (1 - beta1^t),  v^ = v / (1 - beta2^t)
 
