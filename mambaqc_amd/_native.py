@@ -12,6 +12,7 @@ device pointers handed across are then valid on both sides.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import weakref
 import os
 import threading
@@ -172,6 +173,31 @@ def load(path: os.PathLike | str | None = None) -> ctypes.CDLL:
         if path is None:
             _lib = lib
         return lib
+
+
+_host = None
+
+
+def host():
+    """The module _host (csrc/host.cpp): the recurrent stack's operators from tensors to launches, for
+    where a call's host time counts. It calls the library that load() opens."""
+    global _host
+    if _host is not None:
+        return _host
+    load()
+    with _lock:
+        if _host is None:
+            path = LIB_PATH.parent / "_host.so"
+            if not path.exists():
+                raise NativeLibraryMissing(
+                    f"{path} is missing: build it with `python -m mambaqc_amd.build`")
+            spec = importlib.util.spec_from_file_location("_host", path)
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+            if module.abi() != ABI_VERSION:
+                raise NativeLibraryMissing(f"{path}: ABI version {module.abi()} != {ABI_VERSION}; rebuild")
+            _host = module
+    return _host
 
 
 def status_string(status: int) -> str:

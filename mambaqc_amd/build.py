@@ -1,9 +1,11 @@
-"""Build libmambaqc_hip.so, the C-ABI library of HIP kernels, in-tree.
+"""Build libmambaqc_hip.so, the C-ABI library of HIP kernels, and _host.so, the host side of the
+recurrent stack's operators over torch's C++ API, in-tree.
 
     python -m mambaqc_amd.build          # or mambaqc_amd.build.build()
 
 Every ``csrc/*.hip`` file is compiled for gfx950 with hipcc (in parallel) and
-linked into ``mambaqc_amd/lib/libmambaqc_hip.so``. Nothing is cached: each call
+linked into ``mambaqc_amd/lib/libmambaqc_hip.so``; ``csrc/host.cpp`` becomes
+``mambaqc_amd/lib/_host.so``, which calls that library. Nothing is cached: each call
 recompiles, so a stale library can never survive a source change.
 """
 from __future__ import annotations
@@ -14,12 +16,14 @@ import re
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIBDIR = PKG / "lib"
 LIBNAME = "libmambaqc_hip.so"
+HOSTNAME = "_host.so"
 ARCH = os.environ.get("MQC_OFFLOAD_ARCH", "gfx950")
 
 # Packed fp32 VALU instructions are disabled for all device code (the compiler
@@ -97,6 +101,33 @@ def _compile(hipcc: str, src: Path, obj: Path) -> None:
                            "\n  ".join(spills))
 
 
+def _run(cmd: list[str], what: str) -> None:
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{what} failed:\n{r.stderr}")
+
+
+def _compile_host(obj: Path) -> None:
+    """With g++, as torch itself: templates of its headers are mangled differently by clang."""
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    includes = [*include_paths(), "/opt/rocm/include", sysconfig.get_paths()["include"]]
+    _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1",
+          "-DTORCH_EXTENSION_NAME=_host",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+          *(f"-I{i}" for i in includes), "-c", str(CSRC / "host.cpp"), "-o", str(obj)],
+         "g++ on host.cpp")
+
+
+def _link_host(hipcc: str, obj: Path, out: Path) -> None:
+    from torch.utils.cpp_extension import library_paths
+
+    _run([hipcc, "-shared", "-fPIC", str(obj), f"-L{LIBDIR}", f"-l:{LIBNAME}",
+          *(f"-L{p}" for p in library_paths()), "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu",
+          "-ltorch_hip", "-ltorch_python", "-Wl,-rpath,$ORIGIN", "-o", str(out)], "link of _host.so")
+
+
 def build(verbose: bool = True) -> Path:
     hipcc = _hipcc()
     objdir = PKG / "_build"
@@ -107,17 +138,21 @@ def build(verbose: bool = True) -> Path:
         raise RuntimeError(f"no HIP sources under {CSRC}")
     objs = [objdir / (s.stem + ".o") for s in sources]
     jobs = min(len(sources), max(1, min(8, os.cpu_count() or 1)))
+    host = objdir / "host_module.obj"
     with cf.ThreadPoolExecutor(jobs) as ex:
+        task = ex.submit(_compile_host, host)
         list(ex.map(lambda so: _compile(hipcc, *so), zip(sources, objs)))
+        task.result()
     out = LIBDIR / LIBNAME
     tmp = LIBDIR / (LIBNAME + ".tmp")
     cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"link failed:\n{r.stderr}")
+    _run(cmd, "link")
     os.replace(tmp, out)
+    tmp = LIBDIR / (HOSTNAME + ".tmp")
+    _link_host(hipcc, host, tmp)
+    os.replace(tmp, LIBDIR / HOSTNAME)
     if verbose:
-        print(f"built {out} from {len(sources)} sources", file=sys.stderr)
+        print(f"built {out} from {len(sources)} sources, and {HOSTNAME}", file=sys.stderr)
     return out
 
 

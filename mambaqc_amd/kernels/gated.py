@@ -16,14 +16,9 @@ from .. import _native as nat
 
 
 def _rows(t: torch.Tensor, dtype: torch.dtype):
-    """(t, elements between tokens) in dtype, read in place where its tokens are evenly spaced and
-    its last axis is dense."""
-    b, n, d = t.shape
-    t = t.detach().to(dtype)
-    if (d > 1 and t.stride(2) != 1) or (b > 1 and n > 1 and t.stride(0) != n * t.stride(1)) or (
-            b * n > 1 and (t.stride(1) if n > 1 else t.stride(0)) < d):
-        t = t.contiguous()
-    return t, d if b * n <= 1 else t.stride(1) if n > 1 else t.stride(0)
+    """(t [b, n, d], elements between tokens) in dtype, read in place where its tokens are evenly
+    spaced and its last axis is dense."""
+    return nat.host().token_rows(t, dtype)
 
 
 def _check(name, dt_raw, g_raw, x, log_rate, h0, reset=None):
@@ -49,81 +44,13 @@ def scan_chunk() -> int:
     return int(nat.load().mqc_gated_scan_chunk())
 
 
-def _scan_forward(dt_raw, g_raw, x, log_rate, h0, reset, train):
-    """(y, h_last, carries or None, the operands as the kernels read them)."""
-    nat.require_device("gated_scan", x, dt_raw, g_raw, log_rate,
-                       *(v for v in (h0, reset) if v is not None))
-    b, t, d = x.shape
-    ct = _scan_dtype(dt_raw, g_raw, x)
-    (dt, dts), (g, gs), (xv, xs) = (_rows(v, ct) for v in (dt_raw, g_raw, x))
-    lam = nat.param_f32(log_rate)
-    h0 = None if h0 is None else h0.detach().float().contiguous()
-    reset = None if reset is None else reset.detach().contiguous()
-    y = torch.empty(b, t, d, device=x.device, dtype=ct)
-    h_last = torch.empty(b, d, device=x.device, dtype=torch.float32)
-    lib = nat.load()
-    carries = None
-    if train:
-        every = scan_chunk()
-        carries = torch.empty(b, (t + every - 1) // every, d, device=x.device,
-                              dtype=torch.float32)
-    nbytes = lib.mqc_gated_scan_workspace_bytes(b, t, d)
-    ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
-    nat.call("mqc_gated_scan_fwd", xv, dt.data_ptr(), dts, g.data_ptr(), gs, xv.data_ptr(), xs,
-             lam.data_ptr(), nat.ptr(h0), nat.ptr(reset), y.data_ptr(), h_last.data_ptr(),
-             nat.ptr(carries), b, t, d, nat.dtype_code(xv), ws.data_ptr(), nbytes,
-             nat.stream_of(xv))
-    return y, h_last, carries, (dt, g, xv, lam, reset)
+def _operands(name, dt_raw, g_raw, x, log_rate, reset=None):
+    """The operands as the kernels read them, log_rate in fp32."""
+    return nat.host().Scan(name, dt_raw, g_raw, x, nat.param_f32(log_rate), reset)
 
 
-def _scan_backward(operands, carries, dy, dh_last, want_dh0):
-    """(ddt, dg, dx in the operands' dtype, dlog_rate, dh0 or None in fp32)."""
-    dt_raw, g_raw, x, lam, reset = operands
-    b, t, d = x.shape
-    if x.numel() == 0:
-        grads = [torch.empty_like(x, memory_format=torch.contiguous_format) for _ in range(3)]
-        dh0 = None
-        if want_dh0:
-            dh0 = (torch.zeros(b, d, device=x.device) if dh_last is None
-                   else dh_last.float().clone())
-        return (*grads, torch.zeros_like(lam), dh0)
-    (dt, dts), (g, gs), (xv, xs) = (_rows(v, x.dtype) for v in (dt_raw, g_raw, x))
-    dy = (torch.zeros(b, t, d, device=x.device, dtype=x.dtype) if dy is None
-          else dy.to(x.dtype).contiguous())
-    dh_last = None if dh_last is None else dh_last.float().contiguous()
-    ddt, dg, dx = (torch.empty(b, t, d, device=x.device, dtype=x.dtype) for _ in range(3))
-    drate = torch.empty(d, device=x.device, dtype=torch.float32)
-    dh0 = torch.empty(b, d, device=x.device, dtype=torch.float32) if want_dh0 else None
-    nbytes = nat.load().mqc_gated_scan_workspace_bytes(b, t, d)
-    ws = torch.empty(nbytes, device=x.device, dtype=torch.uint8)
-    nat.call("mqc_gated_scan_bwd", xv, dt.data_ptr(), dts, g.data_ptr(), gs, xv.data_ptr(), xs,
-             lam.data_ptr(), nat.ptr(reset), carries.data_ptr(), dy.data_ptr(), nat.ptr(dh_last),
-             ddt.data_ptr(), dg.data_ptr(), dx.data_ptr(), drate.data_ptr(), nat.ptr(dh0), b, t, d,
-             nat.dtype_code(xv), ws.data_ptr(), nbytes, nat.stream_of(xv))
-    return ddt, dg, dx, drate, dh0
-
-
-class _GatedScan(torch.autograd.Function):
-    """The scan with HIP forward (storing the chunks' entry states) and backward."""
-
-    @staticmethod
-    def forward(ctx, dt_raw, g_raw, x, log_rate, h0, reset):
-        y, h_last, carries, ops = _scan_forward(dt_raw, g_raw, x, log_rate, h0, reset, True)
-        ctx.save_for_backward(*ops, carries)
-        ctx.set_materialize_grads(False)
-        ctx.meta = (dt_raw.dtype, g_raw.dtype, x.dtype, log_rate.dtype,
-                    None if h0 is None else h0.dtype)
-        return y, h_last
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy, dh_last):
-        *ops, carries = ctx.saved_tensors
-        t_dt, t_g, t_x, t_rate, t_h0 = ctx.meta
-        ddt, dg, dx, drate, dh0 = _scan_backward(ops, carries, dy, dh_last,
-                                                 t_h0 is not None and ctx.needs_input_grad[4])
-        return (ddt.to(t_dt), dg.to(t_g), dx.to(t_x), drate.to(t_rate),
-                None if dh0 is None else dh0.to(t_h0), None)
+def _state(h0):
+    return None if h0 is None else h0.detach().float().contiguous()
 
 
 def gated_scan(dt_raw: torch.Tensor, g_raw: torch.Tensor, x: torch.Tensor, log_rate: torch.Tensor,
@@ -142,10 +69,12 @@ def gated_scan(dt_raw: torch.Tensor, g_raw: torch.Tensor, x: torch.Tensor, log_r
     if nat.compiling():
         op = torch.ops.mambaqc.gated_scan_train if train else torch.ops.mambaqc.gated_scan
         y, h_last = op(dt_raw, g_raw, x, log_rate, h0, reset)[:2]
-    elif train:
-        y, h_last = _GatedScan.apply(dt_raw, g_raw, x, log_rate, h0, reset)
     else:
-        y, h_last, _, _ = _scan_forward(dt_raw, g_raw, x, log_rate, h0, reset, False)
+        operands = _operands("gated_scan", dt_raw, g_raw, x, log_rate, reset)
+        if train:
+            y, h_last = nat.host().scan_train(dt_raw, g_raw, x, log_rate, h0, operands, _state(h0))
+        else:
+            y, h_last, _ = nat.host().scan_forward(operands, _state(h0), False)
     return (y, h_last) if return_state else y
 
 
@@ -160,11 +89,4 @@ def gated_scan_step_(dt_raw: torch.Tensor, g_raw: torch.Tensor, x: torch.Tensor,
         raise ValueError(f"gated_scan_step_: one token a sequence, got {t}")
     if h.dtype != torch.float32 or not h.is_contiguous():
         raise ValueError(f"gated_scan_step_: h must be contiguous float32, got {h.dtype}")
-    nat.require_device("gated_scan_step_", x, dt_raw, g_raw, log_rate, h)
-    ct = _scan_dtype(dt_raw, g_raw, x)
-    (dt, dts), (g, gs), (xv, xs) = (_rows(v, ct) for v in (dt_raw, g_raw, x))
-    y = torch.empty(b, 1, d, device=x.device, dtype=ct)
-    nat.call("mqc_gated_scan_step", xv, dt.data_ptr(), dts, g.data_ptr(), gs, xv.data_ptr(), xs,
-             nat.param_f32(log_rate).data_ptr(), h.data_ptr(), y.data_ptr(), b, d,
-             nat.dtype_code(xv), nat.stream_of(xv))
-    return y
+    return nat.host().scan_step(_operands("gated_scan_step_", dt_raw, g_raw, x, log_rate), h)

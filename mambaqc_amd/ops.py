@@ -493,7 +493,8 @@ def gated_scan(dt_raw: Tensor, g_raw: Tensor, x: Tensor, log_rate: Tensor,
                h0: Optional[Tensor] = None,
                reset: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
     """Inference: (y in the promoted dtype, h_last fp32 [B, W])."""
-    return gated._scan_forward(dt_raw, g_raw, x, log_rate, h0, reset, False)[:2]
+    ops = gated._operands("gated_scan", dt_raw, g_raw, x, log_rate, reset)
+    return nat.host().scan_forward(ops, gated._state(h0), False)[:2]
 
 
 @gated_scan.register_fake
@@ -508,7 +509,8 @@ def gated_scan_train(dt_raw: Tensor, g_raw: Tensor, x: Tensor, log_rate: Tensor,
                      h0: Optional[Tensor] = None,
                      reset: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
     """(y, h_last, the chunks' entry states for the backward)."""
-    return gated._scan_forward(dt_raw, g_raw, x, log_rate, h0, reset, True)[:3]
+    ops = gated._operands("gated_scan", dt_raw, g_raw, x, log_rate, reset)
+    return nat.host().scan_forward(ops, gated._state(h0), True)
 
 
 @gated_scan_train.register_fake
@@ -525,10 +527,8 @@ def gated_scan_backward(dt_raw: Tensor, g_raw: Tensor, x: Tensor, log_rate: Tens
                         reset: Optional[Tensor], carries: Tensor, dy: Tensor,
                         dh_last: Tensor) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor]:
     """(ddt, dg, dx in the promoted dtype, dlog_rate and dh0 in fp32)."""
-    ct = gated._scan_dtype(dt_raw, g_raw, x)
-    operands = (dt_raw.to(ct), g_raw.to(ct), x.to(ct), nat.param_f32(log_rate),
-                None if reset is None else reset.contiguous())
-    return gated._scan_backward(operands, carries, dy, dh_last, True)
+    ops = gated._operands("gated_scan", dt_raw, g_raw, x, log_rate, reset)
+    return tuple(nat.host().scan_backward(ops, carries, dy, dh_last, True))
 
 
 @gated_scan_backward.register_fake
@@ -563,7 +563,8 @@ def gate_norm_residual(x: Tensor, y: Tensor, z: Optional[Tensor], post_weight: O
                        scale: Tensor, pre_weight: Tensor,
                        eps: float = 1e-6) -> Tuple[Tensor, Tensor, Tensor]:
     """(out, n in the promoted dtype, the rows' inverse norms fp32 [rows, 2])."""
-    return gate_norm._forward(gate_norm._operands(x, y, z, post_weight, scale, pre_weight), eps, True)
+    ops = gate_norm._operands(x, y, z, post_weight, scale, pre_weight)
+    return nat.host().gate_norm_forward(ops, eps, True)
 
 
 @gate_norm_residual.register_fake
@@ -581,7 +582,7 @@ def gate_norm_residual_backward(
     """(dx, dy, dz in the promoted dtype, dpost, dscale, dpre in fp32); dz and dpost are empty where
     they do not apply."""
     ops = gate_norm._operands(x, y, z, post_weight, scale, pre_weight)
-    dx, dy, dz, dpost, dscale, dpre = gate_norm._backward(ops, stats, dout, dn)
+    dx, dy, dz, dpost, dscale, dpre = nat.host().gate_norm_backward(ops, stats, dout, dn)
     return (dx, dy, x.new_empty(0, dtype=dx.dtype) if dz is None else dz,
             dscale.new_empty(0) if dpost is None else dpost, dscale, dpre)
 

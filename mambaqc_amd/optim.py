@@ -14,7 +14,7 @@ step give the same bits.
 """
 from __future__ import annotations
 
-import ctypes
+import array
 import itertools
 import math
 
@@ -30,15 +30,13 @@ def state_blocks(numel: int) -> int:
     return -(-numel // STATE_BLOCK)
 
 
-def _rows(values) -> ctypes.Array:
-    return (ctypes.c_int64 * max(1, len(values)))(*values)
+def _check_lengths(name, *lists):
+    if not all(len(s) == len(lists[0]) for s in lists):
+        raise ValueError(f"{name}: lists of different lengths {[len(s) for s in lists]}")
 
 
 def _check_tensors(name, params, grads, *states):
     """params and grads of one device, dtypes and shapes that match, all dense."""
-    if not all(len(s) == len(params) for s in (grads, *states)):
-        raise ValueError(f"{name}: lists of different lengths "
-                         f"{[len(s) for s in (params, grads, *states)]}")
     for p, g in zip(params, grads):
         if p.shape != g.shape or p.dtype != g.dtype:
             raise ValueError(f"{name}: a gradient is {g.dtype} {tuple(g.shape)}, its parameter "
@@ -67,35 +65,42 @@ def _scalars(step, lr, betas, eps, weight_decay):
             b2, 1 - b2, eps)
 
 
-def _norm_and_clip(grads, max_norm):
-    """(norm, clip) as fp32 scalars on the gradients' device."""
-    dev = grads[0].device
-    rows = _rows([v for g in grads for v in (g.data_ptr(), g.numel(), nat.dtype_code(g))])
-    nbytes = nat.load().mqc_grad_norm_workspace_bytes(rows, len(grads))
+def _tables(name, params, grads, states, scales, seeds):
+    """The rows that mqc_adamw_step or mqc_adamw8_step reads, and mqc_grad_norm's."""
+    got = nat.host().adam_rows((params, grads, *states, *scales), STATE_BLOCK, seeds)
+    if got is None:  # say what is wrong
+        eight = len(scales) > 0
+        for s in states:
+            _check_state(name, "states", params, s, torch.float8_e4m3fn if eight else torch.float32)
+        for s in scales:
+            _check_state(name, "scales", params, s, torch.float32, state_blocks)
+        _check_tensors(name, params, grads, *states, *scales)
+        raise ValueError(f"{name}: tensors that the kernels do not take")
+    return got
+
+
+def _norm_and_clip(rows: bytes, max_norm, like):
+    """(norm, clip) as fp32 scalars on the gradients' device, from mqc_grad_norm's rows."""
+    count = len(rows) // 24
+    nbytes = nat.load().mqc_grad_norm_workspace_bytes(rows, count)
     if nbytes < 0:
         nat.check(nbytes, "mqc_grad_norm")
-    out = torch.empty(2, device=dev, dtype=torch.float32)
-    ws = torch.empty(nbytes, device=dev, dtype=torch.uint8)
-    nat.call("mqc_grad_norm", out, rows, len(grads), float(max_norm), out.data_ptr(),
-             out.data_ptr() + 4, ws.data_ptr(), nbytes, nat.stream_of(out))
+    out = torch.empty(2, device=like.device, dtype=torch.float32)
+    ws = torch.empty(nbytes, device=like.device, dtype=torch.uint8)
+    at = out.data_ptr()
+    nat.call("mqc_grad_norm", out, rows, count, float(max_norm), at, at + 4, ws.data_ptr(),
+             nbytes, nat.stream_of(out))
     return out[0], out[1]
 
 
 def grad_norm(grads: list[torch.Tensor]) -> torch.Tensor:
     """The 2-norm of all elements of the tensors together (fp32 scalar on their device; summed in 64
     bits, in a fixed order)."""
-    grads = [g.detach() for g in grads]
     if not grads:
         raise ValueError("grad_norm: no tensors")
     _check_tensors("grad_norm", grads, grads)
-    return _norm_and_clip(grads, math.inf)[0]
-
-
-def _updated(*lists):
-    """The kernels write through pointers: tell autograd (and whatever keeps copies of parameters by
-    their version, as param_f32 does) that these tensors changed."""
-    for tensors in lists:
-        torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+    rows = array.array("q", [v for g in grads for v in (g.data_ptr(), g.numel(), nat.dtype_code(g))])
+    return _norm_and_clip(rows.tobytes(), math.inf, grads[0])[0]
 
 
 def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float = 1e-3,
@@ -105,25 +110,24 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float = 
     dtype each (fp32, bf16 or fp16), fp32 states. step counts from 1. With max_norm the gradients
     are scaled by min(1, max_norm / (norm + 1e-6)) as they are read (they stay as they are), norm
     over all of them, which is returned (fp32 scalar on the device)."""
-    params, grads = [p.detach() for p in params], [g.detach() for g in grads]
+    params, grads = list(params), list(grads)
     how = _scalars(step, lr, betas, eps, weight_decay)
-    _check_state("adamw_step_", "states", params, exp_avgs, torch.float32)
-    _check_state("adamw_step_", "states", params, exp_avg_sqs, torch.float32)
-    _check_tensors("adamw_step_", params, grads, exp_avgs, exp_avg_sqs)
+    states = (exp_avgs, exp_avg_sqs)
+    _check_lengths("adamw_step_", params, grads, *states)
     if not params:
         return None
-    norm, clip = (None, None) if max_norm is None else _norm_and_clip(grads, max_norm)
-    _launch32(params, grads, exp_avgs, exp_avg_sqs, how, clip)
+    rows, norm_rows = _tables("adamw_step_", params, grads, states, (), ())
+    norm, clip = (None, None) if max_norm is None else _norm_and_clip(norm_rows, max_norm, params[0])
+    _launch32(rows, params, states, how, clip)
     return norm
 
 
-def _launch32(params, grads, ms, vs, how, clip):
-    rows = _rows([x for p, g, m, v in zip(params, grads, ms, vs)
-                  for x in (p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), p.numel(),
-                            nat.dtype_code(p))])
+def _launch32(rows, params, states, how, clip):
     nat.call("mqc_adamw_step", params[0], rows, len(params), *how, nat.ptr(clip),
              nat.stream_of(params[0]))
-    _updated(params, ms, vs)
+    # The kernels write through pointers: tell autograd (and whatever keeps copies of parameters by
+    # their version, as param_f32 does) that these tensors changed.
+    nat.host().changed((params, *states))
 
 
 def adamw8_step_(params, grads, exp_avgs, exp_avg_scales, root_avg_sqs, root_avg_sq_scales, *,
@@ -132,29 +136,23 @@ def adamw8_step_(params, grads, exp_avgs, exp_avg_scales, root_avg_sqs, root_avg
     """adamw_step_ with states in 8 bits: exp_avgs and root_avg_sqs (sqrt(v)) torch.float8_e4m3fn
     tensors of the parameters' sizes, their scales fp32 of state_blocks(numel) elements. What a state
     stands for is its value times its block's scale. Tensor i of the lists rounds by seed + i."""
-    params, grads = [p.detach() for p in params], [g.detach() for g in grads]
+    params, grads = list(params), list(grads)
     how = _scalars(step, lr, betas, eps, weight_decay)
-    for what, states in (("states", exp_avgs), ("states", root_avg_sqs)):
-        _check_state("adamw8_step_", what, params, states, torch.float8_e4m3fn)
-    for what, states in (("scales", exp_avg_scales), ("scales", root_avg_sq_scales)):
-        _check_state("adamw8_step_", what, params, states, torch.float32, state_blocks)
-    _check_tensors("adamw8_step_", params, grads, exp_avgs, exp_avg_scales, root_avg_sqs,
-                   root_avg_sq_scales)
+    states, scales = (exp_avgs, root_avg_sqs), (exp_avg_scales, root_avg_sq_scales)
+    _check_lengths("adamw8_step_", params, grads, *states, *scales)
     if not params:
         return None
-    norm, clip = (None, None) if max_norm is None else _norm_and_clip(grads, max_norm)
-    _launch8(params, grads, exp_avgs, exp_avg_scales, root_avg_sqs, root_avg_sq_scales, how, clip,
-             step, range(seed, seed + len(params)))
+    rows, norm_rows = _tables("adamw8_step_", params, grads, states, scales,
+                              range(seed, seed + len(params)))
+    norm, clip = (None, None) if max_norm is None else _norm_and_clip(norm_rows, max_norm, params[0])
+    _launch8(rows, params, (*states, *scales), how, clip, step)
     return norm
 
 
-def _launch8(params, grads, ms, mscales, rs, rscales, how, clip, step, seeds):
-    rows = _rows([x for p, g, m, a, r, b, s in zip(params, grads, ms, mscales, rs, rscales, seeds)
-                  for x in (p.data_ptr(), g.data_ptr(), m.data_ptr(), r.data_ptr(), a.data_ptr(),
-                            b.data_ptr(), p.numel(), nat.dtype_code(p), s & 0xFFFFFFFF)])
+def _launch8(rows, params, states, how, clip, step):
     nat.call("mqc_adamw8_step", params[0], rows, len(params), *how, nat.ptr(clip),
              step & 0xFFFFFFFF, nat.stream_of(params[0]))
-    _updated(params, ms, mscales, rs, rscales)
+    nat.host().changed((params, *states))
 
 
 class AdamW(torch.optim.Optimizer):
@@ -203,7 +201,7 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW: a step counts on the host and is not captured into a graph")
-        todo, grads, place = {}, [], 0
+        todo, place = {}, 0
         for index, group in enumerate(self.param_groups):
             for p in group["params"]:
                 place += 1
@@ -215,28 +213,31 @@ class AdamW(torch.optim.Optimizer):
                 if g.dtype != p.dtype:
                     g = g.to(p.dtype)
                 s = self._state_of(p, group["state_bits"])
-                grads.append(g)
                 todo.setdefault((index, s["step"], "root_avg_sq" in s), []).append(
                     (p.detach(), g, s, self.seed + place))
-        if not grads:
+        if not todo:
             return loss
-        _check_tensors("AdamW", [p for t in todo.values() for p, *_ in t],
-                       [g for t in todo.values() for _, g, *_ in t])
+        work = []
+        for (index, step, eight), entries in todo.items():
+            params, grads, states, seeds = zip(*entries)
+            keys = ("exp_avg", "root_avg_sq") if eight else ("exp_avg", "exp_avg_sq")
+            held = [[s[k] for s in states] for k in keys]
+            scales = [[s[k + "_scale"] for s in states] for k in keys] if eight else []
+            work.append((index, step, params, states, held + scales,
+                         _tables("AdamW", params, grads, held, scales, seeds)))
         clip = None
         if self.max_norm is not None:
-            self.grad_norm, clip = _norm_and_clip(grads, self.max_norm)
-        for (index, step, eight), entries in todo.items():
+            nat.require_device("AdamW", *(w[2][0] for w in work))  # one norm, on one device
+            self.grad_norm, clip = _norm_and_clip(b"".join(w[-1][1] for w in work), self.max_norm,
+                                                  work[0][2][0])
+        for index, step, params, states, held, (rows, _) in work:
             group = self.param_groups[index]
             how = _scalars(step + 1, group["lr"], group["betas"], group["eps"],
                            group["weight_decay"])
-            params, gs, states, seeds = zip(*entries)
-            if eight:
-                _launch8(params, gs, *([s[k] for s in states] for k in (
-                    "exp_avg", "exp_avg_scale", "root_avg_sq", "root_avg_sq_scale")), how, clip,
-                    step + 1, seeds)
+            if len(held) == 4:
+                _launch8(rows, params, held, how, clip, step + 1)
             else:
-                _launch32(params, gs, *([s[k] for s in states] for k in ("exp_avg", "exp_avg_sq")),
-                          how, clip)
+                _launch32(rows, params, held, how, clip)
             for s in states:
                 s["step"] = step + 1
         return loss
