@@ -31,39 +31,46 @@ struct GateNormArgs {
 };
 
 // Four consecutive elements from wherever they start (rows of odd widths do not start at multiples
-// of a vector; gfx950 loads and stores those as it does aligned ones), `left` of them.
+// of a vector; gfx950 loads and stores those as it does aligned ones), `left` of them, as they are
+// in memory.
 template <typename T>
-__device__ inline void load_part(const T* row, uint32_t i, int left, float (&out)[4]) {
+using Quad = uint32_t __attribute__((ext_vector_type(sizeof(T)), aligned(sizeof(T))));
+template <typename T>
+__device__ inline Quad<T> load_quad(const T* row, uint32_t i, int left) {
   const T* p = row + i;
-  if (left >= 4) {
-    if constexpr (sizeof(T) == 4) {
-      typedef float any4 __attribute__((ext_vector_type(4), aligned(4)));
-      const any4 v = *reinterpret_cast<const any4*>(p);
+  if (left >= 4) return *reinterpret_cast<const Quad<T>*>(p);
+  Quad<T> v = {};
 #pragma unroll
-      for (int c = 0; c < 4; ++c) out[c] = v[c];
-    } else {
-      typedef uint32_t any2 __attribute__((ext_vector_type(2), aligned(2)));
-      const any2 v = *reinterpret_cast<const any2*>(p);
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        out[c] = io<T>::bits_to_f32(c & 1 ? v[c / 2] >> 16 : v[c / 2] & 0xffffu);
+  for (int c = 0; c < 3; ++c)
+    if (c < left) {
+      if constexpr (sizeof(T) == 4) v[c] = __builtin_bit_cast(uint32_t, p[c]);
+      else v[c / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, p[c]) << (16 * (c % 2));
     }
-  } else {
+  return v;
+}
+template <typename T>
+__device__ inline void unpack_quad(Quad<T> v, float (&out)[4]) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) out[c] = c < left ? load_scalar(p + c) : 0.f;
+  for (int c = 0; c < 4; ++c) {
+    if constexpr (sizeof(T) == 4) out[c] = __uint_as_float(v[c]);
+    else out[c] = io<T>::bits_to_f32(c & 1 ? v[c / 2] >> 16 : v[c / 2] & 0xffffu);
   }
 }
 template <typename T>
+__device__ inline void load_part(const T* row, uint32_t i, int left, float (&out)[4]) {
+  unpack_quad<T>(load_quad(row, i, left), out);
+}
+template <bool STREAM = false, typename T>
 __device__ inline void store_part(T* row, uint32_t i, int left, const float (&in)[4]) {
   T* p = row + i;
   if (left >= 4) {
-    if constexpr (sizeof(T) == 4) {
-      typedef float any4 __attribute__((ext_vector_type(4), aligned(4)));
-      *reinterpret_cast<any4*>(p) = any4{in[0], in[1], in[2], in[3]};
-    } else {
-      typedef uint32_t any2 __attribute__((ext_vector_type(2), aligned(2)));
-      *reinterpret_cast<any2*>(p) = any2{pack2<T>(in[0], in[1]), pack2<T>(in[2], in[3])};
-    }
+    Quad<T> v;
+#pragma unroll
+    for (int c = 0; c < (int)sizeof(T); ++c)
+      if constexpr (sizeof(T) == 4) v[c] = __float_as_uint(in[c]);
+      else v[c] = pack2<T>(in[2 * c], in[2 * c + 1]);
+    if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<Quad<T>*>(p));
+    else *reinterpret_cast<Quad<T>*>(p) = v;
   } else {
 #pragma unroll
     for (int c = 0; c < 4; ++c)
@@ -71,13 +78,24 @@ __device__ inline void store_part(T* row, uint32_t i, int left, const float (&in
   }
 }
 
-// A row belongs to a team: one wave (ONE), or all waves of the workgroup. Its sums, the same in every
-// lane; `red` holds 16 floats a sum.
-template <bool ONE, int N>
+// A row belongs to a team of LANES lanes: 16 or 32 for narrow rows (which would leave most of a wave
+// idle), a wave, or all waves of the workgroup (LANES 0). Its sums, the same in every lane; `red` holds
+// 16 floats a sum.
+template <int LANES, int N>
 __device__ inline void team_sum(float (&v)[N], float* red) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = wave_sum_all(v[i]);
-  if constexpr (!ONE) {
+  for (int i = 0; i < N; ++i) {
+    if constexpr (LANES == 16 || LANES == 32) {
+      v[i] += lane_xor1(v[i]);
+      v[i] += lane_xor2(v[i]);
+      v[i] += row_rot4(v[i]);
+      v[i] += row_rot8(v[i]);
+      if constexpr (LANES == 32) v[i] += __shfl_xor(v[i], 16);
+    } else {
+      v[i] = wave_sum_all(v[i]);
+    }
+  }
+  if constexpr (LANES == 0) {
     const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     if ((threadIdx.x & 63) == 0) {
 #pragma unroll
@@ -94,15 +112,23 @@ __device__ inline void team_sum(float (&v)[N], float* red) {
   }
 }
 
-constexpr int kOneRows = 4;  // rows (waves) of a workgroup whose teams are single waves
+// Teams of a workgroup, and a team's number in it (uniform over a wave where that is one team's).
+template <int LANES>
+constexpr int kTeams = LANES ? 256 / LANES : 1;
+template <int LANES>
+__device__ inline int team_number() {
+  if constexpr (LANES == 0) return 0;
+  const int i = threadIdx.x / (LANES ? LANES : 1);
+  return LANES == 64 ? __builtin_amdgcn_readfirstlane(i) : i;
+}
 
 // A lane holds elements 4 (lane + team m) + 0..3 of its row for m < NV.
-template <typename T, int NV, bool ONE>
-__global__ __launch_bounds__(ONE ? 64 * kOneRows : 1024) void gate_norm_fwd_kernel(GateNormArgs<T> k) {
-  __shared__ float red[ONE ? 1 : 32];
-  const int team = ONE ? 64 : blockDim.x, t = ONE ? threadIdx.x & 63 : threadIdx.x;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = (int)k.d;
-  const int64_t row = ONE ? (int64_t)blockIdx.x * kOneRows + wave : blockIdx.x;
+template <typename T, int NV, int LANES, bool STREAM>
+__global__ __launch_bounds__(LANES ? 256 : 1024) void gate_norm_fwd_kernel(GateNormArgs<T> k) {
+  __shared__ float red[LANES ? 1 : 32];
+  const int team = LANES ? LANES : blockDim.x, t = LANES ? threadIdx.x % team : threadIdx.x;
+  const int d = (int)k.d;
+  const int64_t row = (int64_t)blockIdx.x * kTeams<LANES> + team_number<LANES>();
   if (row >= k.rows) return;  // whole teams; a team of several waves has its row
   const int64_t base = row * k.d;
   float x[NV][4], v[NV][4];
@@ -129,7 +155,7 @@ __global__ __launch_bounds__(ONE ? 64 * kOneRows : 1024) void gate_norm_fwd_kern
   const float inv = 1.f / (float)k.d;
   float rho = 1.f;
   if (k.post) {
-    team_sum<ONE>(s, red);
+    team_sum<LANES>(s, red);
     rho = 1.f / sqrtf(s[0] * inv + k.eps);
   }
   s[0] = 0.f;
@@ -146,9 +172,9 @@ __global__ __launch_bounds__(ONE ? 64 * kOneRows : 1024) void gate_norm_fwd_kern
       x[m][c] = fmaf(sc[c], r, x[m][c]);
       s[0] = fmaf(x[m][c], x[m][c], s[0]);
     }
-    store_part(k.out + base, i, left, x[m]);
+    store_part<STREAM>(k.out + base, i, left, x[m]);
   }
-  team_sum<ONE>(s, red + (ONE ? 0 : 16));
+  team_sum<LANES>(s, red + (LANES ? 0 : 16));
   const float tau = 1.f / sqrtf(s[0] * inv + k.eps);
 #pragma unroll
   for (int m = 0; m < NV; ++m) {
@@ -158,7 +184,7 @@ __global__ __launch_bounds__(ONE ? 64 * kOneRows : 1024) void gate_norm_fwd_kern
     load_part(k.pre, i, left, pre);
 #pragma unroll
     for (int c = 0; c < 4; ++c) x[m][c] *= tau * pre[c];
-    store_part(k.n + base, i, left, x[m]);
+    store_part<STREAM>(k.n + base, i, left, x[m]);
   }
   if (k.stats && t == 0) {
     k.stats[2 * row] = rho;
@@ -167,14 +193,17 @@ __global__ __launch_bounds__(ONE ? 64 * kOneRows : 1024) void gate_norm_fwd_kern
 }
 
 // Teams walk rows (their number, + teams, ..) and keep the weights' sums in registers.
-template <typename T, int NV, bool ONE>
-__global__ __launch_bounds__(ONE ? 64 * kOneRows : 1024) void gate_norm_bwd_kernel(GateNormArgs<T> k) {
-  __shared__ float red[2][ONE ? 1 : 48];
-  __shared__ float fold[ONE ? kOneRows - 1 : 1][ONE ? 3 * NV * 256 : 1];
-  const int team = ONE ? 64 : blockDim.x, t = ONE ? threadIdx.x & 63 : threadIdx.x;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), d = (int)k.d;
+template <typename T, int NV, int LANES>
+__global__ __launch_bounds__(LANES ? 256 : 1024) void gate_norm_bwd_kernel(GateNormArgs<T> k) {
+  __shared__ float red[2][LANES ? 1 : 48];
+  __shared__ float fold[LANES ? kTeams<LANES> - 1 : 1][LANES ? 12 * NV : 1][LANES ? LANES : 1];
+  // The weights' sums: in registers, or where 1024 threads have too few, in LDS.
+  constexpr bool IN_LDS = NV > 1;
+  __shared__ float held[IN_LDS ? 3 * NV * 4 : 1][IN_LDS ? 1024 : 1];
+  const int team = LANES ? LANES : blockDim.x, t = LANES ? threadIdx.x % team : threadIdx.x;
+  const int number = team_number<LANES>(), d = (int)k.d;
   const float inv = 1.f / (float)k.d;
-  float sum[3][NV][4], sc[NV][4], po[NV][4], pre[NV][4];
+  float sum[3][IN_LDS ? 1 : NV][4], sc[NV][4], po[NV][4], pre[NV][4];
   const auto weights = [&] {
 #pragma unroll
     for (int m = 0; m < NV; ++m) {
@@ -189,28 +218,64 @@ __global__ __launch_bounds__(ONE ? 64 * kOneRows : 1024) void gate_norm_bwd_kern
   };
   if constexpr (NV == 1) weights();
 #pragma unroll
-  for (int m = 0; m < NV; ++m)
+  for (int j = 0; j < 3; ++j)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) sum[0][m][c] = sum[1][m][c] = sum[2][m][c] = 0.f;
-  const int64_t first = ONE ? (int64_t)blockIdx.x * kOneRows + wave : blockIdx.x;
-  const int64_t step = ONE ? (int64_t)gridDim.x * kOneRows : gridDim.x;
+    for (int m = 0; m < NV; ++m)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if constexpr (IN_LDS) held[(j * NV + m) * 4 + c][t] = 0.f;
+        else sum[j][m][c] = 0.f;
+      }
+  const auto add = [&](int j, int m, int c, float a, float b) {
+    if constexpr (IN_LDS) {
+      float& at = held[(j * NV + m) * 4 + c][t];
+      at = fmaf(a, b, at);
+    } else {
+      sum[j][m][c] = fmaf(a, b, sum[j][m][c]);
+    }
+  };
+  const int64_t first = (int64_t)blockIdx.x * kTeams<LANES> + number;
+  const int64_t step = (int64_t)gridDim.x * kTeams<LANES>;
   int flip = 0;  // two sets of sums: one barrier a row is enough
+  // A row's loads go out while the row before is worked on (workgroups are few: each writes its sums),
+  // where the registers are there for it.
+  constexpr bool AHEAD = NV == 1;
+  Quad<T> raw[5][AHEAD ? NV : 1];
+  float rho = 1.f, tau = 1.f;
+  const auto fetch = [&](int64_t row, int m, int to) {
+    const int64_t base = row * k.d;
+    const uint32_t i = 4 * (t + m * team);
+    const int left = d - (int)i;
+    raw[0][to] = load_quad(k.x + base, i, left);
+    raw[1][to] = load_quad(k.y + base, i, left);
+    if (k.z) raw[2][to] = load_quad(k.z + row * k.z_row, i, left);
+    if (k.dout) raw[3][to] = load_quad(k.dout + base, i, left);
+    if (k.dn) raw[4][to] = load_quad(k.dn + base, i, left);
+  };
+  const auto ahead = [&](int64_t row) {
+    if (!AHEAD || row >= k.rows) return;
+    rho = k.stats[2 * row], tau = k.stats[2 * row + 1];
+#pragma unroll
+    for (int m = 0; m < NV; ++m) fetch(row, m, AHEAD ? m : 0);
+  };
+  ahead(first);
   for (int64_t row = first; row < k.rows; row += step, flip ^= 1) {
     const int64_t base = row * k.d;
-    const float rho = k.stats[2 * row], tau = k.stats[2 * row + 1];
+    const float rho_now = AHEAD ? rho : k.stats[2 * row], tau_now = AHEAD ? tau : k.stats[2 * row + 1];
     float o[NV][4], v[NV][4], sg[NV][4], cg[NV][4], dn[NV][4], g[NV][4];
     float s[3] = {0.f, 0.f, 0.f};
     if constexpr (NV > 1) weights();
 #pragma unroll
     for (int m = 0; m < NV; ++m) {
-      const uint32_t i = 4 * (t + m * team);
-      const int left = d - (int)i;
-      load_part(k.x + base, i, left, o[m]);
-      load_part(k.y + base, i, left, v[m]);
-      if (k.z) load_part(k.z + row * k.z_row, i, left, sg[m]);
-      if (k.dout) load_part(k.dout + base, i, left, g[m]);
-      if (k.dn) load_part(k.dn + base, i, left, dn[m]);
+      const int at = AHEAD ? m : 0;
+      if (!AHEAD) fetch(row, m, at);
+      unpack_quad<T>(raw[0][at], o[m]);
+      unpack_quad<T>(raw[1][at], v[m]);
+      if (k.z) unpack_quad<T>(raw[2][at], sg[m]);
+      if (k.dout) unpack_quad<T>(raw[3][at], g[m]);
+      if (k.dn) unpack_quad<T>(raw[4][at], dn[m]);
     }
+    ahead(row + step);
 #pragma unroll
     for (int m = 0; m < NV; ++m)
 #pragma unroll
@@ -221,18 +286,18 @@ __global__ __launch_bounds__(ONE ? 64 * kOneRows : 1024) void gate_norm_bwd_kern
           sigmoid_pair(sg[m][c], sg[m][c], cg[m][c]);
           v[m][c] *= sg[m][c];
         }
-        o[m][c] = fmaf(sc[m][c], v[m][c] * rho * po[m][c], o[m][c]);
+        o[m][c] = fmaf(sc[m][c], v[m][c] * rho_now * po[m][c], o[m][c]);
         const float u = dn[m][c] * pre[m][c], wv = sc[m][c] * po[m][c] * v[m][c];
-        g[m][c] = fmaf(tau, u, g[m][c]);
-        sum[1][m][c] = fmaf(dn[m][c] * tau, o[m][c], sum[1][m][c]);
+        g[m][c] = fmaf(tau_now, u, g[m][c]);
+        add(1, m, c, dn[m][c] * tau_now, o[m][c]);
         s[0] = fmaf(u, o[m][c], s[0]);
         s[1] = fmaf(wv, g[m][c], s[1]);
         s[2] = fmaf(wv, o[m][c], s[2]);
       }
-    team_sum<ONE>(s, red[flip]);
+    team_sum<LANES>(s, red[flip]);
     if constexpr (NV > 1) weights();  // not held meanwhile, nor z's gates: a lane has 128 registers
-    const float back = tau * tau * tau * s[0] * inv;
-    const float side = k.post ? rho * rho * rho * inv * (s[1] - back * s[2]) : 0.f;
+    const float back = tau_now * tau_now * tau_now * s[0] * inv;
+    const float side = k.post ? rho_now * rho_now * rho_now * inv * (s[1] - back * s[2]) : 0.f;
 #pragma unroll
     for (int m = 0; m < NV; ++m) {
       const uint32_t i = 4 * (t + m * team);
@@ -247,11 +312,11 @@ __global__ __launch_bounds__(ONE ? 64 * kOneRows : 1024) void gate_norm_bwd_kern
       }
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const float O = fmaf(-back, o[m][c], g[m][c]), vr = v[m][c] * rho;
-        sum[0][m][c] = fmaf(O, vr * po[m][c], sum[0][m][c]);
-        sum[2][m][c] = fmaf(sc[m][c] * O, vr, sum[2][m][c]);
+        const float O = fmaf(-back, o[m][c], g[m][c]), vr = v[m][c] * rho_now;
+        add(0, m, c, O, vr * po[m][c]);
+        add(2, m, c, sc[m][c] * O, vr);
         g[m][c] = O;
-        const float dv = fmaf(rho * sc[m][c] * po[m][c], O, -side * v[m][c]);
+        const float dv = fmaf(rho_now * sc[m][c] * po[m][c], O, -side * v[m][c]);
         dy[c] = k.z ? dv * sg[m][c] : dv;
         dz[c] = k.z ? dv * v[m][c] * cg[m][c] : 0.f;
       }
@@ -260,69 +325,90 @@ __global__ __launch_bounds__(ONE ? 64 * kOneRows : 1024) void gate_norm_bwd_kern
       if (k.z) store_part(k.dz + base, i, left, dz);
     }
   }
-  if constexpr (ONE) {  // the workgroup's waves into its first
-    if (wave > 0) {
+  if constexpr (LANES > 0) {  // the workgroup's teams into its first, in order
+    if (number > 0) {
 #pragma unroll
       for (int j = 0; j < 3; ++j)
 #pragma unroll
         for (int m = 0; m < NV; ++m)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) fold[wave - 1][((j * NV + m) * 4 + c) * 64 + t] = sum[j][m][c];
+          for (int c = 0; c < 4; ++c) fold[number - 1][(j * NV + m) * 4 + c][t] = sum[j][m][c];
     }
     __syncthreads();
-    if (wave > 0) return;
-#pragma unroll
-    for (int w = 0; w < kOneRows - 1; ++w)
+    if (number > 0) return;
+#pragma unroll 1
+    for (int w = 0; w < kTeams<LANES> - 1; ++w)
 #pragma unroll
       for (int j = 0; j < 3; ++j)
 #pragma unroll
         for (int m = 0; m < NV; ++m)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) sum[j][m][c] += fold[w][((j * NV + m) * 4 + c) * 64 + t];
+          for (int c = 0; c < 4; ++c) sum[j][m][c] += fold[w][(j * NV + m) * 4 + c][t];
   }
 #pragma unroll
   for (int j = 0; j < 3; ++j)
 #pragma unroll
     for (int m = 0; m < NV; ++m) {
       const uint32_t i = 4 * (t + m * team);
-      store_part(k.part + ((int64_t)j * gridDim.x + blockIdx.x) * k.d, i, d - (int)i, sum[j][m]);
+      if constexpr (IN_LDS) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sum[j][0][c] = held[(j * NV + m) * 4 + c][t];
+      }
+      store_part(k.part + ((int64_t)j * gridDim.x + blockIdx.x) * k.d, i, d - (int)i, sum[j][IN_LDS ? 0 : m]);
     }
 }
 
 constexpr int64_t kGateNormMaxWidth = 8192;
 
+// A backward's workgroups: as many as run at once (16 waves a CU, by their registers), so that all of
+// them walk about as many rows, and no more, since each writes 12 d bytes of sums.
+inline int64_t gate_norm_bwd_teams(int64_t d) { return d <= 64 ? 16 : d <= 128 ? 8 : d <= 256 ? 4 : 1; }
+inline int64_t gate_norm_bwd_waves(int64_t d) {
+  return d <= 256 ? 4 : d <= 4096 ? (d + 255) / 256 : (d + 511) / 512;
+}
 inline int64_t gate_norm_bwd_blocks(int64_t rows, int64_t d) {
-  const int64_t need = d <= 256 ? (rows + kOneRows - 1) / kOneRows : rows;
-  return need < 512 ? need : 512;
+  const int64_t teams = gate_norm_bwd_teams(d), need = (rows + teams - 1) / teams;
+  const int64_t most = 256 * (16 / gate_norm_bwd_waves(d));
+  const int64_t each = (need + most - 1) / most;
+  return (need + each - 1) / each;
 }
 
+// STREAM: stores that leave no copy in the caches, where x, y, z, out and n are more than the 256 MiB
+// of the last of them: 32768 x 1024 in fp16 (320 MiB) 51 us against 74, 32768 x 512 30 and 31; below,
+// the next product finds n in the cache.
+template <typename T, bool STREAM>
+int launch_gate_norm_rows(const GateNormArgs<T>& k, hipStream_t s) {
+#define MQC_GN(NV, LANES)                                                                       \
+  gate_norm_fwd_kernel<T, NV, LANES, STREAM>                                                    \
+      <<<dim3((unsigned)((k.rows + kTeams<LANES> - 1) / kTeams<LANES>)),                        \
+         dim3(LANES ? 256 : 64 * (unsigned)((k.d + 1023) / 1024)), 0, s>>>(k);                  \
+  return launch_status();
+  if (k.d <= 64) { MQC_GN(1, 16) }
+  if (k.d <= 128) { MQC_GN(1, 32) }
+  if (k.d <= 256) { MQC_GN(1, 64) }
+  if (k.d <= 512) { MQC_GN(2, 64) }
+  if (k.d <= 768) { MQC_GN(3, 64) }
+  if (k.d <= 1024) { MQC_GN(4, 64) }
+  MQC_GN(4, 0)
+#undef MQC_GN
+}
 template <typename T>
 int launch_gate_norm_fwd(const GateNormArgs<T>& k, hipStream_t s) {
-#define MQC_GN(NV, ONE, BLOCKS, WAVES)                                                           \
-  gate_norm_fwd_kernel<T, NV, ONE><<<dim3((unsigned)(BLOCKS)), dim3(64 * (WAVES)), 0, s>>>(k);   \
-  return launch_status();
-  const int64_t four = (k.rows + kOneRows - 1) / kOneRows;
-  if (k.d <= 256) { MQC_GN(1, true, four, kOneRows) }
-  if (k.d <= 512) { MQC_GN(2, true, four, kOneRows) }
-  if (k.d <= 768) { MQC_GN(3, true, four, kOneRows) }
-  if (k.d <= 1024) { MQC_GN(4, true, four, kOneRows) }
-  MQC_GN(4, false, k.rows, (k.d + 1023) / 1024)
-#undef MQC_GN
+  const int64_t bytes = k.rows * k.d * (int64_t)sizeof(T) * (k.z ? 5 : 4);
+  return bytes > (256LL << 20) ? launch_gate_norm_rows<T, true>(k, s) : launch_gate_norm_rows<T, false>(k, s);
 }
 
 template <typename T>
 int launch_gate_norm_bwd(const GateNormArgs<T>& k, float* dscale, float* dpre, float* dpost,
                          hipStream_t s) {
-  const int64_t blocks = gate_norm_bwd_blocks(k.rows, k.d);
-#define MQC_GN(NV, ONE, WAVES) \
-  gate_norm_bwd_kernel<T, NV, ONE><<<dim3((unsigned)blocks), dim3(64 * (WAVES)), 0, s>>>(k);
-  if (k.d <= 256) {
-    MQC_GN(1, true, kOneRows)
-  } else if (k.d <= 4096) {
-    MQC_GN(1, false, (k.d + 255) / 256)
-  } else {
-    MQC_GN(2, false, (k.d + 511) / 512)
-  }
+  const int64_t blocks = gate_norm_bwd_blocks(k.rows, k.d), waves = gate_norm_bwd_waves(k.d);
+#define MQC_GN(NV, LANES) \
+  gate_norm_bwd_kernel<T, NV, LANES><<<dim3((unsigned)blocks), dim3(64 * (unsigned)waves), 0, s>>>(k);
+  if (k.d <= 64) { MQC_GN(1, 16) }
+  else if (k.d <= 128) { MQC_GN(1, 32) }
+  else if (k.d <= 256) { MQC_GN(1, 64) }
+  else if (k.d <= 4096) { MQC_GN(1, 0) }
+  else { MQC_GN(2, 0) }
 #undef MQC_GN
   const int st = launch_status();
   if (st != MQC_OK) return st;
