@@ -83,7 +83,7 @@ variable_list once(const char* name, variable_list grads) {
   for (auto& g : grads)
     if (g.defined()) {
       const auto node = std::make_shared<torch::autograd::DelayedError>(message, 1);
-      g = (*node)({g})[0];
+      g = (*node)({g.detach().requires_grad_()})[0];
     }
   return grads;
 }

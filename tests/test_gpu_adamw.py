@@ -379,3 +379,59 @@ def test_block_trains(bits):
         opt.step()
         losses.append(loss.item())
     assert losses[-1] < 0.9 * losses[0]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_many_tensors(bits):
+    """More tensors than one launch's table, of the step (88, with 8-bit states 60) and the norm (160)."""
+    sizes = [3 + 7 * i for i in range(200)]
+    ps, gs, ms, vs = tensors(sizes, [torch.float32, torch.bfloat16])
+    old = [p.clone() for p in ps]
+    if bits == 32:
+        norm = adamw_step_(ps, gs, [m.clone() for m in ms], [v.clone() for v in vs], step=7,
+                           max_norm=0.5, **HOW)
+    else:
+        m8, r8 = [encoded(m) for m in ms], [encoded(v.sqrt()) for v in vs]
+        ms, vs = [decoded(*t) for t in m8], [decoded(*t) ** 2 for t in r8]
+        norm = adamw8_step_(ps, gs, [c for c, _ in m8], [s for _, s in m8], [c for c, _ in r8],
+                            [s for _, s in r8], step=7, max_norm=0.5, **HOW)
+    total = math.sqrt(sum(g.double().square().sum().item() for g in gs))
+    assert abs(norm.item() - total) <= 2.0 ** -23 * total
+    clip = min(1.0, 0.5 / (total + 1e-6))
+    for p, p0, g, m, v in zip(ps, old, gs, ms, vs):
+        want, m1, _, update = formula(p0, g, m, v, 7, clip, **HOW)
+        spread = update.abs() * (0.9 * m.abs() + 0.1 * g.abs() * clip) / m1.abs().clamp_min(1e-30)
+        hold_p(p, want, update.abs() + spread)
+
+
+def test_more_than_the_caches_hold():
+    """States and parameters stored past the caches (over 256 MiB in all)."""
+    ps, gs, ms, vs = tensors([17_000_003], [torch.float32])
+    want, m, v, update = formula(ps[0], gs[0], ms[0], vs[0], 7, **HOW)
+    spread = update.abs() * (0.9 * ms[0].abs() + 0.1 * gs[0].abs()) / m.abs().clamp_min(1e-30)
+    adamw_step_(ps, gs, ms, vs, step=7, **HOW)
+    hold_p(ps[0], want, update.abs() + spread)
+    assert ((vs[0].double() - v).abs() <= 2.0 ** -21 * v + 1e-44).all()
+
+
+@pytest.mark.parametrize("scale", [1e-25, 1e-12, 1.0, 1e12, 1e18])
+def test_8_bit_states_of_any_size(scale):
+    """Values at which a square underflows or overflows, beside ordinary blocks: the same codes as the
+    formula's neighbours, and parameters that follow it."""
+    n = 1024
+    gen = torch.Generator(DEV).manual_seed(3)
+    g = torch.randn(n, generator=gen, device=DEV)
+    g[256:512] *= scale
+    p = torch.zeros(n, device=DEV)
+    (m, a), (r, b) = encoded(torch.zeros(n, device=DEV)), encoded(torch.zeros(n, device=DEV))
+    adamw8_step_([p], [g], [m], [a], [r], [b], step=1, lr=1e-2, betas=(0.9, 0.95), weight_decay=0.0)
+    g64 = g.double()
+    for value, code, sc in ((0.1 * g64, m, a), ((0.05 * (g * g).double()).sqrt(), r, b)):
+        x = value / sc.double().repeat_interleave(256)
+        low, high = neighbours(x * (1 - 2.0 ** -20))[0], neighbours(x * (1 + 2.0 ** -20))[1]
+        got = code.double()
+        assert ((got.abs() >= low) & (got.abs() <= high) | (got == 2.0 ** -9) & (x > 0)).all()
+    big = (g * g) >= 2.0 ** -120
+    step = 1e-2 * g64 / (((g * g).double()).sqrt() + 1e-8)
+    assert ((p.double() + step).abs() <= 2.0 ** -18 * 1e-2)[big].all()
+    assert p.isfinite().all()

@@ -259,3 +259,28 @@ def test_registered_operators(gate, post):
     for a, b in zip(torch.autograd.grad([out, n], some, [dout, dn]),
                     torch.autograd.grad(want, some, [dout, dn])):
         assert torch.equal(a, b)
+
+
+def test_more_than_the_caches_hold():
+    """Outputs stored past the caches (over 256 MiB in all)."""
+    v, _, _ = make((14000, 1026), torch.float32)
+    ref = formula(*v.values())
+    with torch.no_grad():
+        for name, got in zip(("out", "n"), call(v)):
+            hold(name, got, ref[name])
+
+
+def test_second_gradients_are_refused():
+    v, dout, _ = make((4, 30), torch.float32)
+    x = v["x"].requires_grad_()
+    dx, = torch.autograd.grad(call(v)[0], x, dout, create_graph=True)
+    with pytest.raises(RuntimeError, match="gradient of the gradient"):
+        dx.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("rows,d", [(1, 16), (17, 63), (33, 64), (70, 66), (9, 127), (31, 128), (5, 129),
+                                    (20000, 30), (9000, 110)])
+def test_narrow_rows(dtype, rows, d):
+    """Teams of 16, 32 and 64 lanes, their last ones without a row."""
+    check(*make((rows, d), dtype))

@@ -340,3 +340,91 @@ def test_compiled_operators():
     y2 = torch.ops.mambaqc.gated_scan_train(*leaves, cut)[0]
     for u, v in zip(torch.autograd.grad(y2, leaves, dy), torch.autograd.grad(y1, leaves, dy)):
         assert torch.equal(u, v)
+
+
+# The spans, chunks and groups of chunks that the walks are cut into (forward 16, 128 and 2048 steps,
+# backward 16, 64 and 1024), each one short, full and one over.
+@pytest.mark.parametrize("t", [15, 16, 17, 63, 64, 65, 127, 128, 1023, 1024, 1025, 2047, 2048, 2049, 5000])
+@pytest.mark.parametrize("reset", [0.0, 0.01])
+def test_around_spans_chunks_and_groups(t, reset):
+    dt, g, x, lam, h0, cut, dy, dh = make(2, t, 37, torch.float32, reset=reset)
+    ref = walk(dt, g, x, lam, h0, cut, dy, dh)
+    leaves = [v.requires_grad_() for v in (dt, g, x, lam, h0)]
+    y, h = gated_scan(*leaves[:4], h0=h0, reset=cut, return_state=True)
+    hold("y", y, ref["y"])
+    hold("h", h, ref["h"])
+    for name, got in zip(["dt", "g", "x", "rate", "h0"], torch.autograd.grad([y, h], leaves, [dy, dh])):
+        hold(name, got, ref[name])
+
+
+@pytest.mark.parametrize("at", [0, 15, 16, 63, 64, 127, 128, 2047, 2048])
+def test_reset_at_the_ends_of_chunks(at):
+    dt, g, x, lam, h0, _, dy, dh = make(1, 2200, 66, torch.float32)
+    cut = torch.zeros(1, 2200, dtype=torch.bool, device=DEV)
+    cut[0, at] = True
+    ref = walk(dt, g, x, lam, h0, cut, dy, dh)
+    leaves = [v.requires_grad_() for v in (dt, g, x, lam, h0)]
+    y, h = gated_scan(*leaves[:4], h0=h0, reset=cut, return_state=True)
+    hold("y", y, ref["y"])
+    for name, got in zip(["dt", "g", "x", "rate", "h0"], torch.autograd.grad([y, h], leaves, [dy, dh])):
+        hold(name, got, ref[name])
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_nan_goes_through_all_chunks(bad):
+    """States that are not finite pass from chunk to chunk like others, in their channel alone."""
+    dt, g, x, lam, h0, _, dy, dh = make(1, 4500, 70, torch.float32)
+    x[0, 130, 9] = bad
+    leaves = [v.requires_grad_() for v in (dt, g, x)]
+    y, h = gated_scan(*leaves, lam, h0=h0, return_state=True)
+    others = [i for i in range(70) if i != 9]
+    assert not y[0, 130:, 9].isfinite().any() and y[0, :130].isfinite().all()
+    assert y[0][:, others].isfinite().all() and not h[0, 9].isfinite()
+    dy[0, 4000, 11] = bad
+    for v in torch.autograd.grad([y, h], leaves, [dy, dh]):
+        assert v[0][:, [i for i in others if i != 11]].isfinite().all()
+        assert v[0, 4001:, 11].isfinite().all() and not v[0, 3999, 11].isfinite()
+
+
+def test_last_state_may_be_the_first():
+    """The C entry point with h_last = h0, over several chunks and within one."""
+    from mambaqc_amd import _native as nat
+
+    for t in (1, 100, 2500):
+        dt, g, x, lam, h0, _, _, _ = make(2, t, 100, torch.float32)
+        ref = walk(dt, g, x, lam, h0, None)
+        y, h = torch.empty_like(x), h0.clone()
+        nbytes = nat.load().mqc_gated_scan_workspace_bytes(2, t, 100)
+        ws = torch.empty(nbytes, device=DEV, dtype=torch.uint8)
+        nat.call("mqc_gated_scan_fwd", x, dt.data_ptr(), 100, g.data_ptr(), 100, x.data_ptr(), 100,
+                 lam.data_ptr(), h.data_ptr(), None, y.data_ptr(), h.data_ptr(), None, 2, t, 100, 0,
+                 ws.data_ptr(), nbytes, nat.stream_of(x))
+        hold("y", y, ref["y"])
+        hold("h", h, ref["h"])
+
+
+def test_fast_channels_underflow_cleanly():
+    """Gradients that reach back through decays of 2^-100 and less of a state: exact to the gates' error,
+    then 0, and never NaN."""
+    t, d = 300, 64
+    dt = torch.zeros(1, t, d, device=DEV)
+    g, x = torch.zeros_like(dt), torch.ones_like(dt)
+    lam = torch.linspace(-3, 12, d, device=DEV)
+    leaves = [v.requires_grad_() for v in (dt, g, x, lam)]
+    y, h = gated_scan(*leaves, return_state=True)
+    dh = torch.ones(1, d, device=DEV)
+    ref = walk(dt, g, x, lam, None, None, torch.zeros_like(x), dh)
+    for name, got in zip(["dt", "g", "x", "rate"], torch.autograd.grad(h, leaves, dh)):
+        assert got.isfinite().all()
+        want, mag = ref[name]
+        # A decay over n steps carries n gates' errors (2^-21 each) of its own.
+        n = torch.arange(t, 0, -1, device=DEV)[None, :, None] if got.dim() == 3 else t
+        assert ((got.double() - want).abs() <= (REL + n * 2.0 ** -21) * mag + 1e-37).all(), name
+
+
+def test_second_gradients_are_refused():
+    dt, g, x, lam, _, _, dy, _ = make(1, 20, 8, torch.float32)
+    x.requires_grad_()
+    dx, = torch.autograd.grad(gated_scan(dt, g, x, lam), x, dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="gradient of the gradient"):
+        dx.sum().backward()
