@@ -30,9 +30,9 @@ constexpr int kScanGroup = 16;   // chunks that are joined one by one (scan_entr
 static_assert(kScanWaves * kScanSteps % kScanChunk == 0 && kScanChunk % kScanSteps == 0, "stored states");
 
 // log2(1 + 2^v): what rounding 1 + e leaves of e is added to first order.
-__device__ inline float scan_softplus2(float v) {
-  const float e = __builtin_amdgcn_exp2f(-fabsf(v));
-  const float u = 1.f + e;
+__device__ inline float scan_softplus2(float v, float& e, float& u) {
+  e = __builtin_amdgcn_exp2f(-fabsf(v));
+  u = 1.f + e;
   return fmaf(e - (u - 1.f), 1.44269504f, fmaxf(v, 0.f) + __builtin_amdgcn_logf(u));
 }
 
@@ -50,13 +50,15 @@ __device__ inline float scan_slow(float p) {
 }
 __device__ inline float scan_code(float p, float& a) {
   a = __builtin_amdgcn_exp2f(-p);
-  return p < 1.f ? scan_slow(p) : -a;
+  const float w = scan_slow(p);  // (in every lane: a branch here keeps steps from overlapping)
+  return p < 1.f ? w : -a;
 }
 __device__ inline bool scan_fast(float c) { return __float_as_int(c) < 0; }  // c is -a
 __device__ inline float scan_a(float c) { return scan_fast(c) ? -c : 1.f - c; }
 __device__ inline float scan_w(float c) { return scan_fast(c) ? 1.f + c : c; }
-// a v, and a h + (1 - a) s.
-__device__ inline float scan_fade(float c, float v) { return scan_fast(c) ? -c * v : fmaf(-c, v, v); }
+// a v, (1 - a) v, and a h + (1 - a) s.
+__device__ inline float scan_fade(float c, float v) { return fmaf(-c, v, scan_fast(c) ? 0.f : v); }
+__device__ inline float scan_gain(float c, float v) { return fmaf(c, v, scan_fast(c) ? v : 0.f); }
 __device__ inline float scan_step(float c, float s, float h) {
   return fmaf(c, s - h, scan_fast(c) ? s : h);
 }
@@ -68,7 +70,17 @@ __device__ inline ScanRate scan_rate(float log_rate) {
   return {log_rate * kLog2e, r > 3e38f ? 3e38f : r};  // (a gradient times the rate is then 0, not NaN)
 }
 // p of a step. Below dt = -80, where exp(dt) alone would underflow, from the sum of the logarithms.
-__device__ inline float scan_p(float dt, ScanRate r) { return scan_softplus2(dt * kLog2e) * r.rate; }
+__device__ inline float scan_p(float dt, ScanRate r) {
+  float e, u;
+  return scan_softplus2(dt * kLog2e, e, u) * r.rate;
+}
+// And dp/ddt (natural) = rate sigmoid(dt).
+__device__ inline float scan_p(float dt, ScanRate r, float& slope) {
+  float e, u;
+  const float p = scan_softplus2(dt * kLog2e, e, u) * r.rate, s = __builtin_amdgcn_rcpf(u);
+  slope = (dt < 0.f ? e * s : s) * r.rate;
+  return p;
+}
 __device__ inline float scan_p_low(float dt, ScanRate r) {
   return __builtin_amdgcn_exp2f(fmaf(dt, kLog2e, r.log2_rate)) * kLog2e;
 }
@@ -83,7 +95,10 @@ __device__ inline float scan_join(float c, float u, float h) {
 }
 struct ScanDecay {
   float p = 0.f, a = 1.f;
-  __device__ float code() const { return p < 1.f ? scan_slow(p) : -a; }
+  __device__ float code() const {
+    const float w = scan_slow(p);
+    return p < 1.f ? w : -a;
+  }
 };
 // The same of joined codes.
 struct ScanJoint {
@@ -409,13 +424,11 @@ __global__ __launch_bounds__(64 * kBackWaves) void gated_scan_bwd_kernel(ScanArg
       const float x = io<T>::to_f32(raw[2][i]);
       dy[i] = io<T>::to_f32(raw[3][i]);
       low = fminf(low, dt);
-      float cg, cd;
+      float cg;
       sigmoid_pair(g, sg[i], cg);
-      sigmoid_pair(dt, sd[i], cd);
       e[i] = x * sg[i];
       q[i] = e[i] * cg;
-      sd[i] *= rate.rate;
-      ps[i] = scan_p(dt, rate);
+      ps[i] = scan_p(dt, rate, sd[i]);
     }
     if (__builtin_expect(__any(low < -80.f), 0)) {
       ScanRow<T> again(k.dt + row0 * k.dt_row + at.d0, k.dt_row);
@@ -485,7 +498,7 @@ __global__ __launch_bounds__(64 * kBackWaves) void gated_scan_bwd_kernel(ScanArg
       for (int i = kBackSteps - 1; i >= 0; --i)
         if (PLAIN || i < n) {
           const float G = dy[i] + A, aG = scan_fade(c[i], G);
-          const float dp = aG * e[i], ds = scan_w(c[i]) * G;
+          const float dp = aG * e[i], ds = scan_gain(c[i], G);
           ddt.store(off, dp * sd[i]);
           dg.store(off, ds * q[i]);
           dx.store(off, ds * sg[i]);
