@@ -243,11 +243,17 @@ struct ScanRow {
   __device__ void store(uint32_t off, float v) const {
     *(__attribute__((address_space(1))) Raw*)(at + off) = __builtin_bit_cast(Raw, io<T>::from_f32(v));
   }
-  __device__ void next() {
-    at += by;
+  __device__ void next(bool there = true) {  // (else the same row again)
+    at += there ? by : 0;
     asm volatile("" : "+s"(at));
   }
 };
+
+// Every VG steps the compiler may not mix with later ones: enough to overlap, and registers for three
+// workgroups a CU.
+__device__ inline void scan_pace(int i) {
+  if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+}
 
 // The resets of a span's steps as bits (bit i: step i).
 __device__ inline uint32_t scan_resets(const uint8_t* reset, int64_t row, int n) {
@@ -258,7 +264,7 @@ __device__ inline uint32_t scan_resets(const uint8_t* reset, int64_t row, int n)
 
 // Forward: a workgroup takes one chunk of 64 channels.
 template <typename T, bool CHAIN>
-__global__ __launch_bounds__(64 * kScanWaves) void gated_scan_fwd_kernel(ScanArgs<T> k, uint32_t tiles) {
+__global__ __launch_bounds__(64 * kScanWaves, 6) void gated_scan_fwd_kernel(ScanArgs<T> k, uint32_t tiles) {
   __shared__ float part[2][kScanWaves][64];  // c and u of each span
   __shared__ float words[CHAIN ? 2 : 1][kScanGroup][64], entry[64];
   __shared__ uint32_t place;
@@ -286,38 +292,46 @@ __global__ __launch_bounds__(64 * kScanWaves) void gated_scan_fwd_kernel(ScanArg
     T raw[3][kScanSteps];
 #pragma unroll
     for (int i = 0; i < kScanSteps; ++i) {
-      raw[0][i] = dts.load(off), raw[1][i] = gs.load(off), raw[2][i] = xs.load(off);
-      if (PLAIN || i + 1 < n) dts.next(), gs.next(), xs.next();
+      raw[0][i] = dts.load(off);
+      dts.next(PLAIN || i + 1 < n);
+    }
+#pragma unroll
+    for (int i = 0; i < kScanSteps; ++i) {
+      raw[1][i] = gs.load(off), raw[2][i] = xs.load(off);
+      gs.next(PLAIN || i + 1 < n), xs.next(PLAIN || i + 1 < n);
     }
     __builtin_amdgcn_sched_barrier(0);  // all loads first
     float low = 0.f;
 #pragma unroll
     for (int i = 0; i < kScanSteps; ++i) {
-      const float dt = io<T>::to_f32(raw[0][i]), g = io<T>::to_f32(raw[1][i]);
-      const float x = io<T>::to_f32(raw[2][i]);
+      const float dt = io<T>::to_f32(raw[0][i]);
       low = fminf(low, dt);
       c[i] = scan_p(dt, rate);
-      s[i] = x * __builtin_amdgcn_rcpf(1.f + __expf(-g));
+      scan_pace(i);
     }
     if (__builtin_expect(__any(low < -80.f), 0)) {
       ScanRow<T> again(k.dt + row0 * k.dt_row + at.d0, k.dt_row);
 #pragma unroll
       for (int i = 0; i < kScanSteps; ++i) {
         const float dt = io<T>::to_f32(again.load(off));
-        if (PLAIN || i + 1 < n) again.next();
+        again.next(PLAIN || i + 1 < n);
         if (dt < -80.f) c[i] = scan_p_low(dt, rate);
       }
     }
 #pragma unroll
-    for (int i = 0; i < kScanSteps; ++i)
-      if (PLAIN || i < n) {
-        if (!PLAIN && (cuts >> i & 1)) u = 0.f;
-        float a;
-        span.p += c[i];
-        c[i] = scan_code(c[i], a);
-        span.a *= a;
-        u = scan_step(c[i], s[i], u);
+    for (int i = 0; i < kScanSteps; ++i) {
+      s[i] = io<T>::to_f32(raw[2][i]) * __builtin_amdgcn_rcpf(1.f + __expf(-io<T>::to_f32(raw[1][i])));
+      if (!PLAIN) {
+        if (i >= n) c[i] = s[i] = 0.f;  // a step that changes nothing
+        if (cuts >> i & 1) u = 0.f;
       }
+      float a;
+      span.p += c[i];
+      c[i] = scan_code(c[i], a);
+      span.a *= a;
+      u = scan_step(c[i], s[i], u);
+      scan_pace(i);
+    }
   };
   const bool plain = n == kScanSteps && cuts == 0;
   if (plain) walk(std::true_type());
@@ -412,46 +426,53 @@ __global__ __launch_bounds__(64 * kBackWaves) void gated_scan_bwd_kernel(ScanArg
     T raw[4][kBackSteps];
 #pragma unroll
     for (int i = 0; i < kBackSteps; ++i) {
-      raw[0][i] = dts.load(off), raw[1][i] = gs.load(off), raw[2][i] = xs.load(off);
-      raw[3][i] = dys.load(off);
-      if (PLAIN || i + 1 < n) dts.next(), gs.next(), xs.next(), dys.next();
+      raw[0][i] = dts.load(off);
+      dts.next(PLAIN || i + 1 < n);
+    }
+#pragma unroll
+    for (int i = 0; i < kBackSteps; ++i) {
+      raw[1][i] = gs.load(off), raw[2][i] = xs.load(off), raw[3][i] = dys.load(off);
+      gs.next(PLAIN || i + 1 < n), xs.next(PLAIN || i + 1 < n), dys.next(PLAIN || i + 1 < n);
     }
     __builtin_amdgcn_sched_barrier(0);  // all loads first
     float low = 0.f;
 #pragma unroll
     for (int i = 0; i < kBackSteps; ++i) {
-      const float dt = io<T>::to_f32(raw[0][i]), g = io<T>::to_f32(raw[1][i]);
-      const float x = io<T>::to_f32(raw[2][i]);
-      dy[i] = io<T>::to_f32(raw[3][i]);
+      const float dt = io<T>::to_f32(raw[0][i]);
       low = fminf(low, dt);
-      float cg;
-      sigmoid_pair(g, sg[i], cg);
-      e[i] = x * sg[i];
-      q[i] = e[i] * cg;
       ps[i] = scan_p(dt, rate, sd[i]);
+      scan_pace(i);
     }
     if (__builtin_expect(__any(low < -80.f), 0)) {
       ScanRow<T> again(k.dt + row0 * k.dt_row + at.d0, k.dt_row);
 #pragma unroll
       for (int i = 0; i < kBackSteps; ++i) {
         const float dt = io<T>::to_f32(again.load(off));
-        if (PLAIN || i + 1 < n) again.next();
+        again.next(PLAIN || i + 1 < n);
         if (dt < -80.f) ps[i] = scan_p_low(dt, rate), sd[i] = ps[i] * kLn2;
       }
     }
 #pragma unroll
-    for (int i = 0; i < kBackSteps; ++i)
-      if (PLAIN || i < n) {
-        if (!PLAIN && (cuts >> i & 1)) u = 0.f;
-        float a;
-        span.p += ps[i];
-        c[i] = scan_code(ps[i], a);
-        span.a *= a;
-        u = scan_step(c[i], e[i], u);
+    for (int i = 0; i < kBackSteps; ++i) {
+      float cg;
+      sigmoid_pair(io<T>::to_f32(raw[1][i]), sg[i], cg);
+      e[i] = io<T>::to_f32(raw[2][i]) * sg[i];
+      q[i] = e[i] * cg;
+      dy[i] = io<T>::to_f32(raw[3][i]);
+      if (!PLAIN) {
+        if (i >= n) ps[i] = e[i] = dy[i] = 0.f;  // a step that changes nothing
+        if (cuts >> i & 1) u = 0.f;
       }
+      float a;
+      span.p += ps[i];
+      c[i] = scan_code(ps[i], a);
+      span.a *= a;
+      u = scan_step(c[i], e[i], u);
+      scan_pace(i);
+    }
 #pragma unroll
     for (int i = kBackSteps - 1; i >= 0; --i)
-      if (PLAIN || i < n) v = !PLAIN && (cuts >> i & 1) ? 0.f : scan_fade(c[i], dy[i] + v);
+      v = !PLAIN && (cuts >> i & 1) ? 0.f : scan_fade(c[i], dy[i] + v);
   };
   const bool all = n == kBackSteps && cuts == 0;
   if (all) walk(std::true_type());
