@@ -228,7 +228,8 @@ __device__ inline float scan_entry(const ScanArgs<T>& k, const ScanPlace& at, in
 }
 
 // A row that all lanes share, in two scalar registers, from which a lane reads or writes at its byte
-// offset. next() keeps it a running pointer: left alone, the compiler computes all rows' addresses
+// offset (made anew for each access: widened to 64 bits once for all, it costs a sum in every lane for
+// each). next() keeps it a running pointer: left alone, the compiler computes all rows' addresses
 // ahead and spills them.
 template <typename T>
 struct ScanRow {
@@ -238,9 +239,11 @@ struct ScanRow {
   int64_t by;
   __device__ ScanRow(const T* p, int64_t step) : at((Global)(char*)p), by(step * (int64_t)sizeof(T)) {}
   __device__ T load(uint32_t off) const {
+    asm("" : "+v"(off));
     return __builtin_bit_cast(T, *(__attribute__((address_space(1))) Raw*)(at + off));
   }
   __device__ void store(uint32_t off, float v) const {
+    asm("" : "+v"(off));
     *(__attribute__((address_space(1))) Raw*)(at + off) = __builtin_bit_cast(Raw, io<T>::from_f32(v));
   }
   __device__ void next(bool there = true) {  // (else the same row again)
@@ -249,7 +252,7 @@ struct ScanRow {
   }
 };
 
-// Every VG steps the compiler may not mix with later ones: enough to overlap, and registers for three
+// Every four steps the compiler may not mix with later ones: enough to overlap, and registers for three
 // workgroups a CU.
 __device__ inline void scan_pace(int i) {
   if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
