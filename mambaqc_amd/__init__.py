@@ -6,6 +6,7 @@ Drop-in for the reference package's hot path (polux06/mambaqc):
                         ssm_step_fused, ssm_forward_fused, quaternion_layer_norm_fused
   mambaqc_amd.layers    QuaternionLinear, QuaternionLayerNorm, CausalConv1d
   mambaqc_amd           QuaternionMamba2Block, QuaternionMamba2 (+ presets)
+  mambaqc_amd.optim     AdamW over many tensors, states in 32 or 8 bits
   torch.ops.mambaqc.*   the same kernels as registered torch operators with fake
                         kernels and autograd formulas (mambaqc_amd.ops)
 All compute of the quaternion path runs in libmambaqc_hip.so (hand-written

@@ -17,16 +17,24 @@ namespace mqc {
 // Time is cut into chunks, a chunk into one span of steps for each of its waves, and a lane walks one
 // channel of its wave's span: first from zero (u, its last state, and the sum of p, which give what the
 // span makes of any state before it), then, once the state before the span is known, through the
-// states themselves. The spans of a chunk join in LDS. Between chunks the state goes through memory
-// within the launch: see scan_entry.
-
-constexpr int kScanLanes = 64;   // channels of a workgroup
-constexpr int kScanWaves = 8;    // spans of a chunk, forward
-constexpr int kScanSteps = 16;   // steps of a span
-constexpr int kBackWaves = 4;    // and backward (whose steps take three times the registers)
+// states themselves: inputs are read once, and their gates computed once. The spans of a chunk join in
+// LDS. Between chunks the state goes through memory within the launch: see scan_entry.
+//
+// What bounds it: 8 bytes an element forward and 14 backward (bf16) against some 45 and 65 vector
+// instructions, so neither memory (a copy's 5.1 TB/s) nor arithmetic alone, but how well workgroups
+// overlap. bf16: a prompt of 16384 x 1536 56 us (201 MB, 3.6 TB/s; loads and stores alone 32, with LDS
+// and the words between chunks 38); 4 x 2048 x 1536 forward 29 us, backward 43 (176 MB, 4.1 TB/s).
+// Spans and waves, same prompt (two stages earlier, 61 us as here): 8 steps 72, 4 waves of 16 70, 4 of 32
+// 62, 16 waves of 8 72; backward of 4 x 2048 x 1536: 8 waves of 8 steps 53, 4 of 16 45, 4 of 32 65. Not
+// kept: workgroups that stay and load the next chunk ahead (61 to 82: they all wait for one another in
+// turn), spans walked for a guessed chunk while the counter answers (56 to 77: it guesses wrong).
+constexpr int kScanLanes = 64;  // channels of a workgroup
+constexpr int kScanWaves = 8;   // spans of a chunk, forward
+constexpr int kScanSteps = 16;  // steps of a span
+constexpr int kBackWaves = 4;   // and backward (whose steps take three times the registers)
 constexpr int kBackSteps = 16;
 constexpr int kScanChunk = kBackWaves * kBackSteps;  // steps between the states that training stores
-constexpr int kScanGroup = 16;   // chunks that are joined one by one (scan_entry)
+constexpr int kScanGroup = 16;  // chunks that are joined one by one (scan_entry)
 static_assert(kScanWaves * kScanSteps % kScanChunk == 0 && kScanChunk % kScanSteps == 0, "stored states");
 
 // log2(1 + 2^v): what rounding 1 + e leaves of e is added to first order.
@@ -38,8 +46,8 @@ __device__ inline float scan_softplus2(float v, float& e, float& u) {
 
 // A step's decay as one number c. A slow channel has a near 1 and forgets by 1 - a a token: rounding
 // a to fp32 would shift its rate, and with it the gain at rest, by 2^-25 / (1 - a). So c is 1 - a
-// while p < 1 (scan_slow: a minimax fit of (1 - 2^-p) / p on [0, 1], off by 2^-26.6, rounded by 2^-23), and -a
-// after that; the sign bit tells.
+// while p < 1 (scan_slow: a minimax fit of (1 - 2^-p) / p on [0, 1], off by 2^-26.6, rounded by 2^-23),
+// and -a after that; the sign bit tells.
 __device__ inline float scan_slow(float p) {
   float w = fmaf(p, -1.14580565e-4f, 1.29078003e-3f);
   w = fmaf(p, w, -9.5962761e-3f);
@@ -131,8 +139,8 @@ struct ScanArgs {
   float *drate, *dh0;  // drate: [batch, chunks, width]
   // the states between chunks (several of them)
   uint32_t* tickets;  // [batch, tiles of the width]
-  uint32_t* ends;   // [batch, groups, width]
-  uint64_t* spans;  // [batch, chunks, width]
+  uint32_t* ends;     // [batch, groups, width]
+  uint64_t* spans;    // [batch, chunks, width]
 };
 
 // ---------------------------------------------------------------------------
@@ -166,7 +174,8 @@ __global__ __launch_bounds__(256) void scan_clear_kernel(uint4* words, int64_t z
 struct ScanPlace { int64_t n, b, d0; };
 template <bool CHAIN>
 __device__ inline ScanPlace scan_place(uint32_t* tickets, int64_t width, uint32_t tiles, uint32_t* lds) {
-  const uint32_t across = (uint32_t)((width + kScanLanes - 1) / kScanLanes), tile = __builtin_amdgcn_readfirstlane(blockIdx.x % tiles);
+  const uint32_t across = (uint32_t)((width + kScanLanes - 1) / kScanLanes);
+  const uint32_t tile = __builtin_amdgcn_readfirstlane(blockIdx.x % tiles);
   uint32_t n = 0;
   if constexpr (CHAIN) {
     if (threadIdx.x == 0)
@@ -549,7 +558,8 @@ __global__ __launch_bounds__(64 * kBackWaves) void gated_scan_bwd_kernel(ScanArg
   }
 }
 
-// One token for each sequence, the state in place.
+// One token for each sequence, the state in place. 16 x 1536 in fp16 2.7 us, a launch's latency (7 with
+// the host).
 template <typename T>
 __global__ __launch_bounds__(256) void gated_scan_step_kernel(ScanArgs<T> k, float* h) {
   const int64_t d = (int64_t)blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
