@@ -59,6 +59,11 @@ Tensor as_type(const Tensor& t, at::ScalarType type) {
   const at::NoGradGuard none;
   return t.scalar_type() == type ? t.detach() : t.detach().to(type);
 }
+// The kernels write through pointers: tells autograd (and whatever keeps copies of parameters by their
+// version) that a tensor changed.
+void changed(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 Variable edge(const MaybeTensor& t) { return t ? *t : Variable(); }
 MaybeTensor maybe(const Variable& v) { return v.defined() ? MaybeTensor(v) : std::nullopt; }
 // The types that gradients are wanted in, -1 for none.
@@ -326,6 +331,7 @@ Tensor scan_step(const Scan& o, const Tensor& h) {
                             f32(o.rate), (float*)h.data_ptr(), y.data_ptr(), o.b(), o.d(),
                             dtype_code(o.x), stream_of(o.x)),
         "mqc_gated_scan_step");
+  changed(h);
   return y;
 }
 
@@ -374,12 +380,9 @@ std::optional<std::pair<py::bytes, py::bytes>> adam_rows(const Lists& lists, int
   return std::make_pair(bytes(rows), bytes(norm));
 }
 
-// The kernels write through pointers: tells autograd (and whatever keeps copies of parameters by their
-// version) that these tensors changed.
 void changed(const Lists& lists) {
   for (const auto& l : lists)
-    for (const auto& t : l)
-      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    for (const auto& t : l) changed(t);
 }
 
 }  // namespace
@@ -405,6 +408,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("scan_train", &scan_train);
   m.def("scan_step", &scan_step);
   m.def("adam_rows", &adam_rows);
-  m.def("changed", &changed);
+  m.def("changed", [](const Lists& lists) { changed(lists); });
   m.def("abi", [] { return (int64_t)mqc_abi_version(); });
 }

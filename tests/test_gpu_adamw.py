@@ -435,3 +435,28 @@ def test_8_bit_states_of_any_size(scale):
     step = 1e-2 * g64 / (((g * g).double()).sqrt() + 1e-8)
     assert ((p.double() + step).abs() <= 2.0 ** -18 * 1e-2)[big].all()
     assert p.isfinite().all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_offsets_past_32_bits(bits):
+    """Elements more than 2^31 into a tensor, its states' among them."""
+    n = 2 ** 31 + 1025
+    p = torch.zeros(n, device=DEV, dtype=torch.bfloat16)
+    g = torch.zeros_like(p)
+    at = torch.tensor([0, 2 ** 31 - 1, 2 ** 31, 2 ** 31 + 700, n - 1], device=DEV)
+    g[at] = 0.25
+    how = {"step": 1, "lr": 0.5, "betas": (0.9, 0.95), "weight_decay": 0.0}
+    if bits == 32:
+        m, v = torch.zeros(n, device=DEV), torch.zeros(n, device=DEV)
+        adamw_step_([p], [g], [m], [v], **how)
+        assert ((m[at] - 0.025).abs() < 1e-8).all() and int((m != 0).sum()) == 5
+    else:
+        c = [torch.zeros(n, device=DEV, dtype=torch.uint8).view(E4M3) for _ in range(2)]
+        s = [torch.ones(state_blocks(n), device=DEV) for _ in range(2)]
+        adamw8_step_([p], [g], [c[0]], [s[0]], [c[1]], [s[1]], **how)
+        for code, scale, want in ((c[0], s[0], 0.025), (c[1], s[1], 0.25 * 0.05 ** 0.5)):
+            got = code.view(torch.uint8)[at].view(E4M3).float() * scale[at // 256]
+            assert ((got - want).abs() <= want / 8).all()
+            assert int((code.view(torch.uint8) != 0).sum()) == 5
+    assert (p[at] == -0.5).all() and int((p != 0).sum()) == 5
+    assert abs(grad_norm([g]).item() - 0.25 * 5 ** 0.5) < 1e-6

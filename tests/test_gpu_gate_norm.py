@@ -284,3 +284,33 @@ def test_second_gradients_are_refused():
 def test_narrow_rows(dtype, rows, d):
     """Teams of 16, 32 and 64 lanes, their last ones without a row."""
     check(*make((rows, d), dtype))
+
+
+def test_offsets_past_32_bits():
+    """The last rows of tensors of more than 2^32 bytes equal those rows alone, bit for bit."""
+    rows, d = 2_200_000, 1000
+    r = lambda *s: torch.empty(*s, device=DEV, dtype=torch.bfloat16).normal_()
+    v = {"x": r(rows, d), "y": r(rows, d), "z": r(rows, d + 40)[:, 40:], "post": torch.ones(d, device=DEV),
+         "scale": torch.full((d,), 0.5, device=DEV), "pre": torch.ones(d, device=DEV)}
+    dout, dn = r(rows, d), r(rows, d)
+    end = {k: t[-50:] if t.dim() == 2 else t for k, t in v.items()}
+    results = []
+    for w, gs in ((v, [dout, dn]), (end, [dout[-50:], dn[-50:]])):
+        leaves = {k: t.detach().requires_grad_(k in "xyz") for k, t in w.items()}
+        outs = call(leaves)
+        results.append([*outs, *torch.autograd.grad(outs, [leaves[k] for k in "xyz"], gs)])
+    for a, b in zip(*results):
+        assert torch.equal(a[-50:], b)
+
+
+def test_compiles():
+    """Traced through the registered operators, with the same results."""
+    v, dout, dn = make((30, 70), torch.float32)
+    leaves = {k: t.detach().requires_grad_() for k, t in v.items()}
+    fn = lambda *t: call(dict(zip(v, t)))
+    want = fn(*leaves.values())
+    got = torch.compile(fn, backend="aot_eager", fullgraph=True)(*leaves.values())
+    some = list(leaves.values())
+    for a, b in zip([*got, *torch.autograd.grad(got, some, [dout, dn])],
+                    [*want, *torch.autograd.grad(want, some, [dout, dn])]):
+        assert torch.equal(a, b)

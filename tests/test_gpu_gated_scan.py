@@ -428,3 +428,45 @@ def test_second_gradients_are_refused():
     dx, = torch.autograd.grad(gated_scan(dt, g, x, lam), x, dy, create_graph=True)
     with pytest.raises(RuntimeError, match="gradient of the gradient"):
         dx.sum().backward()
+
+
+def test_offsets_past_32_bits():
+    """Rows more than 2^32 bytes into their tensors, read in place and written: what lies behind a reset
+    near the end equals that part alone (another cut into spans: each gate's error, not the same bits)."""
+    t, d, tail = 1_100_000, 1024, 700
+    wide = torch.empty(1, t, 3 * d, device=DEV, dtype=torch.bfloat16).normal_()
+    dt, g, x = wide.split(d, -1)
+    lam = torch.linspace(-6, 0, d, device=DEV)
+    cut = torch.zeros(1, t, dtype=torch.bool, device=DEV)
+    cut[0, t - tail] = True
+    end = [v[:, t - tail:].clone().requires_grad_() for v in (dt, g, x)]
+    leaves = [v.detach().requires_grad_() for v in (dt, g, x)]
+    y, h = gated_scan(*leaves, lam, reset=cut, return_state=True)
+    y1, h1 = gated_scan(*end, lam, return_state=True)
+    ref = walk(*end, lam, None, None, dy := torch.randn_like(y1), torch.ones_like(h1))
+    hold("y", y[:, t - tail:].detach(), ref["y"])
+    hold("h", h.detach(), ref["h"])
+    whole = torch.zeros_like(y)
+    whole[:, t - tail:] = dy
+    for name, got in zip(("dt", "g", "x"), torch.autograd.grad([y, h], leaves, [whole, torch.ones_like(h)])):
+        hold(name, got[:, t - tail:], ref[name])
+        assert (got[:, :t - tail] == 0).all()
+
+
+def test_compiles():
+    """Traced through the registered operators, with the same results."""
+    dt, g, x, lam, h0, cut, dy, _ = make(2, 150, 24, torch.float32, reset=0.02)
+    leaves = [v.requires_grad_() for v in (dt, g, x, lam, h0)]
+    fn = lambda *v: gated_scan(*v[:4], h0=v[4], reset=cut) * 2.0
+    want = fn(*leaves)
+    got = torch.compile(fn, backend="aot_eager", fullgraph=True)(*leaves)
+    assert torch.equal(got, want)
+    for a, b in zip(torch.autograd.grad(got, leaves, dy), torch.autograd.grad(want, leaves, dy)):
+        assert torch.equal(a, b)
+
+
+def test_step_tells_that_the_state_changed():
+    dt, g, x, lam, h0, _, _, _ = make(2, 1, 24, torch.float32)
+    version = h0._version
+    gated_scan_step_(dt, g, x, lam, h0)
+    assert h0._version > version
