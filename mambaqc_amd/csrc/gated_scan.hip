@@ -20,10 +20,10 @@ namespace mqc {
 // states themselves: inputs are read once, and their gates computed once. The spans of a chunk join in
 // LDS. Between chunks the state goes through memory within the launch: see scan_entry.
 //
-// What bounds it: 8 bytes an element forward and 14 backward (bf16) against some 45 and 65 vector
+// What bounds it: 8 bytes an element forward and 14 backward (bf16) against some 40 and 58 vector
 // instructions, so neither memory (a copy's 5.1 TB/s) nor arithmetic alone, but how well workgroups
-// overlap. bf16: a prompt of 16384 x 1536 56 us (201 MB, 3.6 TB/s; loads and stores alone 32, with LDS
-// and the words between chunks 38); 4 x 2048 x 1536 forward 29 us, backward 43 (176 MB, 4.1 TB/s).
+// overlap. bf16: a prompt of 16384 x 1536 55 us (201 MB, 3.7 TB/s; loads and stores alone 32, with LDS
+// and the words between chunks 38); 4 x 2048 x 1536 forward 28 us, backward 42 (176 MB, 4.2 TB/s).
 // Spans and waves, same prompt (two stages earlier, 61 us as here): 8 steps 72, 4 waves of 16 70, 4 of 32
 // 62, 16 waves of 8 72; backward of 4 x 2048 x 1536: 8 waves of 8 steps 53, 4 of 16 45, 4 of 32 65. Not
 // kept: workgroups that stay and load the next chunk ahead (61 to 82: they all wait for one another in
@@ -44,10 +44,7 @@ __device__ inline float scan_softplus2(float v, float& e, float& u) {
   return fmaf(e - (u - 1.f), 1.44269504f, fmaxf(v, 0.f) + __builtin_amdgcn_logf(u));
 }
 
-// A step's decay as one number c. A slow channel has a near 1 and forgets by 1 - a a token: rounding
-// a to fp32 would shift its rate, and with it the gain at rest, by 2^-25 / (1 - a). So c is 1 - a
-// while p < 1 (scan_slow: a minimax fit of (1 - 2^-p) / p on [0, 1], off by 2^-26.6, rounded by 2^-23),
-// and -a after that; the sign bit tells.
+// 1 - 2^-p for p up to 1, by a minimax fit of (1 - 2^-p) / p (off by 2^-26.6, rounded by 2^-23).
 __device__ inline float scan_slow(float p) {
   float w = fmaf(p, -1.14580565e-4f, 1.29078003e-3f);
   w = fmaf(p, w, -9.5962761e-3f);
@@ -56,20 +53,21 @@ __device__ inline float scan_slow(float p) {
   w = fmaf(p, w, 6.93147182e-1f);
   return p * w;
 }
-__device__ inline float scan_code(float p, float& a) {
+// A step's a and w = 1 - a, each to a few 2^-24 of itself.
+__device__ inline void scan_pair(float p, float& a, float& w) {
   a = __builtin_amdgcn_exp2f(-p);
-  const float w = scan_slow(p);  // (in every lane: a branch here keeps steps from overlapping)
-  return p < 1.f ? w : -a;
+  const float slow = scan_slow(p);  // (in every lane: a branch here keeps steps from overlapping)
+  w = p < 1.f ? slow : 1.f - a;
 }
+// A slow channel has a near 1 and forgets by 1 - a a token: an a rounded to fp32 shifts its rate, and
+// with it the gain at rest, by up to 2^-24 / (1 - a). A span's walk takes a as it is, which adds up over
+// 16 steps (2^-20); the decay of a span and of more is kept as one number, c = 1 - a where a is over a
+// half and -a otherwise; the sign bit tells.
 __device__ inline bool scan_fast(float c) { return __float_as_int(c) < 0; }  // c is -a
 __device__ inline float scan_a(float c) { return scan_fast(c) ? -c : 1.f - c; }
 __device__ inline float scan_w(float c) { return scan_fast(c) ? 1.f + c : c; }
-// a v, (1 - a) v, and a h + (1 - a) s.
+// a v.
 __device__ inline float scan_fade(float c, float v) { return fmaf(-c, v, scan_fast(c) ? 0.f : v); }
-__device__ inline float scan_gain(float c, float v) { return fmaf(c, v, scan_fast(c) ? v : 0.f); }
-__device__ inline float scan_step(float c, float s, float h) {
-  return fmaf(c, s - h, scan_fast(c) ? s : h);
-}
 
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 struct ScanRate { float log2_rate, rate; };
@@ -292,9 +290,9 @@ __global__ __launch_bounds__(64 * kScanWaves, 6) void gated_scan_fwd_kernel(Scan
   const int64_t t0 = at.n * chunk + wave * kScanSteps, row0 = b * k.seq + t0;
   const int n = k.seq - t0 < kScanSteps ? (k.seq > t0 ? (int)(k.seq - t0) : 0) : kScanSteps;
   const ScanRate rate = scan_rate(k.log_rate[dc]);
-  float c[kScanSteps], s[kScanSteps];
+  float a[kScanSteps], ws[kScanSteps];  // h = a h + ws; a is p at first
   const uint32_t cuts = scan_resets(k.reset, row0, n);
-  ScanDecay span;
+  ScanDecay decay;
   float u = 0.f;
   // PLAIN: all steps are there and none is a reset.
   const auto walk = [&](auto plain) {
@@ -318,7 +316,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 6) void gated_scan_fwd_kernel(Scan
     for (int i = 0; i < kScanSteps; ++i) {
       const float dt = io<T>::to_f32(raw[0][i]);
       low = fminf(low, dt);
-      c[i] = scan_p(dt, rate);
+      a[i] = scan_p(dt, rate);
       scan_pace(i);
     }
     if (__builtin_expect(__any(low < -80.f), 0)) {
@@ -327,28 +325,29 @@ __global__ __launch_bounds__(64 * kScanWaves, 6) void gated_scan_fwd_kernel(Scan
       for (int i = 0; i < kScanSteps; ++i) {
         const float dt = io<T>::to_f32(again.load(off));
         again.next(PLAIN || i + 1 < n);
-        if (dt < -80.f) c[i] = scan_p_low(dt, rate);
+        if (dt < -80.f) a[i] = scan_p_low(dt, rate);
       }
     }
 #pragma unroll
     for (int i = 0; i < kScanSteps; ++i) {
-      s[i] = io<T>::to_f32(raw[2][i]) * __builtin_amdgcn_rcpf(1.f + __expf(-io<T>::to_f32(raw[1][i])));
+      const float gate = __builtin_amdgcn_rcpf(1.f + __expf(-io<T>::to_f32(raw[1][i])));
+      float s = io<T>::to_f32(raw[2][i]) * gate, p = a[i], w;
       if (!PLAIN) {
-        if (i >= n) c[i] = s[i] = 0.f;  // a step that changes nothing
+        if (i >= n) p = s = 0.f;  // a step that changes nothing
         if (cuts >> i & 1) u = 0.f;
       }
-      float a;
-      span.p += c[i];
-      c[i] = scan_code(c[i], a);
-      span.a *= a;
-      u = scan_step(c[i], s[i], u);
+      scan_pair(p, a[i], w);
+      ws[i] = w * s;
+      decay.p += p;
+      decay.a *= a[i];
+      u = fmaf(a[i], u, ws[i]);
       scan_pace(i);
     }
   };
   const bool plain = n == kScanSteps && cuts == 0;
   if (plain) walk(std::true_type());
   else if (n > 0) walk(std::false_type());
-  part[0][wave][lane] = cuts ? kScanCut : span.code();
+  part[0][wave][lane] = cuts ? kScanCut : decay.code();
   part[1][wave][lane] = u;
   float h = 0.f;
   if (wave == 0 && at.n == 0) {
@@ -387,7 +386,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 6) void gated_scan_fwd_kernel(Scan
   if (plain) {
 #pragma unroll
     for (int i = 0; i < kScanSteps; ++i) {
-      h = scan_step(c[i], s[i], h);
+      h = fmaf(a[i], h, ws[i]);
       y.store(off, h);
       y.next();
     }
@@ -396,7 +395,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 6) void gated_scan_fwd_kernel(Scan
     for (int i = 0; i < kScanSteps; ++i)
       if (i < n) {
         if (cuts >> i & 1) h = 0.f;
-        h = scan_step(c[i], s[i], h);
+        h = fmaf(a[i], h, ws[i]);
         y.store(off, h);
         y.next();
       }
@@ -423,11 +422,11 @@ __global__ __launch_bounds__(64 * kBackWaves) void gated_scan_bwd_kernel(ScanArg
   const int64_t t0 = j * kScanChunk + wave * kBackSteps, row0 = b * k.seq + t0;
   const int n = k.seq - t0 < kBackSteps ? (k.seq > t0 ? (int)(k.seq - t0) : 0) : kBackSteps;
   const ScanRate rate = scan_rate(k.log_rate[dc]);
-  // c; s, later s - h; dy; sigmoid(g); s (1 - sigmoid(g)); dp/ddt = rate sigmoid(dt); p
-  float c[kBackSteps], e[kBackSteps], dy[kBackSteps], sg[kBackSteps], q[kBackSteps], sd[kBackSteps],
-      ps[kBackSteps];
+  // a; s, later s - h; dy; w = 1 - a; sigmoid(g); s (1 - sigmoid(g)); dp/ddt = rate sigmoid(dt); p
+  float a[kBackSteps], e[kBackSteps], dy[kBackSteps], w[kBackSteps], sg[kBackSteps], q[kBackSteps],
+      sd[kBackSteps], ps[kBackSteps];
   const uint32_t cuts = scan_resets(k.reset, row0, n);
-  ScanDecay span;
+  ScanDecay decay;
   float u = 0.f, v = 0.f;
   // PLAIN: all steps are there and none is a reset.
   const auto walk = [&](auto plain) {
@@ -475,21 +474,20 @@ __global__ __launch_bounds__(64 * kBackWaves) void gated_scan_bwd_kernel(ScanArg
         if (i >= n) ps[i] = e[i] = dy[i] = 0.f;  // a step that changes nothing
         if (cuts >> i & 1) u = 0.f;
       }
-      float a;
-      span.p += ps[i];
-      c[i] = scan_code(ps[i], a);
-      span.a *= a;
-      u = scan_step(c[i], e[i], u);
+      scan_pair(ps[i], a[i], w[i]);
+      decay.p += ps[i];
+      decay.a *= a[i];
+      u = fmaf(a[i], u, w[i] * e[i]);
       scan_pace(i);
     }
 #pragma unroll
     for (int i = kBackSteps - 1; i >= 0; --i)
-      v = !PLAIN && (cuts >> i & 1) ? 0.f : scan_fade(c[i], dy[i] + v);
+      v = !PLAIN && (cuts >> i & 1) ? 0.f : a[i] * (dy[i] + v);
   };
   const bool all = n == kBackSteps && cuts == 0;
   if (all) walk(std::true_type());
   else if (n > 0) walk(std::false_type());
-  part[0][wave][lane] = cuts ? kScanCut : span.code();
+  part[0][wave][lane] = cuts ? kScanCut : decay.code();
   part[1][wave][lane] = u;
   part[2][wave][lane] = v;
   __syncthreads();
@@ -523,15 +521,15 @@ __global__ __launch_bounds__(64 * kBackWaves) void gated_scan_bwd_kernel(ScanArg
           if (!PLAIN && (cuts >> i & 1)) h = 0.f;
           const float s = e[i];
           e[i] = s - h;
-          h = scan_step(c[i], s, h);
+          h = fmaf(a[i], h, w[i] * s);
         }
       const int64_t to = (row0 + (PLAIN ? kBackSteps : n) - 1) * k.width + at.d0;
       ScanRow<T> ddt(k.ddt + to, -k.width), dg(k.dg + to, -k.width), dx(k.dx + to, -k.width);
 #pragma unroll
       for (int i = kBackSteps - 1; i >= 0; --i)
         if (PLAIN || i < n) {
-          const float G = dy[i] + A, aG = scan_fade(c[i], G);
-          const float dp = aG * e[i], ds = scan_gain(c[i], G);
+          const float G = dy[i] + A, aG = a[i] * G;
+          const float dp = aG * e[i], ds = w[i] * G;
           ddt.store(off, dp * sd[i]);
           dg.store(off, ds * q[i]);
           dx.store(off, ds * sg[i]);
@@ -567,9 +565,11 @@ __global__ __launch_bounds__(256) void gated_scan_step_kernel(ScanArgs<T> k, flo
   const float dt = load_scalar(k.dt + b * k.dt_row + d), g = load_scalar(k.g + b * k.g_row + d);
   const float s = load_scalar(k.x + b * k.x_row + d) * __builtin_amdgcn_rcpf(1.f + __expf(-g));
   const ScanRate rate = scan_rate(k.log_rate[d]);
-  float a;
-  const float c = scan_code(dt < -80.f ? scan_p_low(dt, rate) : scan_p(dt, rate), a);
-  const float v = scan_step(c, s, h[b * k.width + d]);
+  const float p = dt < -80.f ? scan_p_low(dt, rate) : scan_p(dt, rate), old = h[b * k.width + d];
+  float a, w;
+  scan_pair(p, a, w);
+  // Away from whichever is the larger part: an a near 1, rounded, would leave its mark at each token.
+  const float v = p < 1.f ? fmaf(w, s - old, old) : fmaf(a, old - s, s);
   h[b * k.width + d] = v;
   store_scalar(k.y + b * k.width + d, v);
 }
