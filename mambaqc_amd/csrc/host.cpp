@@ -371,7 +371,7 @@ std::optional<std::pair<py::bytes, py::bytes>> adam_rows(const Lists& lists, int
     for (const auto& l : lists) rows.push_back((int64_t)l[i].data_ptr());
     rows.push_back(n);
     rows.push_back(dtype_code(p));
-    if (eight) rows.push_back(seeds[i] & 0xffffffff);
+    if (eight) rows.push_back(seeds[i]);
     norm.insert(norm.end(), {(int64_t)g.data_ptr(), n, dtype_code(p)});
   }
   const auto bytes = [](const std::vector<int64_t>& v) {

@@ -143,7 +143,7 @@ def adamw8_step_(params, grads, exp_avgs, exp_avg_scales, root_avg_sqs, root_avg
     if not params:
         return None
     rows, norm_rows = _tables("adamw8_step_", params, grads, states, scales,
-                              range(seed, seed + len(params)))
+                              [(seed + i) & 0xFFFFFFFF for i in range(len(params))])
     norm, clip = (None, None) if max_norm is None else _norm_and_clip(norm_rows, max_norm, params[0])
     _launch8(rows, params, (*states, *scales), how, clip, step)
     return norm
@@ -214,7 +214,7 @@ class AdamW(torch.optim.Optimizer):
                     g = g.to(p.dtype)
                 s = self._state_of(p, group["state_bits"])
                 todo.setdefault((index, s["step"], "root_avg_sq" in s), []).append(
-                    (p.detach(), g, s, self.seed + place))
+                    (p.detach(), g, s, (self.seed + place) & 0xFFFFFFFF))
         if not todo:
             return loss
         work = []

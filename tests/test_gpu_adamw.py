@@ -460,3 +460,19 @@ def test_offsets_past_32_bits(bits):
             assert int((code.view(torch.uint8) != 0).sum()) == 5
     assert (p[at] == -0.5).all() and int((p != 0).sum()) == 5
     assert abs(grad_norm([g]).item() - 0.25 * 5 ** 0.5) < 1e-6
+
+
+def test_8_bit_seeds_of_any_size():
+    """Seeds count modulo 2^32, those past 64 bits and negative ones among them."""
+    n = 1000
+    results = []
+    for seed in (7, 7 + (1 << 32), 7 + (5 << 64), 7 - (1 << 32)):
+        gen = torch.Generator(DEV).manual_seed(6)
+        ps, gs = [[torch.randn(n, generator=gen, device=DEV) for _ in range(2)] for _ in range(2)]
+        codes = [[torch.zeros(n, device=DEV, dtype=torch.uint8).view(torch.float8_e4m3fn)
+                  for _ in range(2)] for _ in range(2)]
+        scales = [[torch.ones(state_blocks(n), device=DEV) for _ in range(2)] for _ in range(2)]
+        adamw8_step_(ps, gs, codes[0], scales[0], codes[1], scales[1], step=1, seed=seed)
+        results.append([t.view(torch.uint8) for t in (*ps, *codes[0], *codes[1])])
+    for got in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got, results[0]))
