@@ -22,9 +22,9 @@ namespace mqc {
 //
 // What bounds it: 8 bytes an element forward and 14 backward (bf16) against some 40 and 58 vector
 // instructions, so neither memory (a copy's 5.1 TB/s) nor arithmetic alone, but how well workgroups
-// overlap. bf16: a prompt of 16384 x 1536 55 us (201 MB, 3.7 TB/s; loads and stores alone 32, with LDS
-// and the words between chunks 38); 4 x 2048 x 1536 forward 28 us, backward 42 (176 MB, 4.2 TB/s).
-// Spans and waves, same prompt (two stages earlier, 61 us as here): 8 steps 72, 4 waves of 16 70, 4 of 32
+// overlap. bf16: a prompt of 16384 x 1536 47 us (201 MB, 4.3 TB/s; loads and stores alone 32, with LDS
+// and the words between chunks 38); 4 x 2048 x 1536 forward 25 us, backward 40 (176 MB, 4.4 TB/s).
+// Spans and waves, same prompt (some stages earlier, 61 us as here): 8 steps 72, 4 waves of 16 70, 4 of 32
 // 62, 16 waves of 8 72; backward of 4 x 2048 x 1536: 8 waves of 8 steps 53, 4 of 16 45, 4 of 32 65. Not
 // kept: workgroups that stay and load the next chunk ahead (61 to 82: they all wait for one another in
 // turn), spans walked for a guessed chunk while the counter answers (56 to 77: it guesses wrong).
@@ -167,6 +167,19 @@ __global__ __launch_bounds__(256) void scan_clear_kernel(uint4* words, int64_t z
   if (i < count) words[i] = uint4{v, v, v, v};
 }
 
+// What the card holds at once, three workgroups a CU, begins over some 3 us (NAPS of 64 clocks) forward
+// and 4 backward, in the order of the chain: begun together, the loads of its first chunks, for which
+// all others wait, share the memory with those of its last. It saves some 3 us a launch,
+// 7 where the card was idle: forward of 16384 x 1536 54.8 to 47.3 us, of 4 x 2048 x 1536 28.4 to 25.0 and
+// backward 41.7 to 40.4; launch after launch, 1 x 8192 33.5 to 30.9, backward 55.7 to 51.1, 1 x 65536 219
+// to 216, 144 workgroups of 2 x 700 x 768 10.7 as before.
+constexpr uint32_t kScanHeld = 768;
+template <uint32_t NAPS>
+__device__ inline void scan_stagger() {
+  if (blockIdx.x < kScanHeld)
+    for (uint32_t i = blockIdx.x * NAPS / kScanHeld; i > 0; --i) __builtin_amdgcn_s_sleep(1);
+}
+
 // Which chunk (from the end where the walk starts) of which 64 channels of which sequence. Each of
 // these `tiles` has a counter of its own: one for all cost 8 ns a workgroup.
 struct ScanPlace { int64_t n, b, d0; };
@@ -280,6 +293,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 6) void gated_scan_fwd_kernel(Scan
   __shared__ uint32_t place;
   const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if constexpr (CHAIN) scan_stagger<96>();
   const ScanPlace at = scan_place<CHAIN>(k.tickets, k.width, tiles, &place);
   const int64_t d = at.d0 + lane, b = at.b;
   const bool on = d < k.width;
@@ -412,6 +426,7 @@ __global__ __launch_bounds__(64 * kBackWaves) void gated_scan_bwd_kernel(ScanArg
   __shared__ uint32_t place;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if constexpr (CHAIN) scan_stagger<128>();
   const ScanPlace at = scan_place<CHAIN>(k.tickets, k.width, tiles, &place);
   const int64_t d = at.d0 + lane, b = at.b;
   const bool on = d < k.width;
