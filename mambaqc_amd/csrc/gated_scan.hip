@@ -169,14 +169,15 @@ __global__ __launch_bounds__(256) void scan_clear_kernel(uint4* words, int64_t z
 
 // What the card holds at once, three workgroups a CU, begins over some 3 us (NAPS of 64 clocks) forward
 // and 4 backward, in the order of the chain: begun together, the loads of its first chunks, for which
-// all others wait, share the memory with those of its last. It saves some 3 us a launch,
-// 7 where the card was idle: forward of 16384 x 1536 54.8 to 47.3 us, of 4 x 2048 x 1536 28.4 to 25.0 and
-// backward 41.7 to 40.4; launch after launch, 1 x 8192 33.5 to 30.9, backward 55.7 to 51.1, 1 x 65536 219
-// to 216, 144 workgroups of 2 x 700 x 768 10.7 as before.
+// all others wait, share the memory with those of its last. It saves some 3 us a launch, 7 where the
+// card was idle: forward of 16384 x 1536 54.8 to 47.3 us, of 4 x 2048 x 1536 28.4 to 25.0 and backward
+// 41.7 to 40.4; launch after launch, 1 x 8192 33.5 to 30.9, backward 55.7 to 51.1, 1 x 65536 219 to 216,
+// 64 x 256 44.6 to 41.4. Short chains that the card holds whole begin at once: 16 x 256 x 1536 16.3, or
+// 17.1 over 3 us; chains of 32 (1 x 4096 x 1536) 22.8, or 21.0.
 constexpr uint32_t kScanHeld = 768;
 template <uint32_t NAPS>
-__device__ inline void scan_stagger() {
-  if (blockIdx.x < kScanHeld)
+__device__ inline void scan_stagger(uint32_t tiles) {
+  if (blockIdx.x < kScanHeld && (gridDim.x > kScanHeld || gridDim.x >= 8 * tiles))
     for (uint32_t i = blockIdx.x * NAPS / kScanHeld; i > 0; --i) __builtin_amdgcn_s_sleep(1);
 }
 
@@ -293,7 +294,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 6) void gated_scan_fwd_kernel(Scan
   __shared__ uint32_t place;
   const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if constexpr (CHAIN) scan_stagger<96>();
+  if constexpr (CHAIN) scan_stagger<96>(tiles);
   const ScanPlace at = scan_place<CHAIN>(k.tickets, k.width, tiles, &place);
   const int64_t d = at.d0 + lane, b = at.b;
   const bool on = d < k.width;
@@ -426,7 +427,7 @@ __global__ __launch_bounds__(64 * kBackWaves) void gated_scan_bwd_kernel(ScanArg
   __shared__ uint32_t place;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if constexpr (CHAIN) scan_stagger<128>();
+  if constexpr (CHAIN) scan_stagger<128>(tiles);
   const ScanPlace at = scan_place<CHAIN>(k.tickets, k.width, tiles, &place);
   const int64_t d = at.d0 + lane, b = at.b;
   const bool on = d < k.width;
@@ -571,7 +572,7 @@ __global__ __launch_bounds__(64 * kBackWaves) void gated_scan_bwd_kernel(ScanArg
   }
 }
 
-// One token for each sequence, the state in place. 16 x 1536 in fp16 2.7 us, a launch's latency (7 with
+// One token for each sequence, the state in place. 16 x 1536 in fp16 3 us, a launch's latency (7 with
 // the host).
 template <typename T>
 __global__ __launch_bounds__(256) void gated_scan_step_kernel(ScanArgs<T> k, float* h) {
