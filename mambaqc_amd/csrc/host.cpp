@@ -3,7 +3,9 @@
 // tables. Nothing is computed here. It exists for its host time: what a training step of one small
 // layer waits for is the path from the Python call to the launch (forward and backward of a gate with
 // norms over 3001 x 515, whose kernels take 25 us: 87 us through Python nodes), and a table of 40
-// tensors with 8-bit states took 130 us to check and fill.
+// tensors with 8-bit states took 130 us to check and fill. The decode steps are host time alone: with
+// their arguments checked here too, and weights taken without a call into Python where they are what
+// the kernels read, 5.0 and 7.2 us a call against 7.0 and 10.2.
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
@@ -57,7 +59,20 @@ void on_device(const std::string& name, const Tensor& t, const Tensor& like) {
 // Autograd does not see what the operands go through; their gradients' edges are the node's.
 Tensor as_type(const Tensor& t, at::ScalarType type) {
   const at::NoGradGuard none;
-  return t.scalar_type() == type ? t.detach() : t.detach().to(type);
+  const Tensor v = t.requires_grad() ? t.detach() : t;
+  return v.scalar_type() == type ? v : v.to(type);
+}
+// A parameter as the kernels read it: itself, or `convert`'s (_native.param_f32) where it is not that.
+Tensor weight(const Tensor& t, const py::object& convert) {
+  if (t.scalar_type() == at::kFloat && t.is_contiguous() && (uintptr_t)t.data_ptr() % 16 == 0)
+    return as_type(t, at::kFloat);
+  return convert(t).cast<Tensor>();
+}
+bool records(std::initializer_list<MaybeTensor> inputs) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const auto& t : inputs)
+    if (t && t->requires_grad()) return true;
+  return false;
 }
 // The kernels write through pointers: tells autograd (and whatever keeps copies of parameters by their
 // version) that a tensor changed.
@@ -122,14 +137,15 @@ struct GateNorm {
   Tensor scale, pre;
   GateNorm() = default;
   GateNorm(const Tensor& x_, const Tensor& y_, const MaybeTensor& z_, const MaybeTensor& post_,
-           const Tensor& scale_, const Tensor& pre_)
-      : z_row(0), post(post_), scale(scale_), pre(pre_) {
+           const Tensor& scale_, const Tensor& pre_, const py::object& convert)
+      : z_row(0) {
     for (const Tensor* t : {&x_, &y_, &scale_, &pre_}) on_device("gate_norm_residual", *t, x_);
+    if (post_) on_device("gate_norm_residual", *post_, x_), post = weight(*post_, convert);
+    scale = weight(scale_, convert), pre = weight(pre_, convert);
     auto type = at::promote_types(x_.scalar_type(), y_.scalar_type());
     if (z_) type = at::promote_types(type, z_->scalar_type());
     x = as_type(x_, type).contiguous();
     y = as_type(y_, type).contiguous();
-    if (post) on_device("gate_norm_residual", *post, x_);
     if (z_) {
       on_device("gate_norm_residual", *z_, x_);
       std::tie(z, z_row) = spaced_rows(*z_, type);
@@ -200,11 +216,21 @@ struct GateNormNode : torch::autograd::Function<GateNormNode> {
   }
 };
 
-std::tuple<Tensor, Tensor> gate_norm_train(const Tensor& x, const Tensor& y, const MaybeTensor& z,
-                                           const MaybeTensor& post, const Tensor& scale,
-                                           const Tensor& pre, const GateNorm& o, double eps) {
-  const auto out = GateNormNode::apply(x, y, z, post, scale, pre, o, eps);
-  return {out[0], out[1]};
+// gate_norm_residual (out, n), or nothing where the shapes do not match.
+std::optional<std::tuple<Tensor, Tensor>> gate_norm(const Tensor& x, const Tensor& y, const MaybeTensor& z,
+                                                    const MaybeTensor& post, const Tensor& scale,
+                                                    const Tensor& pre, double eps,
+                                                    const py::object& convert) {
+  if (x.dim() < 1 || y.sizes() != x.sizes() || (z && z->sizes() != x.sizes())) return std::nullopt;
+  const at::IntArrayRef last = x.sizes().slice(x.dim() - 1);
+  if (scale.sizes() != last || pre.sizes() != last || (post && post->sizes() != last)) return std::nullopt;
+  const GateNorm o(x, y, z, post, scale, pre, convert);
+  if (records({x, y, z, post, scale, pre})) {
+    const auto out = GateNormNode::apply(x, y, z, post, scale, pre, o, eps);
+    return std::make_tuple(out[0], out[1]);
+  }
+  auto [out, n, stats] = gate_norm_forward(o, eps, false);
+  return std::make_tuple(out, n);
 }
 
 // --- the gated scan -------------------------------------------------------------------------------
@@ -232,10 +258,10 @@ struct Scan {
   MaybeTensor reset;
   Scan() = default;
   Scan(const std::string& name, const Tensor& dt_, const Tensor& g_, const Tensor& x_, const Tensor& rate_,
-       const MaybeTensor& reset_)
-      : rate(rate_), reset(reset_) {
+       const MaybeTensor& reset_, const py::object& convert) {
     for (const Tensor* t : {&x_, &dt_, &g_, &rate_}) on_device(name, *t, x_);
-    if (reset) on_device(name, *reset, x_), reset = reset->contiguous();
+    rate = weight(rate_, convert);
+    if (reset_) on_device(name, *reset_, x_), reset = reset_->contiguous();
     const auto type =
         at::promote_types(at::promote_types(dt_.scalar_type(), g_.scalar_type()), x_.scalar_type());
     std::tie(dt, dt_row) = token_rows(dt_, type);
@@ -316,14 +342,37 @@ struct ScanNode : torch::autograd::Function<ScanNode> {
   }
 };
 
-std::tuple<Tensor, Tensor> scan_train(const Tensor& dt, const Tensor& g, const Tensor& x,
-                                      const Tensor& log_rate, const MaybeTensor& h0, const Scan& o,
-                                      const MaybeTensor& h0_read) {
-  const auto out = ScanNode::apply(dt, g, x, log_rate, h0, o, h0_read);
-  return {out[0], out[1]};
+bool scan_shapes(const Tensor& dt, const Tensor& g, const Tensor& x, const Tensor& rate,
+                 const MaybeTensor& h, const MaybeTensor& reset) {
+  if (x.dim() != 3 || dt.sizes() != x.sizes() || g.sizes() != x.sizes()) return false;
+  const int64_t b = x.size(0), t = x.size(1), d = x.size(2);
+  return rate.dim() == 1 && rate.size(0) == d && (!h || h->sizes() == at::IntArrayRef{b, d}) &&
+         (!reset || (reset->sizes() == at::IntArrayRef{b, t} && reset->scalar_type() == at::kBool));
 }
 
-Tensor scan_step(const Scan& o, const Tensor& h) {
+// gated_scan (y, last state), or nothing where the arguments do not match.
+std::optional<std::tuple<Tensor, Tensor>> gated_scan(const Tensor& dt, const Tensor& g, const Tensor& x,
+                                                     const Tensor& log_rate, const MaybeTensor& h0,
+                                                     const MaybeTensor& reset, const py::object& convert) {
+  if (!scan_shapes(dt, g, x, log_rate, h0, reset)) return std::nullopt;
+  const Scan o("gated_scan", dt, g, x, log_rate, reset, convert);
+  MaybeTensor state;
+  if (h0) state = as_type(*h0, at::kFloat).contiguous();
+  if (records({dt, g, x, log_rate, h0})) {
+    const auto out = ScanNode::apply(dt, g, x, log_rate, h0, o, state);
+    return std::make_tuple(out[0], out[1]);
+  }
+  auto [y, h, carries] = scan_forward(o, state, false);
+  return std::make_tuple(y, h);
+}
+
+// gated_scan_step_, or nothing where the arguments do not match.
+MaybeTensor gated_scan_step(const Tensor& dt, const Tensor& g, const Tensor& x, const Tensor& log_rate,
+                            const Tensor& h, const py::object& convert) {
+  if (!scan_shapes(dt, g, x, log_rate, h, std::nullopt) || x.size(1) != 1 ||
+      h.scalar_type() != at::kFloat || !h.is_contiguous())
+    return std::nullopt;
+  const Scan o("gated_scan_step_", dt, g, x, log_rate, std::nullopt, convert);
   const c10::DeviceGuard guard(o.x.device());
   on_device("gated_scan_step_", h, o.x);
   Tensor y = at::empty({o.b(), 1, o.d()}, o.x.options());
@@ -390,23 +439,23 @@ void changed(const Lists& lists) {
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   py::class_<GateNorm>(m, "GateNorm")
       .def(py::init<const Tensor&, const Tensor&, const MaybeTensor&, const MaybeTensor&, const Tensor&,
-                    const Tensor&>());
+                    const Tensor&, const py::object&>());
   m.def("spaced_rows", [](const Tensor& t, py::object type) {
     return spaced_rows(t, torch::python::detail::py_object_to_dtype(type));
   });
   m.def("gate_norm_forward", &gate_norm_forward);
   m.def("gate_norm_backward", &gate_norm_backward);
-  m.def("gate_norm_train", &gate_norm_train);
+  m.def("gate_norm", &gate_norm);
   py::class_<Scan>(m, "Scan")
       .def(py::init<const std::string&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
-                    const MaybeTensor&>());
+                    const MaybeTensor&, const py::object&>());
   m.def("token_rows", [](const Tensor& t, py::object type) {
     return token_rows(t, torch::python::detail::py_object_to_dtype(type));
   });
   m.def("scan_forward", &scan_forward);
   m.def("scan_backward", &scan_backward);
-  m.def("scan_train", &scan_train);
-  m.def("scan_step", &scan_step);
+  m.def("gated_scan", &gated_scan);
+  m.def("gated_scan_step", &gated_scan_step);
   m.def("adam_rows", &adam_rows);
   m.def("changed", [](const Lists& lists) { changed(lists); });
   m.def("abi", [] { return (int64_t)mqc_abi_version(); });

@@ -39,8 +39,7 @@ def _z_rows(z: torch.Tensor, dtype: torch.dtype):
 
 def _operands(x, y, z, post_weight, scale, pre_weight):
     """The operands as the kernels read them, weights in fp32."""
-    return nat.host().GateNorm(x, y, z, None if post_weight is None else nat.param_f32(post_weight),
-                               nat.param_f32(scale), nat.param_f32(pre_weight))
+    return nat.host().GateNorm(x, y, z, post_weight, scale, pre_weight, nat.param_f32)
 
 
 def gate_norm_residual(x: torch.Tensor, y: torch.Tensor, z: torch.Tensor | None = None, *,
@@ -55,12 +54,10 @@ def gate_norm_residual(x: torch.Tensor, y: torch.Tensor, z: torch.Tensor | None 
     block's output, out the stream after it and n the next block's input. Norms and sums are fp32,
     and n comes from out before its rounding. d is at most 8192. Differentiable in every tensor
     argument when autograd is recording."""
-    _check(x, y, z, post_weight, scale, pre_weight)
-    train = torch.is_grad_enabled() and any(
-        v is not None and v.requires_grad for v in (x, y, z, post_weight, scale, pre_weight))
     if nat.compiling():
+        _check(x, y, z, post_weight, scale, pre_weight)
         return torch.ops.mambaqc.gate_norm_residual(x, y, z, post_weight, scale, pre_weight, eps)[:2]
-    operands = _operands(x, y, z, post_weight, scale, pre_weight)
-    if train:
-        return nat.host().gate_norm_train(x, y, z, post_weight, scale, pre_weight, operands, eps)
-    return nat.host().gate_norm_forward(operands, eps, False)[:2]
+    got = nat.host().gate_norm(x, y, z, post_weight, scale, pre_weight, eps, nat.param_f32)
+    if got is None:  # say what is wrong
+        _check(x, y, z, post_weight, scale, pre_weight)
+    return got

@@ -46,7 +46,7 @@ def scan_chunk() -> int:
 
 def _operands(name, dt_raw, g_raw, x, log_rate, reset=None):
     """The operands as the kernels read them, log_rate in fp32."""
-    return nat.host().Scan(name, dt_raw, g_raw, x, nat.param_f32(log_rate), reset)
+    return nat.host().Scan(name, dt_raw, g_raw, x, log_rate, reset, nat.param_f32)
 
 
 def _state(h0):
@@ -63,18 +63,17 @@ def gated_scan(dt_raw: torch.Tensor, g_raw: torch.Tensor, x: torch.Tensor, log_r
     h0: the state before the first token (None: zeros). reset: bool [batch, seq_len], true at the
     first token of a packed document: nothing from before it is seen, NaN included. States are
     fp32. Differentiable in every tensor argument when autograd is recording."""
-    _check("gated_scan", dt_raw, g_raw, x, log_rate, h0, reset)
-    train = torch.is_grad_enabled() and any(v is not None and v.requires_grad
-                                            for v in (dt_raw, g_raw, x, log_rate, h0))
     if nat.compiling():
+        _check("gated_scan", dt_raw, g_raw, x, log_rate, h0, reset)
+        train = torch.is_grad_enabled() and any(v is not None and v.requires_grad
+                                                for v in (dt_raw, g_raw, x, log_rate, h0))
         op = torch.ops.mambaqc.gated_scan_train if train else torch.ops.mambaqc.gated_scan
         y, h_last = op(dt_raw, g_raw, x, log_rate, h0, reset)[:2]
     else:
-        operands = _operands("gated_scan", dt_raw, g_raw, x, log_rate, reset)
-        if train:
-            y, h_last = nat.host().scan_train(dt_raw, g_raw, x, log_rate, h0, operands, _state(h0))
-        else:
-            y, h_last, _ = nat.host().scan_forward(operands, _state(h0), False)
+        got = nat.host().gated_scan(dt_raw, g_raw, x, log_rate, h0, reset, nat.param_f32)
+        if got is None:  # say what is wrong
+            _check("gated_scan", dt_raw, g_raw, x, log_rate, h0, reset)
+        y, h_last = got
     return (y, h_last) if return_state else y
 
 
@@ -83,10 +82,10 @@ def gated_scan_step_(dt_raw: torch.Tensor, g_raw: torch.Tensor, x: torch.Tensor,
     """One token of the gated scan for each sequence: dt_raw, g_raw, x [batch, 1, width] and the
     state h, contiguous fp32 [batch, width], updated in place. Returns y [batch, 1, width]. No
     autograd (the decode step)."""
-    _check("gated_scan_step_", dt_raw, g_raw, x, log_rate, h)
-    b, t, d = x.shape
-    if t != 1:
-        raise ValueError(f"gated_scan_step_: one token a sequence, got {t}")
-    if h.dtype != torch.float32 or not h.is_contiguous():
+    y = nat.host().gated_scan_step(dt_raw, g_raw, x, log_rate, h, nat.param_f32)
+    if y is None:  # say what is wrong
+        _check("gated_scan_step_", dt_raw, g_raw, x, log_rate, h)
+        if x.shape[1] != 1:
+            raise ValueError(f"gated_scan_step_: one token a sequence, got {x.shape[1]}")
         raise ValueError(f"gated_scan_step_: h must be contiguous float32, got {h.dtype}")
-    return nat.host().scan_step(_operands("gated_scan_step_", dt_raw, g_raw, x, log_rate), h)
+    return y
