@@ -252,7 +252,8 @@ __device__ inline float scan_entry(const ScanArgs<T>& k, const ScanPlace& at, in
 // offset (made anew for each access: widened to 64 bits once for all, it costs a sum in every lane for
 // each). next() keeps it a running pointer: left alone, the compiler computes all rows' addresses
 // ahead and spills them.
-template <typename T>
+// STREAM: past the caches (scan_stream).
+template <typename T, bool STREAM = false>
 struct ScanRow {
   using Raw = std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>;
   using Global = __attribute__((address_space(1))) char*;
@@ -261,11 +262,15 @@ struct ScanRow {
   __device__ ScanRow(const T* p, int64_t step) : at((Global)(char*)p), by(step * (int64_t)sizeof(T)) {}
   __device__ T load(uint32_t off) const {
     asm("" : "+v"(off));
-    return __builtin_bit_cast(T, *(__attribute__((address_space(1))) Raw*)(at + off));
+    const auto p = (__attribute__((address_space(1))) Raw*)(at + off);
+    return __builtin_bit_cast(T, STREAM ? __builtin_nontemporal_load(p) : *p);
   }
   __device__ void store(uint32_t off, float v) const {
     asm("" : "+v"(off));
-    *(__attribute__((address_space(1))) Raw*)(at + off) = __builtin_bit_cast(Raw, io<T>::from_f32(v));
+    const auto p = (__attribute__((address_space(1))) Raw*)(at + off);
+    const Raw raw = __builtin_bit_cast(Raw, io<T>::from_f32(v));
+    if constexpr (STREAM) __builtin_nontemporal_store(raw, p);
+    else *p = raw;
   }
   __device__ void next(bool there = true) {  // (else the same row again)
     at += there ? by : 0;
@@ -287,11 +292,12 @@ __device__ inline uint32_t scan_resets(const uint8_t* reset, int64_t row, int n)
 }
 
 // Forward: a workgroup takes one chunk of 64 channels.
-template <typename T, bool CHAIN>
+template <typename T, bool CHAIN, int STREAM = 0>
 __global__ __launch_bounds__(64 * kScanWaves, 6) void gated_scan_fwd_kernel(ScanArgs<T> k, uint32_t tiles) {
   __shared__ float part[2][kScanWaves][64];  // c and u of each span
   __shared__ float words[CHAIN ? 2 : 1][kScanGroup][64], entry[64];
   __shared__ uint32_t place;
+  using In = ScanRow<T, STREAM == 2>;
   const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if constexpr (CHAIN) scan_stagger<96>(tiles);
@@ -312,8 +318,8 @@ __global__ __launch_bounds__(64 * kScanWaves, 6) void gated_scan_fwd_kernel(Scan
   // PLAIN: all steps are there and none is a reset.
   const auto walk = [&](auto plain) {
     constexpr bool PLAIN = decltype(plain)::value;
-    ScanRow<T> dts(k.dt + row0 * k.dt_row + at.d0, k.dt_row);
-    ScanRow<T> gs(k.g + row0 * k.g_row + at.d0, k.g_row), xs(k.x + row0 * k.x_row + at.d0, k.x_row);
+    In dts(k.dt + row0 * k.dt_row + at.d0, k.dt_row);
+    In gs(k.g + row0 * k.g_row + at.d0, k.g_row), xs(k.x + row0 * k.x_row + at.d0, k.x_row);
     T raw[3][kScanSteps];
 #pragma unroll
     for (int i = 0; i < kScanSteps; ++i) {
@@ -335,7 +341,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 6) void gated_scan_fwd_kernel(Scan
       scan_pace(i);
     }
     if (__builtin_expect(__any(low < -80.f), 0)) {
-      ScanRow<T> again(k.dt + row0 * k.dt_row + at.d0, k.dt_row);
+      In again(k.dt + row0 * k.dt_row + at.d0, k.dt_row);
 #pragma unroll
       for (int i = 0; i < kScanSteps; ++i) {
         const float dt = io<T>::to_f32(again.load(off));
@@ -397,7 +403,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 6) void gated_scan_fwd_kernel(Scan
     k.carries[(b * every + t0 / kScanChunk) * k.width + d] = h;
   }
   if (!on) return;
-  ScanRow<T> y(k.y + row0 * k.width + at.d0, k.width);
+  ScanRow<T, (STREAM > 0)> y(k.y + row0 * k.width + at.d0, k.width);
   if (plain) {
 #pragma unroll
     for (int i = 0; i < kScanSteps; ++i) {
@@ -420,11 +426,12 @@ __global__ __launch_bounds__(64 * kScanWaves, 6) void gated_scan_fwd_kernel(Scan
 
 // Backward: the chunks from the last to the first, each from its stored entry state. What a span makes
 // of the adjoint A behind it (A = a G of the step after) is v + 2^-p A.
-template <typename T, bool CHAIN>
+template <typename T, bool CHAIN, int STREAM = 0>
 __global__ __launch_bounds__(64 * kBackWaves) void gated_scan_bwd_kernel(ScanArgs<T> k, uint32_t tiles) {
   __shared__ float part[3][kBackWaves][64];  // c, u and v of each span
   __shared__ float words[CHAIN ? 2 : 1][kScanGroup][64], entry[64];
   __shared__ uint32_t place;
+  using In = ScanRow<T, STREAM == 2>;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if constexpr (CHAIN) scan_stagger<128>(tiles);
@@ -447,9 +454,9 @@ __global__ __launch_bounds__(64 * kBackWaves) void gated_scan_bwd_kernel(ScanArg
   // PLAIN: all steps are there and none is a reset.
   const auto walk = [&](auto plain) {
     constexpr bool PLAIN = decltype(plain)::value;
-    ScanRow<T> dts(k.dt + row0 * k.dt_row + at.d0, k.dt_row);
-    ScanRow<T> gs(k.g + row0 * k.g_row + at.d0, k.g_row), xs(k.x + row0 * k.x_row + at.d0, k.x_row);
-    ScanRow<T> dys(k.dy + row0 * k.width + at.d0, k.width);
+    In dts(k.dt + row0 * k.dt_row + at.d0, k.dt_row);
+    In gs(k.g + row0 * k.g_row + at.d0, k.g_row), xs(k.x + row0 * k.x_row + at.d0, k.x_row);
+    In dys(k.dy + row0 * k.width + at.d0, k.width);
     T raw[4][kBackSteps];
 #pragma unroll
     for (int i = 0; i < kBackSteps; ++i) {
@@ -471,7 +478,7 @@ __global__ __launch_bounds__(64 * kBackWaves) void gated_scan_bwd_kernel(ScanArg
       scan_pace(i);
     }
     if (__builtin_expect(__any(low < -80.f), 0)) {
-      ScanRow<T> again(k.dt + row0 * k.dt_row + at.d0, k.dt_row);
+      In again(k.dt + row0 * k.dt_row + at.d0, k.dt_row);
 #pragma unroll
       for (int i = 0; i < kBackSteps; ++i) {
         const float dt = io<T>::to_f32(again.load(off));
@@ -540,7 +547,7 @@ __global__ __launch_bounds__(64 * kBackWaves) void gated_scan_bwd_kernel(ScanArg
           h = fmaf(a[i], h, w[i] * s);
         }
       const int64_t to = (row0 + (PLAIN ? kBackSteps : n) - 1) * k.width + at.d0;
-      ScanRow<T> ddt(k.ddt + to, -k.width), dg(k.dg + to, -k.width), dx(k.dx + to, -k.width);
+      ScanRow<T, (STREAM > 0)> ddt(k.ddt + to, -k.width), dg(k.dg + to, -k.width), dx(k.dx + to, -k.width);
 #pragma unroll
       for (int i = kBackSteps - 1; i >= 0; --i)
         if (PLAIN || i < n) {
@@ -613,6 +620,21 @@ int scan_chain(ScanArgs<T>& k, const ScanSpace& w, char* ws, hipStream_t s) {
   return launch_status();
 }
 
+// What the 256 MiB cache does not hold anyway goes past it: the outputs where they and the inputs are
+// more, the inputs where these alone are. bf16: backward of 8 x 2048 x 1536 (201 MB in, 151 out) 103 us,
+// with outputs streamed 79, with both 96; 1 x 65536 forward 217, 211, 207, backward 414, 399, 383; what
+// fits loses: 4 x 2048 forward 27.7, 27.1, 28.9, backward 46.3, 45.7, 55.5.
+inline int scan_stream(int64_t tensor, int in, int out) {
+  return tensor * in > (256LL << 20) ? 2 : tensor * (in + out) > (256LL << 20) ? 1 : 0;
+}
+#define MQC_SCAN_CHAIN(KERNEL, WAVES, IN, OUT)                                                        \
+  const dim3 grid((unsigned)(tiles * w.chunks)), block(64 * WAVES);                                   \
+  switch (scan_stream(batch * k.seq * k.width * (int64_t)sizeof(T), IN, OUT)) {                       \
+    case 0: KERNEL<T, true, 0><<<grid, block, 0, s>>>(k, (uint32_t)tiles); break;                     \
+    case 1: KERNEL<T, true, 1><<<grid, block, 0, s>>>(k, (uint32_t)tiles); break;                     \
+    default: KERNEL<T, true, 2><<<grid, block, 0, s>>>(k, (uint32_t)tiles); break;                    \
+  }
+
 template <typename T>
 int launch_gated_scan_fwd(ScanArgs<T> k, int64_t batch, char* ws, hipStream_t s) {
   const int64_t tiles = batch * ((k.width + kScanLanes - 1) / kScanLanes);
@@ -620,8 +642,7 @@ int launch_gated_scan_fwd(ScanArgs<T> k, int64_t batch, char* ws, hipStream_t s)
   if (w.chunks > 1) {
     const int st = scan_chain(k, w, ws, s);
     if (st != MQC_OK) return st;
-    gated_scan_fwd_kernel<T, true>
-        <<<dim3((unsigned)(tiles * w.chunks)), dim3(64 * kScanWaves), 0, s>>>(k, (uint32_t)tiles);
+    MQC_SCAN_CHAIN(gated_scan_fwd_kernel, kScanWaves, 3, 1)
   } else {
     const int64_t waves = k.seq > 0 ? (k.seq + kScanSteps - 1) / kScanSteps : 1;
     gated_scan_fwd_kernel<T, false>
@@ -638,8 +659,7 @@ int launch_gated_scan_bwd(ScanArgs<T> k, int64_t batch, float* drate, char* ws, 
   if (w.chunks > 1) {
     const int st = scan_chain(k, w, ws, s);
     if (st != MQC_OK) return st;
-    gated_scan_bwd_kernel<T, true>
-        <<<dim3((unsigned)(tiles * w.chunks)), dim3(64 * kBackWaves), 0, s>>>(k, (uint32_t)tiles);
+    MQC_SCAN_CHAIN(gated_scan_bwd_kernel, kBackWaves, 4, 3)
   } else {
     gated_scan_bwd_kernel<T, false>
         <<<dim3((unsigned)tiles), dim3(64 * kBackWaves), 0, s>>>(k, (uint32_t)tiles);

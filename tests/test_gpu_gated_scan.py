@@ -470,3 +470,24 @@ def test_step_tells_that_the_state_changed():
     version = h0._version
     gated_scan_step_(dt, g, x, lam, h0)
     assert h0._version > version
+
+
+@pytest.mark.parametrize("dtype,shape", [(torch.bfloat16, (1, 7000, 4100)), (torch.bfloat16, (1, 9000, 4100)),
+                                         (torch.bfloat16, (2, 8209, 4100)), (torch.float32, (1, 7000, 2050)),
+                                         (torch.float32, (3, 5000, 2050))])
+def test_sizes_past_the_cache_equal_their_parts(dtype, shape):
+    """Operands past 256 MiB, in all, in the inputs alone or in neither: channel by channel the same
+    bits as a few channels at a time, gradients too."""
+    gen = torch.Generator(DEV).manual_seed(8)
+    full = [torch.randn(shape, generator=gen, device=DEV, dtype=dtype).requires_grad_() for _ in range(3)]
+    rate = (torch.rand(shape[2], generator=gen, device=DEV) * -4).requires_grad_()
+    dy = torch.randn(shape, generator=gen, device=DEV, dtype=dtype)
+    y, h = gated_scan(*full, rate, return_state=True)
+    grads = torch.autograd.grad((y, h), [*full, rate], (dy, torch.ones_like(h)))
+    for start in range(0, shape[2], 1024):
+        part = slice(start, start + 1024)
+        leaves = [t.detach()[..., part].contiguous().requires_grad_() for t in (*full, rate)]
+        some, last = gated_scan(*leaves, return_state=True)
+        want = torch.autograd.grad((some, last), leaves, (dy[..., part], torch.ones_like(last)))
+        assert torch.equal(y[..., part], some) and torch.equal(h[..., part], last)
+        assert all(torch.equal(g[..., part], w) for g, w in zip(grads, want))
