@@ -20,14 +20,16 @@ namespace mqc {
 // states themselves: inputs are read once, and their gates computed once. The spans of a chunk join in
 // LDS. Between chunks the state goes through memory within the launch: see scan_entry.
 //
-// What bounds it: 8 bytes an element forward and 14 backward (bf16) against some 40 and 58 vector
-// instructions, so neither memory (a copy's 5.1 TB/s) nor arithmetic alone, but how well workgroups
-// overlap. bf16: a prompt of 16384 x 1536 47 us (201 MB, 4.3 TB/s; loads and stores alone 32, with LDS
-// and the words between chunks 38); 4 x 2048 x 1536 forward 25 us, backward 40 (176 MB, 4.4 TB/s).
-// Spans and waves, same prompt (some stages earlier, 61 us as here): 8 steps 72, 4 waves of 16 70, 4 of 32
-// 62, 16 waves of 8 72; backward of 4 x 2048 x 1536: 8 waves of 8 steps 53, 4 of 16 45, 4 of 32 65. Not
-// kept: workgroups that stay and load the next chunk ahead (61 to 82: they all wait for one another in
-// turn), spans walked for a guessed chunk while the counter answers (56 to 77: it guesses wrong).
+// What bounds it: 8 bytes an element forward and 14 backward (bf16) against some 33 and 58 vector
+// instructions (5 and 6 of which take four times as long), so neither memory (a copy's 5.1 TB/s) nor
+// arithmetic alone, but how well workgroups overlap. bf16: a prompt of 16384 x 1536 47 us (201 MB,
+// 4.3 TB/s; loads and stores alone 32, with LDS and the words between chunks 38); 4 x 2048 x 1536 forward
+// 25 us, backward 40 (176 MB, 4.4 TB/s); past the last cache, 1 x 65536 x 1536 208 and 385.
+// Spans and waves, same prompt: 8 of 16 steps 47, 8 of 8 66, 4 of 16 68, 4 of 32 52, 16 of 8 62; backward
+// of 4 x 2048 x 1536 (before later stages): 8 waves of 8 steps 53, 4 of 16 45, 4 of 32 65. Chunks joined one
+// by one: 8 or 16 47, 32 49, 64 55. Not kept: workgroups that stay and load the next chunk ahead (61 to
+// 82: they all wait for one another in turn), spans walked for a guessed chunk while the counter answers
+// (56 to 77: it guesses wrong), 64 registers a lane for four workgroups a CU (51 to 57).
 constexpr int kScanLanes = 64;  // channels of a workgroup
 constexpr int kScanWaves = 8;   // spans of a chunk, forward
 constexpr int kScanSteps = 16;  // steps of a span
