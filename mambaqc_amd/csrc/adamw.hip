@@ -33,8 +33,8 @@ namespace mqc {
 
 constexpr int kAdamThreads = 256;
 constexpr int kAdamVec = 4;                                  // elements a lane takes at once
-constexpr int kAdamIters = 4;
-constexpr int kAdamChunk = kAdamThreads * kAdamVec * kAdamIters;  // elements of a workgroup
+constexpr int kAdamIters = 4;                                // and how often, where there are many
+constexpr int kAdamChunk = kAdamThreads * kAdamVec * kAdamIters;  // elements of a workgroup then
 constexpr int kStateBlock = 256;                             // elements that share a scale
 
 template <int MAX>
@@ -96,21 +96,26 @@ __device__ inline void store4(T* p, int n, bool vec, const float (&in)[4]) {
   }
 }
 
-// STREAM: stores that leave no copy in the caches, for more than these hold (launch_adamw).
+// STREAM: for more than the caches hold (mqc_adamw_step), stores that leave no copy there, and sixteen
+// elements a lane; else four, for more workgroups.
+template <bool STREAM>
+constexpr int kAdamTurns = STREAM ? kAdamIters : 1;
 template <typename T, bool STREAM>
 __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamTable tab, AdamScalars k) {
 #pragma clang fp contract(off)
+  constexpr int TURNS = kAdamTurns<STREAM>;
   const int i = table_find(tab.first, tab.count);
   T* p = (T*)tab.p[i];
   const T* grad = (const T*)tab.grad[i];
   float *m = (float*)tab.m[i], *v = (float*)tab.v[i];
   const int64_t n = tab.n[i];
-  const int64_t base = (int64_t)(blockIdx.x - tab.first[i]) * kAdamChunk + threadIdx.x * kAdamVec;
+  const int64_t base = (int64_t)(blockIdx.x - tab.first[i]) * (kAdamThreads * kAdamVec * TURNS) +
+                       threadIdx.x * kAdamVec;
   const bool fits = (((uintptr_t)p | (uintptr_t)grad) % (4 * sizeof(T)) | ((uintptr_t)m | (uintptr_t)v) % 16) == 0;
   const float clip = k.clip ? *k.clip : 1.f;
-  float pv[kAdamIters][4], gv[kAdamIters][4], mv[kAdamIters][4], vv[kAdamIters][4];
+  float pv[TURNS][4], gv[TURNS][4], mv[TURNS][4], vv[TURNS][4];
 #pragma unroll
-  for (int j = 0; j < kAdamIters; ++j) {
+  for (int j = 0; j < TURNS; ++j) {
     const int64_t at = base + j * kAdamThreads * kAdamVec;
     const int left = n - at < 4 ? (int)(n - at) : 4;
     const bool vec = fits && left == 4;
@@ -121,7 +126,7 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_kernel(AdamTable tab, Adam
     load4<float>(v + at, left, vec, vv[j]);
   }
 #pragma unroll
-  for (int j = 0; j < kAdamIters; ++j) {
+  for (int j = 0; j < TURNS; ++j) {
     const int64_t at = base + j * kAdamThreads * kAdamVec;
     const int left = n - at < 4 ? (int)(n - at) : 4;
     const bool vec = fits && left == 4;
@@ -425,13 +430,9 @@ __global__ __launch_bounds__(1024) void grad_norm_end_kernel(const double* parti
 inline bool known_dtype(int64_t d) { return d == MQC_F32 || d == MQC_BF16 || d == MQC_F16; }
 
 template <typename T>
-void launch_adamw(const AdamTable& t, const AdamScalars& k, uint32_t blocks, hipStream_t s) {
-  // 36 M fp32 parameters (1 GB) 166 us streamed, 177 not; what fits the 256 MiB cache is found there
-  // at the next step.
-  if ((int64_t)blocks * kAdamChunk * (int64_t)(2 * sizeof(T) + 8) > (256LL << 20))
-    adamw_kernel<T, true><<<dim3(blocks), dim3(kAdamThreads), 0, s>>>(t, k);
-  else
-    adamw_kernel<T, false><<<dim3(blocks), dim3(kAdamThreads), 0, s>>>(t, k);
+void launch_adamw(const AdamTable& t, const AdamScalars& k, uint32_t blocks, bool stream, hipStream_t s) {
+  if (stream) adamw_kernel<T, true><<<dim3(blocks), dim3(kAdamThreads), 0, s>>>(t, k);
+  else adamw_kernel<T, false><<<dim3(blocks), dim3(kAdamThreads), 0, s>>>(t, k);
 }
 template <typename T>
 void launch_adamw(const Adam8Table& t, const AdamScalars& k, uint32_t blocks, hipStream_t s) {
@@ -517,12 +518,21 @@ extern "C" int mqc_adamw_step(const int64_t* tensors, int64_t count, float decay
     if ((tensors[6 * i + 2] | tensors[6 * i + 3]) % 4) return MQC_E_ALIGN;
   const AdamScalars k{decay, step_size, root_scale, beta1, one_minus_beta1, beta2, one_minus_beta2,
                       eps, clip, 0};
+  // 36 M fp32 parameters (1 GB) 164 us streamed, 177 not; what fits the 256 MiB cache is found there at
+  // the next step. Of a small step, sixteen elements a lane leave workgroups too few: 2.2 M fp32
+  // parameters 11.3 us, or 9.6 with four, 16 M in bf16 57 and 53; 36 M 163 and 165, and their norm, whose
+  // gradients the cache then holds no longer, 27 and 45.
+  int64_t bytes = 0;
+  for (int64_t i = 0; i < count && bytes <= 256LL << 20; ++i)
+    bytes += tensors[6 * i + 4] * (tensors[6 * i + 5] == MQC_F32 ? 16 : 12);
+  const bool many = bytes > 256LL << 20;
+  const int64_t chunk = kAdamThreads * kAdamVec * (many ? kAdamTurns<true> : kAdamTurns<false>);
   return by_tables<AdamTable>(
-      tensors, count, 6, 4, 5, kAdamChunk,
+      tensors, count, 6, 4, 5, chunk,
       [](AdamTable& t, int at, const int64_t* row, uint32_t first) { put_adam(t, at, row, row[4], first); },
       [&](AdamTable& t, int used, uint32_t blocks, int dtype) {
         t.count = used;
-        MQC_LAUNCH(launch_adamw, dtype, t, k, blocks, (hipStream_t)stream)
+        MQC_LAUNCH(launch_adamw, dtype, t, k, blocks, many, (hipStream_t)stream)
       });
 }
 

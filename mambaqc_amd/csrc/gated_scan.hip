@@ -671,6 +671,7 @@ int launch_gated_scan_bwd(ScanArgs<T> k, int64_t batch, float* drate, char* ws, 
   return mqc_sum_rows(k.drate, drate, k.width, nullptr, nullptr, 0, nullptr, nullptr, 0,
                       batch * w.chunks, s);
 }
+#undef MQC_SCAN_CHAIN
 
 template <typename T>
 int launch_gated_scan_step(const ScanArgs<T>& k, float* h, int64_t batch, hipStream_t s) {

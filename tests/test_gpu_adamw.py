@@ -476,3 +476,17 @@ def test_8_bit_seeds_of_any_size():
         results.append([t.view(torch.uint8) for t in (*ps, *codes[0], *codes[1])])
     for got in results[1:]:
         assert all(torch.equal(a, b) for a, b in zip(got, results[0]))
+
+
+def test_a_step_past_the_cache_equals_its_parts():
+    """Parameters and states past 256 MiB in one call: the same bits as tensor by tensor."""
+    sizes = [9_000_001, 4097, 8_500_003, 0, 5]
+    gen = torch.Generator(DEV).manual_seed(7)
+    lists = [[torch.randn(n, generator=gen, device=DEV) for n in sizes] for _ in range(4)]
+    lists[3] = [v.abs() for v in lists[3]]
+    apart = [[t.clone() for t in one] for one in lists]
+    adamw_step_(*lists, step=4, lr=1e-2)
+    for i in range(len(sizes)):
+        adamw_step_(*([one[i]] for one in apart), step=4, lr=1e-2)
+    for got, want in zip(lists, apart):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
