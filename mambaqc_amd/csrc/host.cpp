@@ -62,11 +62,19 @@ Tensor as_type(const Tensor& t, at::ScalarType type) {
   const Tensor v = t.requires_grad() ? t.detach() : t;
   return v.scalar_type() == type ? v : v.to(type);
 }
-// A parameter as the kernels read it: itself, or `convert`'s (_native.param_f32) where it is not that.
-Tensor weight(const Tensor& t, const py::object& convert) {
+// A parameter as the kernels read it: itself, or `convert`'s (_native.param_f32) where it is not that;
+// without one (in a backward, which runs without Python's lock) a copy.
+Tensor weight(const Tensor& t, const py::object* convert) {
   if (t.scalar_type() == at::kFloat && t.is_contiguous() && (uintptr_t)t.data_ptr() % 16 == 0)
     return as_type(t, at::kFloat);
-  return convert(t).cast<Tensor>();
+  return convert ? (*convert)(t).cast<Tensor>() : as_type(t, at::kFloat).contiguous();
+}
+// What a kernel reads beside the operands, dense in `type`, where it has these sizes.
+Tensor beside(const std::string& name, const char* what, const Tensor& t, at::IntArrayRef sizes,
+              at::ScalarType type, const Tensor& like) {
+  on_device(name, t, like);
+  TORCH_CHECK_VALUE(t.sizes() == sizes, name, ": ", what, " must be ", sizes, ", got ", t.sizes());
+  return as_type(t, type).contiguous();
 }
 bool records(std::initializer_list<MaybeTensor> inputs) {
   if (!at::GradMode::is_enabled()) return false;
@@ -135,9 +143,8 @@ struct GateNorm {
   int64_t z_row;
   MaybeTensor post;
   Tensor scale, pre;
-  GateNorm() = default;
   GateNorm(const Tensor& x_, const Tensor& y_, const MaybeTensor& z_, const MaybeTensor& post_,
-           const Tensor& scale_, const Tensor& pre_, const py::object& convert)
+           const Tensor& scale_, const Tensor& pre_, const py::object* convert)
       : z_row(0) {
     for (const Tensor* t : {&x_, &y_, &scale_, &pre_}) on_device("gate_norm_residual", *t, x_);
     if (post_) on_device("gate_norm_residual", *post_, x_), post = weight(*post_, convert);
@@ -169,9 +176,15 @@ std::tuple<Tensor, Tensor, MaybeTensor> gate_norm_forward(const GateNorm& o, dou
 }
 
 // dx, dy, dz, dpost, dscale, dpre.
-std::vector<MaybeTensor> gate_norm_backward(const GateNorm& o, const Tensor& stats, MaybeTensor dout,
+std::vector<MaybeTensor> gate_norm_backward(const GateNorm& o, Tensor stats, MaybeTensor dout,
                                             MaybeTensor dn) {
   const c10::DeviceGuard guard(o.x.device());
+  const auto grad = [&](const char* what, const Tensor& t) {
+    return beside("gate_norm_residual", what, t, o.x.sizes(), o.x.scalar_type(), o.x);
+  };
+  stats = beside("gate_norm_residual", "the rows' inverse norms", stats, {o.rows(), 2}, at::kFloat, o.x);
+  if (dout) dout = grad("the gradient of out", *dout);
+  if (dn) dn = grad("the gradient of n", *dn);
   Tensor dx = at::empty_like(o.x), dy = at::empty_like(o.x);
   MaybeTensor dz, dpost;
   if (o.z) dz = at::empty_like(o.x);
@@ -181,8 +194,6 @@ std::vector<MaybeTensor> gate_norm_backward(const GateNorm& o, const Tensor& sta
   }
   Tensor dscale = at::empty_like(o.scale), dpre = at::empty_like(o.pre);
   if (o.post) dpost = at::empty_like(*o.post);
-  if (dout) dout = dout->to(o.x.scalar_type()).contiguous();
-  if (dn) dn = dn->to(o.x.scalar_type()).contiguous();
   const int64_t bytes = mqc_gate_norm_workspace_bytes(o.rows(), o.d());
   const Tensor ws = workspace(bytes, "mqc_gate_norm_bwd", o.x);
   check(mqc_gate_norm_bwd(o.x.data_ptr(), o.y.data_ptr(), ptr(o.z), o.z_row, f32(o.post), f32(o.scale),
@@ -194,6 +205,13 @@ std::vector<MaybeTensor> gate_norm_backward(const GateNorm& o, const Tensor& sta
   return {dx, dy, dz, dpost, dscale, dpre};
 }
 
+bool gate_norm_shapes(const Tensor& x, const Tensor& y, const MaybeTensor& z, const MaybeTensor& post,
+                      const Tensor& scale, const Tensor& pre) {
+  if (x.dim() < 1 || y.sizes() != x.sizes() || (z && z->sizes() != x.sizes())) return false;
+  const at::IntArrayRef last = x.sizes().slice(x.dim() - 1);
+  return scale.sizes() == last && pre.sizes() == last && (!post || post->sizes() == last);
+}
+
 struct GateNormNode : torch::autograd::Function<GateNormNode> {
   // The first six are what gradients go to; `o` is read.
   static variable_list forward(AutogradContext* ctx, const Variable& x, const Variable& y,
@@ -202,15 +220,15 @@ struct GateNormNode : torch::autograd::Function<GateNormNode> {
     auto [out, n, stats] = gate_norm_forward(o, eps, true);
     ctx->save_for_backward({o.x, o.y, edge(o.z), edge(o.post), o.scale, o.pre, *stats});
     ctx->set_materialize_grads(false);
-    ctx->saved_data["z_row"] = o.z_row;
     ctx->saved_data["types"] = grad_types({x, y, z, post, scale, pre});
     return {out, n};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    // (what hooks on saved tensors give back may be laid out in other ways than what was saved)
     const auto s = ctx->get_saved_variables();
-    GateNorm o;
-    o.x = s[0], o.y = s[1], o.z = maybe(s[2]), o.z_row = ctx->saved_data["z_row"].toInt();
-    o.post = maybe(s[3]), o.scale = s[4], o.pre = s[5];
+    TORCH_CHECK_VALUE(gate_norm_shapes(s[0], s[1], maybe(s[2]), maybe(s[3]), s[4], s[5]),
+                      "gate_norm_residual: the saved tensors came back in other shapes");
+    const GateNorm o(s[0], s[1], maybe(s[2]), maybe(s[3]), s[4], s[5], nullptr);
     const auto got = gate_norm_backward(o, s[6], maybe(grads[0]), maybe(grads[1]));
     return once("gate_norm_residual", as_grads(got, ctx->saved_data["types"].toIntVector(), 8));
   }
@@ -221,10 +239,8 @@ std::optional<std::tuple<Tensor, Tensor>> gate_norm(const Tensor& x, const Tenso
                                                     const MaybeTensor& post, const Tensor& scale,
                                                     const Tensor& pre, double eps,
                                                     const py::object& convert) {
-  if (x.dim() < 1 || y.sizes() != x.sizes() || (z && z->sizes() != x.sizes())) return std::nullopt;
-  const at::IntArrayRef last = x.sizes().slice(x.dim() - 1);
-  if (scale.sizes() != last || pre.sizes() != last || (post && post->sizes() != last)) return std::nullopt;
-  const GateNorm o(x, y, z, post, scale, pre, convert);
+  if (!gate_norm_shapes(x, y, z, post, scale, pre)) return std::nullopt;
+  const GateNorm o(x, y, z, post, scale, pre, &convert);
   if (records({x, y, z, post, scale, pre})) {
     const auto out = GateNormNode::apply(x, y, z, post, scale, pre, o, eps);
     return std::make_tuple(out[0], out[1]);
@@ -256,9 +272,8 @@ struct Scan {
   int64_t x_row;
   Tensor rate;
   MaybeTensor reset;
-  Scan() = default;
   Scan(const std::string& name, const Tensor& dt_, const Tensor& g_, const Tensor& x_, const Tensor& rate_,
-       const MaybeTensor& reset_, const py::object& convert) {
+       const MaybeTensor& reset_, const py::object* convert) {
     for (const Tensor* t : {&x_, &dt_, &g_, &rate_}) on_device(name, *t, x_);
     rate = weight(rate_, convert);
     if (reset_) on_device(name, *reset_, x_), reset = reset_->contiguous();
@@ -273,16 +288,19 @@ struct Scan {
   int64_t d() const { return x.size(2); }
 };
 
+// States that a training forward stores of t steps.
+int64_t chunks(int64_t t) {
+  const int64_t every = mqc_gated_scan_chunk();
+  return (t + every - 1) / every;
+}
+
 std::tuple<Tensor, Tensor, MaybeTensor> scan_forward(const Scan& o, const MaybeTensor& h0, bool train) {
   const c10::DeviceGuard guard(o.x.device());
   if (h0) on_device("gated_scan", *h0, o.x);
   const int64_t b = o.b(), t = o.t(), d = o.d();
   Tensor y = at::empty({b, t, d}, o.x.options()), h = like_f32({b, d}, o.x);
   MaybeTensor carries;
-  if (train) {
-    const int64_t every = mqc_gated_scan_chunk();
-    carries = like_f32({b, (t + every - 1) / every, d}, o.x);
-  }
+  if (train) carries = like_f32({b, chunks(t), d}, o.x);
   const int64_t bytes = mqc_gated_scan_workspace_bytes(b, t, d);
   const Tensor ws = workspace(bytes, "mqc_gated_scan_fwd", o.x);
   check(mqc_gated_scan_fwd(o.dt.data_ptr(), o.dt_row, o.g.data_ptr(), o.g_row, o.x.data_ptr(), o.x_row,
@@ -294,19 +312,21 @@ std::tuple<Tensor, Tensor, MaybeTensor> scan_forward(const Scan& o, const MaybeT
 }
 
 // ddt, dg, dx, dlog_rate, dh0.
-std::vector<MaybeTensor> scan_backward(const Scan& o, const Tensor& carries, MaybeTensor dy,
-                                       MaybeTensor dh, bool want_dh0) {
+std::vector<MaybeTensor> scan_backward(const Scan& o, Tensor carries, MaybeTensor dy, MaybeTensor dh,
+                                       bool want_dh0) {
   const c10::DeviceGuard guard(o.x.device());
   const int64_t b = o.b(), t = o.t(), d = o.d();
+  carries = beside("gated_scan", "the chunks' states", carries, {b, chunks(t), d}, at::kFloat, o.x);
+  if (dy) dy = beside("gated_scan", "the gradient of y", *dy, {b, t, d}, o.x.scalar_type(), o.x);
+  if (dh) dh = beside("gated_scan", "the state's gradient", *dh, {b, d}, at::kFloat, o.x);
   const auto grad = [&] { return at::empty({b, t, d}, o.x.options()); };
   Tensor ddt = grad(), dg = grad(), dx = grad();
-  if (dh) dh = dh->to(at::kFloat).contiguous();
   MaybeTensor dh0;
   if (o.x.numel() == 0) {
     if (want_dh0) dh0 = dh ? dh->clone() : at::zeros({b, d}, o.rate.options());
     return {ddt, dg, dx, at::zeros_like(o.rate), dh0};
   }
-  dy = dy ? dy->to(o.x.scalar_type()).contiguous() : at::zeros({b, t, d}, o.x.options());
+  if (!dy) dy = at::zeros({b, t, d}, o.x.options());
   Tensor drate = at::empty_like(o.rate);
   if (want_dh0) dh0 = like_f32({b, d}, o.x);
   const int64_t bytes = mqc_gated_scan_workspace_bytes(b, t, d);
@@ -319,29 +339,6 @@ std::vector<MaybeTensor> scan_backward(const Scan& o, const Tensor& carries, May
   return {ddt, dg, dx, drate, dh0};
 }
 
-struct ScanNode : torch::autograd::Function<ScanNode> {
-  static variable_list forward(AutogradContext* ctx, const Variable& dt, const Variable& g,
-                               const Variable& x, const Variable& log_rate, const MaybeTensor& h0,
-                               const Scan& o, const MaybeTensor& h0_read) {
-    auto [y, h, carries] = scan_forward(o, h0_read, true);
-    ctx->save_for_backward({o.dt, o.g, o.x, o.rate, edge(o.reset), *carries});
-    ctx->set_materialize_grads(false);
-    ctx->saved_data["rows"] = std::vector<int64_t>{o.dt_row, o.g_row, o.x_row};
-    ctx->saved_data["types"] = grad_types({dt, g, x, log_rate, h0});
-    return {y, h};
-  }
-  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
-    const auto s = ctx->get_saved_variables();
-    const auto rows = ctx->saved_data["rows"].toIntVector();
-    const auto types = ctx->saved_data["types"].toIntVector();
-    Scan o;
-    o.dt = s[0], o.dt_row = rows[0], o.g = s[1], o.g_row = rows[1], o.x = s[2], o.x_row = rows[2];
-    o.rate = s[3], o.reset = maybe(s[4]);
-    const auto got = scan_backward(o, s[5], maybe(grads[0]), maybe(grads[1]), types[4] >= 0);
-    return once("gated_scan", as_grads(got, types, 7));
-  }
-};
-
 bool scan_shapes(const Tensor& dt, const Tensor& g, const Tensor& x, const Tensor& rate,
                  const MaybeTensor& h, const MaybeTensor& reset) {
   if (x.dim() != 3 || dt.sizes() != x.sizes() || g.sizes() != x.sizes()) return false;
@@ -350,12 +347,34 @@ bool scan_shapes(const Tensor& dt, const Tensor& g, const Tensor& x, const Tenso
          (!reset || (reset->sizes() == at::IntArrayRef{b, t} && reset->scalar_type() == at::kBool));
 }
 
+struct ScanNode : torch::autograd::Function<ScanNode> {
+  static variable_list forward(AutogradContext* ctx, const Variable& dt, const Variable& g,
+                               const Variable& x, const Variable& log_rate, const MaybeTensor& h0,
+                               const Scan& o, const MaybeTensor& h0_read) {
+    auto [y, h, carries] = scan_forward(o, h0_read, true);
+    ctx->save_for_backward({o.dt, o.g, o.x, o.rate, edge(o.reset), *carries});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["types"] = grad_types({dt, g, x, log_rate, h0});
+    return {y, h};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    // (laid out anew, as in GateNormNode)
+    const auto s = ctx->get_saved_variables();
+    const auto types = ctx->saved_data["types"].toIntVector();
+    TORCH_CHECK_VALUE(scan_shapes(s[0], s[1], s[2], s[3], std::nullopt, maybe(s[4])),
+                      "gated_scan: the saved tensors came back in other shapes");
+    const Scan o("gated_scan", s[0], s[1], s[2], s[3], maybe(s[4]), nullptr);
+    const auto got = scan_backward(o, s[5], maybe(grads[0]), maybe(grads[1]), types[4] >= 0);
+    return once("gated_scan", as_grads(got, types, 7));
+  }
+};
+
 // gated_scan (y, last state), or nothing where the arguments do not match.
 std::optional<std::tuple<Tensor, Tensor>> gated_scan(const Tensor& dt, const Tensor& g, const Tensor& x,
                                                      const Tensor& log_rate, const MaybeTensor& h0,
                                                      const MaybeTensor& reset, const py::object& convert) {
   if (!scan_shapes(dt, g, x, log_rate, h0, reset)) return std::nullopt;
-  const Scan o("gated_scan", dt, g, x, log_rate, reset, convert);
+  const Scan o("gated_scan", dt, g, x, log_rate, reset, &convert);
   MaybeTensor state;
   if (h0) state = as_type(*h0, at::kFloat).contiguous();
   if (records({dt, g, x, log_rate, h0})) {
@@ -372,7 +391,7 @@ MaybeTensor gated_scan_step(const Tensor& dt, const Tensor& g, const Tensor& x, 
   if (!scan_shapes(dt, g, x, log_rate, h, std::nullopt) || x.size(1) != 1 ||
       h.scalar_type() != at::kFloat || !h.is_contiguous())
     return std::nullopt;
-  const Scan o("gated_scan_step_", dt, g, x, log_rate, std::nullopt, convert);
+  const Scan o("gated_scan_step_", dt, g, x, log_rate, std::nullopt, &convert);
   const c10::DeviceGuard guard(o.x.device());
   on_device("gated_scan_step_", h, o.x);
   Tensor y = at::empty({o.b(), 1, o.d()}, o.x.options());
@@ -438,8 +457,10 @@ void changed(const Lists& lists) {
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   py::class_<GateNorm>(m, "GateNorm")
-      .def(py::init<const Tensor&, const Tensor&, const MaybeTensor&, const MaybeTensor&, const Tensor&,
-                    const Tensor&, const py::object&>());
+      .def(py::init([](const Tensor& x, const Tensor& y, const MaybeTensor& z, const MaybeTensor& post,
+                       const Tensor& scale, const Tensor& pre, const py::object& convert) {
+        return GateNorm(x, y, z, post, scale, pre, &convert);
+      }));
   m.def("spaced_rows", [](const Tensor& t, py::object type) {
     return spaced_rows(t, torch::python::detail::py_object_to_dtype(type));
   });
@@ -447,8 +468,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gate_norm_backward", &gate_norm_backward);
   m.def("gate_norm", &gate_norm);
   py::class_<Scan>(m, "Scan")
-      .def(py::init<const std::string&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
-                    const MaybeTensor&, const py::object&>());
+      .def(py::init([](const std::string& name, const Tensor& dt, const Tensor& g, const Tensor& x,
+                       const Tensor& rate, const MaybeTensor& reset, const py::object& convert) {
+        return Scan(name, dt, g, x, rate, reset, &convert);
+      }));
   m.def("token_rows", [](const Tensor& t, py::object type) {
     return token_rows(t, torch::python::detail::py_object_to_dtype(type));
   });

@@ -314,3 +314,43 @@ def test_compiles():
     for a, b in zip([*got, *torch.autograd.grad(got, some, [dout, dn])],
                     [*want, *torch.autograd.grad(want, some, [dout, dn])]):
         assert torch.equal(a, b)
+
+
+def copies(order):
+    """Hooks on saved tensors that give back dense copies, or ones whose axes lie in another order."""
+    def pack(t):
+        kept = torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+        return kept if order == "dense" or t.dim() < 2 else kept.transpose(0, 1).contiguous().transpose(0, 1)
+    return torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t)
+
+
+@pytest.mark.parametrize("hooks", [lambda: copies("dense"), lambda: copies("turned"),
+                                   torch.autograd.graph.save_on_cpu])
+@pytest.mark.parametrize("shape", [(1, 40), (50, 40), (30, 515), (2, 3, 300)])
+def test_saved_tensors_come_back_laid_out_anew(hooks, shape):
+    """The backward reads what hooks on saved tensors give back, not the forward's rows."""
+    v, dout, dn = make(shape, torch.float32)
+    wide = torch.randn(*shape[:-1], 3 * shape[-1], device=DEV)
+
+    def grads():
+        leaves = {k: t.detach().requires_grad_() for k, t in v.items() if k != "z"}
+        leaf = wide.detach().requires_grad_()
+        outs = call({**leaves, "z": leaf[..., shape[-1]:2 * shape[-1]]})
+        return torch.autograd.grad(outs, [leaf, *leaves.values()], [dout, dn])
+
+    want = grads()
+    with hooks():
+        got = grads()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_saved_tensors_of_other_shapes_are_refused():
+    v, dout, dn = make((30, 40), torch.float32)
+    v["x"].requires_grad_()
+    for shape in [(30, 40), (40,), (30, 2)]:
+        with torch.autograd.graph.saved_tensors_hooks(
+                lambda t: t, lambda t: t[:1] if tuple(t.shape) == shape else t):
+            out, n = call(v)
+        with pytest.raises(ValueError, match="must be|other shapes"):
+            (out * dout + n * dn).sum().backward()

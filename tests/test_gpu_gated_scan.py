@@ -491,3 +491,45 @@ def test_sizes_past_the_cache_equal_their_parts(dtype, shape):
         want = torch.autograd.grad((some, last), leaves, (dy[..., part], torch.ones_like(last)))
         assert torch.equal(y[..., part], some) and torch.equal(h[..., part], last)
         assert all(torch.equal(g[..., part], w) for g, w in zip(grads, want))
+
+
+def copies(order):
+    """Hooks on saved tensors that give back dense copies, or ones whose axes lie in another order."""
+    def pack(t):
+        kept = torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+        return kept if order == "dense" or t.dim() < 2 else kept.transpose(0, 1).contiguous().transpose(0, 1)
+    return torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t)
+
+
+@pytest.mark.parametrize("hooks", [lambda: copies("dense"), lambda: copies("turned"),
+                                   torch.autograd.graph.save_on_cpu])
+@pytest.mark.parametrize("t", [1, 40, 300])
+def test_saved_tensors_come_back_laid_out_anew(hooks, t):
+    """The backward reads what hooks on saved tensors give back, not the forward's rows."""
+    wide = torch.randn(3, t, 5 * 24, generator=torch.Generator(DEV).manual_seed(t), device=DEV)
+    cut = torch.arange(3 * t, device=DEV).reshape(3, t) % 37 == 5
+    dy = torch.randn(3, t, 24, device=DEV)
+
+    def grads():
+        leaf = wide.detach().requires_grad_()
+        lam = torch.linspace(-4, 1, 24, device=DEV).requires_grad_()
+        y, h = gated_scan(leaf[..., 24:48], leaf[..., 48:72], leaf[..., 96:], lam, reset=cut,
+                          return_state=True)
+        return torch.autograd.grad([y, h], [leaf, lam], [dy, torch.ones_like(h)])
+
+    want = grads()
+    with hooks():
+        got = grads()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_saved_tensors_of_other_shapes_are_refused():
+    dt, g, x, lam, _, _, dy, _ = make(2, 70, 24, torch.float32)
+    x.requires_grad_()
+    for shape in [(2, 70, 24), (24,), (2, 2, 24)]:
+        with torch.autograd.graph.saved_tensors_hooks(
+                lambda t: t, lambda t: t[:1] if tuple(t.shape) == shape else t):
+            y = gated_scan(dt, g, x, lam)
+        with pytest.raises(ValueError, match="must be|other shapes"):
+            y.backward(dy)
