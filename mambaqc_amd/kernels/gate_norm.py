@@ -39,6 +39,7 @@ def _z_rows(z: torch.Tensor, dtype: torch.dtype):
 
 def _operands(x, y, z, post_weight, scale, pre_weight):
     """The operands as the kernels read them, weights in fp32."""
+    _check(x, y, z, post_weight, scale, pre_weight)
     return nat.host().GateNorm(x, y, z, post_weight, scale, pre_weight, nat.param_f32)
 
 

@@ -44,8 +44,9 @@ def scan_chunk() -> int:
     return int(nat.load().mqc_gated_scan_chunk())
 
 
-def _operands(name, dt_raw, g_raw, x, log_rate, reset=None):
-    """The operands as the kernels read them, log_rate in fp32."""
+def _operands(name, dt_raw, g_raw, x, log_rate, reset=None, h0=None):
+    """The operands as the kernels read them, log_rate in fp32; h0 is only checked."""
+    _check(name, dt_raw, g_raw, x, log_rate, h0, reset)
     return nat.host().Scan(name, dt_raw, g_raw, x, log_rate, reset, nat.param_f32)
 
 

@@ -493,7 +493,7 @@ def gated_scan(dt_raw: Tensor, g_raw: Tensor, x: Tensor, log_rate: Tensor,
                h0: Optional[Tensor] = None,
                reset: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
     """Inference: (y in the promoted dtype, h_last fp32 [B, W])."""
-    ops = gated._operands("gated_scan", dt_raw, g_raw, x, log_rate, reset)
+    ops = gated._operands("gated_scan", dt_raw, g_raw, x, log_rate, reset, h0)
     return nat.host().scan_forward(ops, gated._state(h0), False)[:2]
 
 
@@ -509,7 +509,7 @@ def gated_scan_train(dt_raw: Tensor, g_raw: Tensor, x: Tensor, log_rate: Tensor,
                      h0: Optional[Tensor] = None,
                      reset: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
     """(y, h_last, the chunks' entry states for the backward)."""
-    ops = gated._operands("gated_scan", dt_raw, g_raw, x, log_rate, reset)
+    ops = gated._operands("gated_scan", dt_raw, g_raw, x, log_rate, reset, h0)
     return nat.host().scan_forward(ops, gated._state(h0), True)
 
 

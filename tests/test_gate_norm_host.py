@@ -74,3 +74,17 @@ def test_fake_kernels():
         grads = torch.ops.mambaqc.gate_norm_residual_backward(x, x, None, w, w, w, stats, x, x)
         assert grads[0].dtype == torch.bfloat16 and grads[2].numel() == 0
         assert all(g.shape == (6,) and g.dtype == torch.float32 for g in grads[3:])
+
+
+def test_registered_operators_check_their_arguments():
+    """torch.ops.mambaqc.gate_norm_residual* refuse what gate_norm_residual refuses."""
+    x, w = torch.zeros(2, 3, 4), torch.zeros(4)
+    for op, rest in ((torch.ops.mambaqc.gate_norm_residual, ()),
+                     (torch.ops.mambaqc.gate_norm_residual_backward, (torch.zeros(6, 2), x, x))):
+        with pytest.raises(ValueError, match="one shape"):
+            op(x, x[:1], None, None, w, w, *rest)
+        with pytest.raises(ValueError, match="z must be"):
+            op(x, x, x[..., :2], None, w, w, *rest)
+        for bad in ((w[:3], w, w), (w, w[:3], w), (w, w, w[:3])):
+            with pytest.raises(ValueError, match="must be \\[4\\]"):
+                op(x, x, x, *bad, *rest)

@@ -92,3 +92,24 @@ def test_fake_kernels():
         assert y.dtype == torch.bfloat16 and carries.dtype == torch.float32
         every = nat.load().mqc_gated_scan_chunk()
         assert carries.shape == (2, -(-70 // every), 6)
+
+
+def test_registered_operators_check_their_arguments():
+    """torch.ops.mambaqc.gated_scan* refuse what gated_scan refuses, before anything reads it."""
+    x, lam, h = z(2, 3, 4), z(4), z(2, 4)
+    ops = torch.ops.mambaqc
+    for op in (ops.gated_scan, ops.gated_scan_train):
+        with pytest.raises(ValueError, match="one shape"):
+            op(z(1, 3, 4), x, x, lam, None, None)
+        with pytest.raises(ValueError, match="one shape"):
+            op(z(3, 4), z(3, 4), z(3, 4), lam, None, None)
+        with pytest.raises(ValueError, match="log_rate"):
+            op(x, x, x, z(3), None, None)
+        with pytest.raises(ValueError, match="state"):
+            op(x, x, x, lam, z(1, 4), None)
+        with pytest.raises(ValueError, match="reset"):
+            op(x, x, x, lam, None, z(2, 3, dtype=torch.int32))
+    with pytest.raises(ValueError, match="one shape"):
+        ops.gated_scan_backward(x, x, z(2, 9, 4), lam, None, z(2, 1, 4), x, h)
+    with pytest.raises(ValueError, match="reset"):
+        ops.gated_scan_backward(x, x, x, lam, z(2, 2, dtype=torch.bool), z(2, 1, 4), x, h)

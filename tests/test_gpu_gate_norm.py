@@ -354,3 +354,16 @@ def test_saved_tensors_of_other_shapes_are_refused():
             out, n = call(v)
         with pytest.raises(ValueError, match="must be|other shapes"):
             (out * dout + n * dn).sum().backward()
+
+
+def test_registered_backward_checks_what_it_reads():
+    v, dout, dn = make((30, 40), torch.float32)
+    ops = (v["x"], v["y"], v["z"], v["post"], v["scale"], v["pre"])
+    stats = torch.ops.mambaqc.gate_norm_residual(*ops)[2]
+    op = torch.ops.mambaqc.gate_norm_residual_backward
+    op(*ops, stats, dout, dn)
+    for bad in ((stats[:29], dout, dn), (stats, dout[:29], dn), (stats, dout, dn[:, :39])):
+        with pytest.raises(ValueError, match="must be"):
+            op(*ops, *bad)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        op(*ops, stats.cpu(), dout, dn)

@@ -533,3 +533,15 @@ def test_saved_tensors_of_other_shapes_are_refused():
             y = gated_scan(dt, g, x, lam)
         with pytest.raises(ValueError, match="must be|other shapes"):
             y.backward(dy)
+
+
+def test_registered_backward_checks_what_it_reads():
+    dt, g, x, lam, _, _, dy, dh = make(2, 70, 24, torch.float32)
+    carries = torch.ops.mambaqc.gated_scan_train(dt, g, x, lam, None, None)[2]
+    op = torch.ops.mambaqc.gated_scan_backward
+    op(dt, g, x, lam, None, carries, dy, dh)
+    for bad in ((carries[:, :1], dy, dh), (carries, dy[:, :69], dh), (carries, dy, dh[:1])):
+        with pytest.raises(ValueError, match="must be"):
+            op(dt, g, x, lam, None, *bad)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        op(dt, g, x, lam, None, carries.cpu(), dy, dh)
