@@ -70,6 +70,7 @@ __device__ inline float scan_a(float c) { return scan_fast(c) ? -c : 1.f - c; }
 __device__ inline float scan_w(float c) { return scan_fast(c) ? 1.f + c : c; }
 // a v.
 __device__ inline float scan_fade(float c, float v) { return fmaf(-c, v, scan_fast(c) ? 0.f : v); }
+__device__ inline bool scan_finite(float v) { return fabsf(v) < __builtin_inff(); }
 
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 struct ScanRate { float log2_rate, rate; };
@@ -100,6 +101,29 @@ __device__ inline float scan_p_low(float dt, ScanRate r) {
 constexpr float kScanCut = 2.f;
 __device__ inline float scan_join(float c, float u, float h) {
   return c == kScanCut ? u : u + scan_fade(c, h);
+}
+// An infinite h stays infinite over any steps, as it does step by step, where its fade is NaN (h - c h, or
+// 0 h where the decay of many steps underflows). Such a NaN lasts to the end of the joins or to a cut, so
+// joins are walked plainly, and again with INF where the last of them is not finite (a test in each join
+// cost 2.5 % of a long scan's forward, this 0 to 1).
+template <bool INF>
+__device__ inline float scan_join_as(float c, float u, float h) {
+  return INF && c != kScanCut && !scan_finite(h) ? u + h : scan_join(c, u, h);
+}
+template <typename Walk>
+__device__ inline float scan_joins(Walk walk, bool on = true) {
+  const float h = walk(std::false_type());
+  if (__builtin_expect(__any(on && !scan_finite(h)), 0)) return walk(std::true_type());
+  return h;
+}
+// h through the spans from, from + by, .. before `to`: their codes c and u.
+__device__ inline float scan_spans(int from, int to, int by, const float (*c)[64], const float (*u)[64],
+                                   float h, int lane) {
+  return scan_joins([&](auto inf) {
+    float v = h;
+    for (int w = from; w != to; w += by) v = scan_join_as<decltype(inf)::value>(c[w][lane], u[w][lane], v);
+    return v;
+  });
 }
 struct ScanDecay {
   float p = 0.f, a = 1.f;
@@ -243,9 +267,15 @@ __device__ inline float scan_entry(const ScanArgs<T>& k, const ScanPlace& at, in
   __syncthreads();
   float h = first;
   if (wave == 0) {
-    if (group > 0) h = words[0][kScanGroup - 1][lane];
-    for (int m = 0; m < member; ++m) h = scan_join(words[0][m][lane], words[1][m][lane], h);
-    if (member == kScanGroup - 1 && on) post(ends + group * k.width + in, word_of(scan_join(c, u, h)));
+    const float before = group > 0 ? words[0][kScanGroup - 1][lane] : first;
+    h = scan_joins([&](auto inf) {
+      float v = before;
+      for (int m = 0; m < member; ++m)
+        v = scan_join_as<decltype(inf)::value>(words[0][m][lane], words[1][m][lane], v);
+      return v;
+    }, on);
+    if (member == kScanGroup - 1 && on)
+      post(ends + group * k.width + in, word_of(scan_join_as<true>(c, u, h)));
   }
   return h;
 }
@@ -379,15 +409,19 @@ __global__ __launch_bounds__(64 * kScanWaves, 6) void gated_scan_fwd_kernel(Scan
   }
   __syncthreads();
   if constexpr (CHAIN) {
-    float cu = h, cc = 0.f;
+    float cu = 0.f, cc = 0.f;
     if (wave == 0) {
       ScanJoint all;
       all.cut = at.n == 0;  // the first chunk posts its state (h0 is not read again: h_last may be h0)
 #pragma unroll
-      for (int w = 0; w < kScanWaves; ++w) {
-        all.then(part[0][w][lane]);
-        cu = scan_join(part[0][w][lane], part[1][w][lane], cu);
-      }
+      for (int w = 0; w < kScanWaves; ++w) all.then(part[0][w][lane]);
+      cu = scan_joins([&](auto inf) {
+        float v = h;
+#pragma unroll
+        for (int w = 0; w < kScanWaves; ++w)
+          v = scan_join_as<decltype(inf)::value>(part[0][w][lane], part[1][w][lane], v);
+        return v;
+      });
       cc = all.code();
     }
     h = scan_entry<kScanWaves, false>(k, at, chunks, in, on, wave, cc, cu, h, words);
@@ -399,7 +433,7 @@ __global__ __launch_bounds__(64 * kScanWaves, 6) void gated_scan_fwd_kernel(Scan
     if (k.seq == 0 && k.h_last && on && wave == 0) k.h_last[b * k.width + d] = h;
     return;
   }
-  for (int w = 0; w < wave; ++w) h = scan_join(part[0][w][lane], part[1][w][lane], h);
+  h = scan_spans(0, wave, 1, part[0], part[1], h, lane);
   if (k.carries && t0 % kScanChunk == 0 && on) {
     const int64_t every = (k.seq + kScanChunk - 1) / kScanChunk;
     k.carries[(b * every + t0 / kScanChunk) * k.width + d] = h;
@@ -522,10 +556,14 @@ __global__ __launch_bounds__(64 * kBackWaves) void gated_scan_bwd_kernel(ScanArg
     if (wave == 0) {
       ScanJoint all;
 #pragma unroll
-      for (int w = kBackWaves - 1; w >= 0; --w) {
-        all.then(part[0][w][lane]);
-        cv = scan_join(part[0][w][lane], part[2][w][lane], cv);
-      }
+      for (int w = kBackWaves - 1; w >= 0; --w) all.then(part[0][w][lane]);
+      cv = scan_joins([&](auto inf) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = kBackWaves - 1; w >= 0; --w)
+          v = scan_join_as<decltype(inf)::value>(part[0][w][lane], part[2][w][lane], v);
+        return v;
+      });
       cc = all.code();
     }
     A = scan_entry<kBackWaves, true>(k, at, chunks, in, on, wave, cc, cv, A, words);
@@ -536,8 +574,8 @@ __global__ __launch_bounds__(64 * kBackWaves) void gated_scan_bwd_kernel(ScanArg
   float drate = 0.f;
   if (n > 0) {
     float h = k.carries[(b * chunks + j) * k.width + dc];
-    for (int w = 0; w < wave; ++w) h = scan_join(part[0][w][lane], part[1][w][lane], h);
-    for (int w = kBackWaves - 1; w > wave; --w) A = scan_join(part[0][w][lane], part[2][w][lane], A);
+    h = scan_spans(0, wave, 1, part[0], part[1], h, lane);
+    A = scan_spans(kBackWaves - 1, wave, -1, part[0], part[2], A, lane);
     const auto back = [&](auto plain) {
       constexpr bool PLAIN = decltype(plain)::value;
 #pragma unroll
@@ -594,7 +632,8 @@ __global__ __launch_bounds__(256) void gated_scan_step_kernel(ScanArgs<T> k, flo
   float a, w;
   scan_pair(p, a, w);
   // Away from whichever is the larger part: an a near 1, rounded, would leave its mark at each token.
-  const float v = p < 1.f ? fmaf(w, s - old, old) : fmaf(a, old - s, s);
+  float v = p < 1.f ? fmaf(w, s - old, old) : fmaf(a, old - s, s);
+  if (!scan_finite(v)) v = fmaf(a, old, w * s);  // infinities do not meet their negatives
   h[b * k.width + d] = v;
   store_scalar(k.y + b * k.width + d, v);
 }

@@ -545,3 +545,48 @@ def test_registered_backward_checks_what_it_reads():
             op(dt, g, x, lam, None, *bad)
     with pytest.raises(RuntimeError, match="ROCm device"):
         op(dt, g, x, lam, None, carries.cpu(), dy, dh)
+
+
+def hold_kinds(what, got, ref):
+    """hold() where the reference is finite; the same infinities, and nothing finite for a NaN."""
+    want, mag = ref
+    fine, inf = want.isfinite(), want.isinf()
+    assert torch.equal(got.double()[inf], want[inf]), what
+    assert not got[want.isnan()].isfinite().any(), what
+    hold(what, torch.where(fine, got, 0), (torch.where(fine, want, 0.0), torch.where(fine, mag, 0.0)))
+
+
+@pytest.mark.parametrize("t", [5, 40, 300, 2500])
+@pytest.mark.parametrize("where", ["h0", "x", "dy", "dh"])
+def test_infinite_states_stay_infinite(t, where):
+    """Slow channels, and ones whose decay over a span underflows, from a state, a token or a gradient
+    that is infinite: inf on and on, as the recurrence has it token by token, and not NaN."""
+    d = 70
+    dt, g, x, _, h0, _, dy, dh = make(1, t, d, torch.float32)
+    lam = torch.linspace(-7, 2.5, d, device=DEV)
+    mid = t // 2
+    for i, v in enumerate((float("inf"), -float("inf"))):
+        {"h0": h0, "x": x[:, mid], "dy": dy[:, mid], "dh": dh}[where][:, i::3] = v
+    ref = walk(dt, g, x, lam, h0, None, dy, dh)
+    assert ref["y"][0].isnan().sum() == 0
+    leaves = [v.requires_grad_() for v in (dt, g, x, lam, h0)]
+    y, h = gated_scan(*leaves[:4], h0=h0, return_state=True)
+    hold_kinds("y", y.detach(), ref["y"])
+    hold_kinds("h", h.detach(), ref["h"])
+    for name, got in zip(["dt", "g", "x", "rate", "h0"], torch.autograd.grad([y, h], leaves, [dy, dh])):
+        hold_kinds(name, got, ref[name])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_step_with_infinities(dtype):
+    dt, g, x, _, h0, _, _, _ = make(2, 6, 90, dtype)
+    lam = torch.linspace(-7, 2.5, 90, device=DEV)
+    h0[0, ::3], h0[1, 1::3] = float("inf"), -float("inf")
+    x[0, 2, 1::3], x[1, 3, ::3] = float("inf"), -float("inf")
+    ref = walk(dt, g, x, lam, h0, None)
+    assert ref["y"][0].isnan().sum() == 0
+    h = h0.clone()
+    for i in range(6):
+        y = gated_scan_step_(dt[:, i:i + 1], g[:, i:i + 1], x[:, i:i + 1], lam, h)
+        hold_kinds("y", y[:, 0], tuple(v[:, i] for v in ref["y"]))
+    hold_kinds("h", h, ref["h"])
