@@ -56,6 +56,12 @@ void on_device(const std::string& name, const Tensor& t, const Tensor& like) {
   TORCH_CHECK(t.device() == like.device(), "mambaqc_amd.", name, ": tensors on different devices (",
               like.device(), ", ", t.device(), ")");
 }
+// Forward-mode gradients would be lost without a word: the kernels see values alone.
+void no_tangents(const std::string& name, std::initializer_list<MaybeTensor> inputs) {
+  for (const auto& t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->_fw_grad(0).defined(), name,
+                                ": forward-mode automatic differentiation is not supported");
+}
 // Autograd does not see what the operands go through; their gradients' edges are the node's.
 Tensor as_type(const Tensor& t, at::ScalarType type) {
   const at::NoGradGuard none;
@@ -72,6 +78,7 @@ Tensor weight(const Tensor& t, const py::object* convert) {
 // What a kernel reads beside the operands, dense in `type`, where it has these sizes.
 Tensor beside(const std::string& name, const char* what, const Tensor& t, at::IntArrayRef sizes,
               at::ScalarType type, const Tensor& like) {
+  no_tangents(name, {t});
   on_device(name, t, like);
   TORCH_CHECK_VALUE(t.sizes() == sizes, name, ": ", what, " must be ", sizes, ", got ", t.sizes());
   return as_type(t, type).contiguous();
@@ -146,6 +153,7 @@ struct GateNorm {
   GateNorm(const Tensor& x_, const Tensor& y_, const MaybeTensor& z_, const MaybeTensor& post_,
            const Tensor& scale_, const Tensor& pre_, const py::object* convert)
       : z_row(0) {
+    no_tangents("gate_norm_residual", {x_, y_, z_, post_, scale_, pre_});
     for (const Tensor* t : {&x_, &y_, &scale_, &pre_}) on_device("gate_norm_residual", *t, x_);
     if (post_) on_device("gate_norm_residual", *post_, x_), post = weight(*post_, convert);
     scale = weight(scale_, convert), pre = weight(pre_, convert);
@@ -272,9 +280,12 @@ struct Scan {
   int64_t x_row;
   Tensor rate;
   MaybeTensor reset;
+  // (the state h is only looked at)
   Scan(const std::string& name, const Tensor& dt_, const Tensor& g_, const Tensor& x_, const Tensor& rate_,
-       const MaybeTensor& reset_, const py::object* convert) {
+       const MaybeTensor& reset_, const MaybeTensor& h, const py::object* convert) {
+    no_tangents(name, {dt_, g_, x_, rate_, h});
     for (const Tensor* t : {&x_, &dt_, &g_, &rate_}) on_device(name, *t, x_);
+    if (h) on_device(name, *h, x_);
     rate = weight(rate_, convert);
     if (reset_) on_device(name, *reset_, x_), reset = reset_->contiguous();
     const auto type =
@@ -296,7 +307,6 @@ int64_t chunks(int64_t t) {
 
 std::tuple<Tensor, Tensor, MaybeTensor> scan_forward(const Scan& o, const MaybeTensor& h0, bool train) {
   const c10::DeviceGuard guard(o.x.device());
-  if (h0) on_device("gated_scan", *h0, o.x);
   const int64_t b = o.b(), t = o.t(), d = o.d();
   Tensor y = at::empty({b, t, d}, o.x.options()), h = like_f32({b, d}, o.x);
   MaybeTensor carries;
@@ -363,7 +373,7 @@ struct ScanNode : torch::autograd::Function<ScanNode> {
     const auto types = ctx->saved_data["types"].toIntVector();
     TORCH_CHECK_VALUE(scan_shapes(s[0], s[1], s[2], s[3], std::nullopt, maybe(s[4])),
                       "gated_scan: the saved tensors came back in other shapes");
-    const Scan o("gated_scan", s[0], s[1], s[2], s[3], maybe(s[4]), nullptr);
+    const Scan o("gated_scan", s[0], s[1], s[2], s[3], maybe(s[4]), std::nullopt, nullptr);
     const auto got = scan_backward(o, s[5], maybe(grads[0]), maybe(grads[1]), types[4] >= 0);
     return once("gated_scan", as_grads(got, types, 7));
   }
@@ -374,7 +384,7 @@ std::optional<std::tuple<Tensor, Tensor>> gated_scan(const Tensor& dt, const Ten
                                                      const Tensor& log_rate, const MaybeTensor& h0,
                                                      const MaybeTensor& reset, const py::object& convert) {
   if (!scan_shapes(dt, g, x, log_rate, h0, reset)) return std::nullopt;
-  const Scan o("gated_scan", dt, g, x, log_rate, reset, &convert);
+  const Scan o("gated_scan", dt, g, x, log_rate, reset, h0, &convert);
   MaybeTensor state;
   if (h0) state = as_type(*h0, at::kFloat).contiguous();
   if (records({dt, g, x, log_rate, h0})) {
@@ -391,9 +401,8 @@ MaybeTensor gated_scan_step(const Tensor& dt, const Tensor& g, const Tensor& x, 
   if (!scan_shapes(dt, g, x, log_rate, h, std::nullopt) || x.size(1) != 1 ||
       h.scalar_type() != at::kFloat || !h.is_contiguous())
     return std::nullopt;
-  const Scan o("gated_scan_step_", dt, g, x, log_rate, std::nullopt, &convert);
+  const Scan o("gated_scan_step_", dt, g, x, log_rate, std::nullopt, h, &convert);
   const c10::DeviceGuard guard(o.x.device());
-  on_device("gated_scan_step_", h, o.x);
   Tensor y = at::empty({o.b(), 1, o.d()}, o.x.options());
   check(mqc_gated_scan_step(o.dt.data_ptr(), o.dt_row, o.g.data_ptr(), o.g_row, o.x.data_ptr(), o.x_row,
                             f32(o.rate), (float*)h.data_ptr(), y.data_ptr(), o.b(), o.d(),
@@ -469,8 +478,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gate_norm", &gate_norm);
   py::class_<Scan>(m, "Scan")
       .def(py::init([](const std::string& name, const Tensor& dt, const Tensor& g, const Tensor& x,
-                       const Tensor& rate, const MaybeTensor& reset, const py::object& convert) {
-        return Scan(name, dt, g, x, rate, reset, &convert);
+                       const Tensor& rate, const MaybeTensor& reset, const MaybeTensor& h0,
+                       const py::object& convert) {
+        return Scan(name, dt, g, x, rate, reset, h0, &convert);
       }));
   m.def("token_rows", [](const Tensor& t, py::object type) {
     return token_rows(t, torch::python::detail::py_object_to_dtype(type));

@@ -54,7 +54,7 @@ def gate_norm_residual(x: torch.Tensor, y: torch.Tensor, z: torch.Tensor | None 
     without z the gate is 1, without post_weight y is not normalised. x is the residual stream, y a
     block's output, out the stream after it and n the next block's input. Norms and sums are fp32,
     and n comes from out before its rounding. d is at most 8192. Differentiable in every tensor
-    argument when autograd is recording."""
+    argument when autograd is recording (in reverse; forward mode is refused)."""
     if nat.compiling():
         _check(x, y, z, post_weight, scale, pre_weight)
         return torch.ops.mambaqc.gate_norm_residual(x, y, z, post_weight, scale, pre_weight, eps)[:2]

@@ -45,9 +45,9 @@ def scan_chunk() -> int:
 
 
 def _operands(name, dt_raw, g_raw, x, log_rate, reset=None, h0=None):
-    """The operands as the kernels read them, log_rate in fp32; h0 is only checked."""
+    """The operands as the kernels read them, log_rate in fp32; h0 is only looked at."""
     _check(name, dt_raw, g_raw, x, log_rate, h0, reset)
-    return nat.host().Scan(name, dt_raw, g_raw, x, log_rate, reset, nat.param_f32)
+    return nat.host().Scan(name, dt_raw, g_raw, x, log_rate, reset, h0, nat.param_f32)
 
 
 def _state(h0):
@@ -63,7 +63,8 @@ def gated_scan(dt_raw: torch.Tensor, g_raw: torch.Tensor, x: torch.Tensor, log_r
 
     h0: the state before the first token (None: zeros). reset: bool [batch, seq_len], true at the
     first token of a packed document: nothing from before it is seen, NaN included. States are
-    fp32. Differentiable in every tensor argument when autograd is recording."""
+    fp32. Differentiable in every tensor argument when autograd is recording (in reverse; forward mode
+    is refused)."""
     if nat.compiling():
         _check("gated_scan", dt_raw, g_raw, x, log_rate, h0, reset)
         train = torch.is_grad_enabled() and any(v is not None and v.requires_grad

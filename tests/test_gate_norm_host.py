@@ -88,3 +88,16 @@ def test_registered_operators_check_their_arguments():
         for bad in ((w[:3], w, w), (w, w[:3], w), (w, w, w[:3])):
             with pytest.raises(ValueError, match="must be \\[4\\]"):
                 op(x, x, x, *bad, *rest)
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_refuses_forward_mode(which):
+    """A tangent would be lost: the kernels see the values alone."""
+    ops = [torch.zeros(3, 4) for _ in range(3)] + [torch.zeros(4) for _ in range(3)]
+    with torch.autograd.forward_ad.dual_level():
+        ops[which] = torch.autograd.forward_ad.make_dual(ops[which], torch.ones_like(ops[which]))
+        x, y, gate, post, scale, pre = ops
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            gate_norm_residual(x, y, gate, scale=scale, pre_weight=pre, post_weight=post)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.ops.mambaqc.gate_norm_residual(*ops)

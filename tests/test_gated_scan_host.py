@@ -113,3 +113,17 @@ def test_registered_operators_check_their_arguments():
         ops.gated_scan_backward(x, x, z(2, 9, 4), lam, None, z(2, 1, 4), x, h)
     with pytest.raises(ValueError, match="reset"):
         ops.gated_scan_backward(x, x, x, lam, z(2, 2, dtype=torch.bool), z(2, 1, 4), x, h)
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_refuses_forward_mode(which):
+    """A tangent would be lost: the kernels see the values alone."""
+    ops = [z(2, 1, 4) for _ in range(3)] + [z(4), z(2, 4)]
+    with torch.autograd.forward_ad.dual_level():
+        ops[which] = torch.autograd.forward_ad.make_dual(ops[which], torch.ones_like(ops[which]))
+        calls = [lambda: gated_scan(*ops[:4], h0=ops[4]), lambda: gated_scan_step_(*ops),
+                 lambda: torch.ops.mambaqc.gated_scan(*ops, None),
+                 lambda: torch.ops.mambaqc.gated_scan_train(*ops, None)]
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()

@@ -367,3 +367,18 @@ def test_registered_backward_checks_what_it_reads():
             op(*ops, *bad)
     with pytest.raises(RuntimeError, match="ROCm device"):
         op(*ops, stats.cpu(), dout, dn)
+
+
+def test_forward_mode_is_refused():
+    v, dout, _ = make((4, 40), torch.float32)
+    x = v["x"].requires_grad_()
+    out = call(v)[0]
+    ad = torch.autograd.forward_ad
+    with ad.dual_level():
+        for grad in (False, True):
+            dual = ad.make_dual(x.detach().requires_grad_(grad), torch.ones_like(x))
+            with pytest.raises(RuntimeError):
+                call({**v, "x": dual})
+        with pytest.raises(RuntimeError):  # a gradient with a tangent
+            torch.autograd.grad(out, x, ad.make_dual(dout, torch.ones_like(dout)))
+    assert call(v)[1].isfinite().all()

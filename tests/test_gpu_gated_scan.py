@@ -590,3 +590,17 @@ def test_step_with_infinities(dtype):
         y = gated_scan_step_(dt[:, i:i + 1], g[:, i:i + 1], x[:, i:i + 1], lam, h)
         hold_kinds("y", y[:, 0], tuple(v[:, i] for v in ref["y"]))
     hold_kinds("h", h, ref["h"])
+
+
+def test_forward_mode_is_refused():
+    dt, g, x, lam, _, _, dy, _ = make(2, 20, 8, torch.float32)
+    y = gated_scan(dt, g, x.requires_grad_(), lam)
+    ad = torch.autograd.forward_ad
+    with ad.dual_level():
+        for grad in (False, True):
+            dual = ad.make_dual(x.detach().requires_grad_(grad), torch.ones_like(x))
+            with pytest.raises(RuntimeError):
+                gated_scan(dt, g, dual, lam)
+        with pytest.raises(RuntimeError):  # a gradient with a tangent
+            torch.autograd.grad(y, x, ad.make_dual(dy, torch.ones_like(dy)))
+    assert gated_scan(dt, g, x, lam).isfinite().all()
