@@ -301,8 +301,10 @@ __global__ __launch_bounds__(LANES ? 256 : 1024) void gate_norm_bwd_kernel(GateN
       }
     team_sum<LANES>(s, red[flip]);
     if constexpr (NV > 1) weights();  // not held meanwhile, nor z's gates: a lane has 128 registers
-    const float back = tau_now * tau_now * tau_now * s[0] * inv;
-    const float side = k.post ? rho_now * rho_now * rho_now * inv * (s[1] - back * s[2]) : 0.f;
+    // Of rows near zero under a small eps, a norm's cube alone would be infinite.
+    const auto cubed = [](float norm, float v) { return norm * (norm * (norm * v)); };
+    const float back = cubed(tau_now, s[0] * inv);
+    const float side = k.post ? cubed(rho_now, (s[1] - back * s[2]) * inv) : 0.f;
 #pragma unroll
     for (int m = 0; m < NV; ++m) {
       const uint32_t i = 4 * (t + m * team);

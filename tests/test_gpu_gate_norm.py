@@ -382,3 +382,21 @@ def test_forward_mode_is_refused():
         with pytest.raises(RuntimeError):  # a gradient with a tangent
             torch.autograd.grad(out, x, ad.make_dual(dout, torch.ones_like(dout)))
     assert call(v)[1].isfinite().all()
+
+
+@pytest.mark.parametrize("d", [40, 300, 1500, 5000])
+@pytest.mark.parametrize("gate", [True, False])
+def test_rows_near_zero_under_a_small_eps(d, gate, monkeypatch):
+    """Inverse norms up to 1e15, whose cubes fp32 does not hold: rows of zeros (padding) and tiny ones."""
+    monkeypatch.setitem(globals(), "EPS", 1e-30)
+    v, dout, dn = make((6, d), torch.float32, gate)
+    size = torch.tensor([0.0, 1e-16, 1e-14, 1.0, 0.0, 1e-10], device=DEV)[:, None]
+    v["x"], v["y"] = v["x"] * size, v["y"] * size
+    ref = formula(*v.values(), dout, dn)
+    leaves = {k: t.detach().requires_grad_() for k, t in v.items() if t is not None}
+    outs = call({**v, **leaves}, eps=EPS)
+    for name, got in zip(("out", "n"), outs):
+        hold(name, got.detach(), ref[name])
+    for name, got in zip(leaves, torch.autograd.grad(outs, list(leaves.values()), [dout, dn])):
+        assert got.isfinite().all(), name
+        hold(name, got, ref[name])
