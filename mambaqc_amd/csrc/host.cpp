@@ -62,10 +62,12 @@ void no_tangents(const std::string& name, std::initializer_list<MaybeTensor> inp
     TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->_fw_grad(0).defined(), name,
                                 ": forward-mode automatic differentiation is not supported");
 }
-// Autograd does not see what the operands go through; their gradients' edges are the node's.
+// Autograd does not see what the operands go through; their gradients' edges are the node's. (Views that
+// torch negates as it reads them, such as the imaginary part of a conjugate, are made what they stand for.)
 Tensor as_type(const Tensor& t, at::ScalarType type) {
   const at::NoGradGuard none;
-  const Tensor v = t.requires_grad() ? t.detach() : t;
+  Tensor v = t.requires_grad() ? t.detach() : t;
+  if (v.is_neg()) v = v.resolve_neg();
   return v.scalar_type() == type ? v : v.to(type);
 }
 // A parameter as the kernels read it: itself, or `convert`'s (_native.param_f32) where it is not that;
@@ -399,7 +401,7 @@ std::optional<std::tuple<Tensor, Tensor>> gated_scan(const Tensor& dt, const Ten
 MaybeTensor gated_scan_step(const Tensor& dt, const Tensor& g, const Tensor& x, const Tensor& log_rate,
                             const Tensor& h, const py::object& convert) {
   if (!scan_shapes(dt, g, x, log_rate, h, std::nullopt) || x.size(1) != 1 ||
-      h.scalar_type() != at::kFloat || !h.is_contiguous())
+      h.scalar_type() != at::kFloat || !h.is_contiguous() || h.is_neg())
     return std::nullopt;
   const Scan o("gated_scan_step_", dt, g, x, log_rate, std::nullopt, h, &convert);
   const c10::DeviceGuard guard(o.x.device());
@@ -430,7 +432,7 @@ std::optional<std::pair<py::bytes, py::bytes>> adam_rows(const Lists& lists, int
   norm.reserve(count * 3);
   const auto dense = [&](const Tensor& t) {
     return t.layout() == at::kStrided && t.is_cuda() && t.device() == lists[0][0].device() &&
-           t.is_contiguous();
+           t.is_contiguous() && !t.is_neg();
   };
   const auto state = eight ? at::kFloat8_e4m3fn : at::kFloat;
   for (size_t i = 0; i < count; ++i) {

@@ -209,7 +209,7 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 if p.grad.layout != torch.strided:
                     raise ValueError("AdamW: sparse gradients are not supported")
-                g = p.grad.detach().contiguous()
+                g = p.grad.detach().contiguous().resolve_neg()
                 if g.dtype != p.dtype:
                     g = g.to(p.dtype)
                 s = self._state_of(p, group["state_bits"])

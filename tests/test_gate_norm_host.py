@@ -101,3 +101,9 @@ def test_refuses_forward_mode(which):
             gate_norm_residual(x, y, gate, scale=scale, pre_weight=pre, post_weight=post)
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.ops.mambaqc.gate_norm_residual(*ops)
+
+
+def test_negated_views_are_read_as_what_they_stand_for():
+    gate = torch.randn(5, 1, dtype=torch.complex64).conj().imag
+    view, row = _z_rows(gate, torch.float32)
+    assert gate.is_neg() and not view.is_neg() and torch.equal(view, gate) and row == view.stride(0)

@@ -127,3 +127,12 @@ def test_refuses_forward_mode(which):
         for call in calls:
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
+
+
+def test_negated_views_are_read_as_what_they_stand_for():
+    x = torch.randn(2, 3, 1, dtype=torch.complex64).conj().imag
+    view, row = _rows(x, torch.float32)
+    assert x.is_neg() and not view.is_neg() and torch.equal(view, x) and row == view.stride(1)
+    one = z(2, 1, 4)
+    with pytest.raises(ValueError, match="contiguous float32"):
+        gated_scan_step_(one, one, one, z(4), torch._neg_view(z(2, 4)))

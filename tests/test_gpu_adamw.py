@@ -490,3 +490,18 @@ def test_a_step_past_the_cache_equals_its_parts():
         adamw_step_(*([one[i]] for one in apart), step=4, lr=1e-2)
     for got, want in zip(lists, apart):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_negated_gradients():
+    """A gradient that torch negates as it reads it (the imaginary part of a conjugate)."""
+    p = torch.nn.Parameter(torch.ones(5, 1, device=DEV))
+    q = torch.nn.Parameter(torch.ones(5, 1, device=DEV))
+    p.grad = torch.ones(5, 1, device=DEV) * torch.arange(5, device=DEV)[:, None]
+    q.grad = torch._neg_view(-p.grad)
+    assert q.grad.is_neg()
+    AdamW([p], lr=0.1).step()
+    AdamW([q], lr=0.1).step()
+    assert torch.equal(p, q)
+    with pytest.raises(ValueError, match="do not take"):
+        adamw_step_([torch._neg_view(torch.ones(5, device=DEV))], [torch.ones(5, device=DEV)],
+                    [torch.zeros(5, device=DEV)], [torch.zeros(5, device=DEV)], step=1)
