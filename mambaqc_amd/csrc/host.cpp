@@ -50,17 +50,19 @@ Tensor workspace(int64_t bytes, const char* name, const Tensor& like) {
 Tensor like_f32(at::IntArrayRef sizes, const Tensor& like) {
   return at::empty(sizes, like.options().dtype(at::kFloat));
 }
-void on_device(const std::string& name, const Tensor& t, const Tensor& like) {
+void on_device(const char* name, const Tensor& t, const Tensor& like) {
   TORCH_CHECK(t.is_cuda(), "mambaqc_amd.", name, ": expected tensors on a ROCm device, got ", t.device(),
               "; this package runs only on the GPU");
   TORCH_CHECK(t.device() == like.device(), "mambaqc_amd.", name, ": tensors on different devices (",
               like.device(), ", ", t.device(), ")");
 }
 // Forward-mode gradients would be lost without a word: the kernels see values alone.
-void no_tangents(const std::string& name, std::initializer_list<MaybeTensor> inputs) {
-  for (const auto& t : inputs)
-    TORCH_CHECK_NOT_IMPLEMENTED(!t || !t->_fw_grad(0).defined(), name,
-                                ": forward-mode automatic differentiation is not supported");
+bool tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
+bool tangent(const MaybeTensor& t) { return t && tangent(*t); }
+template <typename... Inputs>
+void no_tangents(const char* name, const Inputs&... inputs) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(tangent(inputs) || ...), name,
+                              ": forward-mode automatic differentiation is not supported");
 }
 // Autograd does not see what the operands go through; their gradients' edges are the node's. (Views that
 // torch negates as it reads them, such as the imaginary part of a conjugate, are made what they stand for.)
@@ -78,9 +80,9 @@ Tensor weight(const Tensor& t, const py::object* convert) {
   return convert ? (*convert)(t).cast<Tensor>() : as_type(t, at::kFloat).contiguous();
 }
 // What a kernel reads beside the operands, dense in `type`, where it has these sizes.
-Tensor beside(const std::string& name, const char* what, const Tensor& t, at::IntArrayRef sizes,
+Tensor beside(const char* name, const char* what, const Tensor& t, at::IntArrayRef sizes,
               at::ScalarType type, const Tensor& like) {
-  no_tangents(name, {t});
+  no_tangents(name, t);
   on_device(name, t, like);
   TORCH_CHECK_VALUE(t.sizes() == sizes, name, ": ", what, " must be ", sizes, ", got ", t.sizes());
   return as_type(t, type).contiguous();
@@ -155,7 +157,7 @@ struct GateNorm {
   GateNorm(const Tensor& x_, const Tensor& y_, const MaybeTensor& z_, const MaybeTensor& post_,
            const Tensor& scale_, const Tensor& pre_, const py::object* convert)
       : z_row(0) {
-    no_tangents("gate_norm_residual", {x_, y_, z_, post_, scale_, pre_});
+    no_tangents("gate_norm_residual", x_, y_, z_, post_, scale_, pre_);
     for (const Tensor* t : {&x_, &y_, &scale_, &pre_}) on_device("gate_norm_residual", *t, x_);
     if (post_) on_device("gate_norm_residual", *post_, x_), post = weight(*post_, convert);
     scale = weight(scale_, convert), pre = weight(pre_, convert);
@@ -283,9 +285,9 @@ struct Scan {
   Tensor rate;
   MaybeTensor reset;
   // (the state h is only looked at)
-  Scan(const std::string& name, const Tensor& dt_, const Tensor& g_, const Tensor& x_, const Tensor& rate_,
+  Scan(const char* name, const Tensor& dt_, const Tensor& g_, const Tensor& x_, const Tensor& rate_,
        const MaybeTensor& reset_, const MaybeTensor& h, const py::object* convert) {
-    no_tangents(name, {dt_, g_, x_, rate_, h});
+    no_tangents(name, dt_, g_, x_, rate_, h);
     for (const Tensor* t : {&x_, &dt_, &g_, &rate_}) on_device(name, *t, x_);
     if (h) on_device(name, *h, x_);
     rate = weight(rate_, convert);
@@ -482,7 +484,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       .def(py::init([](const std::string& name, const Tensor& dt, const Tensor& g, const Tensor& x,
                        const Tensor& rate, const MaybeTensor& reset, const MaybeTensor& h0,
                        const py::object& convert) {
-        return Scan(name, dt, g, x, rate, reset, h0, &convert);
+        return Scan(name.c_str(), dt, g, x, rate, reset, h0, &convert);
       }));
   m.def("token_rows", [](const Tensor& t, py::object type) {
     return token_rows(t, torch::python::detail::py_object_to_dtype(type));
