@@ -179,6 +179,11 @@ class AdamW(torch.optim.Optimizer):
         self.min_8bit_size, self.max_norm, self.seed = min_8bit_size, max_norm, seed
         self.grad_norm = None
 
+    def __getstate__(self):
+        """What copies and pickles take along: torch's part and this class's own settings."""
+        own = ("min_8bit_size", "max_norm", "seed", "grad_norm")
+        return {**super().__getstate__(), **{k: getattr(self, k) for k in own}}
+
     def _state_of(self, p, bits):
         s = self.state[p]
         if not s:

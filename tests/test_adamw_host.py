@@ -1,5 +1,7 @@
 """The AdamW step's refusals and argument checks, without a GPU."""
+import copy
 import ctypes
+import pickle
 
 import pytest
 import torch
@@ -88,3 +90,15 @@ def test_validation_codes():
     fake = ctypes.c_void_p(4096)
     assert lib.mqc_grad_norm(rows(64, 10, 0), 1, 1.0, None, fake, fake, 64, None) == -1
     assert lib.mqc_grad_norm(rows(64, 10, 0), 1, 1.0, fake, fake, fake, 4, None) == -6
+
+
+@pytest.mark.parametrize("copied", [copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o))])
+def test_copies_keep_their_settings(copied):
+    p = torch.nn.Parameter(torch.ones(3))
+    opt = copied(AdamW([p], lr=0.5, state_bits=8, min_8bit_size=2, max_norm=0.25, seed=11))
+    assert (opt.min_8bit_size, opt.max_norm, opt.seed, opt.grad_norm) == (2, 0.25, 11, None)
+    group, = opt.param_groups
+    assert group["lr"] == 0.5 and group["state_bits"] == 8 and torch.equal(group["params"][0], p)
+    group["params"][0].grad = torch.ones(3)
+    with pytest.raises(RuntimeError, match="ROCm device"):
+        opt.step()

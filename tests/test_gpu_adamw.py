@@ -6,7 +6,9 @@ Tolerances. In fp32, m and v are sums of two products: three roundings, at most 
 absolute values. The update carries at most eight roundings (and the two means' own): 2^-20 of it. p
 takes two more and half a step of its type.
 """
+import copy
 import math
+import pickle
 
 import pytest
 import torch
@@ -505,3 +507,26 @@ def test_negated_gradients():
     with pytest.raises(ValueError, match="do not take"):
         adamw_step_([torch._neg_view(torch.ones(5, device=DEV))], [torch.ones(5, device=DEV)],
                     [torch.zeros(5, device=DEV)], [torch.zeros(5, device=DEV)], step=1)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("copied", [copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o))])
+def test_copies_go_on_with_the_same_bits(copied, bits):
+    gen = torch.Generator(DEV).manual_seed(3)
+    params = [torch.nn.Parameter(torch.randn(n, generator=gen, device=DEV)) for n in (5000, 300)]
+    opt = AdamW(params, lr=0.1, state_bits=bits, min_8bit_size=1000, max_norm=0.5, seed=5)
+
+    def step(params, opt, seed):
+        gen = torch.Generator(DEV).manual_seed(seed)
+        for p in params:
+            p.grad = torch.randn(p.shape, generator=gen, device=DEV)
+        opt.step()
+
+    step(params, opt, 1)
+    other, twins = copied((opt, params))
+    for seed in (2, 3):
+        step(params, opt, seed)
+        step(twins, other, seed)
+        for p, q in zip(params, twins):
+            assert p is not q and torch.equal(p, q)
+        assert torch.equal(opt.grad_norm, other.grad_norm)
