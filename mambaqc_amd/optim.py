@@ -15,6 +15,7 @@ step give the same bits.
 from __future__ import annotations
 
 import array
+import collections
 import itertools
 import math
 
@@ -155,6 +156,12 @@ def _launch8(rows, params, states, how, clip, step):
     nat.host().changed((params, *states))
 
 
+def _viewed(state, from_dtype, to_dtype):
+    """A parameter's state with its tensors of one 8-bit type viewed as the other."""
+    return {k: v.view(to_dtype) if isinstance(v, torch.Tensor) and v.dtype == from_dtype else v
+            for k, v in state.items()}
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW with decoupled weight decay over the kernels of this module.
 
@@ -180,9 +187,18 @@ class AdamW(torch.optim.Optimizer):
         self.grad_norm = None
 
     def __getstate__(self):
-        """What copies and pickles take along: torch's part and this class's own settings."""
-        own = ("min_8bit_size", "max_norm", "seed", "grad_norm")
-        return {**super().__getstate__(), **{k: getattr(self, k) for k in own}}
+        """What copies and pickles take along: torch's part, with 8-bit states as bytes (float8 tensors
+        cannot be unpickled), and this class's own settings."""
+        got = super().__getstate__()
+        got |= {k: getattr(self, k) for k in ("min_8bit_size", "max_norm", "seed", "grad_norm")}
+        got["state"] = collections.defaultdict(dict, {p: _viewed(s, torch.float8_e4m3fn, torch.uint8)
+                                                      for p, s in self.state.items()})
+        return got
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for p, s in self.state.items():
+            self.state[p] = _viewed(s, torch.uint8, torch.float8_e4m3fn)
 
     def _state_of(self, p, bits):
         s = self.state[p]

@@ -102,3 +102,20 @@ def test_copies_keep_their_settings(copied):
     group["params"][0].grad = torch.ones(3)
     with pytest.raises(RuntimeError, match="ROCm device"):
         opt.step()
+
+
+@pytest.mark.parametrize("copied", [copy.deepcopy, lambda o: pickle.loads(pickle.dumps(o))])
+def test_copies_keep_8_bit_states(copied):
+    p = torch.nn.Parameter(torch.ones(3))
+    opt = AdamW([p], state_bits=8)
+    codes = torch.tensor([1.0, -2.0, 0.5]).to(E4M3)
+    opt.state[p] = {"step": 3, "exp_avg": codes, "exp_avg_scale": torch.tensor([0.5])}
+    other = copied(opt)
+    state = other.state[other.param_groups[0]["params"][0]]
+    assert state["step"] == 3 and state["exp_avg"].dtype == E4M3
+    assert torch.equal(state["exp_avg"].float(), codes.float()) and state["exp_avg_scale"].item() == 0.5
+    assert state["exp_avg"].data_ptr() != codes.data_ptr()
+    assert opt.state[p]["exp_avg"].dtype == E4M3
+    new = torch.nn.Parameter(torch.ones(3))
+    other.add_param_group({"params": [new]})
+    assert other.state[new] == {}
