@@ -117,7 +117,9 @@ int mqc_step_norm_out_gate_fits(int64_t M, int64_t d_inner);
  * of them), y is dense. h_last (fp32, or NULL) may be h0. carries (fp32 [batch,
  * ceil(seq_len / mqc_gated_scan_chunk()), width], or NULL): the states that the backward starts
  * from, each chunk's before its first token.
- * workspace (16-byte aligned) of mqc_gated_scan_workspace_bytes. width and seq_len at most 2^31, batch at most 65535.
+ * workspace (16-byte aligned) of mqc_gated_scan_workspace_bytes. MQC_E_LIMIT for width or seq_len
+ * above 2^31, batch above 65535, and walks of 2^32 threads (64 for each 64 channels and 16 steps of a
+ * sequence).
  *
  * Backward: gradients of dt, g, x (dense), log_rate [width], and of h0 (or NULL) from dy and
  * dh_last (or NULL); every size at least 1.
@@ -144,7 +146,8 @@ int mqc_gated_scan_step(const void* dt, int64_t dt_row, const void* g, int64_t g
  *   n = out / sqrt(mean out^2 + eps) pre
  * x, y, out and n dense, rows of z z_row elements apart; z NULL: v = y; post NULL: r = v. post, scale
  * and pre are [d]. stats (fp32 [rows, 2], or NULL) takes the two inverse norms for the backward. out
- * may be x or y, n may be y.
+ * may be x or y, n may be y. MQC_E_LIMIT for a forward of 2^32 threads: 2^28, 2^27 or 2^26 rows of d up
+ * to 64, 128 or 1024, 2^26 / ceil(d / 1024) wider ones.
  * Backward, from dout and dn (dense; either may be NULL, zeros): dx, dy and dz dense, dpost (with
  * post), dscale and dpre [d] summed over the rows in a fixed order; rows at least 1, workspace of
  * mqc_gate_norm_workspace_bytes. */

@@ -449,7 +449,8 @@ void launch_norm(const NormTable& t, double* partial, uint32_t blocks, hipStream
     default: F<f16_t>(__VA_ARGS__); break;            \
   }
 
-// Workgroups of a tensor; a launch holds at most 2^31 - 1 of them.
+// Workgroups of a tensor; a launch (of 256 threads each) holds at most kMaxBlocks of them.
+constexpr int64_t kMaxBlocks = 0xffffffffLL / 256;
 inline int64_t chunks_of(int64_t n, int64_t chunk) { return (n + chunk - 1) / chunk; }
 
 // Fills tables with the tensors of one dtype after another and calls launch(table, blocks, dtype) for
@@ -465,7 +466,7 @@ int by_tables(const int64_t* rows, int64_t count, int width, int n_at, int d_at,
       const int64_t* row = rows + i * width;
       const bool mine = i < count && row[d_at] == dtype && row[n_at] > 0;
       const int64_t more = mine ? chunks_of(row[n_at], chunk) : 0;
-      if (used > 0 && (i == count || (mine && (used == Table::kMax || blocks + more > 0x7fffffffLL)))) {
+      if (used > 0 && (i == count || (mine && (used == Table::kMax || blocks + more > kMaxBlocks)))) {
         launch(t, used, (uint32_t)blocks, dtype);
         const int st = launch_status();
         if (st != MQC_OK) return st;
@@ -485,7 +486,7 @@ inline int check_rows(const int64_t* rows, int64_t count, int width, int pointer
     const int64_t* row = rows + i * width;
     if (row[n_at] < 0) return MQC_E_SHAPE;
     if (!known_dtype(row[d_at])) return MQC_E_DTYPE;
-    if (chunks_of(row[n_at], chunk) > 0x7fffffffLL) return MQC_E_LIMIT;
+    if (chunks_of(row[n_at], chunk) > kMaxBlocks) return MQC_E_LIMIT;
     const uintptr_t size = row[d_at] == MQC_F32 ? 4 : 2;
     for (int c = 0; c < pointers; ++c) {
       if (row[n_at] > 0 && !row[c]) return MQC_E_NULL;

@@ -300,6 +300,9 @@ inline int launch_status() {
   return e == hipSuccess ? MQC_OK : (int)e;
 }
 
+// HIP refuses a launch of 2^32 threads or more along an axis.
+inline bool launchable(int64_t blocks, int64_t threads) { return blocks <= 0xffffffffLL / threads; }
+
 inline bool aligned(const void* p, uintptr_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
 // Whether the byte ranges [a, a + na) and [b, b + nb) share a byte (NULL or

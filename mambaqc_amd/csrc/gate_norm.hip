@@ -431,6 +431,11 @@ inline int gate_norm_shape(int64_t rows, int64_t d, const void* z, int64_t z_row
   if (d > kGateNormMaxWidth || rows > 0x7fffffffLL) return MQC_E_LIMIT;
   return MQC_OK;
 }
+// The forward's rows are bounded by their launch (launch_gate_norm_rows; the backward's workgroups walk).
+inline bool gate_norm_fwd_fits(int64_t rows, int64_t d) {
+  const int64_t teams = d <= 64 ? 16 : d <= 128 ? 8 : d <= 1024 ? 4 : 1;
+  return launchable((rows + teams - 1) / teams, d <= 1024 ? 256 : 64 * ((d + 1023) / 1024));
+}
 
 template <typename T>
 GateNormArgs<T> gate_norm_args(const void* x, const void* y, const void* z, int64_t z_row,
@@ -469,6 +474,7 @@ extern "C" int mqc_gate_norm_fwd(const void* x, const void* y, const void* z, in
   const int st = gate_norm_shape(rows, d, z, z_row, dtype);
   if (st != MQC_OK) return st;
   if (rows == 0) return MQC_OK;
+  if (!gate_norm_fwd_fits(rows, d)) return MQC_E_LIMIT;
   if (!x || !y || !scale || !pre || !out || !n) return MQC_E_NULL;
 #define MQC_F(T)                                                                        \
   [&] {                                                                                 \

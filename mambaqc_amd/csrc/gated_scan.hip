@@ -676,6 +676,10 @@ inline int scan_stream(int64_t tensor, int in, int out) {
     default: KERNEL<T, true, 2><<<grid, block, 0, s>>>(k, (uint32_t)tiles); break;                    \
   }
 
+// A forward's waves of a workgroup: those that have steps.
+inline int scan_waves(int64_t seq) {
+  return seq > kScanWaves * kScanSteps ? kScanWaves : seq > 0 ? (int)((seq + kScanSteps - 1) / kScanSteps) : 1;
+}
 template <typename T>
 int launch_gated_scan_fwd(ScanArgs<T> k, int64_t batch, char* ws, hipStream_t s) {
   const int64_t tiles = batch * ((k.width + kScanLanes - 1) / kScanLanes);
@@ -685,9 +689,8 @@ int launch_gated_scan_fwd(ScanArgs<T> k, int64_t batch, char* ws, hipStream_t s)
     if (st != MQC_OK) return st;
     MQC_SCAN_CHAIN(gated_scan_fwd_kernel, kScanWaves, 3, 1)
   } else {
-    const int64_t waves = k.seq > 0 ? (k.seq + kScanSteps - 1) / kScanSteps : 1;
     gated_scan_fwd_kernel<T, false>
-        <<<dim3((unsigned)tiles), dim3((unsigned)(64 * waves)), 0, s>>>(k, (uint32_t)tiles);
+        <<<dim3((unsigned)tiles), dim3(64 * (unsigned)scan_waves(k.seq)), 0, s>>>(k, (uint32_t)tiles);
   }
   return launch_status();
 }
@@ -726,10 +729,14 @@ inline int scan_shape(int64_t batch, int64_t seq, int64_t width, int64_t dt_row,
   if (dtype != MQC_F32 && dtype != MQC_BF16 && dtype != MQC_F16) return MQC_E_DTYPE;
   if (batch * seq > 1 && (dt_row < width || g_row < width || x_row < width)) return MQC_E_SHAPE;
   if (batch > 65535 || seq > (1LL << 31) || width > (1LL << 31)) return MQC_E_LIMIT;
-  // Workgroups are counted in 31 bits (2^43 elements).
-  if (batch * ((width + kScanLanes - 1) / kScanLanes) > 0x7fffffffLL / (seq / kScanChunk + 1))
-    return MQC_E_LIMIT;
   return MQC_OK;
+}
+// Whether a walk is one launch: 2^36 elements, and of narrow tensors fewer (a width of 1 takes the
+// workgroups of 64).
+inline bool scan_fits(int64_t batch, int64_t seq, int64_t width, int waves) {
+  const int64_t chunk = waves * kScanSteps, chunks = seq > chunk ? (seq + chunk - 1) / chunk : 1;
+  const int64_t tiles = batch * ((width + kScanLanes - 1) / kScanLanes);  // below 2^42
+  return launchable(tiles, 64 * waves) && launchable(tiles * chunks, 64 * waves);
 }
 
 template <typename T>
@@ -772,6 +779,7 @@ extern "C" int mqc_gated_scan_fwd(const void* dt, int64_t dt_row, const void* g,
   const int st = scan_shape(batch, seq_len, width, dt_row, g_row, x_row, dtype);
   if (st != MQC_OK) return st;
   if (batch == 0 || width == 0) return MQC_OK;
+  if (!scan_fits(batch, seq_len, width, scan_waves(seq_len))) return MQC_E_LIMIT;
   if (!log_rate || (seq_len > 0 && (!dt || !g || !x || !y))) return MQC_E_NULL;
   if (seq_len == 0 && !h_last) return MQC_OK;
   if (workspace_bytes < mqc_gated_scan_workspace_bytes(batch, seq_len, width)) return MQC_E_SPACE;
@@ -797,6 +805,7 @@ extern "C" int mqc_gated_scan_bwd(const void* dt, int64_t dt_row, const void* g,
   const int st = scan_shape(batch, seq_len, width, dt_row, g_row, x_row, dtype);
   if (st != MQC_OK) return st;
   if (batch < 1 || seq_len < 1 || width < 1) return MQC_E_SHAPE;
+  if (!scan_fits(batch, seq_len, width, kBackWaves)) return MQC_E_LIMIT;
   if (!dt || !g || !x || !log_rate || !carries || !dy || !ddt || !dg || !dx || !dlog_rate ||
       !workspace)
     return MQC_E_NULL;

@@ -119,3 +119,14 @@ def test_copies_keep_8_bit_states(copied):
     new = torch.nn.Parameter(torch.ones(3))
     other.add_param_group({"params": [new]})
     assert other.state[new] == {}
+
+
+def test_tensors_past_one_launch_are_refused():
+    """2^32 threads and more along an axis, which HIP does not launch. (Without pointers: what is within
+    the limit is refused for those.)"""
+    lib, how = nat.load(), [1.0] * 8
+    most = 4096 * ((1 << 24) - 1)
+    for n, want in ((most, -1), (most + 1, -5)):
+        assert lib.mqc_adamw_step(rows(0, 64, 64, 64, n, 0), 1, *how, None, None) == want
+        assert lib.mqc_adamw8_step(rows(0, 64, 64, 64, 64, 64, n, 0, 0), 1, *how, None, 1, None) == want
+        assert lib.mqc_grad_norm_workspace_bytes(rows(0, 2 * n, 0), 1) == want

@@ -107,3 +107,13 @@ def test_negated_views_are_read_as_what_they_stand_for():
     gate = torch.randn(5, 1, dtype=torch.complex64).conj().imag
     view, row = _z_rows(gate, torch.float32)
     assert gate.is_neg() and not view.is_neg() and torch.equal(view, gate) and row == view.stride(0)
+
+
+@pytest.mark.parametrize("d,rows", [(1, 16 << 24), (64, 16 << 24), (65, 8 << 24), (128, 8 << 24), (129, 4 << 24),
+                                    (1024, 4 << 24), (1025, 1 << 25), (8192, 1 << 23)])
+def test_rows_past_one_launch_are_refused(d, rows):
+    """2^32 threads and more along an axis, which HIP does not launch. (Without pointers: what is within
+    the limit is refused for those.)"""
+    fwd = lambda rows: nat.load().mqc_gate_norm_fwd(None, None, None, 0, None, None, None, None, None, None,
+                                                    rows, d, 1e-6, 0, None)
+    assert fwd(rows) == -5 and fwd(rows - 16) == -1

@@ -136,3 +136,20 @@ def test_negated_views_are_read_as_what_they_stand_for():
     one = z(2, 1, 4)
     with pytest.raises(ValueError, match="contiguous float32"):
         gated_scan_step_(one, one, one, z(4), torch._neg_view(z(2, 4)))
+
+
+def test_sizes_past_one_launch_are_refused():
+    """2^32 threads and more along an axis, which HIP does not launch. (Without pointers: what is within
+    the limit is refused for those.)"""
+    lib = nat.load()
+    fwd = lambda b, t, d: lib.mqc_gated_scan_fwd(None, d, None, d, None, d, None, None, None, None, None,
+                                                 None, b, t, d, 0, None, 0, None)
+    bwd = lambda b, t, d: lib.mqc_gated_scan_bwd(None, d, None, d, None, d, None, None, None, None, None,
+                                                 None, None, None, None, None, b, t, d, 0, None, 0, None)
+    for walk in (fwd, bwd):
+        assert walk(65535, 32768, 1) == -5 and walk(65535, 16384, 1) == -1
+        assert walk(65535, 1, 1 << 31) == -5 and walk(1, 1 << 31, 64) == -5
+        assert walk(1, 1 << 29, 64) == -1
+    assert fwd(65535, 1, 16384) == -1 and fwd(65535, 16, 65536) == -1  # (of short sequences few waves)
+    step = lambda b, d: lib.mqc_gated_scan_step(None, d, None, d, None, d, None, None, None, b, d, 0, None)
+    assert step(65535, 1 << 31) == -1 and step(65536, 1) == -5
