@@ -56,7 +56,9 @@ extern "C" {
 /* Human-readable text for a status code (static storage, never NULL). */
 const char* mqc_status_string(int status);
 
-/* ABI version: bumped whenever a signature or an argument's meaning changes. */
+/* ABI version: bumped whenever a signature or an argument's meaning changes. The constant is what a
+ * caller was compiled against, the function what the library was. */
+#define MQC_ABI_VERSION 8
 int mqc_abi_version(void);
 
 /* out = p (x) q, Hamilton product of n_quat quaternions. p, q, out: dtype.

@@ -495,5 +495,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gated_scan_step", &gated_scan_step);
   m.def("adam_rows", &adam_rows);
   m.def("changed", [](const Lists& lists) { changed(lists); });
-  m.def("abi", [] { return (int64_t)mqc_abi_version(); });
+  m.def("abi", [] { return (int64_t)MQC_ABI_VERSION; });  // of the header this was compiled with
 }

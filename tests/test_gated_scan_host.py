@@ -1,5 +1,8 @@
 """The gated scan's refusals and shape rules, without a GPU."""
 import ctypes
+import shutil
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -153,3 +156,20 @@ def test_sizes_past_one_launch_are_refused():
     assert fwd(65535, 1, 16384) == -1 and fwd(65535, 16, 65536) == -1  # (of short sequences few waves)
     step = lambda b, d: lib.mqc_gated_scan_step(None, d, None, d, None, d, None, None, None, b, d, 0, None)
     assert step(65535, 1 << 31) == -1 and step(65536, 1) == -5
+
+
+def test_host_module_tells_what_it_was_compiled_against(tmp_path):
+    """Beside a library of another version, _host.abi() still gives its own, so that a stale module shows."""
+    other = tmp_path / "other.c"
+    other.write_text("int mqc_abi_version(void) { return 99; }")
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    subprocess.run([cc, "-shared", "-fPIC", str(other), "-o", str(tmp_path / "other.so")], check=True)
+    code = ("import ctypes, importlib.util, sys, torch; ctypes.CDLL(sys.argv[1], mode=ctypes.RTLD_GLOBAL)\n"
+            "spec = importlib.util.spec_from_file_location('_host', sys.argv[2])\n"
+            "module = importlib.util.module_from_spec(spec); spec.loader.exec_module(module)\n"
+            "print(module.abi())")
+    out = subprocess.run([sys.executable, "-c", code, str(tmp_path / "other.so"),
+                          str(nat.LIB_PATH.parent / "_host.so")], capture_output=True, text=True, check=True)
+    assert int(out.stdout) == nat.ABI_VERSION
