@@ -22,6 +22,7 @@ from .lm import (
     quaternion_mamba2_small,
 )
 from . import ops  # registers torch.ops.mambaqc.*
+from . import optim
 
 __all__ = [
     "QuaternionMamba2",

@@ -2,6 +2,9 @@
 import copy
 import ctypes
 import pickle
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -130,3 +133,10 @@ def test_tensors_past_one_launch_are_refused():
         assert lib.mqc_adamw_step(rows(0, 64, 64, 64, n, 0), 1, *how, None, None) == want
         assert lib.mqc_adamw8_step(rows(0, 64, 64, 64, 64, 64, n, 0, 0), 1, *how, None, 1, None) == want
         assert lib.mqc_grad_norm_workspace_bytes(rows(0, 2 * n, 0), 1) == want
+
+
+def test_the_package_has_its_optimizer():
+    """mambaqc_amd.optim.AdamW after `import mambaqc_amd` alone, as mambaqc_amd.kernels and .layers are."""
+    code = "import mambaqc_amd; print(mambaqc_amd.optim.AdamW, mambaqc_amd.kernels, mambaqc_amd.layers)"
+    root = Path(__file__).resolve().parents[1]
+    subprocess.run([sys.executable, "-c", code], cwd=root, check=True)
