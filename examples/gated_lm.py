@@ -71,11 +71,10 @@ class GatedLM(nn.Module):
     @torch.no_grad()
     def generate(self, prompt, count: int):
         """`count` more tokens for each row, the likeliest ones: the prompt once, then a step each."""
-        logits, states = self(prompt)
-        out = [prompt, logits[:, -1:].argmax(-1)]
-        for _ in range(count - 1):
+        out, states = [prompt], None
+        for _ in range(count):
             logits, states = self(out[-1], states=states)
-            out.append(logits.argmax(-1))
+            out.append(logits[:, -1:].argmax(-1))
         return torch.cat(out, 1)
 
 
