@@ -39,10 +39,10 @@ class GatedLayer(nn.Module):
 
     def forward(self, stream, n, reset=None, h=None):
         """(the stream after the layer, the next one's input, the state); h is updated in place for
-        one token without gradients."""
+        one token without gradients and reset."""
         w = self.width
         dt, g, x, z = self.proj(n).split([w, w, w, n.shape[-1]], -1)
-        if h is not None and n.shape[1] == 1 and not torch.is_grad_enabled():
+        if h is not None and n.shape[1] == 1 and reset is None and not torch.is_grad_enabled():
             y = gated_scan_step_(dt, g, x, self.log_rate, h)
         else:
             y, h = gated_scan(dt, g, x, self.log_rate, h0=h, reset=reset, return_state=True)

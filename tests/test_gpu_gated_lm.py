@@ -48,3 +48,19 @@ def test_steps_are_the_whole_forward():
         alone, _ = model(tokens[:, 25:])
         assert (packed[:, 25:] - alone).abs().max() < 2.0 ** -14
         assert (packed[:, :25] - whole[:, :25]).abs().max() < 2.0 ** -14
+
+
+def test_one_token_that_starts_a_document():
+    """A reset at a single token counts, with a state in hand and without gradients."""
+    torch.manual_seed(2)
+    model = gated_lm.GatedLM(50, d_model=48, width=80).to(DEV)
+    tokens = torch.randint(50, (2, 9), device=DEV)
+    with torch.no_grad():
+        _, states = model(tokens[:, :8])
+        fresh, _ = model(tokens[:, 8:])
+        reset = torch.tensor([[True], [False]], device=DEV)
+        got, _ = model(tokens[:, 8:], reset=reset, states=[h.clone() for h in states])
+        whole, _ = model(tokens)
+    assert (got[0] - fresh[0]).abs().max() < 2.0 ** -14
+    assert (got[1] - whole[1, 8:]).abs().max() < 2.0 ** -14
+    assert (fresh[1] - whole[1, 8:]).abs().max() > 2.0 ** -10  # (the state matters)
