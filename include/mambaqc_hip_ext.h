@@ -119,7 +119,8 @@ int mqc_step_norm_out_gate_fits(int64_t M, int64_t d_inner);
  * from, each chunk's before its first token.
  * workspace (16-byte aligned) of mqc_gated_scan_workspace_bytes. MQC_E_LIMIT for width or seq_len
  * above 2^31, batch above 65535, and walks of 2^32 threads (64 for each 64 channels and 16 steps of a
- * sequence).
+ * sequence). Chunks wait for one another within the launch, each for at most about a second; one that
+ * waited in vain gives NaN for what follows it.
  *
  * Backward: gradients of dt, g, x (dense), log_rate [width], and of h0 (or NULL) from dy and
  * dh_last (or NULL); every size at least 1.

@@ -25,8 +25,10 @@
 //
 // All of it is one read and one write of everything, 28 bytes an element with fp32 parameters and
 // 32-bit states, 10 with bf16 and 8-bit ones, so a large copy's 5.1 TB/s bounds it: 36 M fp32 parameters
-// (1 GB) 164 us; 273 M in bf16 with 8-bit states (2.8 GB) 541 us, 5.1 TB/s; 15 M in fp32 with 8-bit
-// states 45 us. Their norm's 143 MB 27 us (one running sum a lane instead of four 47).
+// (1 GB) 163 us; 273 M in bf16 with 8-bit states (2.76 GB) 550 to 560 us step after step, 4.9 to 5.0 TB/s
+// (after an idle second the first two 549, then up to 860 at the fifth and back to that within 60, and 560
+// where 5 ms lie between them: the card taking up load, not the data); 15 M in fp32 with 8-bit states 45 us. The norm of the 36 M (143 MB) 27 us (one running sum a lane
+// instead of four 47).
 #include "common.hpp"
 
 namespace mqc {

@@ -12,9 +12,9 @@
 // Everything between the loads and the stores is fp32; n comes from o before o is rounded.
 //
 // A row stays in registers between its loads and stores, so memory bounds both directions. bf16, 8192 x
-// 768: forward 12.8 us (4.9 TB/s), backward 21 us and 5 for the weights' sums (101 MB, 4.8 TB/s; without
-// the next row's loads ahead 44); 32768 x 1024 in fp16 52 us (6.5 TB/s, its inputs partly in the last
-// cache; 71 when they are not); 65536 x 64 10 and 19 (a wave to a row instead of 16 lanes: 28 and 56).
+// 768: forward 14.4 us (63 MB, 4.4 TB/s), backward 21 us and 5 for the weights' sums (101 MB, 4.8 TB/s;
+// without the next row's loads ahead 44); 32768 x 1024 in fp16 51 us (6.5 TB/s, its inputs partly in the
+// last cache; 71 when they are not), in fp32 144 and 195 (671 and 1074 MB, 4.7 and 5.5 TB/s); 65536 x 64 10 and 19 (a wave to a row instead of 16 lanes: 28 and 56).
 #include "common.hpp"
 
 namespace mqc {

@@ -22,9 +22,10 @@ namespace mqc {
 //
 // What bounds it: 8 bytes an element forward and 14 backward (bf16) against some 33 and 58 vector
 // instructions (5 and 6 of which take four times as long), so neither memory (a copy's 5.1 TB/s) nor
-// arithmetic alone, but how well workgroups overlap. bf16: a prompt of 16384 x 1536 47 us (201 MB,
-// 4.3 TB/s; loads and stores alone 32, with LDS and the words between chunks 38); 4 x 2048 x 1536 forward
-// 25 us, backward 40 (176 MB, 4.4 TB/s); past the last cache, 1 x 65536 x 1536 208 and 385.
+// arithmetic alone, but how well workgroups overlap. The kernels alone, bf16: a prompt of 16384 x 1536 48 us
+// (201 MB, 4.2 TB/s; loads and stores alone 32, with LDS and the words between chunks 38); 4 x 2048 x 1536
+// forward 25 us, backward 41 (176 MB, 4.3 TB/s); past the last cache, 1 x 65536 x 1536 203 and 381. fp32: 81
+// (403 MB, 5.0 TB/s), 33 and 57 (352 MB, 6.2 TB/s).
 // Spans and waves, same prompt: 8 of 16 steps 47, 8 of 8 66, 4 of 16 68, 4 of 32 52, 16 of 8 62; backward
 // of 4 x 2048 x 1536 (before later stages): 8 waves of 8 steps 53, 4 of 16 45, 4 of 32 65. Chunks joined one
 // by one: 8 or 16 47, 32 49, 64 55. Not kept: workgroups that stay and load the next chunk ahead (61 to
@@ -195,11 +196,11 @@ __global__ __launch_bounds__(256) void scan_clear_kernel(uint4* words, int64_t z
 
 // What the card holds at once, three workgroups a CU, begins over some 3 us (NAPS of 64 clocks) forward
 // and 4 backward, in the order of the chain: begun together, the loads of its first chunks, for which
-// all others wait, share the memory with those of its last. It saves some 3 us a launch, 7 where the
-// card was idle: forward of 16384 x 1536 54.8 to 47.3 us, of 4 x 2048 x 1536 28.4 to 25.0 and backward
-// 41.7 to 40.4; launch after launch, 1 x 8192 33.5 to 30.9, backward 55.7 to 51.1, 1 x 65536 219 to 216,
-// 64 x 256 44.6 to 41.4. Short chains that the card holds whole begin at once: 16 x 256 x 1536 16.3, or
-// 17.1 over 3 us; chains of 32 (1 x 4096 x 1536) 22.8, or 21.0.
+// all others wait, share the memory with those of its last. Walks launch after launch, their other launches
+// (2.4 us forward, 6.4 backward) included, begun at once and so: forward of 16384 x 1536 54.3 and 48.8 us, 4 x
+// 2048 29.3 and 25.6, 1 x 8192 34.7 and 29.9, 1 x 4096 22.2 and 19.8; backward 86.3 and 82.0, 44.7 and 43.2,
+// 53.0 and 49.0, 34.8 and 31.7; 64 x 256 39.7 and 39.6. Short chains that the card holds whole begin at once:
+// forward of 16 x 256 14.7, or 15.8 over 3 us.
 constexpr uint32_t kScanHeld = 768;
 template <uint32_t NAPS>
 __device__ inline void scan_stagger(uint32_t tiles) {
@@ -662,9 +663,10 @@ int scan_chain(ScanArgs<T>& k, const ScanSpace& w, char* ws, hipStream_t s) {
 }
 
 // What the 256 MiB cache does not hold anyway goes past it: the outputs where they and the inputs are
-// more, the inputs where these alone are. bf16: backward of 8 x 2048 x 1536 (201 MB in, 151 out) 103 us,
-// with outputs streamed 79, with both 96; 1 x 65536 forward 217, 211, 207, backward 414, 399, 383; what
-// fits loses: 4 x 2048 forward 27.7, 27.1, 28.9, backward 46.3, 45.7, 55.5.
+// more, the inputs where these alone are. bf16, launch after launch with their other launches: backward of 8
+// x 2048 x 1536 (201 MB in, 151 out) 97.5 us, with outputs streamed 73.5, with both 92.7; 1 x 65536 forward
+// 209.8, 204.8, 200.4, backward 405, 392, 375; what fits gains little or loses, and whoever reads its outputs
+// next finds them in the cache: 4 x 2048 forward 25.7, 25.4, 27.5, backward 43.2, 42.2, 52.5.
 inline int scan_stream(int64_t tensor, int in, int out) {
   return tensor * in > (256LL << 20) ? 2 : tensor * (in + out) > (256LL << 20) ? 1 : 0;
 }
