@@ -208,7 +208,8 @@ class AdamW(torch.optim.Optimizer):
                 for k in ("exp_avg", "root_avg_sq"):
                     s[k] = torch.zeros(p.shape, device=p.device, dtype=torch.uint8).view(
                         torch.float8_e4m3fn)
-                    s[k + "_scale"] = torch.ones(state_blocks(p.numel()), device=p.device)
+                    s[k + "_scale"] = torch.ones(state_blocks(p.numel()), device=p.device,
+                                                 dtype=torch.float32)
             else:
                 s["exp_avg"] = torch.zeros(p.shape, device=p.device, dtype=torch.float32)
                 s["exp_avg_sq"] = torch.zeros(p.shape, device=p.device, dtype=torch.float32)

@@ -140,3 +140,21 @@ def test_the_package_has_its_optimizer():
     code = "import mambaqc_amd; print(mambaqc_amd.optim.AdamW, mambaqc_amd.kernels, mambaqc_amd.layers)"
     root = Path(__file__).resolve().parents[1]
     subprocess.run([sys.executable, "-c", code], cwd=root, check=True)
+
+
+@pytest.mark.parametrize("default", [torch.bfloat16, torch.float64])
+def test_states_do_not_follow_the_default_dtype(default):
+    """A step under another default dtype refuses nothing but the CPU."""
+    p, q = (torch.nn.Parameter(torch.ones(n, dtype=torch.float32)) for n in (600, 3))
+    opt = AdamW([p, q], state_bits=8, min_8bit_size=100)
+    before = torch.get_default_dtype()
+    try:
+        torch.set_default_dtype(default)
+        p.grad, q.grad = torch.ones_like(p), torch.ones_like(q)
+        with pytest.raises(RuntimeError, match="ROCm device"):
+            opt.step()
+    finally:
+        torch.set_default_dtype(before)
+    for s, names in ((opt.state[p], ("exp_avg_scale", "root_avg_sq_scale")),
+                     (opt.state[q], ("exp_avg", "exp_avg_sq"))):
+        assert not s or all(s[k].dtype == torch.float32 for k in names)
