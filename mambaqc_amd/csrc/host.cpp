@@ -12,6 +12,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
+#include <algorithm>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -430,8 +431,10 @@ std::optional<std::pair<py::bytes, py::bytes>> adam_rows(const Lists& lists, int
     if (l.size() != count) return std::nullopt;
   if (eight && seeds.size() != count) return std::nullopt;
   std::vector<int64_t> rows, norm;
+  std::vector<std::pair<uintptr_t, uintptr_t>> spans;  // of parameters, whose elements are written side by side
   rows.reserve(count * 9);
   norm.reserve(count * 3);
+  spans.reserve(count);
   const auto dense = [&](const Tensor& t) {
     return t.layout() == at::kStrided && t.is_cuda() && t.device() == lists[0][0].device() &&
            t.is_contiguous() && !t.is_neg();
@@ -454,7 +457,12 @@ std::optional<std::pair<py::bytes, py::bytes>> adam_rows(const Lists& lists, int
     rows.push_back(dtype_code(p));
     if (eight) rows.push_back(seeds[i]);
     norm.insert(norm.end(), {(int64_t)g.data_ptr(), n, dtype_code(p)});
+    const uintptr_t start = (uintptr_t)p.data_ptr();
+    if (n > 0) spans.emplace_back(start, start + n * (type == at::kFloat ? 4 : 2));
   }
+  if (!std::is_sorted(spans.begin(), spans.end())) std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    if (spans[i].first < spans[i - 1].second) return std::nullopt;
   const auto bytes = [](const std::vector<int64_t>& v) {
     return py::bytes((const char*)v.data(), v.size() * sizeof(int64_t));
   };

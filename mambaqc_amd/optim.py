@@ -76,6 +76,9 @@ def _tables(name, params, grads, states, scales, seeds):
         for s in scales:
             _check_state(name, "scales", params, s, torch.float32, state_blocks)
         _check_tensors(name, params, grads, *states, *scales)
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.nbytes) for p in params if p.numel())
+        if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+            raise ValueError(f"{name}: a parameter is there twice, or two of them share memory")
         raise ValueError(f"{name}: tensors that the kernels do not take")
     return got
 
@@ -108,9 +111,10 @@ def adamw_step_(params, grads, exp_avgs, exp_avg_sqs, *, step: int, lr: float = 
                 betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
                 max_norm: float | None = None) -> torch.Tensor | None:
     """One AdamW step in place over lists of tensors: contiguous parameters and gradients of one
-    dtype each (fp32, bf16 or fp16), fp32 states. step counts from 1. With max_norm the gradients
-    are scaled by min(1, max_norm / (norm + 1e-6)) as they are read (they stay as they are), norm
-    over all of them, which is returned (fp32 scalar on the device)."""
+    dtype each (fp32, bf16 or fp16), no two parameters in the same memory, fp32 states. step counts
+    from 1. With max_norm the gradients are scaled by min(1, max_norm / (norm + 1e-6)) as they are
+    read (they stay as they are), norm over all of them, which is returned (fp32 scalar on the
+    device)."""
     params, grads = list(params), list(grads)
     how = _scalars(step, lr, betas, eps, weight_decay)
     states = (exp_avgs, exp_avg_sqs)

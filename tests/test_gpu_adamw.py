@@ -530,3 +530,32 @@ def test_copies_go_on_with_the_same_bits(copied, bits):
         for p, q in zip(params, twins):
             assert p is not q and torch.equal(p, q)
         assert torch.equal(opt.grad_norm, other.grad_norm)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_parameters_that_share_memory_are_refused(bits):
+    """Two workgroups would write one parameter side by side; neighbours in one buffer are fine."""
+    flat = torch.ones(3000, device=DEV)
+    new = lambda n: torch.zeros(n, device=DEV)
+    code = lambda n: torch.zeros(n, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
+
+    def step(params):
+        ns, grads = [p.numel() for p in params], [torch.ones_like(p) for p in params]
+        if bits == 32:
+            return adamw_step_(params, grads, [new(n) for n in ns], [new(n) for n in ns], step=1)
+        scales = lambda: [torch.ones(state_blocks(n), device=DEV) for n in ns]
+        return adamw8_step_(params, grads, [code(n) for n in ns], scales(), [code(n) for n in ns], scales(),
+                            step=1)
+
+    for bad in ([flat[:10], flat[:10]], [flat[100:700], flat[:101]], [flat[:3000], flat[50:60], new(4)]):
+        with pytest.raises(ValueError, match="share memory"):
+            step(bad)
+    assert (flat == 1).all()
+    step([flat[1000:2000], flat[:1000], flat[2000:], flat[500:500]])
+    assert (flat < 1).all()
+    p = torch.nn.Parameter(new(5000))
+    p.grad = torch.ones_like(p)
+    with pytest.warns(UserWarning, match="duplicate parameters"):
+        opt = AdamW([p, p], state_bits=bits)
+    with pytest.raises(ValueError, match="share memory"):
+        opt.step()
