@@ -189,6 +189,49 @@ int64_t mqc_grad_norm_workspace_bytes(const int64_t* tensors, int64_t count);
 int mqc_grad_norm(const int64_t* tensors, int64_t count, double max_norm, float* norm, float* clip,
                   void* workspace, int64_t workspace_bytes, void* stream);
 
+/* The gated delta rule: for each head a state S [k_dim, v_dim] (fp32),
+ *   p = exp(log_decay_t) S_{t-1},  S_t = p + beta_t k_t (v_t - p^T k_t)^T,  o_t = scale S_t^T q_t
+ * from h0 [batch, v_heads, k_dim, v_dim] (NULL: zeros). q and k are [batch, seq_len, k_heads, k_dim], v
+ * [batch, seq_len, v_heads, v_dim], the last axis dense, `strides` the elements between batch rows,
+ * tokens and heads of q, k and v (nine, read before the call returns; none negative); log_decay and beta
+ * [batch, seq_len, v_heads], dense, of decay_dtype and beta_dtype; o dense as v. v_heads is a multiple of
+ * k_heads: value head i has key head i / (v_heads / k_heads). k_dim is at most 128. reset (bytes [batch,
+ * seq_len], or NULL): where it is not 0, S_{t-1} is taken as 0. h_last (fp32, or NULL) may be h0.
+ * For the backward (or NULL, both): states (fp32 [batch, v_heads, chunks, mqc_gated_delta_key_width(k_dim),
+ * mqc_gated_delta_value_width(v_dim)]), each chunk's before its first token, and residuals (fp32 [batch,
+ * v_heads, chunks, mqc_gated_delta_chunk(), value width]), v_t - p^T k_t; chunks =
+ * ceil(seq_len / mqc_gated_delta_chunk()). Both and the workspace are 16-byte aligned.
+ * MQC_E_LIMIT beyond k_dim 128, v_dim 2^20, seq_len 2^31, 2^26 heads in the batch, launches of 2^32 threads
+ * (256 for each chunk of a head, or for 16 columns of v_dim) and 2^40 elements of q a value head.
+ *
+ * Backward: gradients of q, k, v (dense), log_decay and beta (of their types) and of h0 (or NULL), from d_o
+ * (dense) and dh_last (or NULL); batch and seq_len at least 1.
+ * The step: one token of each sequence (strides as above, those between tokens not read), h updated in
+ * place. */
+int mqc_gated_delta_chunk(void);
+int64_t mqc_gated_delta_key_width(int64_t k_dim);
+int64_t mqc_gated_delta_value_width(int64_t v_dim);
+int64_t mqc_gated_delta_workspace_bytes(int64_t batch, int64_t seq_len, int64_t k_heads,
+                                        int64_t v_heads, int64_t k_dim, int64_t v_dim, int dtype,
+                                        int backward);
+int mqc_gated_delta_fwd(const void* q, const void* k, const void* v, const int64_t* strides,
+                        const void* log_decay, int decay_dtype, const void* beta, int beta_dtype,
+                        const void* reset, const float* h0, void* o, float* h_last, float* states,
+                        float* residuals, int64_t batch, int64_t seq_len, int64_t k_heads,
+                        int64_t v_heads, int64_t k_dim, int64_t v_dim, float scale, int dtype,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+int mqc_gated_delta_bwd(const void* q, const void* k, const void* v, const int64_t* strides,
+                        const void* log_decay, int decay_dtype, const void* beta, int beta_dtype,
+                        const void* reset, const float* states, const float* residuals,
+                        const void* d_o, const float* dh_last, void* dq, void* dk, void* dv,
+                        void* dlog_decay, void* dbeta, float* dh0, int64_t batch, int64_t seq_len,
+                        int64_t k_heads, int64_t v_heads, int64_t k_dim, int64_t v_dim, float scale,
+                        int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+int mqc_gated_delta_step(const void* q, const void* k, const void* v, const int64_t* strides,
+                         const void* log_decay, int decay_dtype, const void* beta, int beta_dtype,
+                         float* h, void* o, int64_t batch, int64_t k_heads, int64_t v_heads,
+                         int64_t k_dim, int64_t v_dim, float scale, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -167,6 +167,55 @@ __device__ inline void store_scalar(T* __restrict__ p, float v) {
 }
 
 // ---------------------------------------------------------------------------
+// Four consecutive elements from wherever they start (rows of odd widths do not start at multiples
+// of a vector; gfx950 loads and stores those as it does aligned ones), `left` of them, as they are
+// in memory.
+template <typename T>
+using Quad = uint32_t __attribute__((ext_vector_type(sizeof(T)), aligned(sizeof(T))));
+template <typename T>
+__device__ inline Quad<T> load_quad(const T* row, uint32_t i, int left) {
+  const T* p = row + i;
+  if (left >= 4) return *reinterpret_cast<const Quad<T>*>(p);
+  Quad<T> v = {};
+#pragma unroll
+  for (int c = 0; c < 3; ++c)
+    if (c < left) {
+      if constexpr (sizeof(T) == 4) v[c] = __builtin_bit_cast(uint32_t, p[c]);
+      else v[c / 2] |= (uint32_t)__builtin_bit_cast(uint16_t, p[c]) << (16 * (c % 2));
+    }
+  return v;
+}
+template <typename T>
+__device__ inline void unpack_quad(Quad<T> v, float (&out)[4]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    if constexpr (sizeof(T) == 4) out[c] = __uint_as_float(v[c]);
+    else out[c] = io<T>::bits_to_f32(c & 1 ? v[c / 2] >> 16 : v[c / 2] & 0xffffu);
+  }
+}
+template <typename T>
+__device__ inline void load_part(const T* row, uint32_t i, int left, float (&out)[4]) {
+  unpack_quad<T>(load_quad(row, i, left), out);
+}
+template <bool STREAM = false, typename T>
+__device__ inline void store_part(T* row, uint32_t i, int left, const float (&in)[4]) {
+  T* p = row + i;
+  if (left >= 4) {
+    Quad<T> v;
+#pragma unroll
+    for (int c = 0; c < (int)sizeof(T); ++c)
+      if constexpr (sizeof(T) == 4) v[c] = __float_as_uint(in[c]);
+      else v[c] = pack2<T>(in[2 * c], in[2 * c + 1]);
+    if constexpr (STREAM) __builtin_nontemporal_store(v, reinterpret_cast<Quad<T>*>(p));
+    else *reinterpret_cast<Quad<T>*>(p) = v;
+  } else {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (c < left) store_scalar(p + c, in[c]);
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Hamilton product r = p (x) q (textbook form; reference
 // mambaqc/kernels/quaternion_ops.py:278-281).
 // ---------------------------------------------------------------------------

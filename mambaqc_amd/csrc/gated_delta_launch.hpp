@@ -1,0 +1,60 @@
+#pragma once
+// Launches of the gated delta rule's kernels (gated_delta.hpp) for one type.
+#include "gated_delta.hpp"
+
+namespace mqc {
+namespace delta {
+
+#define MQC_BY_KEYS(F)              \
+  if (a.k_dim <= 32) return F(32);  \
+  if (a.k_dim <= 64) return F(64);  \
+  return F(128);
+
+template <typename T>
+int launch_fwd(const Args<T>& a, hipStream_t s) {
+  const unsigned units = (unsigned)(a.batch * a.k_heads * a.chunks);
+  const unsigned waves = (unsigned)(a.batch * a.v_heads * (a.v_pad / 16));
+#define MQC_F(KD)                                                                        \
+  [&] {                                                                                  \
+    if (units) delta_prep_kernel<T, KD, false><<<dim3(units), dim3(256), 0, s>>>(a);     \
+    delta_fwd_kernel<T, KD><<<dim3(waves), dim3(64), 0, s>>>(a);                         \
+    return launch_status();                                                              \
+  }()
+  MQC_BY_KEYS(MQC_F)
+#undef MQC_F
+}
+
+template <typename T>
+int launch_bwd(const Args<T>& a, hipStream_t s) {
+  const unsigned units = (unsigned)(a.batch * a.k_heads * a.chunks);
+  const unsigned waves = (unsigned)(a.batch * a.v_heads * (a.v_pad / 16));
+  const unsigned parts = (unsigned)(a.batch * a.v_heads * a.chunks);
+  const int64_t shares = (a.batch * a.seq * a.k_heads * a.k_dim + 255) / 256;
+#define MQC_F(KD)                                                                             \
+  [&] {                                                                                       \
+    delta_prep_kernel<T, KD, true><<<dim3(units), dim3(256), 0, s>>>(a);                      \
+    delta_bwd_kernel<T, KD><<<dim3(waves), dim3(64), 0, s>>>(a);                              \
+    delta_grad_kernel<T, KD><<<dim3(parts), dim3(256), 0, s>>>(a);                            \
+    if (a.k_heads != a.v_heads)                                                               \
+      delta_share_kernel<T><<<dim3((unsigned)(shares < 65536 ? shares : 65536)), dim3(256), 0, s>>>(a); \
+    return launch_status();                                                                   \
+  }()
+  MQC_BY_KEYS(MQC_F)
+#undef MQC_F
+}
+
+template <typename T>
+int launch_step(const Args<T>& a, float* h, hipStream_t s) {
+  const unsigned units = (unsigned)(a.batch * a.v_heads * ((a.v_dim + 63) / 64));
+#define MQC_F(KD)                                                                    \
+  [&] {                                                                              \
+    delta_step_kernel<T, KD / 16><<<dim3(units), dim3(256), 0, s>>>(a, h);           \
+    return launch_status();                                                          \
+  }()
+  MQC_BY_KEYS(MQC_F)
+#undef MQC_F
+}
+#undef MQC_BY_KEYS
+
+}  // namespace delta
+}  // namespace mqc

@@ -13,6 +13,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <algorithm>
+#include <cmath>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -417,6 +418,170 @@ MaybeTensor gated_scan_step(const Tensor& dt, const Tensor& g, const Tensor& x, 
   return y;
 }
 
+// --- the gated delta rule -------------------------------------------------------------------------
+// t [b, n, h, d] in `type` with a dense last axis; batch rows, tokens and heads are read where they are.
+Tensor dense_last(const Tensor& t, at::ScalarType type) {
+  const Tensor v = as_type(t, type);
+  return v.size(3) > 1 && v.stride(3) != 1 ? v.contiguous() : v;
+}
+
+// Operands as the kernels read them: q, k and v in the promoted type, the gates in their own
+// (kernels/delta.py).
+struct Delta {
+  Tensor q, k, v, g, beta;
+  MaybeTensor reset;
+  float scale;
+  int64_t strides[9];
+  // (the state h is only looked at)
+  Delta(const char* name, const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g_,
+        const Tensor& beta_, const MaybeTensor& reset_, const MaybeTensor& h,
+        const std::optional<double>& scale_) {
+    no_tangents(name, q_, k_, v_, g_, beta_, h);
+    for (const Tensor* t : {&v_, &q_, &k_, &g_, &beta_}) on_device(name, *t, v_);
+    if (h) on_device(name, *h, v_);
+    if (reset_) on_device(name, *reset_, v_), reset = reset_->contiguous();
+    const auto type =
+        at::promote_types(at::promote_types(q_.scalar_type(), k_.scalar_type()), v_.scalar_type());
+    q = dense_last(q_, type), k = dense_last(k_, type), v = dense_last(v_, type);
+    g = as_type(g_, g_.scalar_type()).contiguous();
+    beta = as_type(beta_, beta_.scalar_type()).contiguous();
+    dtype_code(v), dtype_code(g), dtype_code(beta);
+    scale = (float)(scale_ ? *scale_ : 1 / std::sqrt((double)q.size(3)));
+    const Tensor* const rows[3] = {&q, &k, &v};
+    for (int i = 0; i < 3; ++i)
+      for (int j = 0; j < 3; ++j) strides[3 * i + j] = rows[i]->stride(j);
+  }
+  int64_t b() const { return v.size(0); }
+  int64_t t() const { return v.size(1); }
+  int64_t hk() const { return q.size(2); }
+  int64_t hv() const { return v.size(2); }
+  int64_t dk() const { return q.size(3); }
+  int64_t dv() const { return v.size(3); }
+  // What a training forward stores: the chunks' states, and residuals.
+  std::vector<int64_t> saved(bool states) const {
+    const int64_t c = mqc_gated_delta_chunk(), width = mqc_gated_delta_value_width(dv());
+    return {b(), hv(), (t() + c - 1) / c, states ? mqc_gated_delta_key_width(dk()) : c, width};
+  }
+};
+
+std::tuple<Tensor, Tensor, MaybeTensor, MaybeTensor> delta_forward(const Delta& o, const MaybeTensor& h0,
+                                                                   bool train) {
+  const c10::DeviceGuard guard(o.v.device());
+  const int64_t b = o.b(), t = o.t(), hk = o.hk(), hv = o.hv(), dk = o.dk(), dv = o.dv();
+  const int64_t bytes = mqc_gated_delta_workspace_bytes(b, t, hk, hv, dk, dv, dtype_code(o.v), 0);
+  const Tensor ws = workspace(bytes, "mqc_gated_delta_fwd", o.v);
+  Tensor out = at::empty({b, t, hv, dv}, o.v.options()), h = like_f32({b, hv, dk, dv}, o.v);
+  MaybeTensor states, resid;
+  if (train) states = like_f32(o.saved(true), o.v), resid = like_f32(o.saved(false), o.v);
+  check(mqc_gated_delta_fwd(o.q.data_ptr(), o.k.data_ptr(), o.v.data_ptr(), o.strides, o.g.data_ptr(),
+                            dtype_code(o.g), o.beta.data_ptr(), dtype_code(o.beta), ptr(o.reset),
+                            f32(h0), out.data_ptr(), (float*)h.data_ptr(), (float*)ptr(states),
+                            (float*)ptr(resid), b, t, hk, hv, dk, dv, o.scale, dtype_code(o.v),
+                            ws.data_ptr(), bytes, stream_of(o.v)),
+        "mqc_gated_delta_fwd");
+  return {out, h, states, resid};
+}
+
+// dq, dk, dv, dlog_decay, dbeta, dh0.
+std::vector<MaybeTensor> delta_backward(const Delta& o, Tensor states, Tensor resid, MaybeTensor d_o,
+                                        MaybeTensor dh, bool want_dh0) {
+  const c10::DeviceGuard guard(o.v.device());
+  const int64_t b = o.b(), t = o.t(), hk = o.hk(), hv = o.hv(), dk = o.dk(), dv = o.dv();
+  states = beside("gated_delta", "the chunks' states", states, o.saved(true), at::kFloat, o.v);
+  resid = beside("gated_delta", "the chunks' residuals", resid, o.saved(false), at::kFloat, o.v);
+  if (d_o) d_o = beside("gated_delta", "the gradient of o", *d_o, {b, t, hv, dv}, o.v.scalar_type(), o.v);
+  if (dh) dh = beside("gated_delta", "the state's gradient", *dh, {b, hv, dk, dv}, at::kFloat, o.v);
+  const auto like = [](const Tensor& x) { return at::empty(x.sizes(), x.options()); };
+  Tensor dq = like(o.q), dkk = like(o.k), dvv = like(o.v), dg = like(o.g), dbeta = like(o.beta);
+  MaybeTensor dh0;
+  if (o.v.numel() == 0) {
+    if (want_dh0) dh0 = dh ? dh->clone() : at::zeros({b, hv, dk, dv}, o.v.options().dtype(at::kFloat));
+    return {dq, dkk, dvv, dg, dbeta, dh0};
+  }
+  if (!d_o) d_o = at::zeros({b, t, hv, dv}, o.v.options());
+  if (want_dh0) dh0 = like_f32({b, hv, dk, dv}, o.v);
+  const int64_t bytes = mqc_gated_delta_workspace_bytes(b, t, hk, hv, dk, dv, dtype_code(o.v), 1);
+  const Tensor ws = workspace(bytes, "mqc_gated_delta_bwd", o.v);
+  check(mqc_gated_delta_bwd(o.q.data_ptr(), o.k.data_ptr(), o.v.data_ptr(), o.strides, o.g.data_ptr(),
+                            dtype_code(o.g), o.beta.data_ptr(), dtype_code(o.beta), ptr(o.reset),
+                            f32(states), f32(resid), ptr(d_o), f32(dh), dq.data_ptr(), dkk.data_ptr(),
+                            dvv.data_ptr(), dg.data_ptr(), dbeta.data_ptr(), (float*)ptr(dh0), b, t, hk,
+                            hv, dk, dv, o.scale, dtype_code(o.v), ws.data_ptr(), bytes, stream_of(o.v)),
+        "mqc_gated_delta_bwd");
+  return {dq, dkk, dvv, dg, dbeta, dh0};
+}
+
+bool delta_shapes(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta,
+                  const MaybeTensor& h, const MaybeTensor& reset) {
+  if (q.dim() != 4 || v.dim() != 4 || k.sizes() != q.sizes()) return false;
+  const int64_t b = v.size(0), t = v.size(1), hk = q.size(2), hv = v.size(2), dk = q.size(3),
+                dv = v.size(3);
+  const at::IntArrayRef gates = v.sizes().slice(0, 3);
+  return q.size(0) == b && q.size(1) == t && hk > 0 && hv > 0 && hv % hk == 0 && dk > 0 && dv > 0 &&
+         dk <= 128 && g.sizes() == gates && beta.sizes() == gates &&
+         (!h || h->sizes() == at::IntArrayRef{b, hv, dk, dv}) &&
+         (!reset || (reset->sizes() == at::IntArrayRef{b, t} && reset->scalar_type() == at::kBool));
+}
+
+struct DeltaNode : torch::autograd::Function<DeltaNode> {
+  static variable_list forward(AutogradContext* ctx, const Variable& q, const Variable& k,
+                               const Variable& v, const Variable& g, const Variable& beta,
+                               const MaybeTensor& h0, const Delta& o, const MaybeTensor& h0_read) {
+    auto [out, h, states, resid] = delta_forward(o, h0_read, true);
+    ctx->save_for_backward({o.q, o.k, o.v, o.g, o.beta, edge(o.reset), *states, *resid});
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["types"] = grad_types({q, k, v, g, beta, h0});
+    ctx->saved_data["scale"] = (double)o.scale;
+    return {out, h};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    // (laid out anew, as in GateNormNode)
+    const auto s = ctx->get_saved_variables();
+    const auto types = ctx->saved_data["types"].toIntVector();
+    TORCH_CHECK_VALUE(delta_shapes(s[0], s[1], s[2], s[3], s[4], std::nullopt, maybe(s[5])),
+                      "gated_delta: the saved tensors came back in other shapes");
+    const Delta o("gated_delta", s[0], s[1], s[2], s[3], s[4], maybe(s[5]), std::nullopt,
+                  ctx->saved_data["scale"].toDouble());
+    const auto got = delta_backward(o, s[6], s[7], maybe(grads[0]), maybe(grads[1]), types[5] >= 0);
+    return once("gated_delta", as_grads(got, types, 8));
+  }
+};
+
+// gated_delta (o, last state), or nothing where the arguments do not match.
+std::optional<std::tuple<Tensor, Tensor>> gated_delta(const Tensor& q, const Tensor& k, const Tensor& v,
+                                                      const Tensor& g, const Tensor& beta,
+                                                      const MaybeTensor& h0, const MaybeTensor& reset,
+                                                      const std::optional<double>& scale) {
+  if (!delta_shapes(q, k, v, g, beta, h0, reset)) return std::nullopt;
+  const Delta o("gated_delta", q, k, v, g, beta, reset, h0, scale);
+  MaybeTensor state;
+  if (h0) state = as_type(*h0, at::kFloat).contiguous();
+  if (records({q, k, v, g, beta, h0})) {
+    const auto out = DeltaNode::apply(q, k, v, g, beta, h0, o, state);
+    return std::make_tuple(out[0], out[1]);
+  }
+  auto [out, h, states, resid] = delta_forward(o, state, false);
+  return std::make_tuple(out, h);
+}
+
+// gated_delta_step_, or nothing where the arguments do not match.
+MaybeTensor gated_delta_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
+                             const Tensor& beta, const Tensor& h, const std::optional<double>& scale) {
+  if (!delta_shapes(q, k, v, g, beta, h, std::nullopt) || v.size(1) != 1 ||
+      h.scalar_type() != at::kFloat || !h.is_contiguous() || h.is_neg())
+    return std::nullopt;
+  const Delta o("gated_delta_step_", q, k, v, g, beta, std::nullopt, h, scale);
+  const c10::DeviceGuard guard(o.v.device());
+  Tensor out = at::empty({o.b(), 1, o.hv(), o.dv()}, o.v.options());
+  check(mqc_gated_delta_step(o.q.data_ptr(), o.k.data_ptr(), o.v.data_ptr(), o.strides, o.g.data_ptr(),
+                             dtype_code(o.g), o.beta.data_ptr(), dtype_code(o.beta),
+                             (float*)h.data_ptr(), out.data_ptr(), o.b(), o.hk(), o.hv(), o.dk(), o.dv(),
+                             o.scale, dtype_code(o.v), stream_of(o.v)),
+        "mqc_gated_delta_step");
+  changed(h);
+  return out;
+}
+
 // --- the AdamW step's tables ----------------------------------------------------------------------
 using Lists = std::vector<std::vector<Tensor>>;
 
@@ -501,6 +666,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("scan_backward", &scan_backward);
   m.def("gated_scan", &gated_scan);
   m.def("gated_scan_step", &gated_scan_step);
+  py::class_<Delta>(m, "Delta")
+      .def(py::init([](const std::string& name, const Tensor& q, const Tensor& k, const Tensor& v,
+                       const Tensor& g, const Tensor& beta, const MaybeTensor& reset,
+                       const MaybeTensor& h0, const std::optional<double>& scale) {
+        return Delta(name.c_str(), q, k, v, g, beta, reset, h0, scale);
+      }));
+  m.def("delta_forward", &delta_forward);
+  m.def("delta_backward", &delta_backward);
+  m.def("gated_delta", &gated_delta);
+  m.def("gated_delta_step", &gated_delta_step);
   m.def("adam_rows", &adam_rows);
   m.def("changed", [](const Lists& lists) { changed(lists); });
   m.def("abi", [] { return (int64_t)MQC_ABI_VERSION; });  // of the header this was compiled with

@@ -18,6 +18,7 @@ from .parallel_scan import parallel_scan_quaternion
 from .ssm_fused import (ssm_step_fused, ssm_forward_fused, ssm_forward_fused_dl,
                         ssm_forward_front_dl, ssm_front, ssm_forward_fused_bc)
 from .gated import gated_scan, gated_scan_step_
+from .delta import gated_delta, gated_delta_step_
 from .gate_norm import gate_norm_residual
 from .quaternion_ops import (
     quaternion_multiply,
@@ -45,5 +46,7 @@ __all__ = [
     "ssm_forward_fused_bc",
     "gated_scan",
     "gated_scan_step_",
+    "gated_delta",
+    "gated_delta_step_",
     "gate_norm_residual",
 ]

@@ -25,7 +25,7 @@ from torch.library import custom_op, register_autograd
 
 from . import _native as nat
 from .block import _gate_operands, _out_gate_backward
-from .kernels import cayley_transform, gate_norm, gated, parallel_scan, quaternion_ops
+from .kernels import cayley_transform, delta, gate_norm, gated, parallel_scan, quaternion_ops
 from .kernels import ssm_fused as sf
 from .kernels.quaternion_norm import _qln_backward, _qln_forward
 from .layers.causal_conv1d import _conv_silu_backward, _ConvSiLU, _rows_view
@@ -556,6 +556,77 @@ def _gated_scan_bwd(ctx, dy, dh_last, _gcarries):
 register_autograd(f"{NS}::gated_scan_train", _gated_scan_bwd, setup_context=_gated_scan_setup)
 
 
+# --- the gated delta rule ---------------------------------------------------------
+
+@custom_op(f"{NS}::gated_delta", mutates_args=())
+def gated_delta(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor,
+                h0: Optional[Tensor] = None, reset: Optional[Tensor] = None,
+                scale: Optional[float] = None) -> Tuple[Tensor, Tensor]:
+    """Inference: (o in the promoted dtype, h_last fp32 [B, HV, DK, DV])."""
+    ops = delta._operands("gated_delta", q, k, v, log_decay, beta, reset, h0, scale)
+    return nat.host().delta_forward(ops, gated._state(h0), False)[:2]
+
+
+@gated_delta.register_fake
+def _(q, k, v, log_decay, beta, h0=None, reset=None, scale=None):
+    b, _, hv, dv = v.shape
+    return (v.new_empty(v.shape, dtype=delta._dtype(q, k, v)),
+            v.new_empty(b, hv, q.shape[3], dv, dtype=torch.float32))
+
+
+@custom_op(f"{NS}::gated_delta_train", mutates_args=())
+def gated_delta_train(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor,
+                      h0: Optional[Tensor] = None, reset: Optional[Tensor] = None,
+                      scale: Optional[float] = None) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(o, h_last, the chunks' states and residuals for the backward)."""
+    ops = delta._operands("gated_delta", q, k, v, log_decay, beta, reset, h0, scale)
+    return nat.host().delta_forward(ops, gated._state(h0), True)
+
+
+@gated_delta_train.register_fake
+def _(q, k, v, log_decay, beta, h0=None, reset=None, scale=None):
+    b, _, hv, dv = v.shape
+    states, residuals = delta._saved(q, v)
+    return (v.new_empty(v.shape, dtype=delta._dtype(q, k, v)),
+            v.new_empty(b, hv, q.shape[3], dv, dtype=torch.float32),
+            v.new_empty(states, dtype=torch.float32), v.new_empty(residuals, dtype=torch.float32))
+
+
+@custom_op(f"{NS}::gated_delta_backward", mutates_args=())
+def gated_delta_backward(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor,
+                         reset: Optional[Tensor], states: Tensor, residuals: Tensor, do: Tensor,
+                         dh_last: Tensor, scale: Optional[float] = None,
+                         ) -> Tuple[Tensor, Tensor, Tensor, Tensor, Tensor, Tensor]:
+    """(dq, dk, dv in the promoted dtype, dlog_decay and dbeta in their own, dh0 in fp32)."""
+    ops = delta._operands("gated_delta", q, k, v, log_decay, beta, reset, None, scale)
+    return tuple(nat.host().delta_backward(ops, states, residuals, do, dh_last, True))
+
+
+@gated_delta_backward.register_fake
+def _(q, k, v, log_decay, beta, reset, states, residuals, do, dh_last, scale=None):
+    ct = delta._dtype(q, k, v)
+    return (q.new_empty(q.shape, dtype=ct), q.new_empty(q.shape, dtype=ct),
+            v.new_empty(v.shape, dtype=ct), log_decay.new_empty(log_decay.shape),
+            beta.new_empty(beta.shape), dh_last.new_empty(dh_last.shape, dtype=torch.float32))
+
+
+def _gated_delta_setup(ctx, inputs, output):
+    q, k, v, log_decay, beta, h0, reset, scale = inputs
+    ctx.save_for_backward(q, k, v, log_decay, beta, reset, *output[2:])
+    ctx.scale, ctx.h0_dtype = scale, None if h0 is None else h0.dtype
+
+
+def _gated_delta_bwd(ctx, do, dh_last, _gstates, _gresiduals):
+    q, k, v, log_decay, beta, reset, states, residuals = ctx.saved_tensors
+    dq, dk, dv, dg, dbeta, dh0 = gated_delta_backward(q, k, v, log_decay, beta, reset, states,
+                                                      residuals, do, dh_last, ctx.scale)
+    return (dq.to(q.dtype), dk.to(k.dtype), dv.to(v.dtype), dg, dbeta,
+            None if ctx.h0_dtype is None else dh0.to(ctx.h0_dtype), None, None)
+
+
+register_autograd(f"{NS}::gated_delta_train", _gated_delta_bwd, setup_context=_gated_delta_setup)
+
+
 # --- gate, norms and residual between blocks --------------------------------------
 
 @custom_op(f"{NS}::gate_norm_residual", mutates_args=())
@@ -617,5 +688,6 @@ OPS = (
     "ssm_forward_dl_train", "ssm_backward_dl", "ssm_front", "ssm_front_backward",
     "quaternion_layer_norm", "quaternion_layer_norm_backward", "causal_conv1d_silu",
     "causal_conv1d_silu_backward", "out_gate", "out_gate_backward", "gated_scan", "gated_scan_train",
-    "gated_scan_backward", "gate_norm_residual", "gate_norm_residual_backward",
+    "gated_scan_backward", "gated_delta", "gated_delta_train", "gated_delta_backward",
+    "gate_norm_residual", "gate_norm_residual_backward",
 )
