@@ -232,6 +232,21 @@ int mqc_gated_delta_step(const void* q, const void* k, const void* v, const int6
                          float* h, void* o, int64_t batch, int64_t k_heads, int64_t v_heads,
                          int64_t k_dim, int64_t v_dim, float scale, int dtype, void* stream);
 
+/* Layer norm of each of `rows` rows of d (1 to mqc_layer_norm_max_width()) elements, x_row apart in x,
+ * dense in y: y = (x - mean x) / sqrt(mean (x - mean x)^2 + eps) weight + bias (either may be NULL, 1 and
+ * 0). stats (fp32 [rows, 2], or NULL) takes the mean and the inverse root for the backward. y may be x
+ * where x is dense. MQC_E_LIMIT for a forward of 2^32 threads (a wave to a row of 129 to 1024, as
+ * mqc_gate_norm_fwd).
+ * Backward, from dy (dense): dx (dense), and dweight and dbias [d] (or NULL) summed over the rows in a
+ * fixed order; rows at least 1, workspace of mqc_layer_norm_workspace_bytes where there are sums. */
+int64_t mqc_layer_norm_max_width(void);
+int64_t mqc_layer_norm_workspace_bytes(int64_t rows, int64_t d);
+int mqc_layer_norm_fwd(const void* x, int64_t x_row, const float* weight, const float* bias, void* y,
+                       float* stats, int64_t rows, int64_t d, float eps, int dtype, void* stream);
+int mqc_layer_norm_bwd(const void* x, int64_t x_row, const float* weight, const float* stats,
+                       const void* dy, void* dx, float* dweight, float* dbias, int64_t rows, int64_t d,
+                       int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

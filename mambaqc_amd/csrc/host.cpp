@@ -263,6 +263,94 @@ std::optional<std::tuple<Tensor, Tensor>> gate_norm(const Tensor& x, const Tenso
   return std::make_tuple(out, n);
 }
 
+// --- layer norm -----------------------------------------------------------------------------------
+// Operands as the kernels read them, weights in fp32 (kernels/layer_norm.py).
+struct LayerNorm {
+  Tensor x;
+  int64_t x_row;
+  MaybeTensor w, b;
+  LayerNorm(const Tensor& x_, const MaybeTensor& w_, const MaybeTensor& b_, const py::object* convert) {
+    no_tangents("layer_norm", x_, w_, b_);
+    on_device("layer_norm", x_, x_);
+    if (w_) on_device("layer_norm", *w_, x_), w = weight(*w_, convert);
+    if (b_) on_device("layer_norm", *b_, x_), b = weight(*b_, convert);
+    std::tie(x, x_row) = spaced_rows(x_, x_.scalar_type());
+    dtype_code(x);
+  }
+  int64_t d() const { return x.size(-1); }
+  int64_t rows() const { return d() ? x.numel() / d() : 0; }
+};
+
+std::tuple<Tensor, MaybeTensor> layer_norm_forward(const LayerNorm& o, double eps, bool train) {
+  const c10::DeviceGuard guard(o.x.device());
+  Tensor y = at::empty(o.x.sizes(), o.x.options());
+  MaybeTensor stats;
+  if (train) stats = like_f32({o.rows(), 2}, o.x);
+  if (o.rows() > 0)
+    check(mqc_layer_norm_fwd(o.x.data_ptr(), o.x_row, f32(o.w), f32(o.b), y.data_ptr(),
+                             (float*)ptr(stats), o.rows(), o.d(), (float)eps, dtype_code(o.x),
+                             stream_of(o.x)),
+          "mqc_layer_norm_fwd");
+  return {y, stats};
+}
+
+// dx, dweight, dbias (without their tensors nothing).
+std::vector<MaybeTensor> layer_norm_backward(const LayerNorm& o, Tensor stats, Tensor dy) {
+  const c10::DeviceGuard guard(o.x.device());
+  stats = beside("layer_norm", "the rows' means and inverse roots", stats, {o.rows(), 2}, at::kFloat, o.x);
+  dy = beside("layer_norm", "the gradient of y", dy, o.x.sizes(), o.x.scalar_type(), o.x);
+  Tensor dx = at::empty(o.x.sizes(), o.x.options());
+  MaybeTensor dw, db;
+  if (o.rows() == 0) {
+    if (o.w) dw = at::zeros_like(*o.w);
+    if (o.b) db = at::zeros_like(*o.b);
+    return {dx, dw, db};
+  }
+  if (o.w) dw = at::empty_like(*o.w);
+  if (o.b) db = at::empty_like(*o.b);
+  const int64_t bytes = dw || db ? mqc_layer_norm_workspace_bytes(o.rows(), o.d()) : 0;
+  const Tensor ws = workspace(bytes, "mqc_layer_norm_bwd", o.x);
+  check(mqc_layer_norm_bwd(o.x.data_ptr(), o.x_row, f32(o.w), f32(stats), dy.data_ptr(), dx.data_ptr(),
+                           (float*)ptr(dw), (float*)ptr(db), o.rows(), o.d(), dtype_code(o.x),
+                           ws.data_ptr(), bytes, stream_of(o.x)),
+        "mqc_layer_norm_bwd");
+  return {dx, dw, db};
+}
+
+bool layer_norm_shapes(const Tensor& x, const MaybeTensor& w, const MaybeTensor& b) {
+  if (x.dim() < 1) return false;
+  const at::IntArrayRef last = x.sizes().slice(x.dim() - 1);
+  return (!w || w->sizes() == last) && (!b || b->sizes() == last);
+}
+
+struct LayerNormNode : torch::autograd::Function<LayerNormNode> {
+  static variable_list forward(AutogradContext* ctx, const Variable& x, const MaybeTensor& w,
+                               const MaybeTensor& b, const LayerNorm& o, double eps) {
+    auto [y, stats] = layer_norm_forward(o, eps, true);
+    ctx->save_for_backward({o.x, edge(o.w), edge(o.b), *stats});
+    ctx->saved_data["types"] = grad_types({x, w, b});
+    return {y};
+  }
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    // (laid out anew, as in GateNormNode)
+    const auto s = ctx->get_saved_variables();
+    TORCH_CHECK_VALUE(layer_norm_shapes(s[0], maybe(s[1]), maybe(s[2])),
+                      "layer_norm: the saved tensors came back in other shapes");
+    const LayerNorm o(s[0], maybe(s[1]), maybe(s[2]), nullptr);
+    const auto got = layer_norm_backward(o, s[3], grads[0]);
+    return once("layer_norm", as_grads(got, ctx->saved_data["types"].toIntVector(), 5));
+  }
+};
+
+// layer_norm, or nothing where the shapes do not match.
+MaybeTensor layer_norm(const Tensor& x, const MaybeTensor& w, const MaybeTensor& b, double eps,
+                       const py::object& convert) {
+  if (!layer_norm_shapes(x, w, b)) return std::nullopt;
+  const LayerNorm o(x, w, b, &convert);
+  if (records({x, w, b})) return LayerNormNode::apply(x, w, b, o, eps)[0];
+  return std::get<0>(layer_norm_forward(o, eps, false));
+}
+
 // --- the gated scan -------------------------------------------------------------------------------
 // t [b, n, d] in `type` and the elements between its tokens, read in place where these are evenly
 // spaced and the last axis is dense.
@@ -676,6 +764,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("delta_backward", &delta_backward);
   m.def("gated_delta", &gated_delta);
   m.def("gated_delta_step", &gated_delta_step);
+  py::class_<LayerNorm>(m, "LayerNorm")
+      .def(py::init([](const Tensor& x, const MaybeTensor& w, const MaybeTensor& b,
+                       const py::object& convert) { return LayerNorm(x, w, b, &convert); }));
+  m.def("layer_norm_forward", &layer_norm_forward);
+  m.def("layer_norm_backward", &layer_norm_backward);
+  m.def("layer_norm", &layer_norm);
   m.def("adam_rows", &adam_rows);
   m.def("changed", [](const Lists& lists) { changed(lists); });
   m.def("abi", [] { return (int64_t)MQC_ABI_VERSION; });  // of the header this was compiled with

@@ -5,8 +5,9 @@ of libmambaqc_hip.so, plus the block's fused forms `ssm_forward_fused_dl`
 (delta and s given) and `ssm_forward_front_dl` (from dt_proj / gate_proj outputs),
 `ssm_front` (delta = softplus(dt_raw), s = sigmoid(g_raw) * x), and
 `ssm_forward_fused_bc` (the B/C projections and the SSM in one launch), and the operators of a
-recurrent stack: `gated_scan` with its single-token step `gated_scan_step_`, and
-`gate_norm_residual` between its blocks.
+recurrent stack: `gated_scan` and `gated_delta` (a state of one number a channel, of a matrix a head)
+with their single-token steps `gated_scan_step_` and `gated_delta_step_`, `gate_norm_residual` between
+its blocks, and `layer_norm`.
 
 The submodule `quaternion_norm` (the layer norm) is imported before the
 element-wise ops so that the package attribute `quaternion_norm` ends up bound
@@ -20,6 +21,7 @@ from .ssm_fused import (ssm_step_fused, ssm_forward_fused, ssm_forward_fused_dl,
 from .gated import gated_scan, gated_scan_step_
 from .delta import gated_delta, gated_delta_step_
 from .gate_norm import gate_norm_residual
+from .norm import layer_norm
 from .quaternion_ops import (
     quaternion_multiply,
     quaternion_multiply_batched,
@@ -49,4 +51,5 @@ __all__ = [
     "gated_delta",
     "gated_delta_step_",
     "gate_norm_residual",
+    "layer_norm",
 ]

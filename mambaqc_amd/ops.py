@@ -25,7 +25,7 @@ from torch.library import custom_op, register_autograd
 
 from . import _native as nat
 from .block import _gate_operands, _out_gate_backward
-from .kernels import cayley_transform, delta, gate_norm, gated, parallel_scan, quaternion_ops
+from .kernels import cayley_transform, delta, gate_norm, gated, norm, parallel_scan, quaternion_ops
 from .kernels import ssm_fused as sf
 from .kernels.quaternion_norm import _qln_backward, _qln_forward
 from .layers.causal_conv1d import _conv_silu_backward, _ConvSiLU, _rows_view
@@ -627,6 +627,50 @@ def _gated_delta_bwd(ctx, do, dh_last, _gstates, _gresiduals):
 register_autograd(f"{NS}::gated_delta_train", _gated_delta_bwd, setup_context=_gated_delta_setup)
 
 
+# --- layer norm -------------------------------------------------------------------
+
+@custom_op(f"{NS}::layer_norm", mutates_args=())
+def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None,
+               eps: float = 1e-5) -> Tuple[Tensor, Tensor]:
+    """(y in x's dtype, the rows' means and inverse roots fp32 [rows, 2])."""
+    return nat.host().layer_norm_forward(norm._operands(x, weight, bias), eps, True)
+
+
+@layer_norm.register_fake
+def _(x, weight=None, bias=None, eps=1e-5):
+    rows = x.numel() // x.shape[-1] if x.shape[-1] else 0
+    return x.new_empty(x.shape), x.new_empty(rows, 2, dtype=torch.float32)
+
+
+@custom_op(f"{NS}::layer_norm_backward", mutates_args=())
+def layer_norm_backward(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], stats: Tensor,
+                        dy: Tensor) -> Tuple[Tensor, Tensor, Tensor]:
+    """(dx in x's dtype, dweight and dbias in fp32, empty where they do not apply)."""
+    dx, dw, db = nat.host().layer_norm_backward(norm._operands(x, weight, bias), stats, dy)
+    none = lambda: x.new_empty(0, dtype=torch.float32)
+    return dx, none() if dw is None else dw, none() if db is None else db
+
+
+@layer_norm_backward.register_fake
+def _(x, weight, bias, stats, dy):
+    sums = [x.new_empty(0 if w is None else w.shape[0], dtype=torch.float32) for w in (weight, bias)]
+    return x.new_empty(x.shape), *sums
+
+
+def _layer_norm_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:3], output[1])
+
+
+def _layer_norm_bwd(ctx, dy, _gstats):
+    x, weight, bias, stats = ctx.saved_tensors
+    dx, dw, db = layer_norm_backward(x, weight, bias, stats, dy)
+    return (dx, None if weight is None else dw.to(weight.dtype),
+            None if bias is None else db.to(bias.dtype), None)
+
+
+register_autograd(f"{NS}::layer_norm", _layer_norm_bwd, setup_context=_layer_norm_setup)
+
+
 # --- gate, norms and residual between blocks --------------------------------------
 
 @custom_op(f"{NS}::gate_norm_residual", mutates_args=())
@@ -689,5 +733,5 @@ OPS = (
     "quaternion_layer_norm", "quaternion_layer_norm_backward", "causal_conv1d_silu",
     "causal_conv1d_silu_backward", "out_gate", "out_gate_backward", "gated_scan", "gated_scan_train",
     "gated_scan_backward", "gated_delta", "gated_delta_train", "gated_delta_backward",
-    "gate_norm_residual", "gate_norm_residual_backward",
+    "gate_norm_residual", "gate_norm_residual_backward", "layer_norm", "layer_norm_backward",
 )
