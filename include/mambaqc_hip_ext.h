@@ -1,8 +1,8 @@
 /* Entry points of libmambaqc_hip.so beside the drop-in boundary of mambaqc_hip.h: products
  * and fused steps that the Python layers choose by size, each computing what operators of
  * mambaqc_hip.h or torch compute otherwise, and the operators of a recurrent stack (the gated
- * scan, the gate with norms and residual, the AdamW step). Conventions, status codes and dtype
- * codes are that header's. */
+ * scan, the gated delta rule, the gate with norms and residual, layer norm, the AdamW and the Muon
+ * step). Conventions, status codes and dtype codes are that header's. */
 #ifndef MAMBAQC_HIP_EXT_H
 #define MAMBAQC_HIP_EXT_H
 
@@ -246,6 +246,26 @@ int mqc_layer_norm_fwd(const void* x, int64_t x_row, const float* weight, const 
 int mqc_layer_norm_bwd(const void* x, int64_t x_row, const float* weight, const float* stats,
                        const void* dy, void* dx, float* dweight, float* dbias, int64_t rows, int64_t d,
                        int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Newton's and Schulz's iteration for each of `batch` matrices [rows, cols], dense, x to out (which may be x):
+ *   X = x / max(|x|_F, eps);  `steps` times  A = X X^T,  X = a X + (b A + c A^2) X
+ * (on the shorter side). Singular values of X and of A have to stay below 64 on the way. bf16 matrices pass
+ * through products of fp16 operands, fp32 and fp16 ones through pairs of them (2^-22 of a value). steps 1 to
+ * 100; MQC_E_LIMIT beyond 65535 matrices, a shorter side of 32768, a longer one of 2^24 and launches of 2^32
+ * threads. workspace (256-byte aligned) of mqc_orthogonalize_workspace_bytes.
+ *
+ * mqc_muon_step: for each of `count` matrices, rows of six values p, grad, m, rows, cols, dtype (pointers as
+ * integers, dense, aligned to their elements; m fp32; read before the call returns):
+ *   m = momentum m + (1 - momentum) grad,  u = momentum m + (1 - momentum) grad (nesterov) or m
+ *   p = p decay - rate sqrt(max(1, rows / cols)) X  with X from u as above */
+int64_t mqc_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int dtype);
+int mqc_orthogonalize(const void* x, void* out, int64_t batch, int64_t rows, int64_t cols, int steps,
+                      float a, float b, float c, float eps, int dtype, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+int64_t mqc_muon_workspace_bytes(const int64_t* matrices, int64_t count);
+int mqc_muon_step(const int64_t* matrices, int64_t count, float decay, float rate, float momentum,
+                  int nesterov, int steps, float a, float b, float c, float eps, void* workspace,
+                  int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

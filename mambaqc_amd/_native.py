@@ -119,6 +119,8 @@ SIGNATURES_EXT = {
     "mqc_gated_scan_fwd": [_vp, _i64] * 3 + [_vp] * 6 + [_i64] * 3 + [_int, _vp, _i64, _vp],
     "mqc_gated_scan_bwd": [_vp, _i64] * 3 + [_vp] * 10 + [_i64] * 3 + [_int, _vp, _i64, _vp],
     "mqc_gated_scan_step": [_vp, _i64] * 3 + [_vp] * 3 + [_i64] * 2 + [_int, _vp],
+    "mqc_orthogonalize": [_vp] * 2 + [_i64] * 3 + [_int] + [_f32] * 4 + [_int, _vp, _i64, _vp],
+    "mqc_muon_step": [_vp, _i64] + [_f32] * 3 + [_int] * 2 + [_f32] * 4 + [_vp, _i64, _vp],
     "mqc_layer_norm_fwd": [_vp, _i64] + [_vp] * 4 + [_i64] * 2 + [_f32, _int, _vp],
     "mqc_layer_norm_bwd": [_vp, _i64] + [_vp] * 6 + [_i64] * 2 + [_int, _vp, _i64, _vp],
     "mqc_gated_delta_chunk": [],
@@ -130,6 +132,8 @@ SIGNATURES_EXT = {
                             + [_f32, _int, _vp],
 }
 SIGNATURES_EXT_I64 = {
+    "mqc_orthogonalize_workspace_bytes": [_i64] * 3 + [_int],
+    "mqc_muon_workspace_bytes": [_vp, _i64],
     "mqc_layer_norm_max_width": [],
     "mqc_layer_norm_workspace_bytes": [_i64, _i64],
     "mqc_gated_delta_key_width": [_i64],

@@ -17,10 +17,10 @@
 //
 // Three kinds of kernels. One over all chunks side by side forms the products within them (gram
 // matrices, the triangular inverse) and lays every operand out as the matrix instructions read it. One
-// walks the chunks of a head: columns of S do not depend on one another, so each wave owns 16 of them and
-// keeps them in registers from the first chunk to the last, with no barrier and no word to another wave:
-// what a product leaves (a column a lane, four rows each) is what the next one takes as its right operand
-// if the left one's columns are in the order kPlace. The backward's gradients of q, k, g and beta need
+// walks the chunks of a head: columns of S do not depend on one another, so a workgroup has 16 or 32 of
+// them, in registers from the first chunk to the last. What a product leaves (a column a lane, four rows
+// each) is what the next one takes as its right operand if the left one's columns are in the order that
+// place() gives. The backward's gradients of q, k, g and beta need
 // sums over v_dim: again over all chunks side by side.
 //
 // Products are of bf16 matrix instructions on operands cut into pieces of 8 bits: three hold an fp32
@@ -88,6 +88,14 @@ __device__ inline floatx4 mma(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], floa
       if (order - i >= 0 && order - i < NB)
         acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[order - i], acc, 0, 0, 0);
   return acc;
+}
+
+// After the last product into v and before v is used: eight wait states in the same basic block. (The
+// compiler keeps results of matrix instructions from being read too early, but not in every case where a
+// branch lies between the two: it read the last of four values before its sum was there.)
+__device__ inline floatx4 settled(floatx4 v) {
+  asm volatile("s_nop 7" : "+v"(v));
+  return v;
 }
 
 template <int N>
@@ -312,6 +320,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Args<T> a) {
       kk = mma(kf[i], kn, kk);
       qk = mma(qf[i], kn, qk);
     }
+    kk = settled(kk), qk = settled(qk);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       s.kk[16 * w + 4 * g + r][16 * n + m] = kk[r];
@@ -378,8 +387,43 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Args<T> a) {
 }
 
 // ---------------------------------------------------------------------------
-// The walks. A wave has 16 columns of a head's state.
+// The walks. A workgroup has CT times 16 columns of a head's state, its wave w the tokens 16 w.. of each
+// chunk and the state's rows 16 w.. and 16 (w + 4)... A product's left operand is the wave's own rows, from
+// memory to registers a chunk ahead; its right one (the state, then what the tokens leave) is all waves',
+// and goes through LDS as pieces.
 // ---------------------------------------------------------------------------
+template <int KD, int CT>
+struct WalkShared {
+  static constexpr int KS = KD / 32;
+  uint16_t state[2][CT][KS * kPieces * kFrag];  // of this chunk and of the next
+  uint16_t x[CT][2 * kPieces * kFrag], u[CT][2 * kPieces * kFrag], y[CT][2 * kPieces * kFrag];
+  uint16_t d_o[2][CT][2 * kPieces * kFrag];     // (backward)
+  float xs[2][CT][kC][16];                      // x and u in fp32 where documents meet
+  int bad[2][4];                                // whether a wave has some that are not finite
+};
+
+// A barrier for what is in LDS; accesses to memory stay under way.
+__device__ inline void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// Rows 16 tile.. of a right operand [.., 16], as pieces of its fragments.
+template <int N>
+__device__ inline void put_tile(uint16_t* frags, int tile, const floatx4& v) {
+  const int lane = threadIdx.x & 63;
+  float x[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+  for (int p = 0; p < N; ++p) {
+    uint2 w;
+    w.x = p + 1 < N ? cut2(x[0], x[1]) : pack2<bf16_t>(x[0], x[1]);
+    w.y = p + 1 < N ? cut2(x[2], x[3]) : pack2<bf16_t>(x[2], x[3]);
+    *reinterpret_cast<uint2*>(frags + (tile / 2 * N + p) * kFrag + lane * 8 + tile % 2 * 4) = w;
+    if (p + 1 < N) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) x[c] = rest(x[c]);
+    }
+  }
+}
 
 // Element (row, col) of a triangular matrix that is there as fragments.
 template <bool UPPER>
@@ -394,291 +438,419 @@ __device__ inline float tri_at(const uint16_t* tri, int row, int col) {
 }
 
 __device__ inline bool finite(float v) { return fabsf(v) < __builtin_huge_valf(); }
-__device__ inline bool finite(const floatx4 (&x)[4]) {
-  bool ok = true;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) ok = ok && finite(x[i][r]);
-  return __ballot(!ok) == 0;
-}
 
-// tri x, a triangular matrix [64, 64] (its fragments) times the wave's columns. Where documents meet in
-// the chunk (`mixed`) and x is not finite, term by term: zero times NaN is not zero.
+// The wave's rows of a triangular matrix: fragments of its one or two columns of 32.
 template <bool UPPER>
-__device__ inline void tri_product(const uint16_t* tri, const floatx4 (&x)[4], bool mixed,
-                                   const float* doc, float (*xs)[17], floatx4 (&out)[4]) {
-  const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
-  if (mixed && !finite(x)) {
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) xs[16 * i + 4 * g + r][m] = x[i][r];
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = 16 * i + 4 * g + r;
-        float v = 0.f;
-        for (int j = UPPER ? row : 0; UPPER ? j < kC : j <= row; ++j)
-          if (doc[j] == doc[row]) v = fmaf(tri_at<UPPER>(tri, row, j), xs[j][m], v);
-        out[i][r] = v;
-      }
-    __syncthreads();
-    return;
-  }
-  bf16x8 xf[2][kPieces];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) split<kPieces>(x[2 * s], x[2 * s + 1], xf[s]);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    floatx4 v = {};
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int f = UPPER ? upper_frag(i, s) : lower_frag(i, s);
-      if (f < 0) continue;
-      bf16x8 tf[kPieces];
-      load_frag(tri + f * kPieces * kFrag, lane, tf);
-      v = mma(tf, xf[s], v);
+__device__ inline void load_tri(const uint16_t* tri, int w, bf16x8 (&f)[2][kPieces]) {
+  const int lane = threadIdx.x & 63;
+  const bool both = UPPER ? w < 2 : w >= 2;
+  const int first = UPPER ? (w < 2 ? 2 * w : w + 2) : (w < 2 ? w : 2 * w - 2);
+  load_frag(tri + first * kPieces * kFrag, lane, f[UPPER ? (both ? 0 : 1) : 0]);
+  if (both) load_frag(tri + (first + 1) * kPieces * kFrag, lane, f[1]);
+}
+// Their product with x. Where documents meet in the chunk (`mixed`) and x is not finite somewhere (`bad`, of
+// each wave), term by term: zero times NaN is not zero.
+template <bool UPPER, int NX>
+__device__ inline floatx4 tri_product(const bf16x8 (&f)[2][kPieces], const uint16_t* x, int w, bool mixed,
+                                      const int* bad, const float (*xs)[16], const uint16_t* tri,
+                                      const float* doc) {
+  const int lane = threadIdx.x & 63;
+  floatx4 v = {};
+  if (mixed && (bad[0] | bad[1] | bad[2] | bad[3])) {
+    for (int r = 0; r < 4; ++r) {
+      const int row = 16 * w + 4 * (lane >> 4) + r;
+      float s = 0.f;
+#pragma unroll 1
+      for (int j = UPPER ? row : 0; UPPER ? j < kC : j <= row; ++j)
+        if (doc[j] == doc[row]) s = fmaf(tri_at<UPPER>(tri, row, j), xs[j][lane & 15], s);
+      v[r] = s;
     }
-    out[i] = v;
+    return v;
   }
+  bf16x8 b[NX];
+  if (!UPPER || w < 2) {
+    load_frag(x, lane, b);
+    v = settled(mma(f[0], b, v));
+  }
+  if (UPPER || w >= 2) {
+    load_frag(x + NX * kFrag, lane, b);
+    v = settled(mma(f[1], b, v));
+  }
+  return v;
 }
 
-// rows x S for the chunk's rows (K or Q as fragments by rows) and the state's pieces.
-template <int KS, int NP>
-__device__ inline void row_product(const uint16_t* rows, const bf16x8 (&sf)[KS][kPieces],
-                                   floatx4 (&out)[4]) {
-  const int lane = threadIdx.x & 63;
+// What the two walks share: where a workgroup is, and its operands.
+template <typename T, int KD, bool BWD, int CT>
+struct Walker {
+  static constexpr int NP = kIn<T>, KS = KD / 32, MT = KD / 16 > 4 ? 2 : 1;
+  static constexpr int kPart = KD / 8 * NP * kFrag, kTriPart = kTri * kPieces * kFrag;
+  const Args<T>& a;
+  int lane, w, g, m;
+  int64_t b, hv, hk, bh;
+  int col0;
+  bool holds;  // whether the wave has rows of the state (of 32 only two do)
+  const uint16_t *keys, *tri;
+  const float* vec;
+
+  __device__ explicit Walker(const Args<T>& a_) : a(a_) {
+    lane = threadIdx.x & 63;
+    w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    g = lane >> 4, m = lane & 15;
+    const int groups = (a.v_pad / 16 + CT - 1) / CT;
+    const int64_t unit = xcd_order(blockIdx.x, gridDim.x);
+    bh = unit / groups;
+    b = bh / a.v_heads, hv = bh % a.v_heads, hk = hv / (a.v_heads / a.k_heads);
+    col0 = (int)(unit % groups) * CT * 16;
+    holds = w < KD / 16;
+    keys = a.keys + (b * a.k_heads + hk) * a.chunks * (3 * kPart);
+    tri = a.tri + bh * a.chunks * (2 * kTriPart);
+    vec = a.vec + bh * a.chunks * (4 * kC);
+  }
+  __device__ int col(int ct) const { return col0 + 16 * ct + m; }
+  // Fragments of the wave's tokens of K or Q, and of its rows of K^T or Q^T, of a chunk.
+  __device__ const uint16_t* part(int64_t c, int i) const { return keys + c * (3 * kPart) + i * kPart; }
+  __device__ void load_rows(int64_t c, int i, bf16x8 (&f)[KS][NP]) const {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+    for (int s = 0; s < KS; ++s) load_frag(part(c, i) + (s * 4 + w) * NP * kFrag, lane, f[s]);
+  }
+  __device__ void load_cols(int64_t c, int i, bf16x8 (&f)[MT][2][NP]) const {
+    if (!holds) return;
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+        load_frag(part(c, i) + ((w + 4 * t) * 2 + s) * NP * kFrag, lane, f[t][s]);
+  }
+  // rows x state.
+  __device__ floatx4 row_product(const bf16x8 (&f)[KS][NP], const uint16_t* state) const {
     floatx4 v = {};
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      bf16x8 f[NP];
-      load_frag(rows + (s * 4 + i) * NP * kFrag, lane, f);
-      v = mma(f, sf[s], v);
+      bf16x8 b[kPieces];
+      load_frag(state + s * kPieces * kFrag, lane, b);
+      v = mma(f[s], b, v);
     }
-    out[i] = v;
+    return settled(v);
   }
-}
-
-// S += cols x for K^T or Q^T as fragments; tokens of other documents than `keep` left out where `cut`.
-template <int KD, int NP>
-__device__ inline void col_product(const uint16_t* cols, const floatx4 (&x)[4], bool cut,
-                                   const float* doc, float keep, floatx4 (&S)[KD / 16]) {
-  const int lane = threadIdx.x & 63, g = lane >> 4;
-  bf16x8 xf[2][kPieces];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) split<kPieces>(x[2 * s], x[2 * s + 1], xf[s]);
-  if (cut) {
-    u32x4 mask[2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t e = doc[32 * s + place(g, j)] == keep ? 0xffffu : 0u;
-        mask[s][j / 2] = j % 2 ? mask[s][j / 2] | e << 16 : e;
-      }
-#pragma unroll
-    for (int i = 0; i < KD / 16; ++i)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        bf16x8 f[NP];
-        load_frag(cols + (i * 2 + s) * NP * kFrag, lane, f);
-#pragma unroll
-        for (int p = 0; p < NP; ++p)
-          f[p] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, f[p]) & mask[s]);
-        S[i] = mma(f, xf[s], S[i]);
-      }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < KD / 16; ++i)
+  // S += cols x; tokens of other documents than `keep` left out where `cut`.
+  __device__ void col_product(const bf16x8 (&f)[MT][2][NP], const uint16_t* x, bool cut, const float* doc,
+                              float keep, floatx4 (&S)[MT]) const {
+    if (!holds) return;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      bf16x8 f[NP];
-      load_frag(cols + (i * 2 + s) * NP * kFrag, lane, f);
-      S[i] = mma(f, xf[s], S[i]);
-    }
-}
-
-// The wave's columns of a state [k_dim, v_dim] in memory.
-template <int KD, typename T>
-__device__ inline void load_state(const Args<T>& a, const float* from, int col, floatx4 (&S)[KD / 16]) {
-  const int g = (threadIdx.x & 63) >> 4;
+      bf16x8 xf[kPieces];
+      load_frag(x + s * kPieces * kFrag, lane, xf);
+      if (cut) {
+        u32x4 mask = {};
 #pragma unroll
-  for (int i = 0; i < KD / 16; ++i)
+        for (int j = 0; j < 8; ++j)
+          if (doc[32 * s + place(g, j)] == keep) mask[j / 2] |= j % 2 ? 0xffff0000u : 0xffffu;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+          bf16x8 only[NP];
+#pragma unroll
+          for (int p = 0; p < NP; ++p)
+            only[p] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, f[t][s][p]) & mask);
+          S[t] = settled(mma(only, xf, S[t]));
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) S[t] = mma(f[t][s], xf, S[t]);
+        if (s == 1) {
+#pragma unroll
+          for (int t = 0; t < MT; ++t) S[t] = settled(S[t]);
+        }
+      }
+    }
+  }
+  __device__ void put_state(uint16_t* frags, const floatx4 (&S)[MT]) const {
+    if (!holds) return;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) put_tile<kPieces>(frags, w + 4 * t, S[t]);
+  }
+  // The wave's rows of a state [k_dim, v_dim] in memory.
+  __device__ void load_state(const float* from, int ct, floatx4 (&S)[MT]) const {
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = 16 * (w + 4 * t) + 4 * g + r;
+        S[t][r] = from && d < a.k_dim && col(ct) < a.v_dim
+                      ? from[(bh * a.k_dim + d) * a.v_dim + col(ct)] : 0.f;
+      }
+  }
+  __device__ void store_state(float* to, int ct, const floatx4 (&S)[MT]) const {
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = 16 * (w + 4 * t) + 4 * g + r;
+        if (d < a.k_dim && col(ct) < a.v_dim) to[(bh * a.k_dim + d) * a.v_dim + col(ct)] = S[t][r];
+      }
+  }
+  // The same between chunks, padded.
+  __device__ void store_padded(float* to, int64_t c, int ct, const floatx4 (&S)[MT]) const {
+    if (!holds || col(ct) >= a.v_pad) return;
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        to[((bh * a.chunks + c) * KD + 16 * (w + 4 * t) + 4 * g + r) * a.v_pad + col(ct)] = S[t][r];
+  }
+  __device__ void store_rows(float* to, int64_t c, int ct, const floatx4& v) const {
+    if (col(ct) >= a.v_pad) return;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      to[((bh * a.chunks + c) * kC + 16 * w + 4 * g + r) * a.v_pad + col(ct)] = v[r];
+  }
+  // The wave's tokens of v (or dO) and of o (or dv).
+  __device__ void load_tile(const T* from, int64_t x_b, int64_t x_t, int64_t x_h, int64_t c, int ct,
+                            float (&v)[4]) const {
+    const T* at = from + b * x_b + hv * x_h + col(ct);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int d = 16 * i + 4 * g + r;
-      S[i][r] = from && d < a.k_dim && col < a.v_dim ? from[(int64_t)d * a.v_dim + col] : 0.f;
+      const int64_t t = c * kC + 16 * w + 4 * g + r;
+      v[r] = t < a.seq && col(ct) < a.v_dim ? load_scalar(at + t * x_t) : 0.f;
     }
-}
-template <int KD, typename T>
-__device__ inline void store_state(const Args<T>& a, float* to, int col, const floatx4 (&S)[KD / 16]) {
-  const int g = (threadIdx.x & 63) >> 4;
-#pragma unroll
-  for (int i = 0; i < KD / 16; ++i)
+  }
+  __device__ void store_tile(T* to, int64_t c, int ct, const floatx4& v) const {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int d = 16 * i + 4 * g + r;
-      if (d < a.k_dim && col < a.v_dim) to[(int64_t)d * a.v_dim + col] = S[i][r];
+      const int64_t t = c * kC + 16 * w + 4 * g + r;
+      if (t < a.seq && col(ct) < a.v_dim)
+        store_scalar(to + ((b * a.seq + t) * a.v_heads + hv) * a.v_dim + col(ct), v[r]);
     }
-}
-// The same between chunks, padded.
-template <int KD>
-__device__ inline void store_padded(float* to, int64_t pitch, const floatx4 (&S)[KD / 16]) {
-  const int g = (threadIdx.x & 63) >> 4;
+  }
+  // Rows that are not finite, for tri_product.
+  __device__ void mark(float (*xs)[16], int* bad, const floatx4& v) const {
+    bool ok = true;
 #pragma unroll
-  for (int i = 0; i < KD / 16; ++i)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) to[(16 * i + 4 * g + r) * pitch] = S[i][r];
-}
+    for (int r = 0; r < 4; ++r) {
+      xs[16 * w + 4 * g + r][m] = v[r];
+      ok = ok && finite(v[r]);
+    }
+    const bool some = __ballot(!ok) != 0;
+    if (lane == 0) bad[w] = some;
+  }
+};
 
-template <typename T, int KD>
-__global__ __launch_bounds__(64) void delta_fwd_kernel(Args<T> a) {
-  constexpr int NP = kIn<T>, KS = KD / 32, kPart = KD / 8 * NP * kFrag;
-  __shared__ float xs[kC][17];
-  const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
-  const int tiles = a.v_pad / 16;
-  const int64_t unit = xcd_order(blockIdx.x, gridDim.x), bh = unit / tiles;
-  const int64_t b = bh / a.v_heads, hv = bh % a.v_heads, hk = hv / (a.v_heads / a.k_heads);
-  const int col = (int)(unit % tiles) * 16 + m;
-  const bool real = col < a.v_dim;
-  const T* v = a.v + b * a.v_b + hv * a.v_h + col;
-  const uint16_t* keys = a.keys + (b * a.k_heads + hk) * a.chunks * (3 * kPart);
-  const uint16_t* tri = a.tri + bh * a.chunks * (2 * kTri * kPieces * kFrag);
-  const float* vec = a.vec + bh * a.chunks * (4 * kC);
-  floatx4 S[KD / 16];
-  load_state<KD>(a, a.h0 ? a.h0 + bh * a.k_dim * a.v_dim : nullptr, col, S);
+// A chunk's gates, for the wave's tokens.
+struct RowGates {
+  floatx4 e, end, beta, doc;
+  float all, first, last;
+  __device__ void load(const float* vec, int w, int g) {
+    const int at = 16 * w + 4 * g;
+    e = *reinterpret_cast<const floatx4*>(vec + at);
+    end = *reinterpret_cast<const floatx4*>(vec + kC + at);
+    beta = *reinterpret_cast<const floatx4*>(vec + 2 * kC + at);
+    doc = *reinterpret_cast<const floatx4*>(vec + 3 * kC + at);
+    all = vec[kC - 1], first = vec[3 * kC], last = vec[4 * kC - 1];
+  }
+};
+
+// Waves to a SIMD where their operands leave registers for that (two hide one another's waits).
+template <typename T, int KD, int CT, bool BWD>
+constexpr int kWalkWaves = CT == 1 && (BWD ? (kIn<T> == 1 && KD == 128) || (kIn<T> == 2 && KD < 128)
+                                           : kIn<T> == 1 || (kIn<T> == 2 && KD < 128)) ? 2 : 1;
+
+template <typename T, int KD, int CT>
+__global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, false>)) void delta_fwd_kernel(Args<T> a) {
+  __shared__ __attribute__((aligned(16))) WalkShared<KD, CT> s;
+  const Walker<T, KD, false, CT> k(a);
+  using K = Walker<T, KD, false, CT>;
+  constexpr int NP = K::NP, KS = K::KS, MT = K::MT;
+  floatx4 S[CT][MT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    k.load_state(a.h0, ct, S[ct]);
+    k.put_state(s.state[0][ct], S[ct]);
+  }
+  bf16x8 kf[KS][NP], qf[KS][NP], tf[2][kPieces], pf[2][kPieces], cf[MT][2][NP];
+  float v[CT][4];
+  RowGates next;
+  if (a.chunks > 0) {
+    next.load(k.vec, k.w, k.g);
+    k.load_rows(0, 0, kf);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) k.load_tile(a.v, a.v_b, a.v_t, a.v_h, 0, ct, v[ct]);
+    load_tri<false>(k.tri, k.w, tf);
+    k.load_cols(0, 1, cf);
+    k.load_rows(0, 2, qf);
+    load_tri<false>(k.tri + K::kTriPart, k.w, pf);
+  }
   for (int64_t c = 0; c < a.chunks; ++c) {
-    const float* doc = vec + 3 * kC;
-    const bool mixed = doc[0] != doc[kC - 1];
-    if (a.states) store_padded<KD>(a.states + (bh * a.chunks + c) * KD * a.v_pad + col, a.v_pad, S);
-    bf16x8 sf[KS][kPieces];
+    const RowGates at = next;
+    const float* doc = k.vec + c * 4 * kC + 3 * kC;
+    const uint16_t* tri = k.tri + c * 2 * K::kTriPart;
+    const bool mixed = at.first != at.last, cut = at.last != 0.f, more = c + 1 < a.chunks;
+    lds_barrier();
+    if (more) next.load(k.vec + (c + 1) * 4 * kC, k.w, k.g);
+    floatx4 x[CT];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) split<kPieces>(S[2 * s], S[2 * s + 1], sf[s]);
-    floatx4 x[4], r[4];
-    row_product<KS, NP>(keys, sf, x);
+    for (int ct = 0; ct < CT; ++ct) x[ct] = k.row_product(kf, s.state[c & 1][ct]);
+    if (more) k.load_rows(c + 1, 0, kf);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int row = 16 * i + 4 * g + j;
-        const int64_t t = c * kC + row;
-        const float vt = real && t < a.seq ? load_scalar(v + t * a.v_t) : 0.f;
-        x[i][j] = doc[row] == 0.f && t < a.seq ? fmaf(-vec[row], x[i][j], vt) : vt;
-      }
-    tri_product<false>(tri, x, mixed, doc, xs, r);
-    if (a.resid) {
-      float* to = a.resid + (bh * a.chunks + c) * kC * a.v_pad + col;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) to[(int64_t)(16 * i + 4 * g + j) * a.v_pad] = r[i][j];
+      for (int r = 0; r < 4; ++r)
+        x[ct][r] = at.doc[r] == 0.f && c * kC + 16 * k.w + 4 * k.g + r < a.seq
+                       ? fmaf(-at.e[r], x[ct][r], v[ct][r]) : v[ct][r];
+      put_tile<kPieces>(s.x[ct], k.w, x[ct]);
+      if (mixed) k.mark(s.xs[0][ct], s.bad[0], x[ct]);
+      if (a.states) k.store_padded(a.states, c, ct, S[ct]);
+      if (more) k.load_tile(a.v, a.v_b, a.v_t, a.v_h, c + 1, ct, v[ct]);
     }
+    lds_barrier();
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int ct = 0; ct < CT; ++ct) {
+      floatx4 r = tri_product<false, kPieces>(tf, s.x[ct], k.w, mixed, s.bad[0], s.xs[0][ct], tri, doc);
+      if (a.resid) k.store_rows(a.resid, c, ct, r);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r[i][j] *= vec[2 * kC + 16 * i + 4 * g + j];
-    floatx4 y[4];
-    row_product<KS, NP>(keys + 2 * kPart, sf, x);
-    tri_product<false>(tri + kTri * kPieces * kFrag, r, mixed, doc, xs, y);
+      for (int i = 0; i < 4; ++i) r[i] *= at.beta[i];
+      put_tile<kPieces>(s.u[ct], k.w, r);
+      if (mixed) k.mark(s.xs[1][ct], s.bad[1], r);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i) r[i] = at.doc[i] == at.last ? r[i] * at.end[i] : 0.f;
+      put_tile<kPieces>(s.y[ct], k.w, r);
+    }
+    if (more) load_tri<false>(tri + 2 * K::kTriPart, k.w, tf);
+    lds_barrier();
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int row = 16 * i + 4 * g + j;
-        const int64_t t = c * kC + row;
-        const float ot = a.scale * (doc[row] == 0.f ? fmaf(vec[row], x[i][j], y[i][j]) : y[i][j]);
-        if (real && t < a.seq)
-          store_scalar(a.o + ((b * a.seq + t) * a.v_heads + hv) * a.v_dim + col, ot);
-        r[i][j] = doc[row] == doc[kC - 1] ? r[i][j] * vec[kC + row] : 0.f;
-      }
-    const float all = vec[kC - 1];
-    const bool cut = doc[kC - 1] != 0.f;
+    for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll
-    for (int i = 0; i < KD / 16; ++i)
+      for (int t = 0; t < MT; ++t)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) S[i][j] = cut ? 0.f : S[i][j] * all;
-    col_product<KD, NP>(keys + kPart, r, mixed, doc, doc[kC - 1], S);
-    keys += 3 * kPart;
-    tri += 2 * kTri * kPieces * kFrag;
-    vec += 4 * kC;
+        for (int r = 0; r < 4; ++r) S[ct][t][r] = cut ? 0.f : S[ct][t][r] * at.all;
+      k.col_product(cf, s.y[ct], mixed, doc, at.last, S[ct]);
+      k.put_state(s.state[(c + 1) & 1][ct], S[ct]);
+    }
+    if (more) k.load_cols(c + 1, 1, cf);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      const floatx4 qs = k.row_product(qf, s.state[c & 1][ct]);
+      floatx4 o = tri_product<false, kPieces>(pf, s.u[ct], k.w, mixed, s.bad[1], s.xs[1][ct],
+                                              tri + K::kTriPart, doc);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = a.scale * (at.doc[r] == 0.f ? fmaf(at.e[r], qs[r], o[r]) : o[r]);
+      k.store_tile(a.o, c, ct, o);
+    }
+    if (more) {
+      k.load_rows(c + 1, 2, qf);
+      load_tri<false>(tri + 3 * K::kTriPart, k.w, pf);
+    }
   }
-  if (a.h_last) store_state<KD>(a, a.h_last + bh * a.k_dim * a.v_dim, col, S);
+  if (a.h_last && k.holds) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) k.store_state(a.h_last, ct, S[ct]);
+  }
 }
 
-template <typename T, int KD>
-__global__ __launch_bounds__(64) void delta_bwd_kernel(Args<T> a) {
-  constexpr int NP = kIn<T>, KS = KD / 32, kPart = KD / 8 * NP * kFrag;
-  __shared__ float xs[kC][17];
-  const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
-  const int tiles = a.v_pad / 16;
-  const int64_t unit = xcd_order(blockIdx.x, gridDim.x), bh = unit / tiles;
-  const int64_t b = bh / a.v_heads, hv = bh % a.v_heads, hk = hv / (a.v_heads / a.k_heads);
-  const int col = (int)(unit % tiles) * 16 + m;
-  const bool real = col < a.v_dim;
-  floatx4 S[KD / 16];  // the gradient of the state after the chunk
-  load_state<KD>(a, a.dh_last ? a.dh_last + bh * a.k_dim * a.v_dim : nullptr, col, S);
-  for (int64_t c = a.chunks - 1; c >= 0; --c) {
-    const uint16_t* keys = a.keys + ((b * a.k_heads + hk) * a.chunks + c) * (3 * kPart);
-    const uint16_t* tri = a.tri + (bh * a.chunks + c) * (2 * kTri * kPieces * kFrag);
-    const float* vec = a.vec + (bh * a.chunks + c) * (4 * kC);
-    const float* doc = vec + 3 * kC;
-    const bool mixed = doc[0] != doc[kC - 1], cut = doc[kC - 1] != 0.f;
-    store_padded<KD>(a.dstates + (bh * a.chunks + c) * KD * a.v_pad + col, a.v_pad, S);
-    floatx4 x[4], y[4], z[4];
-    {
-      bf16x8 sf[KS][kPieces];
+template <typename T, int KD, int CT>
+__global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, true>)) void delta_bwd_kernel(Args<T> a) {
+  __shared__ __attribute__((aligned(16))) WalkShared<KD, CT> s;
+  const Walker<T, KD, true, CT> k(a);
+  using K = Walker<T, KD, true, CT>;
+  constexpr int NP = K::NP, KS = K::KS, MT = K::MT;
+  const int64_t heads = a.v_heads * (int64_t)a.v_dim, end = a.chunks - 1;
+  const auto load_grad = [&](int64_t c, int ct, float (&v)[4]) {
+    k.load_tile(a.d_o, a.seq * heads, heads, a.v_dim, c, ct, v);
+  };
+  floatx4 S[CT][MT];  // the gradient of the state after the chunk
+  float v[CT][4], ahead[CT][4];
 #pragma unroll
-      for (int s = 0; s < KS; ++s) split<kPieces>(S[2 * s], S[2 * s + 1], sf[s]);
-      row_product<KS, NP>(keys, sf, y);
+  for (int ct = 0; ct < CT; ++ct) {
+    k.load_state(a.dh_last, ct, S[ct]);
+    k.put_state(s.state[end & 1][ct], S[ct]);
+    load_grad(end, ct, v[ct]);
+    put_tile<NP>(s.d_o[end & 1][ct], k.w, floatx4{v[ct][0], v[ct][1], v[ct][2], v[ct][3]});
+  }
+  bf16x8 kf[KS][NP], tf[2][kPieces], pf[2][kPieces], cf[MT][2][NP], qf[MT][2][NP];
+  RowGates next;
+  {
+    next.load(k.vec + end * 4 * kC, k.w, k.g);
+    k.load_rows(end, 0, kf);
+    load_tri<true>(k.tri + (2 * end + 1) * K::kTriPart, k.w, pf);
+    load_tri<true>(k.tri + 2 * end * K::kTriPart, k.w, tf);
+    k.load_cols(end, 2, qf);
+    k.load_cols(end, 1, cf);
+  }
+  for (int64_t c = end; c >= 0; --c) {
+    const RowGates at = next;
+    const float* doc = k.vec + c * 4 * kC + 3 * kC;
+    const uint16_t* tri = k.tri + c * 2 * K::kTriPart;
+    const bool mixed = at.first != at.last, cut = at.last != 0.f, more = c > 0;
+    if (mixed) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+        k.mark(s.xs[1][ct], s.bad[1], floatx4{v[ct][0], v[ct][1], v[ct][2], v[ct][3]});
+    }
+    lds_barrier();
+    if (more) {
+      next.load(k.vec + (c - 1) * 4 * kC, k.w, k.g);
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) load_grad(c - 1, ct, ahead[ct]);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int ct = 0; ct < CT; ++ct) {
+      const floatx4 y = k.row_product(kf, s.state[c & 1][ct]);
+      floatx4 z = tri_product<true, NP>(pf, s.d_o[c & 1][ct], k.w, mixed, s.bad[1], s.xs[1][ct],
+                                        tri + K::kTriPart, doc);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t t = c * kC + 16 * i + 4 * g + j;
-        x[i][j] = real && t < a.seq
-                      ? a.scale * load_scalar(a.d_o + ((b * a.seq + t) * a.v_heads + hv) * a.v_dim + col)
-                      : 0.f;
+      for (int r = 0; r < 4; ++r) {
+        z[r] *= a.scale;
+        if (at.doc[r] == at.last) z[r] = fmaf(at.end[r], y[r], z[r]);
       }
-    tri_product<true>(tri + kTri * kPieces * kFrag, x, mixed, doc, xs, z);
+      put_tile<kPieces>(s.x[ct], k.w, z);
+      if (mixed) k.mark(s.xs[0][ct], s.bad[0], z);
+      // e dO, for the state.
+      floatx4 x;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+      for (int r = 0; r < 4; ++r) x[r] = at.doc[r] == 0.f ? v[ct][r] * (a.scale * at.e[r]) : 0.f;
+      put_tile<kPieces>(s.u[ct], k.w, x);
+      k.store_padded(a.dstates, c, ct, S[ct]);
+    }
+    if (more) {
+      k.load_rows(c - 1, 0, kf);
+      load_tri<true>(tri - K::kTriPart, k.w, pf);
+    }
+    lds_barrier();
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int row = 16 * i + 4 * g + j;
-        if (doc[row] == doc[kC - 1]) z[i][j] = fmaf(vec[kC + row], y[i][j], z[i][j]);
+    for (int ct = 0; ct < CT; ++ct) {
+      floatx4 z = tri_product<true, kPieces>(tf, s.x[ct], k.w, mixed, s.bad[0], s.xs[0][ct], tri, doc);
+      k.store_rows(a.z, c, ct, z);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) z[r] *= at.beta[r];
+      k.store_tile(a.dv, c, ct, z);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) z[r] = at.doc[r] == 0.f ? -z[r] * at.e[r] : 0.f;
+      put_tile<kPieces>(s.y[ct], k.w, z);
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[ct][t][r] = cut ? 0.f : S[ct][t][r] * at.all;
+      k.col_product(qf, s.u[ct], cut, doc, 0.f, S[ct]);
+    }
+    if (more) {
+      load_tri<true>(tri - 2 * K::kTriPart, k.w, tf);
+      k.load_cols(c - 1, 2, qf);
+    }
+    lds_barrier();
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      k.col_product(cf, s.y[ct], cut, doc, 0.f, S[ct]);
+      k.put_state(s.state[(c + 1) & 1][ct], S[ct]);
+      if (more) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[ct][r] = ahead[ct][r];
+        put_tile<NP>(s.d_o[(c + 1) & 1][ct], k.w, floatx4{v[ct][0], v[ct][1], v[ct][2], v[ct][3]});
       }
-    tri_product<true>(tri, z, mixed, doc, xs, y);
-    float* zs = a.z + (bh * a.chunks + c) * kC * a.v_pad + col;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int row = 16 * i + 4 * g + j;
-        const int64_t t = c * kC + row;
-        zs[(int64_t)row * a.v_pad] = y[i][j];
-        const float dv = vec[2 * kC + row] * y[i][j];
-        if (real && t < a.seq)
-          store_scalar(a.dv + ((b * a.seq + t) * a.v_heads + hv) * a.v_dim + col, dv);
-        x[i][j] = doc[row] == 0.f ? x[i][j] * vec[row] : 0.f;
-        y[i][j] = doc[row] == 0.f ? -dv * vec[row] : 0.f;
-      }
-    const float all = vec[kC - 1];
-#pragma unroll
-    for (int i = 0; i < KD / 16; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) S[i][j] = cut ? 0.f : S[i][j] * all;
-    col_product<KD, NP>(keys + 2 * kPart, x, cut, doc, 0.f, S);
-    col_product<KD, NP>(keys + kPart, y, cut, doc, 0.f, S);
+    }
+    if (more) k.load_cols(c - 1, 1, cf);
   }
-  if (a.dh0) store_state<KD>(a, a.dh0 + bh * a.k_dim * a.v_dim, col, S);
+  if (a.dh0 && k.holds) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) k.store_state(a.dh0, ct, S[ct]);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -808,6 +980,7 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(Args<T> a) {
   float wrote = 0.f;  // k . (dS' u)
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
+    dq[i] = settled(dq[i]), ka[i] = settled(ka[i]), kb[i] = settled(kb[i]);
     const int d = 16 * i + 4 * g;
     float kv[4] = {0.f, 0.f, 0.f, 0.f};
     if (here && d < a.k_dim) load_part(krow, d, a.k_dim - d, kv);
@@ -823,6 +996,7 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(Args<T> a) {
 #pragma unroll
   for (int n = 0; n < 5; ++n) {
     const bool turned = n <= w;
+    p[n] = settled(p[n]), mm[n] = settled(mm[n]);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int other = 16 * (turned ? n : n - 1) + 4 * g + r;
@@ -871,6 +1045,7 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(Args<T> a) {
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const int d = 16 * i + 4 * g;
+    dq[i] = settled(dq[i]), ka[i] = settled(ka[i]), kb[i] = settled(kb[i]);
     if (!here || d >= a.k_dim) continue;
     float qv[4], kv[4], dk[4], dqv[4];
     load_part(qrow, d, a.k_dim - d, qv);

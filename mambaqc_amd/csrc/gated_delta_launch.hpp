@@ -10,15 +10,30 @@ namespace delta {
   if (a.k_dim <= 64) return F(64);  \
   return F(128);
 
+// Columns of the state to a workgroup: 16 as long as the card has room for more workgroups.
+template <typename T, int KD, bool BWD>
+int launch_walk(const Args<T>& a, hipStream_t s) {
+  const int64_t tiles = a.v_pad / 16, heads = a.batch * a.v_heads;
+  if (heads * tiles <= 512) {
+    const dim3 grid((unsigned)(heads * tiles));
+    if constexpr (BWD) delta_bwd_kernel<T, KD, 1><<<grid, dim3(256), 0, s>>>(a);
+    else delta_fwd_kernel<T, KD, 1><<<grid, dim3(256), 0, s>>>(a);
+  } else {
+    const dim3 grid((unsigned)(heads * (tiles / 2)));
+    if constexpr (BWD) delta_bwd_kernel<T, KD, 2><<<grid, dim3(256), 0, s>>>(a);
+    else delta_fwd_kernel<T, KD, 2><<<grid, dim3(256), 0, s>>>(a);
+  }
+  return launch_status();
+}
+
 template <typename T>
 int launch_fwd(const Args<T>& a, hipStream_t s) {
   const unsigned units = (unsigned)(a.batch * a.k_heads * a.chunks);
-  const unsigned waves = (unsigned)(a.batch * a.v_heads * (a.v_pad / 16));
 #define MQC_F(KD)                                                                        \
   [&] {                                                                                  \
     if (units) delta_prep_kernel<T, KD, false><<<dim3(units), dim3(256), 0, s>>>(a);     \
-    delta_fwd_kernel<T, KD><<<dim3(waves), dim3(64), 0, s>>>(a);                         \
-    return launch_status();                                                              \
+    const int st = launch_status();                                                      \
+    return st != MQC_OK ? st : launch_walk<T, KD, false>(a, s);                          \
   }()
   MQC_BY_KEYS(MQC_F)
 #undef MQC_F
@@ -27,13 +42,14 @@ int launch_fwd(const Args<T>& a, hipStream_t s) {
 template <typename T>
 int launch_bwd(const Args<T>& a, hipStream_t s) {
   const unsigned units = (unsigned)(a.batch * a.k_heads * a.chunks);
-  const unsigned waves = (unsigned)(a.batch * a.v_heads * (a.v_pad / 16));
   const unsigned parts = (unsigned)(a.batch * a.v_heads * a.chunks);
   const int64_t shares = (a.batch * a.seq * a.k_heads * a.k_dim + 255) / 256;
 #define MQC_F(KD)                                                                             \
   [&] {                                                                                       \
     delta_prep_kernel<T, KD, true><<<dim3(units), dim3(256), 0, s>>>(a);                      \
-    delta_bwd_kernel<T, KD><<<dim3(waves), dim3(64), 0, s>>>(a);                              \
+    int st = launch_status();                                                                 \
+    if (st == MQC_OK) st = launch_walk<T, KD, true>(a, s);                                    \
+    if (st != MQC_OK) return st;                                                              \
     delta_grad_kernel<T, KD><<<dim3(parts), dim3(256), 0, s>>>(a);                            \
     if (a.k_heads != a.v_heads)                                                               \
       delta_share_kernel<T><<<dim3((unsigned)(shares < 65536 ? shares : 65536)), dim3(256), 0, s>>>(a); \

@@ -1,5 +1,7 @@
-"""AdamW on the GPU: one launch for 88 tensors of a dtype (60 with 8-bit states), states in 32 or in 8
-bits, the gradients' norm and its clipping on the device.
+"""AdamW and Muon on the GPU.
+
+AdamW: one launch for 88 tensors of a dtype (60 with 8-bit states), states in 32 or in 8 bits, the
+gradients' norm and its clipping on the device.
 
     p <- p (1 - lr weight_decay) - lr m^ / (sqrt(v^) + eps),  m^ = m / (1 - beta1^t),  v^ = v / (1 - beta2^t)
 
@@ -11,6 +13,15 @@ clip to 1.0, then the step); `adamw_step_`, `adamw8_step_` and `grad_norm` are t
 of a tensor: 2.03 bytes a parameter instead of 8 (a 14.66 B parameter model: 30 GB instead of 117).
 Their rounding keeps the means of m and of v (csrc/adamw.hip); it needs a seed, and the same seed and
 step give the same bits.
+
+Muon, for matrices: momentum, the nearest orthogonal matrix by Newton's and Schulz's iteration, the step.
+
+    m <- mu m + (1 - mu) g,  u = mu m + (1 - mu) g (nesterov) or m,  X = u / max(|u|_F, eps)
+    X <- a X + (b A + c A^2) X with A = X X^T, `steps` times
+    p <- p (1 - lr weight_decay) - lr max(1, rows / cols)^1/2 X
+
+`Muon` is the optimizer, `muon_step_` and `orthogonalize` are the operators under it (csrc/ortho.hip). All
+matrices of a type go through the same launches, up to 64 of 16 shapes at a time.
 """
 from __future__ import annotations
 
@@ -271,6 +282,164 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict):
         """torch's loading casts floating states to the parameter's dtype: the states' own are
         put back from what was saved."""
+        super().load_state_dict(state_dict)
+        ids = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
+        params = itertools.chain.from_iterable(g["params"] for g in self.param_groups)
+        for i, p in zip(ids, params):
+            saved = state_dict["state"].get(i)
+            if saved is not None:
+                self.state[p] = {k: v.detach().to(p.device, copy=True).contiguous()
+                                 if isinstance(v, torch.Tensor) else v for k, v in saved.items()}
+
+
+# --- orthogonalised updates of matrices ------------------------------------------------------------
+
+COEFFICIENTS = (3.4445, -4.775, 2.0315)  # of Muon: a steep start, and an end between 0.7 and 1.2
+
+
+def _iteration(name, steps, coefficients, eps):
+    if not 1 <= steps <= 100:
+        raise ValueError(f"{name}: steps is 1 to 100, got {steps}")
+    if len(coefficients) != 3:
+        raise ValueError(f"{name}: three coefficients, got {coefficients}")
+    if not eps >= 0:
+        raise ValueError(f"{name}: eps is not negative, got {eps}")
+    return (steps, *map(float, coefficients), eps)
+
+
+def _workspace(nbytes, name, like):
+    if nbytes < 0:
+        nat.check(nbytes, name)
+    return torch.empty(nbytes, device=like.device, dtype=torch.uint8)
+
+
+@torch.no_grad()
+def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=COEFFICIENTS,
+                  eps: float = 1e-7) -> torch.Tensor:
+    """x [..., rows, cols] (fp32, bf16 or fp16) after `steps` of Newton's and Schulz's iteration, in its
+    dtype: each matrix over max(its 2-norm, eps), then X <- a X + (b A + c A^2) X with A = X X^T, which
+    brings its singular values near 1. The coefficients have to keep them below 64 on the way. fp32 and
+    fp16 matrices are iterated at fp32's accuracy, bf16 ones with 11-bit operands (off by an eighth of what
+    the matrix' own 8 bits do). No autograd."""
+    how = _iteration("orthogonalize", steps, coefficients, eps)
+    if x.dim() < 2:
+        raise ValueError(f"orthogonalize: x is [..., rows, cols], got {tuple(x.shape)}")
+    dtype = nat.dtype_code(x)
+    nat.require_device("orthogonalize", x)
+    x = x.detach().contiguous().resolve_neg()
+    out = torch.empty_like(x)
+    if x.numel() == 0:
+        return out
+    rows, cols = x.shape[-2:]
+    batch = x.numel() // (rows * cols)
+    nbytes = nat.load().mqc_orthogonalize_workspace_bytes(batch, rows, cols, dtype)
+    ws = _workspace(nbytes, "mqc_orthogonalize", x)
+    nat.call("mqc_orthogonalize", x, x.data_ptr(), out.data_ptr(), batch, rows, cols, *how, dtype,
+             ws.data_ptr(), nbytes, nat.stream_of(x))
+    return out
+
+
+def _muon_rows(name, params, grads, momenta):
+    """The rows that mqc_muon_step reads."""
+    _check_lengths(name, params, grads, momenta)
+    for p in params:
+        if p.dim() != 2:
+            raise ValueError(f"{name}: parameters are matrices, got {tuple(p.shape)}")
+    _check_state(name, "momenta", params, momenta, torch.float32)
+    _check_tensors(name, params, grads, momenta)
+    if any(t.is_neg() for t in itertools.chain(params, grads, momenta)):
+        raise ValueError(f"{name}: tensors that the kernels do not take")
+    written = [t for t in itertools.chain(params, momenta) if t.numel()]
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.nbytes) for t in written)
+    if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
+        raise ValueError(f"{name}: a parameter is there twice, or two of them share memory")
+    return [(p.data_ptr(), g.data_ptr(), m.data_ptr(), *p.shape, nat.dtype_code(p))
+            for p, g, m in zip(params, grads, momenta) if p.numel()]
+
+
+@torch.no_grad()
+def muon_step_(params, grads, momenta, *, lr: float = 1e-3, momentum: float = 0.95, nesterov: bool = True,
+               weight_decay: float = 0.1, steps: int = 5, coefficients=COEFFICIENTS,
+               eps: float = 1e-7) -> None:
+    """One Muon step in place over lists of matrices: contiguous parameters and gradients of one dtype each
+    (fp32, bf16 or fp16), no two parameters in the same memory, fp32 momenta of their sizes. The iteration
+    is orthogonalize's."""
+    params, grads, momenta = list(params), list(grads), list(momenta)
+    how = _iteration("muon_step_", steps, coefficients, eps)
+    rows = _muon_rows("muon_step_", params, grads, momenta)
+    _launch_muon(rows, (params, momenta), lr, momentum, nesterov, weight_decay, how)
+
+
+def _launch_muon(rows, changed, lr, momentum, nesterov, weight_decay, how):
+    if not rows:
+        return
+    table = array.array("q", itertools.chain.from_iterable(rows)).tobytes()
+    like = changed[0][0]
+    nbytes = nat.load().mqc_muon_workspace_bytes(table, len(rows))
+    ws = _workspace(nbytes, "mqc_muon_step", like)
+    lr = float(lr)
+    nat.call("mqc_muon_step", like, table, len(rows), 1 - lr * weight_decay, lr, momentum, int(nesterov),
+             *how, ws.data_ptr(), nbytes, nat.stream_of(like))
+    nat.host().changed(changed)
+
+
+class Muon(torch.optim.Optimizer):
+    """Muon over the kernels of this module, for parameters that are matrices (embeddings, heads, norms and
+    biases belong to an AdamW beside it). Momenta are fp32."""
+
+    def __init__(self, params, lr: float = 1e-3, momentum: float = 0.95, nesterov: bool = True,
+                 weight_decay: float = 0.1, steps: int = 5, coefficients=COEFFICIENTS,
+                 eps: float = 1e-7):
+        if lr < 0 or weight_decay < 0:
+            raise ValueError(f"Muon: lr {lr} and weight_decay {weight_decay} are not negative")
+        if not 0 <= momentum < 1:
+            raise ValueError(f"Muon: momentum is in [0, 1), got {momentum}")
+        _iteration("Muon", steps, coefficients, eps)
+        super().__init__(params, {"lr": lr, "momentum": momentum, "nesterov": nesterov,
+                                  "weight_decay": weight_decay, "steps": steps,
+                                  "coefficients": tuple(coefficients), "eps": eps})
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() != 2:
+                self.param_groups.pop()
+                raise ValueError(f"Muon: parameters are matrices, got {tuple(p.shape)}")
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        work = []
+        for group in self.param_groups:
+            entries = []
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.layout != torch.strided:
+                    raise ValueError("Muon: sparse gradients are not supported")
+                g = p.grad.detach().contiguous().resolve_neg()
+                s = self.state[p]
+                if "momentum_buffer" not in s:
+                    s["momentum_buffer"] = torch.zeros(p.shape, device=p.device, dtype=torch.float32)
+                entries.append((p.detach(), g.to(p.dtype), s["momentum_buffer"]))
+            if entries:
+                work.append((group, entries))
+        if not work:
+            return loss
+        lists = [list(x) for x in zip(*itertools.chain.from_iterable(e for _, e in work))]
+        _muon_rows("Muon", *lists)  # no two in the same memory, over all groups
+        for group, entries in work:
+            params, grads, momenta = map(list, zip(*entries))
+            how = _iteration("Muon", group["steps"], group["coefficients"], group["eps"])
+            _launch_muon(_muon_rows("Muon", params, grads, momenta), (params, momenta), group["lr"],
+                         group["momentum"], group["nesterov"], group["weight_decay"], how)
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """torch's loading casts momenta to the parameter's dtype: they are put back as they were saved."""
         super().load_state_dict(state_dict)
         ids = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
         params = itertools.chain.from_iterable(g["params"] for g in self.param_groups)
