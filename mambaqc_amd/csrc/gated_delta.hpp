@@ -439,44 +439,50 @@ __device__ inline float tri_at(const uint16_t* tri, int row, int col) {
 
 __device__ inline bool finite(float v) { return fabsf(v) < __builtin_huge_valf(); }
 
-// The wave's rows of a triangular matrix: fragments of its one or two columns of 32.
+// The wave's rows of a triangular matrix: fragments of its two columns of 32, one of which may be zero.
 template <bool UPPER>
 __device__ inline void load_tri(const uint16_t* tri, int w, bf16x8 (&f)[2][kPieces]) {
   const int lane = threadIdx.x & 63;
   const bool both = UPPER ? w < 2 : w >= 2;
-  const int first = UPPER ? (w < 2 ? 2 * w : w + 2) : (w < 2 ? w : 2 * w - 2);
-  load_frag(tri + first * kPieces * kFrag, lane, f[UPPER ? (both ? 0 : 1) : 0]);
-  if (both) load_frag(tri + (first + 1) * kPieces * kFrag, lane, f[1]);
+  const int first = UPPER ? (w < 2 ? 2 * w : w + 1) : (w < 2 ? w : 2 * w - 2);
+  constexpr int part = UPPER ? 0 : 1;  // that may be missing
+  const uint16_t* at = tri + first * kPieces * kFrag;
+  load_frag(UPPER && !both ? at + kPieces * kFrag : at, lane, f[0]);
+  load_frag(both || UPPER ? at + kPieces * kFrag : at, lane, f[1]);
+  if (!both) {
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p) f[part][p] = __builtin_bit_cast(bf16x8, (u32x4){});
+  }
 }
-// Their product with x. Where documents meet in the chunk (`mixed`) and x is not finite somewhere (`bad`, of
-// each wave), term by term: zero times NaN is not zero.
-template <bool UPPER, int NX>
-__device__ inline floatx4 tri_product(const bf16x8 (&f)[2][kPieces], const uint16_t* x, int w, bool mixed,
-                                      const int* bad, const float (*xs)[16], const uint16_t* tri,
-                                      const float* doc) {
+// Their product with x.
+template <int NX>
+__device__ inline floatx4 tri_product(const bf16x8 (&f)[2][kPieces], const uint16_t* x) {
   const int lane = threadIdx.x & 63;
-  floatx4 v = {};
-  if (mixed && (bad[0] | bad[1] | bad[2] | bad[3])) {
-    for (int r = 0; r < 4; ++r) {
-      const int row = 16 * w + 4 * (lane >> 4) + r;
-      float s = 0.f;
+  floatx4 v[2] = {};
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    bf16x8 b[NX];
+    load_frag(x + s * NX * kFrag, lane, b);
+    v[s] = mma(f[s], b, v[s]);
+  }
+  return settled(v[0]) + settled(v[1]);
+}
+// The same where documents meet in the chunk and x is not finite somewhere (`bad`, of each wave): term by
+// term, since zero times NaN is not zero.
+template <bool UPPER>
+__device__ inline bool tri_apart(const int* bad, const float (*xs)[16], const uint16_t* tri, const float* doc,
+                                 int w, floatx4& out) {
+  if (!(bad[0] | bad[1] | bad[2] | bad[3])) return false;
+  const int lane = threadIdx.x & 63;
+  for (int r = 0; r < 4; ++r) {
+    const int row = 16 * w + 4 * (lane >> 4) + r;
+    float s = 0.f;
 #pragma unroll 1
-      for (int j = UPPER ? row : 0; UPPER ? j < kC : j <= row; ++j)
-        if (doc[j] == doc[row]) s = fmaf(tri_at<UPPER>(tri, row, j), xs[j][lane & 15], s);
-      v[r] = s;
-    }
-    return v;
+    for (int j = UPPER ? row : 0; UPPER ? j < kC : j <= row; ++j)
+      if (doc[j] == doc[row]) s = fmaf(tri_at<UPPER>(tri, row, j), xs[j][lane & 15], s);
+    out[r] = s;
   }
-  bf16x8 b[NX];
-  if (!UPPER || w < 2) {
-    load_frag(x, lane, b);
-    v = settled(mma(f[0], b, v));
-  }
-  if (UPPER || w >= 2) {
-    load_frag(x + NX * kFrag, lane, b);
-    v = settled(mma(f[1], b, v));
-  }
-  return v;
+  return true;
 }
 
 // What the two walks share: where a workgroup is, and its operands.
@@ -514,53 +520,61 @@ struct Walker {
     for (int s = 0; s < KS; ++s) load_frag(part(c, i) + (s * 4 + w) * NP * kFrag, lane, f[s]);
   }
   __device__ void load_cols(int64_t c, int i, bf16x8 (&f)[MT][2][NP]) const {
-    if (!holds) return;
+    const int tile = holds ? w : 0;
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
       for (int s = 0; s < 2; ++s)
-        load_frag(part(c, i) + ((w + 4 * t) * 2 + s) * NP * kFrag, lane, f[t][s]);
+        load_frag(part(c, i) + ((tile + 4 * t) * 2 + s) * NP * kFrag, lane, f[t][s]);
   }
-  // rows x state.
+  // rows x state (K's, and in the forward Q's too: each piece of the state is read once).
   __device__ floatx4 row_product(const bf16x8 (&f)[KS][NP], const uint16_t* state) const {
-    floatx4 v = {};
+    floatx4 v[2] = {};
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       bf16x8 b[kPieces];
       load_frag(state + s * kPieces * kFrag, lane, b);
-      v = mma(f[s], b, v);
+      v[s % 2] = mma(f[s], b, v[s % 2]);
     }
-    return settled(v);
+    return KS > 1 ? settled(v[0]) + settled(v[1]) : settled(v[0]);
   }
-  // S += cols x; tokens of other documents than `keep` left out where `cut`.
-  __device__ void col_product(const bf16x8 (&f)[MT][2][NP], const uint16_t* x, bool cut, const float* doc,
-                              float keep, floatx4 (&S)[MT]) const {
-    if (!holds) return;
+  __device__ void row_products(const bf16x8 (&f)[KS][NP], const bf16x8 (&h)[KS][NP], const uint16_t* state,
+                               floatx4& x, floatx4& y) const {
+    x = (floatx4){}, y = (floatx4){};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      bf16x8 b[kPieces];
+      load_frag(state + s * kPieces * kFrag, lane, b);
+      x = mma(f[s], b, x);
+      y = mma(h[s], b, y);
+    }
+    x = settled(x), y = settled(y);
+  }
+  // S += cols x.
+  __device__ void col_product(const bf16x8 (&f)[MT][2][NP], const uint16_t* x, floatx4 (&S)[MT]) const {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       bf16x8 xf[kPieces];
       load_frag(x + s * kPieces * kFrag, lane, xf);
-      if (cut) {
-        u32x4 mask = {};
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (doc[32 * s + place(g, j)] == keep) mask[j / 2] |= j % 2 ? 0xffff0000u : 0xffffu;
+      for (int t = 0; t < MT; ++t) S[t] = mma(f[t][s], xf, S[t]);
+    }
 #pragma unroll
-        for (int t = 0; t < MT; ++t) {
-          bf16x8 only[NP];
+    for (int t = 0; t < MT; ++t) S[t] = settled(S[t]);
+  }
+  // The columns of tokens of other documents than `keep` as zero.
+  __device__ void cut_cols(bf16x8 (&f)[MT][2][NP], const float* doc, float keep) const {
 #pragma unroll
-          for (int p = 0; p < NP; ++p)
-            only[p] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, f[t][s][p]) & mask);
-          S[t] = settled(mma(only, xf, S[t]));
-        }
-      } else {
+    for (int s = 0; s < 2; ++s) {
+      u32x4 mask = {};
 #pragma unroll
-        for (int t = 0; t < MT; ++t) S[t] = mma(f[t][s], xf, S[t]);
-        if (s == 1) {
+      for (int j = 0; j < 8; ++j)
+        if (doc[32 * s + place(g, j)] == keep) mask[j / 2] |= j % 2 ? 0xffff0000u : 0xffffu;
 #pragma unroll
-          for (int t = 0; t < MT; ++t) S[t] = settled(S[t]);
-        }
-      }
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+          f[t][s][p] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, f[t][s][p]) & mask);
     }
   }
   __device__ void put_state(uint16_t* frags, const floatx4 (&S)[MT]) const {
@@ -603,22 +617,30 @@ struct Walker {
     for (int r = 0; r < 4; ++r)
       to[((bh * a.chunks + c) * kC + 16 * w + 4 * g + r) * a.v_pad + col(ct)] = v[r];
   }
-  // The wave's tokens of v (or dO) and of o (or dv).
+  // The wave's tokens of v (or dO), past the ends the last one's and its last column; and of o (or dv).
   __device__ void load_tile(const T* from, int64_t x_b, int64_t x_t, int64_t x_h, int64_t c, int ct,
-                            float (&v)[4]) const {
-    const T* at = from + b * x_b + hv * x_h + col(ct);
+                            T (&v)[4]) const {
+    const T* at = from + b * x_b + hv * x_h + (col(ct) < a.v_dim ? col(ct) : a.v_dim - 1);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int64_t t = c * kC + 16 * w + 4 * g + r;
-      v[r] = t < a.seq && col(ct) < a.v_dim ? load_scalar(at + t * x_t) : 0.f;
+      v[r] = at[(t < a.seq ? t : a.seq - 1) * x_t];
     }
   }
+  __device__ bool here(int64_t c, int r) const { return c * kC + 16 * w + 4 * g + r < a.seq; }
+  __device__ float tile_value(const T (&v)[4], int64_t c, int ct, int r) const {
+    return here(c, r) && col(ct) < a.v_dim ? load_scalar(&v[r]) : 0.f;
+  }
   __device__ void store_tile(T* to, int64_t c, int ct, const floatx4& v) const {
+    T* at = to + ((b * a.seq + c * kC + 16 * w + 4 * g) * a.v_heads + hv) * a.v_dim + col(ct);
+    const int64_t step = a.v_heads * (int64_t)a.v_dim;
+    if ((c + 1) * kC <= a.seq && col0 + 16 * CT <= a.v_dim) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int64_t t = c * kC + 16 * w + 4 * g + r;
-      if (t < a.seq && col(ct) < a.v_dim)
-        store_scalar(to + ((b * a.seq + t) * a.v_heads + hv) * a.v_dim + col(ct), v[r]);
+      for (int r = 0; r < 4; ++r) store_scalar(at + r * step, v[r]);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (here(c, r) && col(ct) < a.v_dim) store_scalar(at + r * step, v[r]);
     }
   }
   // Rows that are not finite, for tri_product.
@@ -656,8 +678,8 @@ constexpr int kWalkWaves = CT == 1 && (BWD ? (kIn<T> == 1 && KD == 128) || (kIn<
 template <typename T, int KD, int CT>
 __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, false>)) void delta_fwd_kernel(Args<T> a) {
   __shared__ __attribute__((aligned(16))) WalkShared<KD, CT> s;
-  const Walker<T, KD, false, CT> k(a);
   using K = Walker<T, KD, false, CT>;
+  const K k(a);
   constexpr int NP = K::NP, KS = K::KS, MT = K::MT;
   floatx4 S[CT][MT];
 #pragma unroll
@@ -666,77 +688,87 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, false>)) void delta_fwd
     k.put_state(s.state[0][ct], S[ct]);
   }
   bf16x8 kf[KS][NP], qf[KS][NP], tf[2][kPieces], pf[2][kPieces], cf[MT][2][NP];
-  float v[CT][4];
+  T v[CT][4];
   RowGates next;
   if (a.chunks > 0) {
     next.load(k.vec, k.w, k.g);
     k.load_rows(0, 0, kf);
+    k.load_rows(0, 2, qf);
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) k.load_tile(a.v, a.v_b, a.v_t, a.v_h, 0, ct, v[ct]);
     load_tri<false>(k.tri, k.w, tf);
     k.load_cols(0, 1, cf);
-    k.load_rows(0, 2, qf);
     load_tri<false>(k.tri + K::kTriPart, k.w, pf);
   }
   for (int64_t c = 0; c < a.chunks; ++c) {
+    // What comes next goes out as soon as its place is free (behind the last chunk, once more its own).
+    const int64_t ahead = c + 1 < a.chunks ? c + 1 : c;
     const RowGates at = next;
     const float* doc = k.vec + c * 4 * kC + 3 * kC;
-    const uint16_t* tri = k.tri + c * 2 * K::kTriPart;
-    const bool mixed = at.first != at.last, cut = at.last != 0.f, more = c + 1 < a.chunks;
+    const uint16_t *tri = k.tri + c * 2 * K::kTriPart, *tri_ahead = k.tri + ahead * 2 * K::kTriPart;
+    const bool mixed = at.first != at.last, cut = at.last != 0.f;
     lds_barrier();
-    if (more) next.load(k.vec + (c + 1) * 4 * kC, k.w, k.g);
-    floatx4 x[CT];
+    next.load(k.vec + ahead * 4 * kC, k.w, k.g);
+    floatx4 x[CT], qs[CT];
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) x[ct] = k.row_product(kf, s.state[c & 1][ct]);
-    if (more) k.load_rows(c + 1, 0, kf);
+    for (int ct = 0; ct < CT; ++ct) k.row_products(kf, qf, s.state[c & 1][ct], x[ct], qs[ct]);
+    k.load_rows(ahead, 0, kf);
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        x[ct][r] = at.doc[r] == 0.f && c * kC + 16 * k.w + 4 * k.g + r < a.seq
-                       ? fmaf(-at.e[r], x[ct][r], v[ct][r]) : v[ct][r];
+      for (int r = 0; r < 4; ++r) {
+        const float vt = k.tile_value(v[ct], c, ct, r);
+        x[ct][r] = at.doc[r] == 0.f && k.here(c, r) ? fmaf(-at.e[r], x[ct][r], vt) : vt;
+      }
       put_tile<kPieces>(s.x[ct], k.w, x[ct]);
       if (mixed) k.mark(s.xs[0][ct], s.bad[0], x[ct]);
-      if (a.states) k.store_padded(a.states, c, ct, S[ct]);
-      if (more) k.load_tile(a.v, a.v_b, a.v_t, a.v_h, c + 1, ct, v[ct]);
     }
     lds_barrier();
+    k.load_rows(ahead, 2, qf);
+    floatx4 r[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      floatx4 r = tri_product<false, kPieces>(tf, s.x[ct], k.w, mixed, s.bad[0], s.xs[0][ct], tri, doc);
-      if (a.resid) k.store_rows(a.resid, c, ct, r);
+      k.load_tile(a.v, a.v_b, a.v_t, a.v_h, ahead, ct, v[ct]);
+      if (!mixed || !tri_apart<false>(s.bad[0], s.xs[0][ct], tri, doc, k.w, r[ct]))
+        r[ct] = tri_product<kPieces>(tf, s.x[ct]);
+      floatx4 u, y;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] *= at.beta[i];
-      put_tile<kPieces>(s.u[ct], k.w, r);
-      if (mixed) k.mark(s.xs[1][ct], s.bad[1], r);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = at.doc[i] == at.last ? r[i] * at.end[i] : 0.f;
-      put_tile<kPieces>(s.y[ct], k.w, r);
+      for (int i = 0; i < 4; ++i) {
+        u[i] = r[ct][i] * at.beta[i];
+        y[i] = at.doc[i] == at.last ? u[i] * at.end[i] : 0.f;
+      }
+      put_tile<kPieces>(s.u[ct], k.w, u);
+      put_tile<kPieces>(s.y[ct], k.w, y);
+      if (mixed) k.mark(s.xs[1][ct], s.bad[1], u);
     }
-    if (more) load_tri<false>(tri + 2 * K::kTriPart, k.w, tf);
+    load_tri<false>(tri_ahead, k.w, tf);
+    if (mixed) k.cut_cols(cf, doc, at.last);
     lds_barrier();
+    if (a.states) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) k.store_padded(a.states, c, ct, S[ct]);
+    }
+    floatx4 o[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll
       for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) S[ct][t][r] = cut ? 0.f : S[ct][t][r] * at.all;
-      k.col_product(cf, s.y[ct], mixed, doc, at.last, S[ct]);
+        for (int i = 0; i < 4; ++i) S[ct][t][i] = cut ? 0.f : S[ct][t][i] * at.all;
+      k.col_product(cf, s.y[ct], S[ct]);
+      if (!mixed || !tri_apart<false>(s.bad[1], s.xs[1][ct], tri + K::kTriPart, doc, k.w, o[ct]))
+        o[ct] = tri_product<kPieces>(pf, s.u[ct]);
       k.put_state(s.state[(c + 1) & 1][ct], S[ct]);
     }
-    if (more) k.load_cols(c + 1, 1, cf);
+    k.load_cols(ahead, 1, cf);
+    load_tri<false>(tri_ahead + K::kTriPart, k.w, pf);
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      const floatx4 qs = k.row_product(qf, s.state[c & 1][ct]);
-      floatx4 o = tri_product<false, kPieces>(pf, s.u[ct], k.w, mixed, s.bad[1], s.xs[1][ct],
-                                              tri + K::kTriPart, doc);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) o[r] = a.scale * (at.doc[r] == 0.f ? fmaf(at.e[r], qs[r], o[r]) : o[r]);
-      k.store_tile(a.o, c, ct, o);
-    }
-    if (more) {
-      k.load_rows(c + 1, 2, qf);
-      load_tri<false>(tri + 3 * K::kTriPart, k.w, pf);
+      for (int i = 0; i < 4; ++i)
+        o[ct][i] = a.scale * (at.doc[i] == 0.f ? fmaf(at.e[i], qs[ct][i], o[ct][i]) : o[ct][i]);
+      k.store_tile(a.o, c, ct, o[ct]);
+      if (a.resid) k.store_rows(a.resid, c, ct, r[ct]);
     }
   }
   if (a.h_last && k.holds) {
@@ -748,104 +780,107 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, false>)) void delta_fwd
 template <typename T, int KD, int CT>
 __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, true>)) void delta_bwd_kernel(Args<T> a) {
   __shared__ __attribute__((aligned(16))) WalkShared<KD, CT> s;
-  const Walker<T, KD, true, CT> k(a);
   using K = Walker<T, KD, true, CT>;
+  const K k(a);
   constexpr int NP = K::NP, KS = K::KS, MT = K::MT;
   const int64_t heads = a.v_heads * (int64_t)a.v_dim, end = a.chunks - 1;
-  const auto load_grad = [&](int64_t c, int ct, float (&v)[4]) {
+  const auto load_grad = [&](int64_t c, int ct, T (&v)[4]) {
     k.load_tile(a.d_o, a.seq * heads, heads, a.v_dim, c, ct, v);
   };
-  floatx4 S[CT][MT];  // the gradient of the state after the chunk
-  float v[CT][4], ahead[CT][4];
+  const auto put_grad = [&](int64_t c, int ct, const T (&raw)[4], floatx4& v) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = k.tile_value(raw, c, ct, r);
+    put_tile<NP>(s.d_o[c & 1][ct], k.w, v);
+  };
+  floatx4 S[CT][MT], v[CT];  // the gradient of the state after the chunk; the wave's tokens of dO
+  T raw[CT][4];
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     k.load_state(a.dh_last, ct, S[ct]);
     k.put_state(s.state[end & 1][ct], S[ct]);
-    load_grad(end, ct, v[ct]);
-    put_tile<NP>(s.d_o[end & 1][ct], k.w, floatx4{v[ct][0], v[ct][1], v[ct][2], v[ct][3]});
+    load_grad(end, ct, raw[ct]);
+    put_grad(end, ct, raw[ct], v[ct]);
   }
   bf16x8 kf[KS][NP], tf[2][kPieces], pf[2][kPieces], cf[MT][2][NP], qf[MT][2][NP];
   RowGates next;
-  {
-    next.load(k.vec + end * 4 * kC, k.w, k.g);
-    k.load_rows(end, 0, kf);
-    load_tri<true>(k.tri + (2 * end + 1) * K::kTriPart, k.w, pf);
-    load_tri<true>(k.tri + 2 * end * K::kTriPart, k.w, tf);
-    k.load_cols(end, 2, qf);
-    k.load_cols(end, 1, cf);
-  }
+  next.load(k.vec + end * 4 * kC, k.w, k.g);
+  k.load_rows(end, 0, kf);
+  load_tri<true>(k.tri + (2 * end + 1) * K::kTriPart, k.w, pf);
+  load_tri<true>(k.tri + 2 * end * K::kTriPart, k.w, tf);
+  k.load_cols(end, 2, qf);
+  k.load_cols(end, 1, cf);
   for (int64_t c = end; c >= 0; --c) {
+    const int64_t ahead = c > 0 ? c - 1 : 0;
     const RowGates at = next;
     const float* doc = k.vec + c * 4 * kC + 3 * kC;
-    const uint16_t* tri = k.tri + c * 2 * K::kTriPart;
-    const bool mixed = at.first != at.last, cut = at.last != 0.f, more = c > 0;
+    const uint16_t *tri = k.tri + c * 2 * K::kTriPart, *tri_ahead = k.tri + ahead * 2 * K::kTriPart;
+    const bool mixed = at.first != at.last, cut = at.last != 0.f;
     if (mixed) {
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-        k.mark(s.xs[1][ct], s.bad[1], floatx4{v[ct][0], v[ct][1], v[ct][2], v[ct][3]});
+      for (int ct = 0; ct < CT; ++ct) k.mark(s.xs[1][ct], s.bad[1], v[ct]);
+    }
+    if (cut) {
+      k.cut_cols(qf, doc, 0.f);
+      k.cut_cols(cf, doc, 0.f);
     }
     lds_barrier();
-    if (more) {
-      next.load(k.vec + (c - 1) * 4 * kC, k.w, k.g);
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) load_grad(c - 1, ct, ahead[ct]);
-    }
+    next.load(k.vec + ahead * 4 * kC, k.w, k.g);
+    floatx4 y[CT], z[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      const floatx4 y = k.row_product(kf, s.state[c & 1][ct]);
-      floatx4 z = tri_product<true, NP>(pf, s.d_o[c & 1][ct], k.w, mixed, s.bad[1], s.xs[1][ct],
-                                        tri + K::kTriPart, doc);
+      load_grad(ahead, ct, raw[ct]);
+      y[ct] = k.row_product(kf, s.state[c & 1][ct]);
+      if (!mixed || !tri_apart<true>(s.bad[1], s.xs[1][ct], tri + K::kTriPart, doc, k.w, z[ct]))
+        z[ct] = tri_product<NP>(pf, s.d_o[c & 1][ct]);
+    }
+    k.load_rows(ahead, 0, kf);
+    load_tri<true>(tri_ahead + K::kTriPart, k.w, pf);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      floatx4 x;  // e dO, for the state
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        z[r] *= a.scale;
-        if (at.doc[r] == at.last) z[r] = fmaf(at.end[r], y[r], z[r]);
+        z[ct][r] *= a.scale;
+        if (at.doc[r] == at.last) z[ct][r] = fmaf(at.end[r], y[ct][r], z[ct][r]);
+        x[r] = at.doc[r] == 0.f ? v[ct][r] * (a.scale * at.e[r]) : 0.f;
       }
-      put_tile<kPieces>(s.x[ct], k.w, z);
-      if (mixed) k.mark(s.xs[0][ct], s.bad[0], z);
-      // e dO, for the state.
-      floatx4 x;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) x[r] = at.doc[r] == 0.f ? v[ct][r] * (a.scale * at.e[r]) : 0.f;
+      put_tile<kPieces>(s.x[ct], k.w, z[ct]);
       put_tile<kPieces>(s.u[ct], k.w, x);
-      k.store_padded(a.dstates, c, ct, S[ct]);
-    }
-    if (more) {
-      k.load_rows(c - 1, 0, kf);
-      load_tri<true>(tri - K::kTriPart, k.w, pf);
+      if (mixed) k.mark(s.xs[0][ct], s.bad[0], z[ct]);
     }
     lds_barrier();
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      floatx4 z = tri_product<true, kPieces>(tf, s.x[ct], k.w, mixed, s.bad[0], s.xs[0][ct], tri, doc);
-      k.store_rows(a.z, c, ct, z);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) z[r] *= at.beta[r];
-      k.store_tile(a.dv, c, ct, z);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) z[r] = at.doc[r] == 0.f ? -z[r] * at.e[r] : 0.f;
-      put_tile<kPieces>(s.y[ct], k.w, z);
+      k.store_padded(a.dstates, c, ct, S[ct]);
 #pragma unroll
       for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) S[ct][t][r] = cut ? 0.f : S[ct][t][r] * at.all;
-      k.col_product(qf, s.u[ct], cut, doc, 0.f, S[ct]);
+      if (!mixed || !tri_apart<true>(s.bad[0], s.xs[0][ct], tri, doc, k.w, z[ct]))
+        z[ct] = tri_product<kPieces>(tf, s.x[ct]);
+      k.col_product(qf, s.u[ct], S[ct]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        y[ct][r] = at.beta[r] * z[ct][r];
+        v[ct][r] = at.doc[r] == 0.f ? -y[ct][r] * at.e[r] : 0.f;
+      }
+      put_tile<kPieces>(s.y[ct], k.w, v[ct]);
     }
-    if (more) {
-      load_tri<true>(tri - 2 * K::kTriPart, k.w, tf);
-      k.load_cols(c - 1, 2, qf);
-    }
+    load_tri<true>(tri_ahead, k.w, tf);
+    k.load_cols(ahead, 2, qf);
     lds_barrier();
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      k.col_product(cf, s.y[ct], cut, doc, 0.f, S[ct]);
+      k.col_product(cf, s.y[ct], S[ct]);
       k.put_state(s.state[(c + 1) & 1][ct], S[ct]);
-      if (more) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[ct][r] = ahead[ct][r];
-        put_tile<NP>(s.d_o[(c + 1) & 1][ct], k.w, floatx4{v[ct][0], v[ct][1], v[ct][2], v[ct][3]});
-      }
+      put_grad(ahead, ct, raw[ct], v[ct]);
     }
-    if (more) k.load_cols(c - 1, 1, cf);
+    k.load_cols(ahead, 1, cf);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      k.store_rows(a.z, c, ct, z[ct]);
+      k.store_tile(a.dv, c, ct, y[ct]);
+    }
   }
   if (a.dh0 && k.holds) {
 #pragma unroll
