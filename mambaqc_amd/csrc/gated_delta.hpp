@@ -98,6 +98,12 @@ __device__ inline floatx4 settled(floatx4 v) {
   return v;
 }
 
+// The same for the fp32 instruction, whose result takes 32 cycles.
+__device__ inline floatx4 settled32(floatx4 v) {
+  asm volatile("s_nop 15" : "+v"(v));
+  return v;
+}
+
 template <int N>
 __device__ inline void load_frag(const uint16_t* at, int lane, bf16x8 (&f)[N]) {
 #pragma unroll
@@ -207,55 +213,74 @@ __device__ inline Gates chunk_gates(const Args<T>& a, int64_t b, int64_t hv, int
 
 // ---------------------------------------------------------------------------
 // The products within chunks. A workgroup of four waves takes a chunk of a key head and of the value heads
-// that share it; wave w rows 16 w.
+// that share it; wave w rows 16 w.., whose gram products stay in its registers.
 // ---------------------------------------------------------------------------
-template <typename T, int KD, bool BWD>
+template <typename T, int KD>
 struct PrepShared {
   uint16_t frags[KD / 8 * kIn<T> * kFrag];  // K by rows; then Q, to be turned
-  float kk[kC][kC + 1], qk[kC][kC + 1];     // below the diagonal and on it
-  float m[kC][kC + 1], inv[kC][kC + 1], y[3][16][17];
+  float m[kC][kC + 4], inv[kC][kC + 4];     // (rows at multiples of 16 bytes)
   double G[kC];
   float beta[kC];
   int doc[kC];
 };
 
-// X = (I + m)^-1 for a strictly lower triangular m, rows by substitution in blocks of 16, then block
-// diagonal by block diagonal: X_ij = -X_ii (sum over j <= l < i of m_il X_lj).
+// 16 x 16 x 4 in fp32: lane 16 g + m holds a's row m, b's column m and of both the columns (rows) that it
+// takes as number g.
+__device__ inline floatx4 mma32(float a, float b, floatx4 acc) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, acc, 0, 0, 0);
+}
+
+// X = (I + m)^-1 for a strictly lower triangular m: its diagonal blocks of 16 by substitution, a column to a
+// lane (products of powers of m would lose digits where keys repeat), then block diagonal by block diagonal,
+// X_ij = -X_ii Y with Y = sum over j <= l < i of m_il X_lj, wave i. A sum over the 16 of a block takes them in
+// the order 4 g + r, r = 0..3, in which Y leaves its product. Everything in fp32.
 template <typename S>
 __device__ inline void invert(S& s) {
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, o = 16 * w;
-  if (lane < 16) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, o = 16 * w, g = lane >> 4, c = lane & 15;
+  {
     float x[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      float v = i == lane ? 1.f : 0.f;
+      float v = i == c ? 1.f : 0.f;
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (j < i) v = fmaf(-s.m[o + i][o + j], x[j], v);
-      x[i] = i < lane ? 0.f : v;
-      s.inv[o + i][o + lane] = x[i];
+      for (int q = 0; q < 4; ++q) {
+        if (4 * q >= i) continue;
+        const floatx4 row = *reinterpret_cast<const floatx4*>(&s.m[o + i][o + 4 * q]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (4 * q + j < i) v = fmaf(-row[j], x[4 * q + j], v);
+      }
+      x[i] = i < c ? 0.f : v;  // (a NaN of rows in between is none above the diagonal)
     }
-  }
-  const int r = tid >> 4, c = tid & 15;
+    if (g == 0) {
 #pragma unroll
-  for (int d = 1; d < 4; ++d) {
-    __syncthreads();
-    for (int b = 0; b + d < 4; ++b) {
-      const int i = 16 * (b + d), j = 16 * b;
-      float v = 0.f;
-      for (int l = j; l < i; ++l) v = fmaf(s.m[i + r][l], s.inv[l][j + c], v);
-      s.y[b][r][c] = v;
-    }
-    __syncthreads();
-    for (int b = 0; b + d < 4; ++b) {
-      const int i = 16 * (b + d), j = 16 * b;
-      float v = 0.f;
-#pragma unroll
-      for (int l = 0; l < 16; ++l) v = fmaf(-s.inv[i + r][i + l], s.y[b][l][c], v);
-      s.inv[i + r][j + c] = v;
+      for (int i = 0; i < 16; ++i) s.inv[o + i][o + c] = x[i];
     }
   }
   __syncthreads();
+  const floatx4 own = *reinterpret_cast<const floatx4*>(&s.inv[o + c][o + 4 * g]);  // X_ii
+#pragma unroll
+  for (int d = 1; d < 4; ++d) {
+    if (w >= d) {
+      const int j = 16 * (w - d);
+      floatx4 y = {};
+#pragma unroll
+      for (int n = 0; n < d; ++n) {
+        const int l = j + 16 * n;
+        const floatx4 left = *reinterpret_cast<const floatx4*>(&s.m[o + c][l + 4 * g]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y = mma32(left[r], s.inv[l + 4 * g + r][j + c], y);
+      }
+      y = settled32(y);
+      floatx4 x = {};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x = mma32(-own[r], y[r], x);
+      x = settled32(x);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) s.inv[o + 4 * g + r][j + c] = x[r];
+    }
+    __syncthreads();
+  }
 }
 
 // K or Q, by rows in `frags`, by columns into `to`.
@@ -283,13 +308,27 @@ __device__ inline void write_turned(const uint16_t* frags, uint16_t* to) {
 template <typename T, int KD, bool BWD>
 __global__ __launch_bounds__(256) void delta_prep_kernel(Args<T> a) {
   constexpr int NP = kIn<T>, KS = KD / 32;
-  __shared__ __attribute__((aligned(16))) PrepShared<T, KD, BWD> s;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, g = lane >> 4, m = lane & 15;
+  __shared__ __attribute__((aligned(16))) PrepShared<T, KD> s;
+  const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t unit = blockIdx.x, chunk = unit % a.chunks, bh = unit / a.chunks;
   const int64_t b = bh / a.k_heads, hk = bh % a.k_heads, t0 = chunk * kC, t = t0 + 16 * w + m;
   const int group = (int)(a.v_heads / a.k_heads);
   uint16_t* keys = a.keys + unit * (3 * KD / 8 * NP * kFrag);
   constexpr int kPart = KD / 8 * NP * kFrag;
+  // The gates of a value head, by one wave.
+  const auto gates = [&](int64_t hv) {
+    const Gates x = chunk_gates(a, b, hv, t0);
+    s.G[lane] = x.G;
+    s.beta[lane] = x.beta;
+    s.doc[lane] = x.doc;
+    const double end = __shfl(x.G, 63);
+    float* vec = a.vec + ((b * a.v_heads + hv) * a.chunks + chunk) * 4 * kC;
+    vec[lane] = x.doc == 0 ? expf((float)x.G) : 0.f;
+    vec[kC + lane] = x.doc == __shfl(x.doc, 63) ? expf((float)(end - x.G)) : 0.f;
+    vec[2 * kC + lane] = x.beta;
+    vec[3 * kC + lane] = (float)x.doc;
+  };
 
   // Rows of K and Q as fragments.
   bf16x8 kf[KS][NP], qf[KS][NP];
@@ -299,33 +338,34 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Args<T> a) {
     const int dim = t < a.seq ? a.k_dim : 0;
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
-      float x[8];
+      float x[8], y[8];
       load_row8(krow, i, g, dim, x);
+      load_row8(qrow, i, g, dim, y);
       split<NP>(x, kf[i]);
-      load_row8(qrow, i, g, dim, x);
-      split<NP>(x, qf[i]);
-      const int at = (i * 4 + w) * NP * kFrag;
-      store_frag(keys + at, lane, kf[i]);
-      store_frag(s.frags + at, lane, kf[i]);
-      if constexpr (!BWD) store_frag(keys + 2 * kPart + at, lane, qf[i]);
+      split<NP>(y, qf[i]);
     }
   }
+  if (w == 3) gates(hk * group);
+#pragma unroll
+  for (int i = 0; i < KS; ++i) {
+    const int at = (i * 4 + w) * NP * kFrag;
+    store_frag(s.frags + at, lane, kf[i]);
+    store_frag(keys + at, lane, kf[i]);
+    if constexpr (!BWD) store_frag(keys + 2 * kPart + at, lane, qf[i]);
+  }
   __syncthreads();
-  for (int n = 0; n <= w; ++n) {
-    floatx4 kk = {}, qk = {};
+  floatx4 kk[4] = {}, qk[4] = {};
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    if (n > w) continue;
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
       bf16x8 kn[NP];
       load_frag(s.frags + (i * 4 + n) * NP * kFrag, lane, kn);
-      kk = mma(kf[i], kn, kk);
-      qk = mma(qf[i], kn, qk);
+      kk[n] = mma(kf[i], kn, kk[n]);
+      qk[n] = mma(qf[i], kn, qk[n]);
     }
-    kk = settled(kk), qk = settled(qk);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      s.kk[16 * w + 4 * g + r][16 * n + m] = kk[r];
-      s.qk[16 * w + 4 * g + r][16 * n + m] = qk[r];
-    }
+    kk[n] = settled(kk[n]), qk[n] = settled(qk[n]);
   }
   write_turned<T, KD>(s.frags, keys + kPart);
   if constexpr (BWD) {
@@ -338,46 +378,52 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Args<T> a) {
 
   for (int j = 0; j < group; ++j) {
     const int64_t hv = hk * group + j, at = (b * a.v_heads + hv) * a.chunks + chunk;
-    __syncthreads();  // the head before is done with what follows
-    if (w == 0) {
-      const Gates x = chunk_gates(a, b, hv, t0);
-      s.G[lane] = x.G;
-      s.beta[lane] = x.beta;
-      s.doc[lane] = x.doc;
-      const double end = __shfl(x.G, 63);
-      float* vec = a.vec + at * 4 * kC;
-      vec[lane] = x.doc == 0 ? expf((float)x.G) : 0.f;
-      vec[kC + lane] = x.doc == __shfl(x.doc, 63) ? expf((float)(end - x.G)) : 0.f;
-      vec[2 * kC + lane] = x.beta;
-      vec[3 * kC + lane] = (float)x.doc;
+    if (j > 0) {
+      __syncthreads();  // the head before is done with what follows
+      if (w == 3) gates(hv);
+      __syncthreads();
     }
-    __syncthreads();
-    // m and P (over m's and qk's places above the diagonal nothing is read but as zero).
-    float P[kC * kC / 256];
-    for (int i = 0; i < kC * kC / 256; ++i) {
-      const int row = i * 4 + w, col = lane;
-      const bool seen = col <= row && s.doc[row] == s.doc[col];
-      const float D = seen ? expf((float)(s.G[row] - s.G[col])) : 0.f;
-      s.m[row][col] = seen && col < row ? D * s.kk[row][col] * s.beta[BWD ? row : col] : 0.f;
-      P[i] = seen ? D * s.qk[row][col] : 0.f;
-      s.inv[row][col] = 0.f;
+    // m, and P in registers (above the diagonal nothing is read).
+    floatx4 P[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      P[n] = (floatx4){};
+      if (n > w) continue;
+      const int col = 16 * n + m;
+      const double Gc = s.G[col];
+      const int dc = s.doc[col];
+      const float bc = s.beta[col];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = 16 * w + 4 * g + r;
+        const bool seen = col <= row && s.doc[row] == dc;
+        const float D = seen ? expf((float)(s.G[row] - Gc)) : 0.f;
+        s.m[row][col] = seen && col < row ? D * kk[n][r] * (BWD ? s.beta[row] : bc) : 0.f;
+        if (seen) P[n][r] = D * qk[n][r];
+      }
     }
     __syncthreads();
     invert(s);
-    for (int i = 0; i < kC * kC / 256; ++i) s.m[i * 4 + w][lane] = P[i];
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      if (n <= w) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s.m[16 * w + 4 * g + r][16 * n + m] = P[n][r];
+      }
     __syncthreads();
     uint16_t* tri = a.tri + at * (2 * kTri * kPieces * kFrag);
     for (int f = w; f < 2 * kTri; f += 4) {
       const int n = f % kTri;  // which rows of 16 and columns of 32
       const int mt = BWD ? (n < 4 ? n / 2 : n - 2) : (n < 2 ? n : n / 2 + 1);
       const int ks = BWD ? (n < 4 ? n % 2 : 1) : (n < 2 ? 0 : n % 2);
+      const float(*from)[kC + 4] = f < kTri ? s.inv : s.m;
       float x[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int row = 16 * mt + m, col = 32 * ks + place(g, e);
         const int i = BWD ? col : row, l = BWD ? row : col;
         // Not of another document (whose NaN may have come here) and not above the diagonal.
-        x[e] = l > i || s.doc[i] != s.doc[l] ? 0.f : f < kTri ? s.inv[i][l] : s.m[i][l];
+        x[e] = l > i || s.doc[i] != s.doc[l] ? 0.f : from[i][l];
       }
       bf16x8 p[kPieces];
       split<kPieces>(x, p);
@@ -893,12 +939,17 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, true>)) void delta_bwd_
 // columns 16 w.. of everything turned (tokens as columns). Operands pass through LDS 32 columns of v_dim
 // at a time, as fragments with their columns in order.
 // ---------------------------------------------------------------------------
+// Of wide keys two waves have a column each, and half of k_dim: their gradients of q and k are what
+// registers are needed for.
+template <int KD>
+constexpr int kGradHalves = KD > 64 ? 2 : 1;
+
 template <typename T, int KD>
 struct GradShared {
   uint16_t u[4 * kPieces * kFrag], z[4 * kPieces * kFrag], d_o[4 * kIn<T> * kFrag];
   uint16_t S[KD / 16 * kPieces * kFrag], dS[KD / 16 * kPieces * kFrag];
   double G[kC];
-  float beta[kC], dG[kC], w[kC], dbeta[kC], dot[4];
+  float beta[kC], dG[2][kC], w[2][kC], dbeta[kC], dot[8];
   int doc[kC];
 };
 
@@ -911,29 +962,30 @@ __device__ inline void stage(uint16_t* to, int row, int c, float (&x)[8]) {
 }
 
 template <typename T, int KD>
-__global__ __launch_bounds__(256) void delta_grad_kernel(Args<T> a) {
-  constexpr int NP = kIn<T>, MT = KD / 16, kPart = KD / 8 * NP * kFrag;
+__global__ __launch_bounds__(256 * kGradHalves<KD>, 2) void delta_grad_kernel(Args<T> a) {
+  constexpr int NP = kIn<T>, H = kGradHalves<KD>, MT = KD / 16 / H, kPart = KD / 8 * NP * kFrag;
   __shared__ __attribute__((aligned(16))) GradShared<T, KD> s;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, m = lane & 15;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = wave & 3, half = wave >> 2;
   const int64_t unit = xcd_order(blockIdx.x, gridDim.x), chunk = unit % a.chunks, bh = unit / a.chunks;
   const int64_t b = bh / a.v_heads, hv = bh % a.v_heads, hk = hv / (a.v_heads / a.k_heads);
   const int64_t t0 = chunk * kC;
-  if (w == 0) {
+  if (wave == 0) {
     const Gates x = chunk_gates(a, b, hv, t0);
     s.G[lane] = x.G;
     s.beta[lane] = x.beta;
     s.doc[lane] = x.doc;
   }
   __syncthreads();
-  const int row = tid >> 2, c8 = tid & 3;  // what this thread stages
-  const float* resid = a.resid + (unit * kC + row) * a.v_pad + 8 * c8;
-  const float* zs = a.z + (unit * kC + row) * a.v_pad + 8 * c8;
+  // What this thread stages: a row of the states; one of u and z or (of two halves the second) of dO.
+  const int row = tid >> 2, c8 = tid & 3, token = row & 63;
+  const float* resid = a.resid + (unit * kC + token) * a.v_pad + 8 * c8;
+  const float* zs = a.z + (unit * kC + token) * a.v_pad + 8 * c8;
   const float* st = a.states + (unit * KD + row) * a.v_pad + 8 * c8;
   const float* ds = a.dstates + (unit * KD + row) * a.v_pad + 8 * c8;
-  const T* d_o = a.d_o + ((b * a.seq + t0 + row) * a.v_heads + hv) * a.v_dim;
-  const bool in = t0 + row < a.seq;
-  const float beta = s.beta[row];
+  const T* d_o = a.d_o + ((b * a.seq + t0 + token) * a.v_heads + hv) * a.v_dim;
+  const bool in = t0 + token < a.seq;
+  const float beta = s.beta[token];
   float dot_b = 0.f, dot_s = 0.f;
 
   // Slot n of the first w + 1: rows of u (tokens 16 n..) against the wave's columns of dO and of z; slot
@@ -942,34 +994,36 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(Args<T> a) {
   for (int v0 = 0; v0 < a.v_pad; v0 += 32) {
     __syncthreads();
     float x[8], y[8];
-    load_vec<float, 8>(resid + v0, x);
-    load_vec<float, 8>(zs + v0, y);
+    if (H == 1 || half == 0) {
+      load_vec<float, 8>(resid + v0, x);
+      load_vec<float, 8>(zs + v0, y);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      dot_b = fmaf(x[i], y[i], dot_b);
-      x[i] *= beta;
-    }
-    stage<kPieces>(s.u, row, c8, x);
-    stage<kPieces>(s.z, row, c8, y);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int at = v0 + 8 * c8 + 4 * h;
-      float q[4] = {0.f, 0.f, 0.f, 0.f};
-      if (in && at < a.v_dim) load_part(d_o, at, a.v_dim - at, q);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[4 * h + i] = q[i];
-    }
-    stage<NP>(s.d_o, row, c8, x);
-#pragma unroll
-    for (int h = 0; h < (KD + 63) / 64; ++h)
-      if (KD >= 64 || row < KD) {
-        load_vec<float, 8>(st + (int64_t)64 * h * a.v_pad + v0, x);
-        load_vec<float, 8>(ds + (int64_t)64 * h * a.v_pad + v0, y);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) dot_s = fmaf(x[i], y[i], dot_s);
-        stage<kPieces>(s.S, row + 64 * h, c8, x);
-        stage<kPieces>(s.dS, row + 64 * h, c8, y);
+      for (int i = 0; i < 8; ++i) {
+        dot_b = fmaf(x[i], y[i], dot_b);
+        x[i] *= beta;
       }
+      stage<kPieces>(s.u, token, c8, x);
+      stage<kPieces>(s.z, token, c8, y);
+    }
+    if (H == 1 || half == 1) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int at = v0 + 8 * c8 + 4 * h;
+        float q[4] = {0.f, 0.f, 0.f, 0.f};
+        if (in && at < a.v_dim) load_part(d_o, at, a.v_dim - at, q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[4 * h + i] = q[i];
+      }
+      stage<NP>(s.d_o, token, c8, x);
+    }
+    if (KD >= 64 || row < KD) {
+      load_vec<float, 8>(st + v0, x);
+      load_vec<float, 8>(ds + v0, y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dot_s = fmaf(x[i], y[i], dot_s);
+      stage<kPieces>(s.S, row, c8, x);
+      stage<kPieces>(s.dS, row, c8, y);
+    }
     __syncthreads();
     bf16x8 uw[kPieces], zw[kPieces], ow[NP];
     load_frag(s.u + w * kPieces * kFrag, lane, uw);
@@ -977,8 +1031,7 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(Args<T> a) {
     load_frag(s.d_o + w * NP * kFrag, lane, ow);
 #pragma unroll
     for (int n = 0; n < 5; ++n) {
-      const bool turned = n <= w;
-      if (turned) {
+      if (n <= w) {
         bf16x8 un[kPieces];
         load_frag(s.u + n * kPieces * kFrag, lane, un);
         p[n] = mma(un, ow, p[n]);
@@ -993,11 +1046,12 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(Args<T> a) {
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
+      const int tile = half * MT + i;
       bf16x8 f[kPieces];
-      load_frag(s.S + i * kPieces * kFrag, lane, f);
+      load_frag(s.S + tile * kPieces * kFrag, lane, f);
       dq[i] = mma(f, ow, dq[i]);
       ka[i] = mma(f, zw, ka[i]);
-      load_frag(s.dS + i * kPieces * kFrag, lane, f);
+      load_frag(s.dS + tile * kPieces * kFrag, lane, f);
       kb[i] = mma(f, uw, kb[i]);
     }
   }
@@ -1016,7 +1070,7 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(Args<T> a) {
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     dq[i] = settled(dq[i]), ka[i] = settled(ka[i]), kb[i] = settled(kb[i]);
-    const int d = 16 * i + 4 * g;
+    const int d = 16 * (half * MT + i) + 4 * g;
     float kv[4] = {0.f, 0.f, 0.f, 0.f};
     if (here && d < a.k_dim) load_part(krow, d, a.k_dim - d, kv);
 #pragma unroll
@@ -1043,7 +1097,8 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(Args<T> a) {
       mm[n][r] = one && other != mine ? mm[n][r] * (-bi * D) : 0.f;
     }
   }
-  const uint16_t* kt = a.keys + ((b * a.k_heads + hk) * a.chunks + chunk) * (3 * kPart) + kPart;
+  const uint16_t* kt = a.keys + ((b * a.k_heads + hk) * a.chunks + chunk) * (3 * kPart) + kPart +
+                       half * MT * 2 * NP * kFrag;
   const uint16_t* qt = kt + kPart;
   const floatx4 none = {};
 #pragma unroll
@@ -1079,7 +1134,7 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(Args<T> a) {
   const bool shared = a.k_heads != a.v_heads;
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
-    const int d = 16 * i + 4 * g;
+    const int d = 16 * (half * MT + i) + 4 * g;
     dq[i] = settled(dq[i]), ka[i] = settled(ka[i]), kb[i] = settled(kb[i]);
     if (!here || d >= a.k_dim) continue;
     float qv[4], kv[4], dk[4], dqv[4];
@@ -1107,20 +1162,27 @@ __global__ __launch_bounds__(256) void delta_grad_kernel(Args<T> a) {
   wrote += __shfl_xor(wrote, 16);
   wrote += __shfl_xor(wrote, 32);
   if (g == 0) {
-    s.dG[mine] = dG;
-    s.w[mine] = wrote;
+    s.dG[half][mine] = dG;
+    s.w[half][mine] = wrote;
   }
   dot_b += lane_xor1(dot_b);
   dot_b += lane_xor2(dot_b);
-  if (c8 == 0) s.dbeta[row] = dot_b;
+  if (c8 == 0 && half == 0) s.dbeta[token] = dot_b;
   dot_s = wave_sum_all(dot_s);
-  if (lane == 0) s.dot[w] = dot_s;
+  if (lane == 0) s.dot[wave] = dot_s;
   __syncthreads();
-  if (w == 0) {
+  if (wave == 0) {
     const int d = s.doc[lane];
-    double v = s.dG[lane];
-    float ends = wave_sum_all(s.w[lane]);  // zero for tokens of other documents than the last
-    if (last == 0) ends = fmaf(expf((float)s.G[kC - 1]), (s.dot[0] + s.dot[1]) + (s.dot[2] + s.dot[3]), ends);
+    double v = s.dG[0][lane];
+    float ends = s.w[0][lane], all = 0.f;
+    if (H == 2) {
+      v += s.dG[1][lane];
+      ends += s.w[1][lane];
+    }
+    ends = wave_sum_all(ends);  // zero for tokens of other documents than the last
+#pragma unroll
+    for (int n = 0; n < 4 * H; ++n) all += s.dot[n];
+    if (last == 0) ends = fmaf(expf((float)s.G[kC - 1]), all, ends);
     if (lane == kC - 1) v += ends;
 #pragma unroll
     for (int n = 1; n < 64; n *= 2) {

@@ -50,7 +50,7 @@ int launch_bwd(const Args<T>& a, hipStream_t s) {
     int st = launch_status();                                                                 \
     if (st == MQC_OK) st = launch_walk<T, KD, true>(a, s);                                    \
     if (st != MQC_OK) return st;                                                              \
-    delta_grad_kernel<T, KD><<<dim3(parts), dim3(256), 0, s>>>(a);                            \
+    delta_grad_kernel<T, KD><<<dim3(parts), dim3(256 * kGradHalves<KD>), 0, s>>>(a);                            \
     if (a.k_heads != a.v_heads)                                                               \
       delta_share_kernel<T><<<dim3((unsigned)(shares < 65536 ? shares : 65536)), dim3(256), 0, s>>>(a); \
     return launch_status();                                                                   \
