@@ -396,10 +396,12 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Args<T> a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int row = 16 * w + 4 * g + r;
-        const bool seen = col <= row && s.doc[row] == dc;
-        const float D = seen ? expf((float)(s.G[row] - Gc)) : 0.f;
-        s.m[row][col] = seen && col < row ? D * kk[n][r] * (BWD ? s.beta[row] : bc) : 0.f;
-        if (seen) P[n][r] = D * qk[n][r];
+        const bool seen = (col <= row) & (s.doc[row] == dc);
+        const float gap = (float)(s.G[row] - Gc);
+        const float D = expf(seen ? gap : -1e4f);  // else 0
+        const float by = D * (BWD ? s.beta[row] : bc);
+        s.m[row][col] = seen & (col < row) ? by * kk[n][r] : 0.f;
+        P[n][r] = seen ? D * qk[n][r] : 0.f;
       }
     }
     __syncthreads();
@@ -939,17 +941,24 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, true>)) void delta_bwd_
 // columns 16 w.. of everything turned (tokens as columns). Operands pass through LDS 32 columns of v_dim
 // at a time, as fragments with their columns in order.
 // ---------------------------------------------------------------------------
-// Of wide keys two waves have a column each, and half of k_dim: their gradients of q and k are what
-// registers are needed for.
+// Of wide keys four waves have the same columns and a quarter of k_dim each: with the gradients of q and k
+// in the registers of one, a SIMD had room for two waves, which could not hide what they wait for.
 template <int KD>
-constexpr int kGradHalves = KD > 64 ? 2 : 1;
+constexpr int kGradParts = KD > 64 ? 4 : 1;
 
 template <typename T, int KD>
 struct GradShared {
-  uint16_t u[4 * kPieces * kFrag], z[4 * kPieces * kFrag], d_o[4 * kIn<T> * kFrag];
-  uint16_t S[KD / 16 * kPieces * kFrag], dS[KD / 16 * kPieces * kFrag];
+  union {
+    struct {
+      uint16_t u[4 * kPieces * kFrag], z[4 * kPieces * kFrag], d_o[4 * kIn<T> * kFrag];
+      uint16_t S[KD / 16 * kPieces * kFrag], dS[KD / 16 * kPieces * kFrag];
+    };
+    // Then, of several parts, D dP and M of each wave's columns: the one or two fragments of what its
+    // tokens read and those of what reads them, three in all.
+    uint16_t tokens[kGradParts<KD> > 1 ? 2 : 1][kGradParts<KD> > 1 ? 4 : 1][3 * kPieces * kFrag];
+  };
   double G[kC];
-  float beta[kC], dG[2][kC], w[2][kC], dbeta[kC], dot[8];
+  float beta[kC], dG[kGradParts<KD>][kC], w[kGradParts<KD>][kC], dbeta[kC], dot[16];
   int doc[kC];
 };
 
@@ -962,11 +971,11 @@ __device__ inline void stage(uint16_t* to, int row, int c, float (&x)[8]) {
 }
 
 template <typename T, int KD>
-__global__ __launch_bounds__(256 * kGradHalves<KD>, 2) void delta_grad_kernel(Args<T> a) {
-  constexpr int NP = kIn<T>, H = kGradHalves<KD>, MT = KD / 16 / H, kPart = KD / 8 * NP * kFrag;
+__global__ __launch_bounds__(256 * kGradParts<KD>, kGradParts<KD> > 1 ? 4 : 2) void delta_grad_kernel(Args<T> a) {
+  constexpr int NP = kIn<T>, H = kGradParts<KD>, MT = KD / 16 / H, kPart = KD / 8 * NP * kFrag;
   __shared__ __attribute__((aligned(16))) GradShared<T, KD> s;
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, m = lane & 15;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = wave & 3, half = wave >> 2;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = wave & 3, part = wave >> 2;
   const int64_t unit = xcd_order(blockIdx.x, gridDim.x), chunk = unit % a.chunks, bh = unit / a.chunks;
   const int64_t b = bh / a.v_heads, hv = bh % a.v_heads, hk = hv / (a.v_heads / a.k_heads);
   const int64_t t0 = chunk * kC;
@@ -977,26 +986,24 @@ __global__ __launch_bounds__(256 * kGradHalves<KD>, 2) void delta_grad_kernel(Ar
     s.doc[lane] = x.doc;
   }
   __syncthreads();
-  // What this thread stages: a row of the states; one of u and z or (of two halves the second) of dO.
+  // What this thread stages: a row of the states (parts 0 and 1), of u and z (part 2), of dO (part 3).
   const int row = tid >> 2, c8 = tid & 3, token = row & 63;
-  const float* resid = a.resid + (unit * kC + token) * a.v_pad + 8 * c8;
-  const float* zs = a.z + (unit * kC + token) * a.v_pad + 8 * c8;
-  const float* st = a.states + (unit * KD + row) * a.v_pad + 8 * c8;
-  const float* ds = a.dstates + (unit * KD + row) * a.v_pad + 8 * c8;
-  const T* d_o = a.d_o + ((b * a.seq + t0 + token) * a.v_heads + hv) * a.v_dim;
-  const bool in = t0 + token < a.seq;
-  const float beta = s.beta[token];
+  const uint32_t at_token = token * a.v_pad + 8 * c8, at_row = row * a.v_pad + 8 * c8;
+  const float *resid = a.resid + unit * kC * a.v_pad, *zs = a.z + unit * kC * a.v_pad;
+  const float *st = a.states + unit * KD * a.v_pad, *ds = a.dstates + unit * KD * a.v_pad;
   float dot_b = 0.f, dot_s = 0.f;
 
   // Slot n of the first w + 1: rows of u (tokens 16 n..) against the wave's columns of dO and of z; slot
-  // n + 1 of the others: rows of dO and of z against its columns of u.
-  floatx4 p[5] = {}, mm[5] = {}, dq[MT] = {}, ka[MT] = {}, kb[MT] = {};
+  // n + 1 of the others: rows of dO and of z against its columns of u. (Of several parts the first takes
+  // dO and the second z, both in p.)
+  floatx4 p[5] = {}, mm[H == 1 ? 5 : 1] = {}, dq[MT] = {}, ka[MT] = {}, kb[MT] = {};
   for (int v0 = 0; v0 < a.v_pad; v0 += 32) {
     __syncthreads();
     float x[8], y[8];
-    if (H == 1 || half == 0) {
-      load_vec<float, 8>(resid + v0, x);
-      load_vec<float, 8>(zs + v0, y);
+    if (H == 1 || part == 2) {
+      load_vec<float, 8>(resid + (at_token + v0), x);
+      load_vec<float, 8>(zs + (at_token + v0), y);
+      const float beta = s.beta[token];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         dot_b = fmaf(x[i], y[i], dot_b);
@@ -1005,20 +1012,21 @@ __global__ __launch_bounds__(256 * kGradHalves<KD>, 2) void delta_grad_kernel(Ar
       stage<kPieces>(s.u, token, c8, x);
       stage<kPieces>(s.z, token, c8, y);
     }
-    if (H == 1 || half == 1) {
+    if (H == 1 || part == 3) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int at = v0 + 8 * c8 + 4 * h;
         float q[4] = {0.f, 0.f, 0.f, 0.f};
-        if (in && at < a.v_dim) load_part(d_o, at, a.v_dim - at, q);
+        if (t0 + token < a.seq && at < a.v_dim)
+          load_part(a.d_o + ((b * a.seq + t0 + token) * a.v_heads + hv) * a.v_dim, at, a.v_dim - at, q);
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[4 * h + i] = q[i];
       }
       stage<NP>(s.d_o, token, c8, x);
     }
-    if (KD >= 64 || row < KD) {
-      load_vec<float, 8>(st + v0, x);
-      load_vec<float, 8>(ds + v0, y);
+    if (row < KD) {
+      load_vec<float, 8>(st + (at_row + v0), x);
+      load_vec<float, 8>(ds + (at_row + v0), y);
 #pragma unroll
       for (int i = 0; i < 8; ++i) dot_s = fmaf(x[i], y[i], dot_s);
       stage<kPieces>(s.S, row, c8, x);
@@ -1034,19 +1042,26 @@ __global__ __launch_bounds__(256 * kGradHalves<KD>, 2) void delta_grad_kernel(Ar
       if (n <= w) {
         bf16x8 un[kPieces];
         load_frag(s.u + n * kPieces * kFrag, lane, un);
-        p[n] = mma(un, ow, p[n]);
-        mm[n] = mma(un, zw, mm[n]);
+        if (part == 0) p[n] = mma(un, ow, p[n]);
+        if constexpr (H == 1) mm[n] = mma(un, zw, mm[n]);
+        else if (part == 1) p[n] = mma(un, zw, p[n]);
       } else {
-        bf16x8 zn[kPieces], on[NP];
-        load_frag(s.d_o + (n - 1) * NP * kFrag, lane, on);
-        load_frag(s.z + (n - 1) * kPieces * kFrag, lane, zn);
-        p[n] = mma(on, uw, p[n]);
-        mm[n] = mma(zn, uw, mm[n]);
+        if (part == 0) {
+          bf16x8 on[NP];
+          load_frag(s.d_o + (n - 1) * NP * kFrag, lane, on);
+          p[n] = mma(on, uw, p[n]);
+        }
+        if (H == 1 || part == 1) {
+          bf16x8 zn[kPieces];
+          load_frag(s.z + (n - 1) * kPieces * kFrag, lane, zn);
+          if constexpr (H == 1) mm[n] = mma(zn, uw, mm[n]);
+          else p[n] = mma(zn, uw, p[n]);
+        }
       }
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-      const int tile = half * MT + i;
+      const int tile = part * MT + i;
       bf16x8 f[kPieces];
       load_frag(s.S + tile * kPieces * kFrag, lane, f);
       dq[i] = mma(f, ow, dq[i]);
@@ -1070,7 +1085,7 @@ __global__ __launch_bounds__(256 * kGradHalves<KD>, 2) void delta_grad_kernel(Ar
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     dq[i] = settled(dq[i]), ka[i] = settled(ka[i]), kb[i] = settled(kb[i]);
-    const int d = 16 * (half * MT + i) + 4 * g;
+    const int d = 16 * (part * MT + i) + 4 * g;
     float kv[4] = {0.f, 0.f, 0.f, 0.f};
     if (here && d < a.k_dim) load_part(krow, d, a.k_dim - d, kv);
 #pragma unroll
@@ -1082,32 +1097,72 @@ __global__ __launch_bounds__(256 * kGradHalves<KD>, 2) void delta_grad_kernel(Ar
     }
   }
   // D dP (turned in the first w + 1 slots), and M.
+  if (H == 1 || part < 2) {
 #pragma unroll
-  for (int n = 0; n < 5; ++n) {
-    const bool turned = n <= w;
-    p[n] = settled(p[n]), mm[n] = settled(mm[n]);
+    for (int n = 0; n < 5; ++n) {
+      const bool turned = n <= w;
+      const int first = 16 * (turned ? n : n - 1) + 4 * g, way = turned ? 1 : -1;
+      p[n] = settled(p[n]);
+      if constexpr (H == 1) mm[n] = settled(mm[n]);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int other = 16 * (turned ? n : n - 1) + 4 * g + r;
-      const bool one = s.doc[other] == doc && (turned ? other <= mine : other >= mine);
-      const double G = s.G[other];
-      const float D = one ? expf((float)(turned ? Gm - G : G - Gm)) : 0.f;
-      const float bi = turned ? bm : s.beta[other];
-      p[n][r] = one ? p[n][r] * (D * a.scale) : 0.f;
-      mm[n][r] = one && other != mine ? mm[n][r] * (-bi * D) : 0.f;
+      for (int r = 0; r < 4; ++r) {
+        const int other = first + r, apart = (mine - other) * way;
+        const bool one = (s.doc[other] == doc) & (apart >= 0);
+        const float gap = (float)((Gm - s.G[other]) * way);
+        const float D = expf(one ? gap : -1e4f);  // else 0
+        const float bi = turned ? bm : s.beta[other], below = apart ? -bi * D : 0.f;
+        if constexpr (H == 1) {
+          p[n][r] = one ? p[n][r] * (D * a.scale) : 0.f;
+          mm[n][r] = one && apart ? mm[n][r] * below : 0.f;
+        } else {
+          const float by = part == 0 ? D * a.scale : below;
+          p[n][r] = one && (part == 0 || apart) ? p[n][r] * by : 0.f;
+        }
+      }
     }
   }
-  const uint16_t* kt = a.keys + ((b * a.k_heads + hk) * a.chunks + chunk) * (3 * kPart) + kPart +
-                       half * MT * 2 * NP * kFrag;
-  const uint16_t* qt = kt + kPart;
   const floatx4 none = {};
+  // The slots as right operands: columns that the wave's tokens read (ks of the first two), and that read
+  // them.
+  const auto reads = [&](const floatx4 (&v)[5], int ks, bf16x8 (&f)[kPieces]) {
+    split<kPieces>(v[2 * ks], 2 * ks + 1 <= w ? v[2 * ks + 1] : none, f);
+  };
+  const auto read_by = [&](const floatx4 (&v)[5], int ks, bf16x8 (&f)[kPieces]) {
+    split<kPieces>(2 * ks >= w ? v[2 * ks + 1] : none, v[2 * ks + 2], f);
+  };
+  if constexpr (H > 1) {
+    __syncthreads();
+    uint16_t* to = s.tokens[part & 1][w];
+    bf16x8 f[kPieces];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      if (part > 1) break;
+      // In their order: ks of what is read, then of what reads.
+      if (2 * ks <= w) {
+        reads(p, ks, f);
+        store_frag(to + ks * kPieces * kFrag, lane, f);
+      }
+      if (2 * ks + 1 >= w) {
+        read_by(p, ks, f);
+        store_frag(to + (w < 2 ? 1 + ks : 2) * kPieces * kFrag, lane, f);
+      }
+    }
+    __syncthreads();
+  }
+  const uint16_t* kt = a.keys + ((b * a.k_heads + hk) * a.chunks + chunk) * (3 * kPart) + kPart +
+                       part * MT * 2 * NP * kFrag;
+  const uint16_t* qt = kt + kPart;
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) {
-    const int n = 2 * ks;
-    if (n <= w) {  // turned: columns that this token reads
+    if (2 * ks <= w) {
       bf16x8 pf[kPieces], mf[kPieces];
-      split<kPieces>(p[n], n + 1 <= w ? p[n + 1] : none, pf);
-      split<kPieces>(mm[n], n + 1 <= w ? mm[n + 1] : none, mf);
+      if constexpr (H == 1) {
+        reads(p, ks, pf);
+        reads(mm, ks, mf);
+      } else {
+        load_frag(s.tokens[0][w] + ks * kPieces * kFrag, lane, pf);
+        load_frag(s.tokens[1][w] + ks * kPieces * kFrag, lane, mf);
+      }
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         bf16x8 f[NP];
@@ -1116,10 +1171,16 @@ __global__ __launch_bounds__(256 * kGradHalves<KD>, 2) void delta_grad_kernel(Ar
         ka[i] = mma(f, mf, ka[i]);
       }
     }
-    if (n + 1 >= w) {  // tokens that read this one
+    if (2 * ks + 1 >= w) {
       bf16x8 pf[kPieces], mf[kPieces];
-      split<kPieces>(n >= w ? p[n + 1] : none, p[n + 2], pf);
-      split<kPieces>(n >= w ? mm[n + 1] : none, mm[n + 2], mf);
+      if constexpr (H == 1) {
+        read_by(p, ks, pf);
+        read_by(mm, ks, mf);
+      } else {
+        const int at = (w < 2 ? 1 + ks : 2) * kPieces * kFrag;
+        load_frag(s.tokens[0][w] + at, lane, pf);
+        load_frag(s.tokens[1][w] + at, lane, mf);
+      }
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         bf16x8 f[NP];
@@ -1134,7 +1195,7 @@ __global__ __launch_bounds__(256 * kGradHalves<KD>, 2) void delta_grad_kernel(Ar
   const bool shared = a.k_heads != a.v_heads;
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
-    const int d = 16 * (half * MT + i) + 4 * g;
+    const int d = 16 * (part * MT + i) + 4 * g;
     dq[i] = settled(dq[i]), ka[i] = settled(ka[i]), kb[i] = settled(kb[i]);
     if (!here || d >= a.k_dim) continue;
     float qv[4], kv[4], dk[4], dqv[4];
@@ -1162,12 +1223,12 @@ __global__ __launch_bounds__(256 * kGradHalves<KD>, 2) void delta_grad_kernel(Ar
   wrote += __shfl_xor(wrote, 16);
   wrote += __shfl_xor(wrote, 32);
   if (g == 0) {
-    s.dG[half][mine] = dG;
-    s.w[half][mine] = wrote;
+    s.dG[part][mine] = dG;
+    s.w[part][mine] = wrote;
   }
   dot_b += lane_xor1(dot_b);
   dot_b += lane_xor2(dot_b);
-  if (c8 == 0 && half == 0) s.dbeta[token] = dot_b;
+  if (c8 == 0 && part == (H == 1 ? 0 : 2)) s.dbeta[token] = dot_b;
   dot_s = wave_sum_all(dot_s);
   if (lane == 0) s.dot[wave] = dot_s;
   __syncthreads();
@@ -1175,9 +1236,10 @@ __global__ __launch_bounds__(256 * kGradHalves<KD>, 2) void delta_grad_kernel(Ar
     const int d = s.doc[lane];
     double v = s.dG[0][lane];
     float ends = s.w[0][lane], all = 0.f;
-    if (H == 2) {
-      v += s.dG[1][lane];
-      ends += s.w[1][lane];
+#pragma unroll
+    for (int n = 1; n < H; ++n) {
+      v += s.dG[n][lane];
+      ends += s.w[n][lane];
     }
     ends = wave_sum_all(ends);  // zero for tokens of other documents than the last
 #pragma unroll

@@ -14,7 +14,7 @@ namespace delta {
 template <typename T, int KD, bool BWD>
 int launch_walk(const Args<T>& a, hipStream_t s) {
   const int64_t tiles = a.v_pad / 16, heads = a.batch * a.v_heads;
-  if (heads * tiles <= 512) {
+  if (heads * tiles <= 256) {
     const dim3 grid((unsigned)(heads * tiles));
     if constexpr (BWD) delta_bwd_kernel<T, KD, 1><<<grid, dim3(256), 0, s>>>(a);
     else delta_fwd_kernel<T, KD, 1><<<grid, dim3(256), 0, s>>>(a);
@@ -50,7 +50,7 @@ int launch_bwd(const Args<T>& a, hipStream_t s) {
     int st = launch_status();                                                                 \
     if (st == MQC_OK) st = launch_walk<T, KD, true>(a, s);                                    \
     if (st != MQC_OK) return st;                                                              \
-    delta_grad_kernel<T, KD><<<dim3(parts), dim3(256 * kGradHalves<KD>), 0, s>>>(a);                            \
+    delta_grad_kernel<T, KD><<<dim3(parts), dim3(256 * kGradParts<KD>), 0, s>>>(a);                            \
     if (a.k_heads != a.v_heads)                                                               \
       delta_share_kernel<T><<<dim3((unsigned)(shares < 65536 ? shares : 65536)), dim3(256), 0, s>>>(a); \
     return launch_status();                                                                   \
