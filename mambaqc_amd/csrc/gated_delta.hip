@@ -11,7 +11,7 @@ int64_t chunk_count(int64_t seq) { return (seq + delta::kC - 1) / delta::kC; }
 
 // Where the workspace's parts begin, each a multiple of 256 bytes long.
 struct Space {
-  int64_t keys, tri, vec, dstates, z, dq, dk, bytes;
+  int64_t keys, tri, zeros, vec, dstates, z, dq, dk, bytes;
 };
 Space space(int64_t batch, int64_t seq, int64_t k_heads, int64_t v_heads, int64_t k_dim, int64_t v_dim,
             int dtype, bool backward) {
@@ -27,6 +27,7 @@ Space space(int64_t batch, int64_t seq, int64_t k_heads, int64_t v_heads, int64_
   };
   w.keys = take(units * 3 * kd / 8 * pieces * frag);
   w.tri = take(parts * 2 * delta::kTri * delta::kPieces * frag);
+  w.zeros = take(delta::kPieces * frag);
   w.vec = take(parts * 4 * delta::kC * 4);
   if (backward) {
     w.dstates = take(parts * kd * vp * 4);
@@ -77,6 +78,7 @@ template <typename T>
 void place_space(delta::Args<T>& a, const Space& w, char* ws) {
   a.keys = (uint16_t*)(ws + w.keys);
   a.tri = (uint16_t*)(ws + w.tri);
+  a.zeros = (uint16_t*)(ws + w.zeros);
   a.vec = (float*)(ws + w.vec);
 }
 

@@ -140,7 +140,7 @@ struct Args {
   // The operands as fragments: of each key head and chunk K, K^T and Q (or, for the backward, Q^T), of
   // each value head and chunk T and P (or T~^T and P^T), and four vectors: e, D_63, beta, and the number
   // of documents begun since the chunk's start.
-  uint16_t *keys, *tri;
+  uint16_t *keys, *tri, *zeros;  // (zeros: one fragment's pieces)
   float* vec;  // [batch, v_heads, chunks, 4, 64]
   // forward
   T* o;
@@ -316,6 +316,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Args<T> a) {
   const int group = (int)(a.v_heads / a.k_heads);
   uint16_t* keys = a.keys + unit * (3 * KD / 8 * NP * kFrag);
   constexpr int kPart = KD / 8 * NP * kFrag;
+  if (unit == 0 && w < kPieces) *reinterpret_cast<u32x4*>(a.zeros + w * kFrag + lane * 8) = (u32x4){};
   // The gates of a value head, by one wave.
   const auto gates = [&](int64_t hv) {
     const Gates x = chunk_gates(a, b, hv, t0);
@@ -350,8 +351,9 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Args<T> a) {
   for (int i = 0; i < KS; ++i) {
     const int at = (i * 4 + w) * NP * kFrag;
     store_frag(s.frags + at, lane, kf[i]);
-    store_frag(keys + at, lane, kf[i]);
-    if constexpr (!BWD) store_frag(keys + 2 * kPart + at, lane, qf[i]);
+    const int to = (w * KS + i) * NP * kFrag;  // a wave of the walk reads its own together
+    store_frag(keys + to, lane, kf[i]);
+    if constexpr (!BWD) store_frag(keys + 2 * kPart + to, lane, qf[i]);
   }
   __syncthreads();
   floatx4 kk[4] = {}, qk[4] = {};
@@ -488,19 +490,15 @@ __device__ inline float tri_at(const uint16_t* tri, int row, int col) {
 __device__ inline bool finite(float v) { return fabsf(v) < __builtin_huge_valf(); }
 
 // The wave's rows of a triangular matrix: fragments of its two columns of 32, one of which may be zero.
+// (The zeros come from memory too: what is there already would be waited for.)
 template <bool UPPER>
-__device__ inline void load_tri(const uint16_t* tri, int w, bf16x8 (&f)[2][kPieces]) {
+__device__ inline void load_tri(const uint16_t* tri, const uint16_t* zeros, int w,
+                                bf16x8 (&f)[2][kPieces]) {
   const int lane = threadIdx.x & 63;
-  const bool both = UPPER ? w < 2 : w >= 2;
   const int first = UPPER ? (w < 2 ? 2 * w : w + 1) : (w < 2 ? w : 2 * w - 2);
-  constexpr int part = UPPER ? 0 : 1;  // that may be missing
   const uint16_t* at = tri + first * kPieces * kFrag;
-  load_frag(UPPER && !both ? at + kPieces * kFrag : at, lane, f[0]);
-  load_frag(both || UPPER ? at + kPieces * kFrag : at, lane, f[1]);
-  if (!both) {
-#pragma unroll
-    for (int p = 0; p < kPieces; ++p) f[part][p] = __builtin_bit_cast(bf16x8, (u32x4){});
-  }
+  load_frag(UPPER && w >= 2 ? zeros : at, lane, f[0]);
+  load_frag(!UPPER && w < 2 ? zeros : at + kPieces * kFrag, lane, f[1]);
 }
 // Their product with x.
 template <int NX>
@@ -565,7 +563,7 @@ struct Walker {
   __device__ const uint16_t* part(int64_t c, int i) const { return keys + c * (3 * kPart) + i * kPart; }
   __device__ void load_rows(int64_t c, int i, bf16x8 (&f)[KS][NP]) const {
 #pragma unroll
-    for (int s = 0; s < KS; ++s) load_frag(part(c, i) + (s * 4 + w) * NP * kFrag, lane, f[s]);
+    for (int s = 0; s < KS; ++s) load_frag(part(c, i) + (w * KS + s) * NP * kFrag, lane, f[s]);
   }
   __device__ void load_cols(int64_t c, int i, bf16x8 (&f)[MT][2][NP]) const {
     const int tile = holds ? w : 0;
@@ -653,43 +651,23 @@ struct Walker {
   // The same between chunks, padded.
   __device__ void store_padded(float* to, int64_t c, int ct, const floatx4 (&S)[MT]) const {
     if (!holds || col(ct) >= a.v_pad) return;
+    float* base = to + (bh * a.chunks + c) * KD * a.v_pad;
 #pragma unroll
     for (int t = 0; t < MT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        to[((bh * a.chunks + c) * KD + 16 * (w + 4 * t) + 4 * g + r) * a.v_pad + col(ct)] = S[t][r];
+        base[(uint32_t)((16 * (w + 4 * t) + 4 * g + r) * a.v_pad + col(ct))] = S[t][r];
   }
   __device__ void store_rows(float* to, int64_t c, int ct, const floatx4& v) const {
     if (col(ct) >= a.v_pad) return;
+    float* base = to + (bh * a.chunks + c) * kC * a.v_pad;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      to[((bh * a.chunks + c) * kC + 16 * w + 4 * g + r) * a.v_pad + col(ct)] = v[r];
-  }
-  // The wave's tokens of v (or dO), past the ends the last one's and its last column; and of o (or dv).
-  __device__ void load_tile(const T* from, int64_t x_b, int64_t x_t, int64_t x_h, int64_t c, int ct,
-                            T (&v)[4]) const {
-    const T* at = from + b * x_b + hv * x_h + (col(ct) < a.v_dim ? col(ct) : a.v_dim - 1);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int64_t t = c * kC + 16 * w + 4 * g + r;
-      v[r] = at[(t < a.seq ? t : a.seq - 1) * x_t];
-    }
+    for (int r = 0; r < 4; ++r) base[(uint32_t)((16 * w + 4 * g + r) * a.v_pad + col(ct))] = v[r];
   }
   __device__ bool here(int64_t c, int r) const { return c * kC + 16 * w + 4 * g + r < a.seq; }
+  __device__ bool whole(int64_t c) const { return (c + 1) * kC <= a.seq && col0 + 16 * CT <= a.v_dim; }
   __device__ float tile_value(const T (&v)[4], int64_t c, int ct, int r) const {
     return here(c, r) && col(ct) < a.v_dim ? load_scalar(&v[r]) : 0.f;
-  }
-  __device__ void store_tile(T* to, int64_t c, int ct, const floatx4& v) const {
-    T* at = to + ((b * a.seq + c * kC + 16 * w + 4 * g) * a.v_heads + hv) * a.v_dim + col(ct);
-    const int64_t step = a.v_heads * (int64_t)a.v_dim;
-    if ((c + 1) * kC <= a.seq && col0 + 16 * CT <= a.v_dim) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) store_scalar(at + r * step, v[r]);
-    } else {
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (here(c, r) && col(ct) < a.v_dim) store_scalar(at + r * step, v[r]);
-    }
   }
   // Rows that are not finite, for tri_product.
   __device__ void mark(float (*xs)[16], int* bad, const floatx4& v) const {
@@ -701,6 +679,46 @@ struct Walker {
     }
     const bool some = __ballot(!ok) != 0;
     if (lane == 0) bad[w] = some;
+  }
+};
+
+// The wave's tokens of v (or dO), and of o (or dv): elements of a chunk from its first token, 16 columns.
+template <typename T>
+struct TileRows {
+  T* first;       // of the head
+  int64_t token;  // elements between tokens
+  int64_t at[4];  // of the lane's four in a chunk, at its column
+  __device__ TileRows(T* x, int64_t token_, int w, int g, int col) : first(x), token(token_) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) at[r] = (16 * w + 4 * g + r) * token_ + col;
+  }
+  // (of `whole` chunks; else past the ends the last token's and the last column)
+  template <typename V, typename K>
+  __device__ void load(const K& k, int64_t c, int ct, V (&v)[4]) const {
+    if (k.whole(c)) {
+      const T* base = first + c * kC * token + 16 * ct;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = base[at[r]];
+    } else {
+      const int col = k.col(ct) < k.a.v_dim ? k.col(ct) : k.a.v_dim - 1;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t t = c * kC + 16 * k.w + 4 * k.g + r;
+        v[r] = first[(t < k.a.seq ? t : k.a.seq - 1) * token + col];
+      }
+    }
+  }
+  template <typename K>
+  __device__ void store(const K& k, int64_t c, int ct, const floatx4& v) const {
+    T* base = first + c * kC * token + 16 * ct;
+    if (k.whole(c)) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) store_scalar(base + at[r], v[r]);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (k.here(c, r) && k.col(ct) < k.a.v_dim) store_scalar(base + at[r], v[r]);
+    }
   }
 };
 
@@ -737,16 +755,19 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, false>)) void delta_fwd
   }
   bf16x8 kf[KS][NP], qf[KS][NP], tf[2][kPieces], pf[2][kPieces], cf[MT][2][NP];
   T v[CT][4];
+  const int64_t heads = a.v_heads * (int64_t)a.v_dim;
+  const TileRows<const T> from(a.v + k.b * a.v_b + k.hv * a.v_h, a.v_t, k.w, k.g, k.col(0));
+  const TileRows<T> to(a.o + k.b * a.seq * heads + k.hv * a.v_dim, heads, k.w, k.g, k.col(0));
   RowGates next;
   if (a.chunks > 0) {
     next.load(k.vec, k.w, k.g);
     k.load_rows(0, 0, kf);
     k.load_rows(0, 2, qf);
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) k.load_tile(a.v, a.v_b, a.v_t, a.v_h, 0, ct, v[ct]);
-    load_tri<false>(k.tri, k.w, tf);
+    for (int ct = 0; ct < CT; ++ct) from.load(k, 0, ct, v[ct]);
+    load_tri<false>(k.tri, a.zeros, k.w, tf);
     k.load_cols(0, 1, cf);
-    load_tri<false>(k.tri + K::kTriPart, k.w, pf);
+    load_tri<false>(k.tri + K::kTriPart, a.zeros, k.w, pf);
   }
   for (int64_t c = 0; c < a.chunks; ++c) {
     // What comes next goes out as soon as its place is free (behind the last chunk, once more its own).
@@ -776,7 +797,7 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, false>)) void delta_fwd
     floatx4 r[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      k.load_tile(a.v, a.v_b, a.v_t, a.v_h, ahead, ct, v[ct]);
+      from.load(k, ahead, ct, v[ct]);
       if (!mixed || !tri_apart<false>(s.bad[0], s.xs[0][ct], tri, doc, k.w, r[ct]))
         r[ct] = tri_product<kPieces>(tf, s.x[ct]);
       floatx4 u, y;
@@ -789,7 +810,7 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, false>)) void delta_fwd
       put_tile<kPieces>(s.y[ct], k.w, y);
       if (mixed) k.mark(s.xs[1][ct], s.bad[1], u);
     }
-    load_tri<false>(tri_ahead, k.w, tf);
+    load_tri<false>(tri_ahead, a.zeros, k.w, tf);
     if (mixed) k.cut_cols(cf, doc, at.last);
     lds_barrier();
     if (a.states) {
@@ -809,13 +830,13 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, false>)) void delta_fwd
       k.put_state(s.state[(c + 1) & 1][ct], S[ct]);
     }
     k.load_cols(ahead, 1, cf);
-    load_tri<false>(tri_ahead + K::kTriPart, k.w, pf);
+    load_tri<false>(tri_ahead + K::kTriPart, a.zeros, k.w, pf);
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         o[ct][i] = a.scale * (at.doc[i] == 0.f ? fmaf(at.e[i], qs[ct][i], o[ct][i]) : o[ct][i]);
-      k.store_tile(a.o, c, ct, o[ct]);
+      to.store(k, c, ct, o[ct]);
       if (a.resid) k.store_rows(a.resid, c, ct, r[ct]);
     }
   }
@@ -832,9 +853,9 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, true>)) void delta_bwd_
   const K k(a);
   constexpr int NP = K::NP, KS = K::KS, MT = K::MT;
   const int64_t heads = a.v_heads * (int64_t)a.v_dim, end = a.chunks - 1;
-  const auto load_grad = [&](int64_t c, int ct, T (&v)[4]) {
-    k.load_tile(a.d_o, a.seq * heads, heads, a.v_dim, c, ct, v);
-  };
+  const int64_t first = k.b * a.seq * heads + k.hv * a.v_dim;
+  const TileRows<const T> from(a.d_o + first, heads, k.w, k.g, k.col(0));
+  const TileRows<T> to(a.dv + first, heads, k.w, k.g, k.col(0));
   const auto put_grad = [&](int64_t c, int ct, const T (&raw)[4], floatx4& v) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) v[r] = k.tile_value(raw, c, ct, r);
@@ -846,15 +867,15 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, true>)) void delta_bwd_
   for (int ct = 0; ct < CT; ++ct) {
     k.load_state(a.dh_last, ct, S[ct]);
     k.put_state(s.state[end & 1][ct], S[ct]);
-    load_grad(end, ct, raw[ct]);
+    from.load(k, end, ct, raw[ct]);
     put_grad(end, ct, raw[ct], v[ct]);
   }
   bf16x8 kf[KS][NP], tf[2][kPieces], pf[2][kPieces], cf[MT][2][NP], qf[MT][2][NP];
   RowGates next;
   next.load(k.vec + end * 4 * kC, k.w, k.g);
   k.load_rows(end, 0, kf);
-  load_tri<true>(k.tri + (2 * end + 1) * K::kTriPart, k.w, pf);
-  load_tri<true>(k.tri + 2 * end * K::kTriPart, k.w, tf);
+  load_tri<true>(k.tri + (2 * end + 1) * K::kTriPart, a.zeros, k.w, pf);
+  load_tri<true>(k.tri + 2 * end * K::kTriPart, a.zeros, k.w, tf);
   k.load_cols(end, 2, qf);
   k.load_cols(end, 1, cf);
   for (int64_t c = end; c >= 0; --c) {
@@ -876,13 +897,13 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, true>)) void delta_bwd_
     floatx4 y[CT], z[CT];
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
-      load_grad(ahead, ct, raw[ct]);
+      from.load(k, ahead, ct, raw[ct]);
       y[ct] = k.row_product(kf, s.state[c & 1][ct]);
       if (!mixed || !tri_apart<true>(s.bad[1], s.xs[1][ct], tri + K::kTriPart, doc, k.w, z[ct]))
         z[ct] = tri_product<NP>(pf, s.d_o[c & 1][ct]);
     }
     k.load_rows(ahead, 0, kf);
-    load_tri<true>(tri_ahead + K::kTriPart, k.w, pf);
+    load_tri<true>(tri_ahead + K::kTriPart, a.zeros, k.w, pf);
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       floatx4 x;  // e dO, for the state
@@ -914,7 +935,7 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, true>)) void delta_bwd_
       }
       put_tile<kPieces>(s.y[ct], k.w, v[ct]);
     }
-    load_tri<true>(tri_ahead, k.w, tf);
+    load_tri<true>(tri_ahead, a.zeros, k.w, tf);
     k.load_cols(ahead, 2, qf);
     lds_barrier();
 #pragma unroll
@@ -927,7 +948,7 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, true>)) void delta_bwd_
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       k.store_rows(a.z, c, ct, z[ct]);
-      k.store_tile(a.dv, c, ct, y[ct]);
+      to.store(k, c, ct, y[ct]);
     }
   }
   if (a.dh0 && k.holds) {

@@ -14,7 +14,7 @@ namespace delta {
 template <typename T, int KD, bool BWD>
 int launch_walk(const Args<T>& a, hipStream_t s) {
   const int64_t tiles = a.v_pad / 16, heads = a.batch * a.v_heads;
-  if (heads * tiles <= 256) {
+  if (heads * tiles <= 512) {
     const dim3 grid((unsigned)(heads * tiles));
     if constexpr (BWD) delta_bwd_kernel<T, KD, 1><<<grid, dim3(256), 0, s>>>(a);
     else delta_fwd_kernel<T, KD, 1><<<grid, dim3(256), 0, s>>>(a);
