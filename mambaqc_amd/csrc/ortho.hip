@@ -43,6 +43,8 @@ struct Group {
   int mp, np;            // padded to 64
   int count, first;      // matrices, and the first one's row
   int tiles;             // workgroups before this group's, by kernel
+  int splits;            // workgroups that share a tile's columns in the first product
+  int64_t shares;        // bytes: where their sums begin
   int sums;              // workgroups that add a matrix's squares
   float rate;
 };
@@ -60,6 +62,7 @@ struct Args {
   float a, b, c, eps, mu, decay;
   int nesterov;
   int flip;     // which X^T is read
+  int side;     // of the first product's tiles
 };
 
 template <bool PAIR>
@@ -140,15 +143,7 @@ __global__ __launch_bounds__(256) void ortho_sum_kernel(Args a) {
 }
 
 // --- X_0 by rows and turned ------------------------------------------------------------------------------
-// One value (times kScale) into a row.
-template <bool PAIR>
-__device__ inline void put(char* row, int col, float v) {
-  _Float16* to = (_Float16*)row + (PAIR ? col / 32 * 64 + col % 32 : col);
-  const _Float16 hi = (_Float16)v;
-  to[0] = hi;
-  if constexpr (PAIR) to[32] = (_Float16)(v - (float)hi);
-}
-// Four of them, col a multiple of 4; the second pieces `second` bytes on (0: none).
+// Four values (times kScale) into a row, col a multiple of 4; the second pieces `second` bytes on (0: none).
 __device__ inline float half_of(const u32x2& v, int c) {
   return io<f16_t>::bits_to_f32(c & 1 ? v[c / 2] >> 16 : v[c / 2] & 0xffffu);
 }
@@ -163,15 +158,6 @@ __device__ inline void put4(char* row, int col, const float (&v)[4], int64_t sec
     for (int c = 0; c < 4; ++c) r[c] = v[c] - half_of(hi, c);
     *(u32x2*)(to + second) = u32x2{pack2<f16_t>(r[0], r[1]), pack2<f16_t>(r[2], r[3])};
   }
-}
-template <bool PAIR>
-__device__ inline void get4(const char* row, int col, float (&v)[4], int64_t second = PAIR ? 64 : 0) {
-  const char* from = row + 2 * (PAIR ? col / 32 * 64 + col % 32 : col);
-  const u32x2 hi = *(const u32x2*)from;
-  u32x2 lo = {0u, 0u};
-  if (second) lo = *(const u32x2*)(from + second);
-#pragma unroll
-  for (int c = 0; c < 4; ++c) v[c] = half_of(hi, c) + half_of(lo, c);
 }
 // From a value of X^T to its second piece.
 template <bool PAIR>
@@ -229,127 +215,198 @@ __global__ __launch_bounds__(256) void ortho_init_kernel(Args a) {
 }
 
 // --- the products ------------------------------------------------------------------------------------------
-enum Stage { GRAM, POLY, APPLY, LAST };
+// JOIN: the first product's tiles from the sums of those that shared their columns.
+enum Stage { GRAM, JOIN, POLY, APPLY, LAST };
 
-template <int STAGE, int T>
+template <int S>
+__host__ __device__ inline int symmetric_tiles(const Group& g) {
+  const int t = ceil_div(g.m, S);
+  return t * (t + 1) / 2;
+}
+template <int STAGE, int S>
 __host__ __device__ inline int tile_count(const Group& g) {
-  const int t = ceil_div(g.m, T);
-  return STAGE == GRAM || STAGE == POLY ? t * (t + 1) / 2 : t * ceil_div(g.n, T);
+  if (STAGE == GRAM) return symmetric_tiles<S>(g) * g.splits;
+  if (STAGE == JOIN) return g.splits > 1 ? symmetric_tiles<S>(g) : 0;
+  if (STAGE == POLY) return symmetric_tiles<S>(g);
+  return ceil_div(g.m, S) * ceil_div(g.n, S);
 }
 
+// Eight values of a row, col a multiple of 8; second pieces as in put4.
+template <bool PAIR>
+__device__ inline void put8(char* row, int col, const float (&v)[8], int64_t second = PAIR ? 64 : 0) {
+  char* to = row + 2 * (PAIR ? col / 32 * 64 + col % 32 : col);
+  u32x4 hi, lo;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    hi[c] = pack2<f16_t>(v[2 * c], v[2 * c + 1]);
+    lo[c] = pack2<f16_t>(v[2 * c] - io<f16_t>::bits_to_f32(hi[c] & 0xffffu),
+                         v[2 * c + 1] - io<f16_t>::bits_to_f32(hi[c] >> 16));
+  }
+  *(u32x4*)to = hi;
+  if (second) *(u32x4*)(to + second) = lo;
+}
+template <bool PAIR>
+__device__ inline void get8(const char* row, int col, float (&v)[8], int64_t second = PAIR ? 64 : 0) {
+  const char* from = row + 2 * (PAIR ? col / 32 * 64 + col % 32 : col);
+  const u32x4 hi = *(const u32x4*)from;
+  u32x4 lo = {};
+  if (second) lo = *(const u32x4*)(from + second);
+#pragma unroll
+  for (int c = 0; c < 8; ++c)
+    v[c] = io<f16_t>::bits_to_f32(c & 1 ? hi[c / 2] >> 16 : hi[c / 2] & 0xffffu) +
+           io<f16_t>::bits_to_f32(c & 1 ? lo[c / 2] >> 16 : lo[c / 2] & 0xffffu);
+}
+// Eight elements of a matrix's row (its parameter's update where MUON).
+template <typename T, bool MUON>
+__device__ inline void put_result(T* to, int left, float (&v)[8], float decay, float rate) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if (left <= 4 * h) break;
+    float y[4], p[4];
+    if constexpr (MUON) load_part((const T*)to, 4 * h, left - 4 * h, p);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      y[c] = v[4 * h + c] * (1.f / kScale);
+      if constexpr (MUON) y[c] = fmaf(-rate, y[c], p[c] * decay);
+    }
+    store_part(to, 4 * h, left - 4 * h, y);
+  }
+}
+
+// A tile's rows w of the left operand and x of the right one, S of each. What it leaves goes through LDS,
+// the columns of a wave at a time: rows of x are written along w, and (the mirrored half of a symmetric
+// product, X by rows, a wide matrix) rows of w along x, 16 bytes a lane. Written from the registers, two
+// bytes a lane, they took longer than the products: 75 us of 12 matrices of 768 x 1536 for the last one.
 template <typename T, typename Cfg, bool PAIR, int STAGE, bool MUON>
 __global__ __launch_bounds__(Cfg::kThreads) void ortho_product_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  constexpr int S = Cfg::TW;
-  static_assert(Cfg::TW == Cfg::TX, "square tiles");
+  constexpr int S = Cfg::TW, XW = S / Cfg::NW_X, P = S + 4;
+  static_assert(Cfg::TW == Cfg::TX && XW * P * 4 <= Cfg::kStagesBytes, "square tiles, a wave's columns in LDS");
+  constexpr bool SYMMETRIC = STAGE == GRAM || STAGE == JOIN || STAGE == POLY;
   const int64_t n = gridDim.x, lin = blockIdx.x;
   const int64_t block = n % kXCDs ? lin : (lin % kXCDs) * (n / kXCDs) + lin / kXCDs;
   int i, left;
   const Group& g = find(a, block, [](const Group& g) { return tile_count<STAGE, S>(g); }, i, left);
   char* ws = a.ws + g.base + i * g.each;
-  // Rows of both operands (w: four consecutive ones to a lane).
-  int w0, x0;
+  int w0, x0, tile = 0, share = 0, k0 = 0;
   const char *W, *X;
-  int wn, xn, K;
-  bool turned = false;
-  if constexpr (STAGE == GRAM || STAGE == POLY) {
+  int wn = g.m, xn, K;
+  if constexpr (SYMMETRIC) {
+    if constexpr (STAGE == GRAM) share = left % g.splits, left /= g.splits;
+    tile = left;
     int tw = (int)((sqrtf(8.f * (float)left + 1.f) - 1.f) * 0.5f);
     while (tw * (tw + 1) / 2 > left) --tw;
     while ((tw + 1) * (tw + 2) / 2 <= left) ++tw;
     w0 = tw * S, x0 = (left - tw * (tw + 1) / 2) * S;
-    W = X = ws + (STAGE == GRAM ? 0 : at_a<PAIR>(g, 0));
-    wn = xn = g.m, K = STAGE == GRAM ? g.np : g.mp;
+    W = X = ws + (STAGE == POLY ? at_a<PAIR>(g, 0) : 0);
+    xn = g.m, K = STAGE == POLY ? g.mp : g.np;
   } else {
-    const int down = ceil_div(g.m, S), tm = left % down, tn = left / down;
+    const int down = ceil_div(g.m, S);
+    w0 = left % down * S, x0 = left / down * S;
     W = ws + at_a<PAIR>(g, 1), X = ws + at_xt<PAIR>(g, a.flip);
-    w0 = tm * S, x0 = tn * S, wn = g.m, xn = g.n, K = g.mp;
-    // The last product's lanes write along the rows of the matrix: of a wide one X^T's rows come first.
-    turned = STAGE == LAST && g.rows <= g.cols;
-    if (turned) {
-      const char* o = W;
-      W = X, X = o;
-      w0 = tn * S, x0 = tm * S, wn = g.n, xn = g.m;
-    }
+    xn = g.n, K = g.mp;
   }
   const int64_t rp = pitch<PAIR>(K);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   floatx4 acc[Cfg::WB][Cfg::XB];
 #pragma unroll
   for (int u = 0; u < Cfg::WB; ++u)
 #pragma unroll
     for (int v = 0; v < Cfg::XB; ++v) acc[u][v] = (floatx4){};
-  // Rows past the matrix read its last one; what comes of them is not written.
-  const auto rows = [&](const char* from, int r0, int count) {
-    return [=](int gr, int k0, int j, uint32_t& voff, const DmaLane& dl) -> const void* {
-      const int base = r0 + gr < count ? r0 + gr : count - 1;
-      const int r = r0 + gr + dl.lrow < count ? r0 + gr + dl.lrow : count - 1;
-      voff = (uint32_t)((r - base) * rp) + dl.cb(j);
-      return from + base * rp + (int64_t)k0 * 2;
-    };
-  };
-  tile_kloop_cfg<Cfg, _Float16, PAIR>(PAIR ? 2 * K : K, lds, acc, rows(W, w0, wn), rows(X, x0, xn));
-
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wr = w0 + wave / Cfg::NW_X * (S / Cfg::NW_W) + 4 * (lane >> 4);
-  const int xr = x0 + wave % Cfg::NW_X * (S / Cfg::NW_X) + (lane & 15);
-  const int64_t mpitch = pitch<PAIR>(g.mp);
+  // Sums of the workgroups that share a tile: [share][register][thread].
+  floatx4* sums = nullptr;
+  if constexpr (STAGE == GRAM || STAGE == JOIN)
+    sums = (floatx4*)(a.ws + g.shares) +
+           (((int64_t)i * symmetric_tiles<S>(g) + tile) * g.splits + share) * (S * S / 4) + tid;
+  if constexpr (STAGE == JOIN) {
+    for (int s = 0; s < g.splits; ++s)
 #pragma unroll
-  for (int u = 0; u < Cfg::WB; ++u)
+      for (int u = 0; u < Cfg::WB; ++u)
 #pragma unroll
-    for (int v = 0; v < Cfg::XB; ++v) {
-      const int w = wr + 16 * u, x = xr + 16 * v;
-      if (x >= xn) continue;
-      float y[4], old[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) y[c] = acc[u][v][c] * (1.f / kScale);
-      if constexpr (STAGE == GRAM || STAGE == POLY) {
-        if (w >= g.mp) continue;
-        char* to = ws + at_a<PAIR>(g, STAGE == POLY);
-        if constexpr (STAGE == POLY) get4<PAIR>(ws + at_a<PAIR>(g, 0) + x * mpitch, w, old);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if constexpr (STAGE == POLY) y[c] = fmaf(a.c, y[c], a.b * old[c]);
-          if (w + c >= wn) y[c] = 0.f;
-        }
-        put4<PAIR>(to + x * mpitch, w, y);
-        if (w0 != x0) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (w + c < wn) put<PAIR>(to + (w + c) * mpitch, x, y[c]);
-        }
-      } else if constexpr (STAGE == APPLY) {
-        if (w >= g.mp) continue;
-        get4<PAIR>(ws + at_xt<PAIR>(g, a.flip) + x * mpitch, w, old, second_piece<PAIR>(g));
-#pragma unroll
-        for (int c = 0; c < 4; ++c) y[c] = w + c < wn ? fmaf(a.a, old[c], y[c]) : 0.f;
-        put4<PAIR>(ws + at_xt<PAIR>(g, a.flip ^ 1) + x * mpitch, w, y, second_piece<PAIR>(g));
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (w + c < wn) put<PAIR>(ws + (w + c) * pitch<PAIR>(g.np), x, y[c]);
-      } else {
-        if (w >= wn) continue;
-        const char* from = ws + at_xt<PAIR>(g, a.flip);
-        if (turned) {
-          const char* at = from + 2 * (PAIR ? x / 32 * 64 + x % 32 : x);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const _Float16* one = (const _Float16*)(at + (w + c < wn ? w + c : w) * mpitch);
-            old[c] = (float)one[0] + (float)one[second_piece<PAIR>(g) / 2];
-          }
-        } else {
-          get4<PAIR>(from + x * mpitch, w, old, second_piece<PAIR>(g));
-        }
-        T* to = target<T>(a, g, i) + (int64_t)x * g.cols;
-        const int most = wn - w;
-        float p[4];
-        if constexpr (MUON) load_part((const T*)to, w, most, p);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          y[c] = fmaf(a.a, old[c], y[c]) * (1.f / kScale);
-          if constexpr (MUON) y[c] = fmaf(-g.rate, y[c], p[c] * a.decay);
-        }
-        store_part(to, w, most, y);
-      }
+        for (int v = 0; v < Cfg::XB; ++v)
+          acc[u][v] += sums[(int64_t)s * (S * S / 4) + (u * Cfg::XB + v) * Cfg::kThreads];
+  } else {
+    if constexpr (STAGE == GRAM) {
+      const int steps = K / 64, each = ceil_div(steps, g.splits);
+      k0 = share * each * 64;
+      K = each * 64 < K - k0 ? each * 64 : K - k0;
     }
+    // Rows past the matrix read its last one; what comes of them is not written.
+    const auto rows = [&](const char* from, int r0, int count) {
+      from += (int64_t)k0 * (PAIR ? 4 : 2);
+      return [=](int gr, int k, int j, uint32_t& voff, const DmaLane& dl) -> const void* {
+        const int base = r0 + gr < count ? r0 + gr : count - 1;
+        const int r = r0 + gr + dl.lrow < count ? r0 + gr + dl.lrow : count - 1;
+        voff = (uint32_t)((r - base) * rp) + dl.cb(j);
+        return from + base * rp + (int64_t)k * 2;
+      };
+    };
+    if (K > 0) tile_kloop_cfg<Cfg, _Float16, PAIR>(PAIR ? 2 * K : K, lds, acc, rows(W, w0, wn), rows(X, x0, xn));
+  }
+  if (STAGE == GRAM && g.splits > 1) {
+#pragma unroll
+    for (int u = 0; u < Cfg::WB; ++u)
+#pragma unroll
+      for (int v = 0; v < Cfg::XB; ++v) sums[(u * Cfg::XB + v) * Cfg::kThreads] = acc[u][v];
+    return;
+  }
+
+  float(*y)[P] = (float(*)[P])lds;  // [x][w]
+  const int64_t mpitch = pitch<PAIR>(g.mp), npitch = pitch<PAIR>(g.np), second = second_piece<PAIR>(g);
+  const bool tall = g.rows > g.cols;
+  char* xt = ws + at_xt<PAIR>(g, a.flip);
+#pragma unroll
+  for (int pass = 0; pass < Cfg::NW_X; ++pass) {
+    const int xb = x0 + pass * XW;
+    __syncthreads();  // the last stage, or the pass before, has been read
+    if (wave % Cfg::NW_X == pass) {
+#pragma unroll
+      for (int u = 0; u < Cfg::WB; ++u)
+#pragma unroll
+        for (int v = 0; v < Cfg::XB; ++v)
+          *(floatx4*)&y[16 * v + (lane & 15)][wave / Cfg::NW_X * (S / Cfg::NW_W) + 16 * u + 4 * (lane >> 4)] =
+              acc[u][v] * (1.f / kScale);
+    }
+    __syncthreads();
+    for (int at = tid; at < XW * (S / 8); at += Cfg::kThreads) {
+      const int xl = at / (S / 8), wl = at % (S / 8) * 8, x = xb + xl, w = w0 + wl;
+      if (w >= g.mp) continue;
+      float v[8], old[8];
+      load_vec<float, 8>(&y[xl][wl], v);
+      if (x < xn) {
+        if constexpr (STAGE == POLY) {
+          get8<PAIR>(ws + at_a<PAIR>(g, 0) + x * mpitch, w, old);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) v[c] = fmaf(a.c, v[c], a.b * old[c]);
+        }
+        if constexpr (!SYMMETRIC) {
+          get8<PAIR>(xt + x * mpitch, w, old, second);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) v[c] = fmaf(a.a, old[c], v[c]);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 8; ++c) v[c] = w + c < wn && x < xn ? v[c] : 0.f;
+      store_vec<float, 8>(&y[xl][wl], v);
+      if (x >= xn) continue;
+      if constexpr (SYMMETRIC) put8<PAIR>(ws + at_a<PAIR>(g, STAGE == POLY) + x * mpitch, w, v);
+      else if constexpr (STAGE == APPLY) put8<PAIR>(ws + at_xt<PAIR>(g, a.flip ^ 1) + x * mpitch, w, v, second);
+      else if (tall && w < wn)
+        put_result<T, MUON>(target<T>(a, g, i) + (int64_t)x * g.cols + w, wn - w, v, a.decay, g.rate);
+    }
+    if (SYMMETRIC ? w0 == x0 : STAGE == LAST && tall) continue;
+    __syncthreads();
+    for (int at = tid; at < S * (XW / 8); at += Cfg::kThreads) {
+      const int wl = at / (XW / 8), xl = at % (XW / 8) * 8, w = w0 + wl, x = xb + xl;
+      if (w >= wn || x >= (STAGE == LAST ? xn : SYMMETRIC ? g.mp : g.np)) continue;
+      float v[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) v[c] = y[xl + c][wl];
+      if constexpr (SYMMETRIC) put8<PAIR>(ws + at_a<PAIR>(g, STAGE == POLY) + w * mpitch, x, v);
+      else if constexpr (STAGE == APPLY) put8<PAIR>(ws + w * npitch, x, v);
+      else put_result<T, MUON>(target<T>(a, g, i) + (int64_t)w * g.cols + x, xn - x, v, a.decay, g.rate);
+    }
+  }
 }
 
 }  // namespace ortho
@@ -383,9 +440,30 @@ Group group_of(int64_t rows, int64_t cols) {
   g.sums = (int)std::min(parts, ortho::kMaxParts);
   return g;
 }
-// Where the groups' buffers and sums lie; returns the workspace's bytes.
+using Tile64 = mfma::TileCfg<64, 64, 2, 2>;
+using Tile128 = mfma::TileCfg<128, 128, 2, 2>;
+using mfma::Tile256;
+
+template <typename Count>
+int64_t total(const Args& a, const Count& count) {
+  int64_t n = 0;
+  for (int i = 0; i < a.count; ++i) n += (int64_t)a.groups[i].count * count(a.groups[i]);
+  return n;
+}
+// The side of a launch's tiles. Of 256 rows by 256 the products run at twice the rate of 128 by 128 (a byte
+// brought to LDS serves twice as many), but a CU holds one such tile, and fewer than three in four CUs with
+// one lose that; of fewer than 128 tiles of 128, four times as many of 64.
+template <int STAGE>
+int tile_side(const Args& a) {
+  if (total(a, ortho::tile_count<STAGE, 256>) >= 192) return 256;
+  return total(a, ortho::tile_count<STAGE, 128>) >= 128 ? 128 : 64;
+}
+
+// Where the groups' buffers and sums lie; returns the workspace's bytes. Long sides are shared among
+// workgroups in the first product where its tiles alone would not fill the card (512 of 128 by 128), in
+// shares of at least 512 columns; and of at most 8192, beyond which an fp32 sum loses more than its operands.
 int64_t lay_out(Args& a, bool pair) {
-  int64_t bytes = 0, parts = 0;
+  int64_t bytes = 0, parts = 0, steps = 0;
   for (int i = 0; i < a.count; ++i) {
     Group& g = a.groups[i];
     g.each = pair ? ortho::matrix_bytes<true>(g) : ortho::matrix_bytes<false>(g);
@@ -393,6 +471,25 @@ int64_t lay_out(Args& a, bool pair) {
     bytes += g.each * g.count;
     g.parts = parts;
     parts += (int64_t)g.count * g.sums;
+    g.splits = 1;
+  }
+  a.side = tile_side<ortho::POLY>(a);
+  const int64_t slots = a.side == 256 ? 256 : a.side == 128 ? 512 : 1024;
+  const auto tiles = [&](const Group& g) -> int64_t {
+    return a.side == 256   ? ortho::symmetric_tiles<256>(g)
+           : a.side == 128 ? ortho::symmetric_tiles<128>(g)
+                           : ortho::symmetric_tiles<64>(g);
+  };
+  steps = total(a, [&](const Group& g) { return tiles(g) * (g.np / 64); });
+  const int64_t least = std::max<int64_t>(8, (steps + slots - 1) / slots);
+  for (int i = 0; i < a.count; ++i) {
+    Group& g = a.groups[i];
+    const int64_t have = g.np / 64;
+    const int64_t want = std::max(have / least, (have + 127) / 128);
+    const int64_t each = (have + want - 1) / std::max<int64_t>(want, 1);
+    g.splits = (int)((have + each - 1) / each);  // none without columns
+    g.shares = bytes;
+    if (g.splits > 1) bytes += g.count * tiles(g) * g.splits * a.side * a.side * 4;
   }
   a.sums = (double*)bytes;  // (an offset until the workspace is known)
   return bytes + (parts * 8 + 255) / 256 * 256;
@@ -410,35 +507,56 @@ int64_t number(Args& a, const Each& each, int64_t threads) {
   return n;
 }
 
+constexpr int kMaxDevices = 64;
 template <typename T, typename Cfg, bool PAIR, int STAGE, bool MUON>
-int launch_product(Args& a, hipStream_t s) {
+int launch_tiles(Args& a, hipStream_t s) {
   const int64_t n = number(a, ortho::tile_count<STAGE, Cfg::TW>, Cfg::kThreads);
   if (n < 0) return MQC_E_LIMIT;
-  ortho::ortho_product_kernel<T, Cfg, PAIR, STAGE, MUON>
-      <<<dim3((unsigned)n), dim3(Cfg::kThreads), Cfg::kStagesBytes, s>>>(a);
+  if (n == 0) return MQC_OK;
+  const auto kernel = ortho::ortho_product_kernel<T, Cfg, PAIR, STAGE, MUON>;
+  if (Cfg::kStagesBytes > 65536) {  // has to be asked for, once on each device
+    static bool done[kMaxDevices] = {};
+    int device = -1;
+    hipError_t e = hipGetDevice(&device);
+    if (e != hipSuccess) return (int)e;
+    if (device < 0 || device >= kMaxDevices) return MQC_E_LIMIT;
+    if (!done[device]) {
+      e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+                              Cfg::kStagesBytes);
+      if (e != hipSuccess) return (int)e;
+      done[device] = true;
+    }
+  }
+  kernel<<<dim3((unsigned)n), dim3(Cfg::kThreads), Cfg::kStagesBytes, s>>>(a);
   return launch_status();
 }
+template <typename T, bool PAIR, int STAGE, bool MUON>
+int launch_product(Args& a, hipStream_t s) {
+  // (the first product's tiles are those that its shares were laid out for)
+  const int side = STAGE == ortho::GRAM || STAGE == ortho::JOIN ? a.side : tile_side<STAGE>(a);
+  if (side == 256) return launch_tiles<T, Tile256, PAIR, STAGE, MUON>(a, s);
+  if (side == 128) return launch_tiles<T, Tile128, PAIR, STAGE, MUON>(a, s);
+  return launch_tiles<T, Tile64, PAIR, STAGE, MUON>(a, s);
+}
 
-template <typename T, typename Cfg, bool PAIR, bool MUON>
+template <typename T, bool PAIR, bool MUON>
 int iterate(Args& a, int steps, hipStream_t s) {
   int st = MQC_OK;
   a.flip = 0;
   for (int i = 0; i < steps && st == MQC_OK; ++i) {
-    st = launch_product<float, Cfg, PAIR, ortho::GRAM, false>(a, s);
-    if (st == MQC_OK) st = launch_product<float, Cfg, PAIR, ortho::POLY, false>(a, s);
+    st = launch_product<float, PAIR, ortho::GRAM, false>(a, s);
+    if (st == MQC_OK) st = launch_product<float, PAIR, ortho::JOIN, false>(a, s);
+    if (st == MQC_OK) st = launch_product<float, PAIR, ortho::POLY, false>(a, s);
     if (st != MQC_OK) break;
     if (i + 1 < steps) {
-      st = launch_product<float, Cfg, PAIR, ortho::APPLY, false>(a, s);
+      st = launch_product<float, PAIR, ortho::APPLY, false>(a, s);
       a.flip ^= 1;
     } else {
-      st = launch_product<T, Cfg, PAIR, ortho::LAST, MUON>(a, s);
+      st = launch_product<T, PAIR, ortho::LAST, MUON>(a, s);
     }
   }
   return st;
 }
-
-using Small = mfma::TileCfg<64, 64, 2, 2>;
-using Large = mfma::TileCfg<128, 128, 2, 2>;
 
 bool paired(int dtype, int64_t rows, int64_t cols) {
   return dtype != MQC_BF16 || std::min(rows, cols) < ortho::kOnePiece;
@@ -458,8 +576,7 @@ int run_pieces(Args& a, int steps, char* ws, hipStream_t s) {
   ortho::ortho_init_kernel<T, PAIR, MUON><<<dim3((unsigned)n), dim3(256), 0, s>>>(a);
   st = launch_status();
   if (st != MQC_OK) return st;
-  const int64_t large = number(a, ortho::tile_count<ortho::GRAM, Large::TW>, Large::kThreads);
-  return large >= 128 ? iterate<T, Large, PAIR, MUON>(a, steps, s) : iterate<T, Small, PAIR, MUON>(a, steps, s);
+  return iterate<T, PAIR, MUON>(a, steps, s);
 }
 template <bool MUON>
 int run(Args& a, int dtype, int steps, char* ws, hipStream_t s) {
