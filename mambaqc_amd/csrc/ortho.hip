@@ -19,6 +19,7 @@
 // of eight strong directions comes out off by 3e-4 of it, without that piece by 0.04, iterated in bf16 by
 // 0.3; gradients with a sixteenth of strong directions by 8e-4).
 #include <algorithm>
+#include <climits>
 #include <vector>
 
 #include "mfma_tile.hpp"
@@ -82,16 +83,20 @@ __host__ __device__ inline int64_t matrix_bytes(const Group& g) {
   return (at_a<PAIR>(g, 2) + 255) / 256 * 256;
 }
 
-// The workgroup's group, the matrix in it and what is left of its number, `each` workgroups to a matrix.
+// The workgroup's group, the matrix in it and what is left of its number, `each` workgroups to a matrix;
+// null for those that fill a group's last eight. An eighth of each group's go to an XCD, consecutive ones:
+// tiles of one matrix share its rows in L2, and every XCD gets as much of the long shapes as of the short
+// ones (in eighths of the whole launch, the longest of four shapes lay on one: 133 us for 80).
 template <typename Each>
-__device__ inline const Group& find(const Args& a, int64_t block, const Each& each, int& matrix, int& left) {
+__device__ inline const Group* find(const Args& a, const Each& each, int& matrix, int& left) {
+  const int at = blockIdx.x / kXCDs, xcd = blockIdx.x % kXCDs;
   int i = 0;
-  while (i + 1 < a.count && block >= a.groups[i + 1].tiles) ++i;
+  while (i + 1 < a.count && at >= a.groups[i + 1].tiles) ++i;
   const Group& g = a.groups[i];
-  const int n = each(g), rest = (int)block - g.tiles;
+  const int n = each(g), rest = xcd * ((n * g.count + kXCDs - 1) / kXCDs) + at - g.tiles;
   matrix = rest / n;
   left = rest % n;
-  return g;
+  return matrix < g.count && at - g.tiles < (n * g.count + kXCDs - 1) / kXCDs ? &g : nullptr;
 }
 template <typename T>
 __device__ inline const T* source(const Args& a, const Group& g, int i) {
@@ -113,7 +118,9 @@ template <typename T, bool MUON>
 __global__ __launch_bounds__(256) void ortho_sum_kernel(Args a) {
   __shared__ double red[4];
   int i, part;
-  const Group& g = find(a, blockIdx.x, [](const Group& g) { return g.sums; }, i, part);
+  const Group* group = find(a, [](const Group& g) { return g.sums; }, i, part);
+  if (!group) return;
+  const Group& g = *group;
   const int64_t n = (int64_t)g.rows * g.cols;
   const T* from = source<T>(a, g, i);
   float* mom = MUON ? a.matrices[g.first + i].m : nullptr;
@@ -172,8 +179,10 @@ __global__ __launch_bounds__(256) void ortho_init_kernel(Args a) {
   __shared__ float tile[64][65];
   __shared__ double total;
   int i, left;
-  const Group& g = find(a, blockIdx.x,
-                        [](const Group& g) { return ceil_div(g.rows, 64) * ceil_div(g.cols, 64); }, i, left);
+  const Group* group =
+      find(a, [](const Group& g) { return ceil_div(g.rows, 64) * ceil_div(g.cols, 64); }, i, left);
+  if (!group) return;
+  const Group& g = *group;
   if (threadIdx.x < 64) {
     double s = 0.0;
     for (int k = threadIdx.x; k < g.sums; k += 64) s += a.sums[g.parts + (int64_t)i * g.sums + k];
@@ -226,7 +235,7 @@ __host__ __device__ inline int symmetric_tiles(const Group& g) {
 template <int STAGE, int S>
 __host__ __device__ inline int tile_count(const Group& g) {
   if (STAGE == GRAM) return symmetric_tiles<S>(g) * g.splits;
-  if (STAGE == JOIN) return g.splits > 1 ? symmetric_tiles<S>(g) : 0;
+  if (STAGE == JOIN) return g.splits > 1 ? symmetric_tiles<64>(g) : 0;
   if (STAGE == POLY) return symmetric_tiles<S>(g);
   return ceil_div(g.m, S) * ceil_div(g.n, S);
 }
@@ -245,16 +254,17 @@ __device__ inline void put8(char* row, int col, const float (&v)[8], int64_t sec
   *(u32x4*)to = hi;
   if (second) *(u32x4*)(to + second) = lo;
 }
+// Eight values of a row, col a multiple of 8, and their sums.
 template <bool PAIR>
-__device__ inline void get8(const char* row, int col, float (&v)[8], int64_t second = PAIR ? 64 : 0) {
+__device__ inline void load8(const char* row, int col, u32x4 (&v)[2], int64_t second = PAIR ? 64 : 0) {
   const char* from = row + 2 * (PAIR ? col / 32 * 64 + col % 32 : col);
-  const u32x4 hi = *(const u32x4*)from;
-  u32x4 lo = {};
-  if (second) lo = *(const u32x4*)(from + second);
-#pragma unroll
-  for (int c = 0; c < 8; ++c)
-    v[c] = io<f16_t>::bits_to_f32(c & 1 ? hi[c / 2] >> 16 : hi[c / 2] & 0xffffu) +
-           io<f16_t>::bits_to_f32(c & 1 ? lo[c / 2] >> 16 : lo[c / 2] & 0xffffu);
+  v[0] = *(const u32x4*)from;
+  v[1] = second ? *(const u32x4*)(from + second) : u32x4{0u, 0u, 0u, 0u};
+}
+__device__ inline float joined(const u32x4 (&v)[2], int c) {
+  const uint32_t hi = v[0][c / 2], lo = v[1][c / 2];
+  return io<f16_t>::bits_to_f32(c & 1 ? hi >> 16 : hi & 0xffffu) +
+         io<f16_t>::bits_to_f32(c & 1 ? lo >> 16 : lo & 0xffffu);
 }
 // Eight elements of a matrix's row (its parameter's update where MUON).
 template <typename T, bool MUON>
@@ -278,15 +288,15 @@ __device__ inline void put_result(T* to, int left, float (&v)[8], float decay, f
 // product, X by rows, a wide matrix) rows of w along x, 16 bytes a lane. Written from the registers, two
 // bytes a lane, they took longer than the products: 75 us of 12 matrices of 768 x 1536 for the last one.
 template <typename T, typename Cfg, bool PAIR, int STAGE, bool MUON>
-__global__ __launch_bounds__(Cfg::kThreads) void ortho_product_kernel(Args a) {
+__global__ __launch_bounds__(Cfg::kThreads, 2) void ortho_product_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   constexpr int S = Cfg::TW, XW = S / Cfg::NW_X, P = S + 4;
   static_assert(Cfg::TW == Cfg::TX && XW * P * 4 <= Cfg::kStagesBytes, "square tiles, a wave's columns in LDS");
   constexpr bool SYMMETRIC = STAGE == GRAM || STAGE == JOIN || STAGE == POLY;
-  const int64_t n = gridDim.x, lin = blockIdx.x;
-  const int64_t block = n % kXCDs ? lin : (lin % kXCDs) * (n / kXCDs) + lin / kXCDs;
   int i, left;
-  const Group& g = find(a, block, [](const Group& g) { return tile_count<STAGE, S>(g); }, i, left);
+  const Group* group = find(a, [](const Group& g) { return tile_count<STAGE, S>(g); }, i, left);
+  if (!group) return;
+  const Group& g = *group;
   char* ws = a.ws + g.base + i * g.each;
   int w0, x0, tile = 0, share = 0, k0 = 0;
   const char *W, *X;
@@ -313,18 +323,21 @@ __global__ __launch_bounds__(Cfg::kThreads) void ortho_product_kernel(Args a) {
   for (int u = 0; u < Cfg::WB; ++u)
 #pragma unroll
     for (int v = 0; v < Cfg::XB; ++v) acc[u][v] = (floatx4){};
-  // Sums of the workgroups that share a tile: [share][register][thread].
-  floatx4* sums = nullptr;
-  if constexpr (STAGE == GRAM || STAGE == JOIN)
-    sums = (floatx4*)(a.ws + g.shares) +
-           (((int64_t)i * symmetric_tiles<S>(g) + tile) * g.splits + share) * (S * S / 4) + tid;
+  // Where the lane's sums lie in the tile.
+  const int wl = wave / Cfg::NW_X * (S / Cfg::NW_W) + 4 * (lane >> 4);
+  const int xl = wave % Cfg::NW_X * XW + (lane & 15);
+  // The sums of the workgroups that share a tile: [tile][share][x][w].
   if constexpr (STAGE == JOIN) {
-    for (int s = 0; s < g.splits; ++s)
+    const int tw = w0 / a.side, tx = x0 / a.side, down = ceil_div(g.m, a.side);
+    const int64_t each = (int64_t)a.side * a.side;
+    const float* from = (const float*)(a.ws + g.shares) +
+                        ((int64_t)i * (down * (down + 1) / 2) + tw * (tw + 1) / 2 + tx) * g.splits * each +
+                        (int64_t)(x0 % a.side + xl) * a.side + w0 % a.side + wl;
+    for (int s = 0; s < g.splits; ++s, from += each)
 #pragma unroll
       for (int u = 0; u < Cfg::WB; ++u)
 #pragma unroll
-        for (int v = 0; v < Cfg::XB; ++v)
-          acc[u][v] += sums[(int64_t)s * (S * S / 4) + (u * Cfg::XB + v) * Cfg::kThreads];
+        for (int v = 0; v < Cfg::XB; ++v) acc[u][v] += *(const floatx4*)(from + 16 * v * a.side + 16 * u);
   } else {
     if constexpr (STAGE == GRAM) {
       const int steps = K / 64, each = ceil_div(steps, g.splits);
@@ -343,51 +356,68 @@ __global__ __launch_bounds__(Cfg::kThreads) void ortho_product_kernel(Args a) {
     };
     if (K > 0) tile_kloop_cfg<Cfg, _Float16, PAIR>(PAIR ? 2 * K : K, lds, acc, rows(W, w0, wn), rows(X, x0, xn));
   }
+#pragma unroll
+  for (int u = 0; u < Cfg::WB; ++u)
+#pragma unroll
+    for (int v = 0; v < Cfg::XB; ++v) acc[u][v] *= STAGE == JOIN ? 1.f : 1.f / kScale;
   if (STAGE == GRAM && g.splits > 1) {
+    char* to = a.ws + g.shares +
+               (((int64_t)i * symmetric_tiles<S>(g) + tile) * g.splits + share) * (S * S * 4);
+    const uint32_t own = (uint32_t)(xl * S + wl) * 4;
 #pragma unroll
-    for (int u = 0; u < Cfg::WB; ++u)
+    for (int v = 0; v < Cfg::XB; ++v, to += 16 * S * 4)
 #pragma unroll
-      for (int v = 0; v < Cfg::XB; ++v) sums[(u * Cfg::XB + v) * Cfg::kThreads] = acc[u][v];
+      for (int u = 0; u < Cfg::WB; ++u) *(floatx4*)(to + own + 64 * u) = acc[u][v];
     return;
   }
 
-  float(*y)[P] = (float(*)[P])lds;  // [x][w]
+  // [x][w], the groups of eight columns in an order that both ways of reading find in distinct banks.
+  float(*y)[P] = (float(*)[P])lds;
+  const auto at8 = [](int x, int w) { return w ^ ((x >> 3 & 7) << 3); };
+  constexpr int ITEMS = XW * (S / 8) / Cfg::kThreads;
+  static_assert(XW * (S / 8) % Cfg::kThreads == 0, "whole items");
   const int64_t mpitch = pitch<PAIR>(g.mp), npitch = pitch<PAIR>(g.np), second = second_piece<PAIR>(g);
   const bool tall = g.rows > g.cols;
   char* xt = ws + at_xt<PAIR>(g, a.flip);
-#pragma unroll
+#pragma unroll 1
   for (int pass = 0; pass < Cfg::NW_X; ++pass) {
     const int xb = x0 + pass * XW;
+    u32x4 old[ITEMS][2];
+    if constexpr (STAGE == POLY || !SYMMETRIC) {
+#pragma unroll
+      for (int it = 0; it < ITEMS; ++it) {
+        const int at = tid + it * Cfg::kThreads, x = xb + at / (S / 8), w = w0 + at % (S / 8) * 8;
+        if (x >= xn || w >= g.mp) continue;
+        if constexpr (STAGE == POLY) load8<PAIR>(ws + at_a<PAIR>(g, 0) + x * mpitch, w, old[it]);
+        else load8<PAIR>(xt + x * mpitch, w, old[it], second);
+      }
+    }
     __syncthreads();  // the last stage, or the pass before, has been read
     if (wave % Cfg::NW_X == pass) {
 #pragma unroll
       for (int u = 0; u < Cfg::WB; ++u)
 #pragma unroll
-        for (int v = 0; v < Cfg::XB; ++v)
-          *(floatx4*)&y[16 * v + (lane & 15)][wave / Cfg::NW_X * (S / Cfg::NW_W) + 16 * u + 4 * (lane >> 4)] =
-              acc[u][v] * (1.f / kScale);
+        for (int v = 0; v < Cfg::XB; ++v) {
+          const int x = 16 * v + (lane & 15);
+          *(floatx4*)&y[x][at8(x, wl + 16 * u)] = acc[u][v];
+        }
     }
     __syncthreads();
-    for (int at = tid; at < XW * (S / 8); at += Cfg::kThreads) {
-      const int xl = at / (S / 8), wl = at % (S / 8) * 8, x = xb + xl, w = w0 + wl;
+#pragma unroll
+    for (int it = 0; it < ITEMS; ++it) {
+      const int at = tid + it * Cfg::kThreads, xr = at / (S / 8), wr = at % (S / 8) * 8;
+      const int x = xb + xr, w = w0 + wr;
       if (w >= g.mp) continue;
-      float v[8], old[8];
-      load_vec<float, 8>(&y[xl][wl], v);
-      if (x < xn) {
-        if constexpr (STAGE == POLY) {
-          get8<PAIR>(ws + at_a<PAIR>(g, 0) + x * mpitch, w, old);
+      float* from = &y[xr][at8(xr, wr)];
+      float v[8];
+      load_vec<float, 8>(from, v);
 #pragma unroll
-          for (int c = 0; c < 8; ++c) v[c] = fmaf(a.c, v[c], a.b * old[c]);
-        }
-        if constexpr (!SYMMETRIC) {
-          get8<PAIR>(xt + x * mpitch, w, old, second);
-#pragma unroll
-          for (int c = 0; c < 8; ++c) v[c] = fmaf(a.a, old[c], v[c]);
-        }
+      for (int c = 0; c < 8; ++c) {
+        if constexpr (STAGE == POLY) v[c] = fmaf(a.c, v[c], a.b * joined(old[it], c));
+        if constexpr (!SYMMETRIC) v[c] = fmaf(a.a, joined(old[it], c), v[c]);
+        v[c] = w + c < wn && x < xn ? v[c] : 0.f;
       }
-#pragma unroll
-      for (int c = 0; c < 8; ++c) v[c] = w + c < wn && x < xn ? v[c] : 0.f;
-      store_vec<float, 8>(&y[xl][wl], v);
+      if constexpr (STAGE == POLY || !SYMMETRIC) store_vec<float, 8>(from, v);
       if (x >= xn) continue;
       if constexpr (SYMMETRIC) put8<PAIR>(ws + at_a<PAIR>(g, STAGE == POLY) + x * mpitch, w, v);
       else if constexpr (STAGE == APPLY) put8<PAIR>(ws + at_xt<PAIR>(g, a.flip ^ 1) + x * mpitch, w, v, second);
@@ -396,12 +426,14 @@ __global__ __launch_bounds__(Cfg::kThreads) void ortho_product_kernel(Args a) {
     }
     if (SYMMETRIC ? w0 == x0 : STAGE == LAST && tall) continue;
     __syncthreads();
-    for (int at = tid; at < S * (XW / 8); at += Cfg::kThreads) {
-      const int wl = at / (XW / 8), xl = at % (XW / 8) * 8, w = w0 + wl, x = xb + xl;
+#pragma unroll
+    for (int it = 0; it < ITEMS; ++it) {
+      const int at = tid + it * Cfg::kThreads, wr = at / (XW / 8), xr = at % (XW / 8) * 8;
+      const int x = xb + xr, w = w0 + wr;
       if (w >= wn || x >= (STAGE == LAST ? xn : SYMMETRIC ? g.mp : g.np)) continue;
       float v[8];
 #pragma unroll
-      for (int c = 0; c < 8; ++c) v[c] = y[xl + c][wl];
+      for (int c = 0; c < 8; ++c) v[c] = x + c < xn ? y[xr + c][at8(xr, wr)] : 0.f;
       if constexpr (SYMMETRIC) put8<PAIR>(ws + at_a<PAIR>(g, STAGE == POLY) + w * mpitch, x, v);
       else if constexpr (STAGE == APPLY) put8<PAIR>(ws + w * npitch, x, v);
       else put_result<T, MUON>(target<T>(a, g, i) + (int64_t)w * g.cols + x, xn - x, v, a.decay, g.rate);
@@ -450,18 +482,19 @@ int64_t total(const Args& a, const Count& count) {
   for (int i = 0; i < a.count; ++i) n += (int64_t)a.groups[i].count * count(a.groups[i]);
   return n;
 }
-// The side of a launch's tiles. Of 256 rows by 256 the products run at twice the rate of 128 by 128 (a byte
-// brought to LDS serves twice as many), but a CU holds one such tile, and fewer than three in four CUs with
-// one lose that; of fewer than 128 tiles of 128, four times as many of 64.
+// The side of a launch's tiles. The last product's are of 256 rows by 256 where they fill the card (half the
+// bytes to LDS: with 8 bf16 matrices of 2048 x 2048 a call takes 1930 us for 2074 at 128; with two, of 128
+// such tiles, 772 for 653), the symmetric ones, of fewer and with half a tile lost on the diagonal, of 128
+// (all at 256: 2136); where fewer than 128 of these are left, of 64.
 template <int STAGE>
 int tile_side(const Args& a) {
-  if (total(a, ortho::tile_count<STAGE, 256>) >= 192) return 256;
+  if ((STAGE == ortho::APPLY || STAGE == ortho::LAST) && total(a, ortho::tile_count<STAGE, 256>) >= 256) return 256;
   return total(a, ortho::tile_count<STAGE, 128>) >= 128 ? 128 : 64;
 }
 
 // Where the groups' buffers and sums lie; returns the workspace's bytes. Long sides are shared among
 // workgroups in the first product where its tiles alone would not fill the card (512 of 128 by 128), in
-// shares of at least 512 columns; and of at most 8192, beyond which an fp32 sum loses more than its operands.
+// shares of about as many columns as a workgroup has on average, at least 512; and of at most 8192, beyond which an fp32 sum loses more than its operands.
 int64_t lay_out(Args& a, bool pair) {
   int64_t bytes = 0, parts = 0, steps = 0;
   for (int i = 0; i < a.count; ++i) {
@@ -474,20 +507,18 @@ int64_t lay_out(Args& a, bool pair) {
     g.splits = 1;
   }
   a.side = tile_side<ortho::POLY>(a);
-  const int64_t slots = a.side == 256 ? 256 : a.side == 128 ? 512 : 1024;
+  const int64_t slots = a.side == 128 ? 512 : 1024;
   const auto tiles = [&](const Group& g) -> int64_t {
-    return a.side == 256   ? ortho::symmetric_tiles<256>(g)
-           : a.side == 128 ? ortho::symmetric_tiles<128>(g)
-                           : ortho::symmetric_tiles<64>(g);
+    return a.side == 128 ? ortho::symmetric_tiles<128>(g) : ortho::symmetric_tiles<64>(g);
   };
   steps = total(a, [&](const Group& g) { return tiles(g) * (g.np / 64); });
   const int64_t least = std::max<int64_t>(8, (steps + slots - 1) / slots);
   for (int i = 0; i < a.count; ++i) {
     Group& g = a.groups[i];
     const int64_t have = g.np / 64;
-    const int64_t want = std::max(have / least, (have + 127) / 128);
-    const int64_t each = (have + want - 1) / std::max<int64_t>(want, 1);
-    g.splits = (int)((have + each - 1) / each);  // none without columns
+    const int64_t want = std::max((have + least - 1) / least, (have + 127) / 128);
+    const int64_t each = (have + want - 1) / want;
+    g.splits = (int)((have + each - 1) / each);
     g.shares = bytes;
     if (g.splits > 1) bytes += g.count * tiles(g) * g.splits * a.side * a.side * 4;
   }
@@ -495,16 +526,17 @@ int64_t lay_out(Args& a, bool pair) {
   return bytes + (parts * 8 + 255) / 256 * 256;
 }
 
-// Workgroups of a launch, of which `each` are one matrix's: where each group's begin. -1: too many.
+// Workgroups of a launch, of which `each` are one matrix's: where each group's begin in an XCD. -1: too many.
 template <typename Each>
 int64_t number(Args& a, const Each& each, int64_t threads) {
   int64_t n = 0;
   for (int i = 0; i < a.count; ++i) {
+    const int64_t of_group = (int64_t)a.groups[i].count * each(a.groups[i]);
     a.groups[i].tiles = (int)n;
-    n += (int64_t)a.groups[i].count * each(a.groups[i]);
-    if (!launchable(n, threads)) return -1;
+    n += (of_group + kXCDs - 1) / kXCDs;
+    if (of_group > INT_MAX - kXCDs || !launchable(n * kXCDs, threads)) return -1;
   }
-  return n;
+  return n * kXCDs;
 }
 
 constexpr int kMaxDevices = 64;
@@ -533,9 +565,11 @@ int launch_tiles(Args& a, hipStream_t s) {
 template <typename T, bool PAIR, int STAGE, bool MUON>
 int launch_product(Args& a, hipStream_t s) {
   // (the first product's tiles are those that its shares were laid out for)
-  const int side = STAGE == ortho::GRAM || STAGE == ortho::JOIN ? a.side : tile_side<STAGE>(a);
-  if (side == 256) return launch_tiles<T, Tile256, PAIR, STAGE, MUON>(a, s);
-  if (side == 128) return launch_tiles<T, Tile128, PAIR, STAGE, MUON>(a, s);
+  const int side = STAGE == ortho::GRAM ? a.side : STAGE == ortho::JOIN ? 64 : tile_side<STAGE>(a);
+  if constexpr (STAGE == ortho::APPLY || STAGE == ortho::LAST)
+    if (side == 256) return launch_tiles<T, Tile256, PAIR, STAGE, MUON>(a, s);
+  if constexpr (STAGE != ortho::JOIN)
+    if (side == 128) return launch_tiles<T, Tile128, PAIR, STAGE, MUON>(a, s);
   return launch_tiles<T, Tile64, PAIR, STAGE, MUON>(a, s);
 }
 
@@ -601,7 +635,8 @@ void batches(const int64_t* rows, int64_t count, float rate, std::vector<Batch>&
         order.push_back(i);
     std::stable_sort(order.begin(), order.end(), [&](int64_t x, int64_t y) {
       const int64_t *u = rows + 6 * x, *v = rows + 6 * y;
-      return u[3] != v[3] ? u[3] < v[3] : u[4] < v[4];
+      const int64_t a = std::max(u[3], u[4]), b = std::max(v[3], v[4]);  // long ones begin first
+      return a != b ? a > b : u[3] != v[3] ? u[3] < v[3] : u[4] < v[4];
     });
     size_t at = 0;
     while (at < order.size()) {
