@@ -202,7 +202,8 @@ int mqc_grad_norm(const int64_t* tensors, int64_t count, double max_norm, float*
  * v_heads, chunks, mqc_gated_delta_chunk(), value width]), v_t - p^T k_t; chunks =
  * ceil(seq_len / mqc_gated_delta_chunk()). Both and the workspace are 16-byte aligned.
  * MQC_E_LIMIT beyond k_dim 128, v_dim 2^20, seq_len 2^31, 2^26 heads in the batch, launches of 2^32 threads
- * (256 for each chunk of a head, or for 16 columns of v_dim) and 2^40 elements of q a value head.
+ * (256 for 16 columns of v_dim or for each chunk of a head, 1024 for these in the backward and the forward
+ * before one) and 2^40 elements of q a value head.
  *
  * Backward: gradients of q, k, v (dense), log_decay and beta (of their types) and of h0 (or NULL), from d_o
  * (dense) and dh_last (or NULL); batch and seq_len at least 1.

@@ -41,7 +41,7 @@ Space space(int64_t batch, int64_t seq, int64_t k_heads, int64_t v_heads, int64_
 }
 
 int shape(int64_t batch, int64_t seq, int64_t k_heads, int64_t v_heads, int64_t k_dim, int64_t v_dim,
-          int dtype, int g_type, int beta_type) {
+          int dtype, int g_type, int beta_type, bool backward) {
   if (batch < 0 || seq < 0 || k_heads < 1 || v_heads < 1 || k_dim < 1 || v_dim < 1 ||
       v_heads % k_heads)
     return MQC_E_SHAPE;
@@ -51,7 +51,7 @@ int shape(int64_t batch, int64_t seq, int64_t k_heads, int64_t v_heads, int64_t 
       seq > (1LL << 31))
     return MQC_E_LIMIT;
   const int64_t heads = batch * v_heads;  // at most 2^48; the rest below 2^63 once this is small
-  if (heads > (1 << 26) || !launchable(heads * chunk_count(seq), 256) ||
+  if (heads > (1 << 26) || !launchable(heads * chunk_count(seq), backward ? 1024 : 256) ||
       !launchable(heads * (value_width(v_dim) / 16), 256))
     return MQC_E_LIMIT;
   if (batch * seq > (1LL << 40) / (v_heads * k_dim)) return MQC_E_LIMIT;
@@ -102,7 +102,8 @@ extern "C" int64_t mqc_gated_delta_value_width(int64_t v_dim) {
 extern "C" int64_t mqc_gated_delta_workspace_bytes(int64_t batch, int64_t seq_len, int64_t k_heads,
                                                    int64_t v_heads, int64_t k_dim, int64_t v_dim,
                                                    int dtype, int backward) {
-  const int st = shape(batch, seq_len, k_heads, v_heads, k_dim, v_dim, dtype, MQC_F32, MQC_F32);
+  const int st = shape(batch, seq_len, k_heads, v_heads, k_dim, v_dim, dtype, MQC_F32, MQC_F32,
+                       backward != 0);
   if (st != MQC_OK) return st;
   return space(batch, seq_len, k_heads, v_heads, k_dim, v_dim, dtype, backward != 0).bytes;
 }
@@ -114,7 +115,8 @@ extern "C" int mqc_gated_delta_fwd(const void* q, const void* k, const void* v, 
                                    int64_t seq_len, int64_t k_heads, int64_t v_heads, int64_t k_dim,
                                    int64_t v_dim, float scale, int dtype, void* workspace,
                                    int64_t workspace_bytes, void* stream) {
-  const int st = shape(batch, seq_len, k_heads, v_heads, k_dim, v_dim, dtype, decay_dtype, beta_dtype);
+  const int st = shape(batch, seq_len, k_heads, v_heads, k_dim, v_dim, dtype, decay_dtype, beta_dtype,
+                       states || residuals);
   if (st != MQC_OK) return st;
   if (batch == 0) return MQC_OK;
   if (seq_len > 0 && (!q || !k || !v || !strides || !log_decay || !beta || !o || !workspace))
@@ -145,7 +147,7 @@ extern "C" int mqc_gated_delta_bwd(const void* q, const void* k, const void* v, 
                                    float* dh0, int64_t batch, int64_t seq_len, int64_t k_heads,
                                    int64_t v_heads, int64_t k_dim, int64_t v_dim, float scale,
                                    int dtype, void* workspace, int64_t workspace_bytes, void* stream) {
-  const int st = shape(batch, seq_len, k_heads, v_heads, k_dim, v_dim, dtype, decay_dtype, beta_dtype);
+  const int st = shape(batch, seq_len, k_heads, v_heads, k_dim, v_dim, dtype, decay_dtype, beta_dtype, true);
   if (st != MQC_OK) return st;
   if (batch < 1 || seq_len < 1) return MQC_E_SHAPE;
   if (!q || !k || !v || !strides || !log_decay || !beta || !states || !residuals || !d_o || !dq || !dk ||
@@ -177,7 +179,7 @@ extern "C" int mqc_gated_delta_step(const void* q, const void* k, const void* v,
                                     int beta_dtype, float* h, void* o, int64_t batch, int64_t k_heads,
                                     int64_t v_heads, int64_t k_dim, int64_t v_dim, float scale,
                                     int dtype, void* stream) {
-  const int st = shape(batch, 1, k_heads, v_heads, k_dim, v_dim, dtype, decay_dtype, beta_dtype);
+  const int st = shape(batch, 1, k_heads, v_heads, k_dim, v_dim, dtype, decay_dtype, beta_dtype, false);
   if (st != MQC_OK) return st;
   if (batch == 0) return MQC_OK;
   if (!q || !k || !v || !strides || !log_decay || !beta || !h || !o) return MQC_E_NULL;

@@ -402,7 +402,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Args<T> a) {
         const float gap = (float)(s.G[row] - Gc);
         const float D = expf(seen ? gap : -1e4f);  // else 0
         const float by = D * (BWD ? s.beta[row] : bc);
-        s.m[row][col] = seen & (col < row) ? by * kk[n][r] : 0.f;
+        s.m[row][col] = (seen & (col < row)) ? by * kk[n][r] : 0.f;
         P[n][r] = seen ? D * qk[n][r] : 0.f;
       }
     }

@@ -100,6 +100,10 @@ def test_validation_codes():
     assert fwd(t=(1 << 31) + 1) == -5 and fwd(b=1 << 10, t=1 << 31) == -5
     # 2^32 threads: chunks of a head, columns of 16.
     assert fwd(b=1, hk=1, hv=1, t=64 << 24, ptr=None) == -5 and fwd(b=1, hk=1, hv=1, t=63 << 24, ptr=None) == -1
+    # (in the backward, and in a forward that stores what it reads, four times as many for chunks)
+    assert bwd(b=1, hk=1, hv=1, t=64 << 22, ptr=None) == -5 and bwd(b=1, hk=1, hv=1, t=63 << 22, ptr=None) == -1
+    assert fwd(b=1, hk=1, hv=1, t=64 << 22, ptr=None, saved=FAKE) == -5
+    assert fwd(b=1, hk=1, hv=1, t=63 << 22, ptr=None, saved=FAKE) == -1
     assert step(b=1 << 20, hv=1, dv=256, ptr=None) == -5 and step(b=1 << 19, hv=1, dv=256, ptr=None) == -1
     size = lib.mqc_gated_delta_workspace_bytes
     assert size(-1, 1, 1, 1, 1, 1, 0, 0) == -2 and size(1, 1, 1, 1, 200, 1, 0, 0) == -5
