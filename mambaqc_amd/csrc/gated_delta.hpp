@@ -546,7 +546,7 @@ struct Walker {
 
   __device__ explicit Walker(const Args<T>& a_) : a(a_) {
     lane = threadIdx.x & 63;
-    w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
     g = lane >> 4, m = lane & 15;
     const int groups = (a.v_pad / 16 + CT - 1) / CT;
     const int64_t unit = xcd_order(blockIdx.x, gridDim.x);
@@ -844,6 +844,105 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, false>)) void delta_fwd
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) k.store_state(a.h_last, ct, S[ct]);
   }
+}
+
+// The same by eight waves, for workgroups that have a CU each: four take the state from chunk to chunk, and
+// four make the outputs beside them, their products with the state while the tokens' x is made, those with
+// what the tokens leave while the next state is. A chunk takes 1.95 us for 2.3 (96 workgroups, 128 keys,
+// bf16); where two workgroups share a CU, four waves each are faster (384 of them: 162 us for 181).
+template <typename T, int KD>
+__global__ __launch_bounds__(512, 2) void delta_fwd_beside_kernel(Args<T> a) {
+  __shared__ __attribute__((aligned(16))) WalkShared<KD, 1> s;
+  using K = Walker<T, KD, false, 1>;
+  const K k(a);
+  constexpr int NP = K::NP, KS = K::KS, MT = K::MT;
+  const auto ahead_of = [&](int64_t c) { return c + 1 < a.chunks ? c + 1 : c; };
+  RowGates next;
+  if (a.chunks > 0) next.load(k.vec, k.w, k.g);
+  if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 8)) {
+    bf16x8 qf[KS][NP], pf[2][kPieces];
+    const int64_t heads = a.v_heads * (int64_t)a.v_dim;
+    const TileRows<T> to(a.o + k.b * a.seq * heads + k.hv * a.v_dim, heads, k.w, k.g, k.col(0));
+    if (a.chunks > 0) {
+      k.load_rows(0, 2, qf);
+      load_tri<false>(k.tri + K::kTriPart, a.zeros, k.w, pf);
+    }
+    for (int64_t c = 0; c < a.chunks; ++c) {
+      const int64_t ahead = ahead_of(c);
+      const RowGates at = next;
+      const float* doc = k.vec + c * 4 * kC + 3 * kC;
+      lds_barrier();
+      next.load(k.vec + ahead * 4 * kC, k.w, k.g);
+      const floatx4 qs = k.row_product(qf, s.state[c & 1][0]);
+      k.load_rows(ahead, 2, qf);
+      lds_barrier();
+      lds_barrier();
+      floatx4 o;
+      if (at.first == at.last ||
+          !tri_apart<false>(s.bad[1], s.xs[1][0], k.tri + (2 * c + 1) * K::kTriPart, doc, k.w, o))
+        o = tri_product<kPieces>(pf, s.u[0]);
+      load_tri<false>(k.tri + (2 * ahead + 1) * K::kTriPart, a.zeros, k.w, pf);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = a.scale * (at.doc[i] == 0.f ? fmaf(at.e[i], qs[i], o[i]) : o[i]);
+      to.store(k, c, 0, o);
+    }
+    return;
+  }
+  floatx4 S[MT];
+  k.load_state(a.h0, 0, S);
+  k.put_state(s.state[0][0], S);
+  bf16x8 kf[KS][NP], tf[2][kPieces], cf[MT][2][NP];
+  T v[4];
+  const TileRows<const T> from(a.v + k.b * a.v_b + k.hv * a.v_h, a.v_t, k.w, k.g, k.col(0));
+  if (a.chunks > 0) {
+    k.load_rows(0, 0, kf);
+    from.load(k, 0, 0, v);
+    load_tri<false>(k.tri, a.zeros, k.w, tf);
+    k.load_cols(0, 1, cf);
+  }
+  for (int64_t c = 0; c < a.chunks; ++c) {
+    const int64_t ahead = ahead_of(c);
+    const RowGates at = next;
+    const float* doc = k.vec + c * 4 * kC + 3 * kC;
+    const bool mixed = at.first != at.last, cut = at.last != 0.f;
+    lds_barrier();
+    next.load(k.vec + ahead * 4 * kC, k.w, k.g);
+    floatx4 x = k.row_product(kf, s.state[c & 1][0]);
+    k.load_rows(ahead, 0, kf);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float vt = k.tile_value(v, c, 0, i);
+      x[i] = at.doc[i] == 0.f && k.here(c, i) ? fmaf(-at.e[i], x[i], vt) : vt;
+    }
+    put_tile<kPieces>(s.x[0], k.w, x);
+    if (mixed) k.mark(s.xs[0][0], s.bad[0], x);
+    lds_barrier();
+    from.load(k, ahead, 0, v);
+    floatx4 r, u, y;
+    if (!mixed || !tri_apart<false>(s.bad[0], s.xs[0][0], k.tri + 2 * c * K::kTriPart, doc, k.w, r))
+      r = tri_product<kPieces>(tf, s.x[0]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u[i] = r[i] * at.beta[i];
+      y[i] = at.doc[i] == at.last ? u[i] * at.end[i] : 0.f;
+    }
+    put_tile<kPieces>(s.u[0], k.w, u);
+    put_tile<kPieces>(s.y[0], k.w, y);
+    if (mixed) k.mark(s.xs[1][0], s.bad[1], u);
+    load_tri<false>(k.tri + 2 * ahead * K::kTriPart, a.zeros, k.w, tf);
+    if (mixed) k.cut_cols(cf, doc, at.last);
+    lds_barrier();
+    if (a.states) k.store_padded(a.states, c, 0, S);
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) S[t][i] = cut ? 0.f : S[t][i] * at.all;
+    k.col_product(cf, s.y[0], S);
+    k.put_state(s.state[(c + 1) & 1][0], S);
+    k.load_cols(ahead, 1, cf);
+    if (a.resid) k.store_rows(a.resid, c, 0, r);
+  }
+  if (a.h_last && k.holds) k.store_state(a.h_last, 0, S);
 }
 
 template <typename T, int KD, int CT>
