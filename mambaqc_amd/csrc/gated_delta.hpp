@@ -1056,6 +1056,128 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, true>)) void delta_bwd_
   }
 }
 
+// The same by eight waves (as forward): four take the state's gradient from chunk to chunk, and four bring them
+// what does not depend on it, P^T dO of the next chunk and Q^T (e dO) of this one.
+template <int KD>
+struct BesideShared {
+  floatx4 z[4][64], s[KD / 16 > 4 ? 2 : 1][4][64];  // as the chain's waves hold z and the state
+};
+template <typename T, int KD>
+__global__ __launch_bounds__(512, 2) void delta_bwd_beside_kernel(Args<T> a) {
+  __shared__ __attribute__((aligned(16))) WalkShared<KD, 1> s;
+  __shared__ BesideShared<KD> beside;
+  using K = Walker<T, KD, true, 1>;
+  const K k(a);
+  constexpr int NP = K::NP, KS = K::KS, MT = K::MT;
+  const int64_t heads = a.v_heads * (int64_t)a.v_dim, end = a.chunks - 1;
+  const int64_t first = k.b * a.seq * heads + k.hv * a.v_dim;
+  const auto ahead_of = [](int64_t c) { return c > 0 ? c - 1 : 0; };
+  if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 8)) {
+    const TileRows<const T> from(a.d_o + first, heads, k.w, k.g, k.col(0));
+    bf16x8 pf[2][kPieces], qf[MT][2][NP];
+    T raw[4];
+    RowGates at;
+    // dO of a chunk, and e dO, to LDS.
+    const auto put = [&](int64_t c) {
+      floatx4 v, x;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        v[r] = k.tile_value(raw, c, 0, r);
+        x[r] = at.doc[r] == 0.f ? v[r] * (a.scale * at.e[r]) : 0.f;
+      }
+      put_tile<NP>(s.d_o[0][0], k.w, v);
+      put_tile<kPieces>(s.u[0], k.w, x);
+      if (at.first != at.last) k.mark(s.xs[1][0], s.bad[1], v);
+    };
+    const auto make_z = [&](int64_t c) {
+      floatx4 z;
+      if (at.first == at.last || !tri_apart<true>(s.bad[1], s.xs[1][0], k.tri + (2 * c + 1) * K::kTriPart,
+                                                  k.vec + c * 4 * kC + 3 * kC, k.w, z))
+        z = tri_product<NP>(pf, s.d_o[0][0]);
+      beside.z[k.w][k.lane] = z;
+    };
+    at.load(k.vec + end * 4 * kC, k.w, k.g);
+    from.load(k, end, 0, raw);
+    load_tri<true>(k.tri + (2 * end + 1) * K::kTriPart, a.zeros, k.w, pf);
+    k.load_cols(end, 2, qf);
+    put(end);
+    lds_barrier();
+    make_z(end);
+    for (int64_t c = end; c >= 0; --c) {
+      const int64_t ahead = ahead_of(c);
+      from.load(k, ahead, 0, raw);
+      load_tri<true>(k.tri + (2 * ahead + 1) * K::kTriPart, a.zeros, k.w, pf);
+      if (at.last != 0.f) k.cut_cols(qf, k.vec + c * 4 * kC + 3 * kC, 0.f);
+      lds_barrier();
+      at.load(k.vec + ahead * 4 * kC, k.w, k.g);
+      floatx4 S[MT] = {};
+      k.col_product(qf, s.u[0], S);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) beside.s[t][k.w][k.lane] = S[t];
+      k.load_cols(ahead, 2, qf);
+      lds_barrier();
+      put(ahead);
+      lds_barrier();
+      make_z(ahead);
+    }
+    return;
+  }
+  const TileRows<T> to(a.dv + first, heads, k.w, k.g, k.col(0));
+  floatx4 S[MT];  // the gradient of the state after the chunk
+  k.load_state(a.dh_last, 0, S);
+  k.put_state(s.state[end & 1][0], S);
+  bf16x8 kf[KS][NP], tf[2][kPieces], cf[MT][2][NP];
+  RowGates next;
+  next.load(k.vec + end * 4 * kC, k.w, k.g);
+  k.load_rows(end, 0, kf);
+  load_tri<true>(k.tri + 2 * end * K::kTriPart, a.zeros, k.w, tf);
+  k.load_cols(end, 1, cf);
+  lds_barrier();
+  for (int64_t c = end; c >= 0; --c) {
+    const int64_t ahead = ahead_of(c);
+    const RowGates at = next;
+    const float* doc = k.vec + c * 4 * kC + 3 * kC;
+    const bool mixed = at.first != at.last, cut = at.last != 0.f;
+    if (cut) k.cut_cols(cf, doc, 0.f);
+    lds_barrier();
+    next.load(k.vec + ahead * 4 * kC, k.w, k.g);
+    const floatx4 ks = k.row_product(kf, s.state[c & 1][0]);
+    k.load_rows(ahead, 0, kf);
+    floatx4 z = beside.z[k.w][k.lane], y, v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      z[r] *= a.scale;
+      if (at.doc[r] == at.last) z[r] = fmaf(at.end[r], ks[r], z[r]);
+    }
+    put_tile<kPieces>(s.x[0], k.w, z);
+    if (mixed) k.mark(s.xs[0][0], s.bad[0], z);
+    lds_barrier();
+    k.store_padded(a.dstates, c, 0, S);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      const floatx4 q = beside.s[t][k.w][k.lane];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) S[t][r] = cut ? q[r] : fmaf(S[t][r], at.all, q[r]);
+    }
+    if (!mixed || !tri_apart<true>(s.bad[0], s.xs[0][0], k.tri + 2 * c * K::kTriPart, doc, k.w, z))
+      z = tri_product<kPieces>(tf, s.x[0]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      y[r] = at.beta[r] * z[r];
+      v[r] = at.doc[r] == 0.f ? -y[r] * at.e[r] : 0.f;
+    }
+    put_tile<kPieces>(s.y[0], k.w, v);
+    load_tri<true>(k.tri + 2 * ahead * K::kTriPart, a.zeros, k.w, tf);
+    lds_barrier();
+    k.col_product(cf, s.y[0], S);
+    k.put_state(s.state[(c + 1) & 1][0], S);
+    k.load_cols(ahead, 1, cf);
+    k.store_rows(a.z, c, 0, z);
+    to.store(k, c, 0, y);
+  }
+  if (a.dh0 && k.holds) k.store_state(a.dh0, 0, S);
+}
+
 // ---------------------------------------------------------------------------
 // The gradients of q, k, g and beta: a chunk of a value head to a workgroup of four waves, wave w the
 // columns 16 w.. of everything turned (tokens as columns). Operands pass through LDS 32 columns of v_dim

@@ -14,9 +14,11 @@ namespace delta {
 template <typename T, int KD, bool BWD>
 int launch_walk(const Args<T>& a, hipStream_t s) {
   const int64_t tiles = a.v_pad / 16, heads = a.batch * a.v_heads;
-  if constexpr (!BWD && (kIn<T> < 3 || KD < 128)) {  // (fp32's operands of 128 keys leave no registers for it)
+  if constexpr (kIn<T> < 3 || KD < 128) {  // (fp32's operands of 128 keys leave no registers for it)
     if (heads * tiles <= 256) {
-      delta_fwd_beside_kernel<T, KD><<<dim3((unsigned)(heads * tiles)), dim3(512), 0, s>>>(a);
+      const dim3 grid((unsigned)(heads * tiles));
+      if constexpr (BWD) delta_bwd_beside_kernel<T, KD><<<grid, dim3(512), 0, s>>>(a);
+      else delta_fwd_beside_kernel<T, KD><<<grid, dim3(512), 0, s>>>(a);
       return launch_status();
     }
   }
