@@ -449,7 +449,7 @@ struct WalkShared {
   uint16_t x[CT][2 * kPieces * kFrag], u[CT][2 * kPieces * kFrag], y[CT][2 * kPieces * kFrag];
   uint16_t d_o[2][CT][2 * kPieces * kFrag];     // (backward)
   float xs[2][CT][kC][16];                      // x and u in fp32 where documents meet
-  int bad[2][4];                                // whether a wave has some that are not finite
+  int bad[2][CT][4];                            // whether a wave has some that are not finite
 };
 
 // A barrier for what is in LDS; accesses to memory stay under way.
@@ -790,7 +790,7 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, false>)) void delta_fwd
         x[ct][r] = at.doc[r] == 0.f && k.here(c, r) ? fmaf(-at.e[r], x[ct][r], vt) : vt;
       }
       put_tile<kPieces>(s.x[ct], k.w, x[ct]);
-      if (mixed) k.mark(s.xs[0][ct], s.bad[0], x[ct]);
+      if (mixed) k.mark(s.xs[0][ct], s.bad[0][ct], x[ct]);
     }
     lds_barrier();
     k.load_rows(ahead, 2, qf);
@@ -798,7 +798,7 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, false>)) void delta_fwd
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
       from.load(k, ahead, ct, v[ct]);
-      if (!mixed || !tri_apart<false>(s.bad[0], s.xs[0][ct], tri, doc, k.w, r[ct]))
+      if (!mixed || !tri_apart<false>(s.bad[0][ct], s.xs[0][ct], tri, doc, k.w, r[ct]))
         r[ct] = tri_product<kPieces>(tf, s.x[ct]);
       floatx4 u, y;
 #pragma unroll
@@ -808,7 +808,7 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, false>)) void delta_fwd
       }
       put_tile<kPieces>(s.u[ct], k.w, u);
       put_tile<kPieces>(s.y[ct], k.w, y);
-      if (mixed) k.mark(s.xs[1][ct], s.bad[1], u);
+      if (mixed) k.mark(s.xs[1][ct], s.bad[1][ct], u);
     }
     load_tri<false>(tri_ahead, a.zeros, k.w, tf);
     if (mixed) k.cut_cols(cf, doc, at.last);
@@ -825,7 +825,7 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, false>)) void delta_fwd
 #pragma unroll
         for (int i = 0; i < 4; ++i) S[ct][t][i] = cut ? 0.f : S[ct][t][i] * at.all;
       k.col_product(cf, s.y[ct], S[ct]);
-      if (!mixed || !tri_apart<false>(s.bad[1], s.xs[1][ct], tri + K::kTriPart, doc, k.w, o[ct]))
+      if (!mixed || !tri_apart<false>(s.bad[1][ct], s.xs[1][ct], tri + K::kTriPart, doc, k.w, o[ct]))
         o[ct] = tri_product<kPieces>(pf, s.u[ct]);
       k.put_state(s.state[(c + 1) & 1][ct], S[ct]);
     }
@@ -879,7 +879,7 @@ __global__ __launch_bounds__(512, 2) void delta_fwd_beside_kernel(Args<T> a) {
       lds_barrier();
       floatx4 o;
       if (at.first == at.last ||
-          !tri_apart<false>(s.bad[1], s.xs[1][0], k.tri + (2 * c + 1) * K::kTriPart, doc, k.w, o))
+          !tri_apart<false>(s.bad[1][0], s.xs[1][0], k.tri + (2 * c + 1) * K::kTriPart, doc, k.w, o))
         o = tri_product<kPieces>(pf, s.u[0]);
       load_tri<false>(k.tri + (2 * ahead + 1) * K::kTriPart, a.zeros, k.w, pf);
 #pragma unroll
@@ -915,11 +915,11 @@ __global__ __launch_bounds__(512, 2) void delta_fwd_beside_kernel(Args<T> a) {
       x[i] = at.doc[i] == 0.f && k.here(c, i) ? fmaf(-at.e[i], x[i], vt) : vt;
     }
     put_tile<kPieces>(s.x[0], k.w, x);
-    if (mixed) k.mark(s.xs[0][0], s.bad[0], x);
+    if (mixed) k.mark(s.xs[0][0], s.bad[0][0], x);
     lds_barrier();
     from.load(k, ahead, 0, v);
     floatx4 r, u, y;
-    if (!mixed || !tri_apart<false>(s.bad[0], s.xs[0][0], k.tri + 2 * c * K::kTriPart, doc, k.w, r))
+    if (!mixed || !tri_apart<false>(s.bad[0][0], s.xs[0][0], k.tri + 2 * c * K::kTriPart, doc, k.w, r))
       r = tri_product<kPieces>(tf, s.x[0]);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -928,7 +928,7 @@ __global__ __launch_bounds__(512, 2) void delta_fwd_beside_kernel(Args<T> a) {
     }
     put_tile<kPieces>(s.u[0], k.w, u);
     put_tile<kPieces>(s.y[0], k.w, y);
-    if (mixed) k.mark(s.xs[1][0], s.bad[1], u);
+    if (mixed) k.mark(s.xs[1][0], s.bad[1][0], u);
     load_tri<false>(k.tri + 2 * ahead * K::kTriPart, a.zeros, k.w, tf);
     if (mixed) k.cut_cols(cf, doc, at.last);
     lds_barrier();
@@ -985,7 +985,7 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, true>)) void delta_bwd_
     const bool mixed = at.first != at.last, cut = at.last != 0.f;
     if (mixed) {
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) k.mark(s.xs[1][ct], s.bad[1], v[ct]);
+      for (int ct = 0; ct < CT; ++ct) k.mark(s.xs[1][ct], s.bad[1][ct], v[ct]);
     }
     if (cut) {
       k.cut_cols(qf, doc, 0.f);
@@ -998,7 +998,7 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, true>)) void delta_bwd_
     for (int ct = 0; ct < CT; ++ct) {
       from.load(k, ahead, ct, raw[ct]);
       y[ct] = k.row_product(kf, s.state[c & 1][ct]);
-      if (!mixed || !tri_apart<true>(s.bad[1], s.xs[1][ct], tri + K::kTriPart, doc, k.w, z[ct]))
+      if (!mixed || !tri_apart<true>(s.bad[1][ct], s.xs[1][ct], tri + K::kTriPart, doc, k.w, z[ct]))
         z[ct] = tri_product<NP>(pf, s.d_o[c & 1][ct]);
     }
     k.load_rows(ahead, 0, kf);
@@ -1014,7 +1014,7 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, true>)) void delta_bwd_
       }
       put_tile<kPieces>(s.x[ct], k.w, z[ct]);
       put_tile<kPieces>(s.u[ct], k.w, x);
-      if (mixed) k.mark(s.xs[0][ct], s.bad[0], z[ct]);
+      if (mixed) k.mark(s.xs[0][ct], s.bad[0][ct], z[ct]);
     }
     lds_barrier();
 #pragma unroll
@@ -1024,7 +1024,7 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, true>)) void delta_bwd_
       for (int t = 0; t < MT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) S[ct][t][r] = cut ? 0.f : S[ct][t][r] * at.all;
-      if (!mixed || !tri_apart<true>(s.bad[0], s.xs[0][ct], tri, doc, k.w, z[ct]))
+      if (!mixed || !tri_apart<true>(s.bad[0][ct], s.xs[0][ct], tri, doc, k.w, z[ct]))
         z[ct] = tri_product<kPieces>(tf, s.x[ct]);
       k.col_product(qf, s.u[ct], S[ct]);
 #pragma unroll
@@ -1087,11 +1087,11 @@ __global__ __launch_bounds__(512, 2) void delta_bwd_beside_kernel(Args<T> a) {
       }
       put_tile<NP>(s.d_o[0][0], k.w, v);
       put_tile<kPieces>(s.u[0], k.w, x);
-      if (at.first != at.last) k.mark(s.xs[1][0], s.bad[1], v);
+      if (at.first != at.last) k.mark(s.xs[1][0], s.bad[1][0], v);
     };
     const auto make_z = [&](int64_t c) {
       floatx4 z;
-      if (at.first == at.last || !tri_apart<true>(s.bad[1], s.xs[1][0], k.tri + (2 * c + 1) * K::kTriPart,
+      if (at.first == at.last || !tri_apart<true>(s.bad[1][0], s.xs[1][0], k.tri + (2 * c + 1) * K::kTriPart,
                                                   k.vec + c * 4 * kC + 3 * kC, k.w, z))
         z = tri_product<NP>(pf, s.d_o[0][0]);
       beside.z[k.w][k.lane] = z;
@@ -1150,7 +1150,7 @@ __global__ __launch_bounds__(512, 2) void delta_bwd_beside_kernel(Args<T> a) {
       if (at.doc[r] == at.last) z[r] = fmaf(at.end[r], ks[r], z[r]);
     }
     put_tile<kPieces>(s.x[0], k.w, z);
-    if (mixed) k.mark(s.xs[0][0], s.bad[0], z);
+    if (mixed) k.mark(s.xs[0][0], s.bad[0][0], z);
     lds_barrier();
     k.store_padded(a.dstates, c, 0, S);
 #pragma unroll
@@ -1159,7 +1159,7 @@ __global__ __launch_bounds__(512, 2) void delta_bwd_beside_kernel(Args<T> a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) S[t][r] = cut ? q[r] : fmaf(S[t][r], at.all, q[r]);
     }
-    if (!mixed || !tri_apart<true>(s.bad[0], s.xs[0][0], k.tri + 2 * c * K::kTriPart, doc, k.w, z))
+    if (!mixed || !tri_apart<true>(s.bad[0][0], s.xs[0][0], k.tri + 2 * c * K::kTriPart, doc, k.w, z))
       z = tri_product<kPieces>(tf, s.x[0]);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {

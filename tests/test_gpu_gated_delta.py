@@ -441,3 +441,27 @@ def test_many_tokens_past_32_bit_offsets():
     o1, h1 = gated_delta(*(x[:, t - tail:] for x in (q, k, v, g, beta)), return_state=True)
     hold("o", o[:, t - tail:], o1.double(), REL + torch.finfo(torch.bfloat16).eps)
     hold("h", h, h1.double(), REL)
+
+
+# Beyond 256 tiles of 16 columns two workgroups share a CU, beyond 512 one has two tiles.
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("batch", [4, 7])
+@pytest.mark.parametrize("dk", [20, 60, 128])
+def test_many_heads(dtype, batch, dk):
+    check(*make(batch, 150, 8, 16, dk, 70, dtype, reset=0.02))
+
+
+@pytest.mark.parametrize("batch", [70, 140])
+@pytest.mark.parametrize("what", range(5))
+def test_nan_stays_before_a_reset_with_many_heads(batch, what):
+    ops, _, do, dh = make(batch, 150, 1, 2, 40, 24, torch.float32)
+    cut = torch.zeros(batch, 150, dtype=torch.bool, device=DEV)
+    cut[:, 40] = True
+    good = gated_delta(*ops[:5], h0=ops[5], reset=cut, return_state=True)
+    ops[what][::3, 20, ..., 0] = float("nan")
+    leaves = [x.requires_grad_() for x in ops]
+    o, h = gated_delta(*leaves[:5], h0=leaves[5], reset=cut, return_state=True)
+    hold("o", o[:, 40:].detach(), good[0][:, 40:].double(), REL)
+    hold("h", h.detach(), good[1].double(), REL)
+    for v in torch.autograd.grad([o, h], leaves, [do, dh])[:5]:
+        assert v[:, 64:].isfinite().all() and v[1::3].isfinite().all()
