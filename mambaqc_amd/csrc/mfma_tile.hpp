@@ -273,7 +273,7 @@ __device__ inline void tile_issue_x(int kt, int slot, int wave, uint32_t lds0, c
   }
 }
 
-template <typename Cfg, int NSW, int NSX, typename E, typename WRow, typename XRow>
+template <typename Cfg, int NSW, int NSX, typename E, bool SPLIT = false, typename WRow, typename XRow>
 __device__ inline void tile_kloop_deep(int K, char* lds, floatx4 (&acc)[Cfg::WB][Cfg::XB],
                                        const WRow& wrow, const XRow& xrow) {
   static_assert(NSX == 2 || NSX == NSW, "the waits below");
@@ -333,13 +333,14 @@ __device__ inline void tile_kloop_deep(int K, char* lds, floatx4 (&acc)[Cfg::WB]
       for (int mb = 0; mb < XB; ++mb)
         xf[kk][mb] = *(const frag*)(xb + xoff[kk] + mb * 16 * kRowBytes);
     }
+    // (of rows in two pieces high by high, high by low and low by high, as above)
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
+    for (int kk = 0; kk < (SPLIT ? 3 : 2); ++kk)
 #pragma unroll
       for (int nb = 0; nb < WB; ++nb)
 #pragma unroll
         for (int mb = 0; mb < XB; ++mb)
-          acc[nb][mb] = mfma16(wf[kk][nb], xf[kk][mb], acc[nb][mb]);
+          acc[nb][mb] = mfma16(wf[SPLIT ? kk / 2 : kk][nb], xf[SPLIT ? kk % 2 : kk][mb], acc[nb][mb]);
     __builtin_amdgcn_sched_barrier(0);
   }
 }

@@ -31,7 +31,7 @@ using namespace mfma;
 
 constexpr int kMatrices = 64, kGroups = 16;  // of a launch
 constexpr float kScale = 256.f;
-constexpr int64_t kPartElems = 16384;        // elements that a workgroup adds the squares of
+constexpr int64_t kPartElems = 4096;        // elements that a workgroup adds the squares of
 constexpr int64_t kMaxParts = 256;
 constexpr int kOnePiece = 256;
 
@@ -240,6 +240,12 @@ __host__ __device__ inline int tile_count(const Group& g) {
   return ceil_div(g.m, S) * ceil_div(g.n, S);
 }
 
+// Stages in LDS. Launches of the smallest tiles have few of them on a CU to hide what a stage waits for (0.5 us
+// of two stages, each of 16 KB): there three are under way.
+constexpr int kSlots = 4;
+template <typename Cfg>
+constexpr int kLdsBytes = Cfg::TW == 64 ? kSlots * Cfg::kStageBytes : Cfg::kStagesBytes;
+
 // Eight values of a row, col a multiple of 8; second pieces as in put4.
 template <bool PAIR>
 __device__ inline void put8(char* row, int col, const float (&v)[8], int64_t second = PAIR ? 64 : 0) {
@@ -291,7 +297,7 @@ template <typename T, typename Cfg, bool PAIR, int STAGE, bool MUON>
 __global__ __launch_bounds__(Cfg::kThreads, 2) void ortho_product_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   constexpr int S = Cfg::TW, XW = S / Cfg::NW_X, P = S + 4;
-  static_assert(Cfg::TW == Cfg::TX && XW * P * 4 <= Cfg::kStagesBytes, "square tiles, a wave's columns in LDS");
+  static_assert(Cfg::TW == Cfg::TX && XW * P * 4 <= kLdsBytes<Cfg>, "square tiles, a wave's columns in LDS");
   constexpr bool SYMMETRIC = STAGE == GRAM || STAGE == JOIN || STAGE == POLY;
   int i, left;
   const Group* group = find(a, [](const Group& g) { return tile_count<STAGE, S>(g); }, i, left);
@@ -354,7 +360,20 @@ __global__ __launch_bounds__(Cfg::kThreads, 2) void ortho_product_kernel(Args a)
         return from + base * rp + (int64_t)k * 2;
       };
     };
-    if (K > 0) tile_kloop_cfg<Cfg, _Float16, PAIR>(PAIR ? 2 * K : K, lds, acc, rows(W, w0, wn), rows(X, x0, xn));
+    const int k2 = PAIR ? 2 * K : K;
+    const auto wrow = rows(W, w0, wn), xrow = rows(X, x0, xn);
+    if constexpr (S == 64) {
+      const DmaLane dl(lane);
+#pragma unroll
+      for (int kt = 0; kt < kSlots - 1; ++kt) {
+        if (kt * kBK >= k2) break;
+        tile_issue_w<Cfg, kSlots>(kt, kt, wave, lds_addr(lds), dl, wrow);
+        tile_issue_x<Cfg, kSlots>(kt, kt, wave, lds_addr(lds), dl, xrow);
+      }
+      tile_kloop_deep<Cfg, kSlots, kSlots, _Float16, PAIR>(k2, lds, acc, wrow, xrow);
+    } else {
+      tile_kloop_cfg<Cfg, _Float16, PAIR>(k2, lds, acc, wrow, xrow);
+    }
   }
 #pragma unroll
   for (int u = 0; u < Cfg::WB; ++u)
@@ -546,7 +565,7 @@ int launch_tiles(Args& a, hipStream_t s) {
   if (n < 0) return MQC_E_LIMIT;
   if (n == 0) return MQC_OK;
   const auto kernel = ortho::ortho_product_kernel<T, Cfg, PAIR, STAGE, MUON>;
-  if (Cfg::kStagesBytes > 65536) {  // has to be asked for, once on each device
+  if (ortho::kLdsBytes<Cfg> > 65536) {  // has to be asked for, once on each device
     static bool done[kMaxDevices] = {};
     int device = -1;
     hipError_t e = hipGetDevice(&device);
@@ -554,12 +573,12 @@ int launch_tiles(Args& a, hipStream_t s) {
     if (device < 0 || device >= kMaxDevices) return MQC_E_LIMIT;
     if (!done[device]) {
       e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
-                              Cfg::kStagesBytes);
+                              ortho::kLdsBytes<Cfg>);
       if (e != hipSuccess) return (int)e;
       done[device] = true;
     }
   }
-  kernel<<<dim3((unsigned)n), dim3(Cfg::kThreads), Cfg::kStagesBytes, s>>>(a);
+  kernel<<<dim3((unsigned)n), dim3(Cfg::kThreads), ortho::kLdsBytes<Cfg>, s>>>(a);
   return launch_status();
 }
 template <typename T, bool PAIR, int STAGE, bool MUON>
