@@ -1201,7 +1201,7 @@ struct GradShared {
   };
   double G[kC];
   float beta[kC], dG[kGradParts<KD>][kC], w[kGradParts<KD>][kC], dbeta[kC], dot[16];
-  int doc[kC];
+  int doc[kC], some[4 * kGradParts<KD>];  // (some: whether a wave saw a state that is not zero)
 };
 
 // Eight values of row `row`, columns 8 c.., into fragments of N pieces.
@@ -1234,6 +1234,7 @@ __global__ __launch_bounds__(256 * kGradParts<KD>, kGradParts<KD> > 1 ? 4 : 2) v
   const float *resid = a.resid + unit * kC * a.v_pad, *zs = a.z + unit * kC * a.v_pad;
   const float *st = a.states + unit * KD * a.v_pad, *ds = a.dstates + unit * KD * a.v_pad;
   float dot_b = 0.f, dot_s = 0.f;
+  uint32_t bits = 0;  // of the state
 
   // Slot n of the first w + 1: rows of u (tokens 16 n..) against the wave's columns of dO and of z; slot
   // n + 1 of the others: rows of dO and of z against its columns of u. (Of several parts the first takes
@@ -1270,7 +1271,10 @@ __global__ __launch_bounds__(256 * kGradParts<KD>, kGradParts<KD> > 1 ? 4 : 2) v
       load_vec<float, 8>(st + (at_row + v0), x);
       load_vec<float, 8>(ds + (at_row + v0), y);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) dot_s = fmaf(x[i], y[i], dot_s);
+      for (int i = 0; i < 8; ++i) {
+        dot_s = fmaf(x[i], y[i], dot_s);
+        bits |= __float_as_uint(x[i]);
+      }
       stage<kPieces>(s.S, row, c8, x);
       stage<kPieces>(s.dS, row, c8, y);
     }
@@ -1472,12 +1476,14 @@ __global__ __launch_bounds__(256 * kGradParts<KD>, kGradParts<KD> > 1 ? 4 : 2) v
   dot_b += lane_xor2(dot_b);
   if (c8 == 0 && part == (H == 1 ? 0 : 2)) s.dbeta[token] = dot_b;
   dot_s = wave_sum_all(dot_s);
-  if (lane == 0) s.dot[wave] = dot_s;
+  const bool some = __ballot((bits & 0x7fffffffu) != 0) != 0;
+  if (lane == 0) s.dot[wave] = dot_s, s.some[wave] = some;
   __syncthreads();
   if (wave == 0) {
     const int d = s.doc[lane];
     double v = s.dG[0][lane];
     float ends = s.w[0][lane], all = 0.f;
+    int seen = 0;
 #pragma unroll
     for (int n = 1; n < H; ++n) {
       v += s.dG[n][lane];
@@ -1485,7 +1491,10 @@ __global__ __launch_bounds__(256 * kGradParts<KD>, kGradParts<KD> > 1 ? 4 : 2) v
     }
     ends = wave_sum_all(ends);  // zero for tokens of other documents than the last
 #pragma unroll
-    for (int n = 0; n < 4 * H; ++n) all += s.dot[n];
+    for (int n = 0; n < 4 * H; ++n) {
+      all += s.dot[n];
+      seen |= s.some[n];
+    }
     if (last == 0) ends = fmaf(expf((float)s.G[kC - 1]), all, ends);
     if (lane == kC - 1) v += ends;
 #pragma unroll
@@ -1495,7 +1504,8 @@ __global__ __launch_bounds__(256 * kGradParts<KD>, kGradParts<KD> > 1 ? 4 : 2) v
       if (lane + n < 64 && other == d) v += after;
     }
     const int before = __shfl_up(d, 1);
-    if (d != (lane == 0 ? 0 : before)) v = 0.0;  // a document's first token: nothing decays into it
+    // Nothing decays into a document's first token, nor into one before which the state is zero.
+    if (d != (lane == 0 ? 0 : before) || (lane == 0 && !seen)) v = 0.0;
     const int64_t to = (b * a.seq + t0 + lane) * a.v_heads + hv;
     if (t0 + lane < a.seq) {
       store_any(a.dg, to, a.g_type, (float)v);

@@ -465,3 +465,22 @@ def test_nan_stays_before_a_reset_with_many_heads(batch, what):
     hold("h", h.detach(), good[1].double(), REL)
     for v in torch.autograd.grad([o, h], leaves, [do, dh])[:5]:
         assert v[:, 64:].isfinite().all() and v[1::3].isfinite().all()
+
+
+@pytest.mark.parametrize("dk", [24, 100])
+def test_what_nothing_decays_into_has_no_gradient(dk):
+    """log_decay of the first token without a state, of a document's first one and where the state is zero."""
+    ops, _, do, dh = make(2, 140, 1, 2, dk, 40, torch.float32, h0=False)
+    cut = torch.zeros(2, 140, dtype=torch.bool, device=DEV)
+    cut[0, [5, 64, 100]] = True
+    g = ops[3].requires_grad_()
+    for reset, h0 in ((None, None), (cut, None), (cut, torch.zeros(2, 2, dk, 40, device=DEV))):
+        o, h = gated_delta(*ops[:5], h0=h0, reset=reset, return_state=True)
+        got, = torch.autograd.grad([o, h], g, [do, dh])
+        assert (got[:, 0] == 0).all() and (got[:, 1:4] != 0).any()
+        if reset is not None:
+            assert (got[cut] == 0).all()
+    with torch.no_grad():
+        ops[2][:, :64] = 0  # nothing is written in the first chunk
+    o, h = gated_delta(*ops[:5], return_state=True)
+    assert (torch.autograd.grad([o, h], g, [do, dh])[0][:, 64] == 0).all()
