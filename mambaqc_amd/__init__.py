@@ -4,9 +4,9 @@ Drop-in for the reference package's hot path (polux06/mambaqc):
   mambaqc_amd.kernels   cayley_discretization_fused, parallel_scan_quaternion,
                         quaternion_multiply (+ conjugate/inverse/norm),
                         ssm_step_fused, ssm_forward_fused, quaternion_layer_norm_fused
-  mambaqc_amd.layers    QuaternionLinear, QuaternionLayerNorm, CausalConv1d
+  mambaqc_amd.layers    QuaternionLinear, QuaternionLayerNorm, CausalConv1d, LayerNorm
   mambaqc_amd           QuaternionMamba2Block, QuaternionMamba2 (+ presets)
-  mambaqc_amd.optim     AdamW over many tensors, states in 32 or 8 bits
+  mambaqc_amd.optim     AdamW over many tensors, states in 32 or 8 bits; Muon for matrices
   torch.ops.mambaqc.*   the same kernels as registered torch operators with fake
                         kernels and autograd formulas (mambaqc_amd.ops)
 All compute of the quaternion path runs in libmambaqc_hip.so (hand-written

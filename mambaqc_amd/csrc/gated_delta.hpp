@@ -213,7 +213,9 @@ __device__ inline Gates chunk_gates(const Args<T>& a, int64_t b, int64_t hv, int
 
 // ---------------------------------------------------------------------------
 // The products within chunks. A workgroup of four waves takes a chunk of a key head and of the value heads
-// that share it; wave w rows 16 w.., whose gram products stay in its registers.
+// that share it; wave w rows 16 w.., whose gram products stay in its registers. Of 1536 chunks of 128 keys
+// in bf16 49 us (the backward's operands 53), 1.5 TB/s of what it reads and writes: the triangular inverse,
+// whose steps wait for one another.
 // ---------------------------------------------------------------------------
 template <typename T, int KD>
 struct PrepShared {
@@ -440,7 +442,9 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(Args<T> a) {
 // The walks. A workgroup has CT times 16 columns of a head's state, its wave w the tokens 16 w.. of each
 // chunk and the state's rows 16 w.. and 16 (w + 4)... A product's left operand is the wave's own rows, from
 // memory to registers a chunk ahead; its right one (the state, then what the tokens leave) is all waves',
-// and goes through LDS as pieces.
+// and goes through LDS as pieces. A chunk waits for the one before, three barriers each: with a workgroup to
+// a CU for 2.3 us (128 keys, bf16), of which matrix instructions take 0.4 and vector instructions 0.75. With
+// operands brought to LDS by a workgroup of one wave each it was 12.
 // ---------------------------------------------------------------------------
 template <int KD, int CT>
 struct WalkShared {
@@ -736,7 +740,8 @@ struct RowGates {
   }
 };
 
-// Waves to a SIMD where their operands leave registers for that (two hide one another's waits).
+// Waves to a SIMD where their operands leave registers for that (two hide one another's waits: 384 workgroups
+// of 32 chunks walk forward in 159 us and back in 171).
 template <typename T, int KD, int CT, bool BWD>
 constexpr int kWalkWaves = CT == 1 && (BWD ? (kIn<T> == 1 && KD == 128) || (kIn<T> == 2 && KD < 128)
                                            : kIn<T> == 1 || (kIn<T> == 2 && KD < 128)) ? 2 : 1;
@@ -1057,7 +1062,8 @@ __global__ __launch_bounds__(256, (kWalkWaves<T, KD, CT, true>)) void delta_bwd_
 }
 
 // The same by eight waves (as forward): four take the state's gradient from chunk to chunk, and four bring them
-// what does not depend on it, P^T dO of the next chunk and Q^T (e dO) of this one.
+// what does not depend on it, P^T dO of the next chunk and Q^T (e dO) of this one. In fp32 with 64 keys 105
+// workgroups take 57 us for 84; 384 of them in bf16 183, with four waves 172.
 template <int KD>
 struct BesideShared {
   floatx4 z[4][64], s[KD / 16 > 4 ? 2 : 1][4][64];  // as the chain's waves hold z and the state
@@ -1181,7 +1187,8 @@ __global__ __launch_bounds__(512, 2) void delta_bwd_beside_kernel(Args<T> a) {
 // ---------------------------------------------------------------------------
 // The gradients of q, k, g and beta: a chunk of a value head to a workgroup of four waves, wave w the
 // columns 16 w.. of everything turned (tokens as columns). Operands pass through LDS 32 columns of v_dim
-// at a time, as fragments with their columns in order.
+// at a time, as fragments with their columns in order. 1536 chunks of 128 by 128 in 193 us, 475 MB at
+// 2.5 TB/s: what is loaded is cut into pieces by the lanes that load it, and all waits for that.
 // ---------------------------------------------------------------------------
 // Of wide keys four waves have the same columns and a quarter of k_dim each: with the gradients of q and k
 // in the registers of one, a SIMD had room for two waves, which could not hide what they wait for.
@@ -1533,7 +1540,8 @@ __global__ __launch_bounds__(256) void delta_share_kernel(Args<T> a) {
 
 // ---------------------------------------------------------------------------
 // One token of each sequence: the state is read and written once, a workgroup 64 columns of a head; lane
-// l of wave w has columns 4 (l % 16).. of rows l / 16 + 4 w + 16 n.
+// l of wave w has columns 4 (l % 16).. of rows l / 16 + 4 w + 16 n. 192 states of 128 by 128 (25 MB) take
+// 9.8 us: one load's wait, two sums over the rows and a store one after another.
 // ---------------------------------------------------------------------------
 template <typename T, int ROWS>
 __global__ __launch_bounds__(256) void delta_step_kernel(Args<T> a, float* h) {

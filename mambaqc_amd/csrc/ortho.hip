@@ -14,10 +14,10 @@
 // Operands are fp16 times 2^8 (X, A and B have values up to about 3, and most near n^-1/2), accumulators
 // fp32. For matrices in fp32 and fp16 a value is two fp16 pieces, held to 2^-23 of itself or 2^-33, and a
 // product three: off by 2e-6. For those in bf16 it is one (of shorter sides from kOnePiece on: roundings
-// average out over a side, and short ones take no less time with one), but X itself, which a X goes on from, keeps its
-// second piece: weak directions grow 3.4 times a step by a X alone, and a rounding of X with them (a matrix
-// of eight strong directions comes out off by 3e-4 of it, without that piece by 0.04, iterated in bf16 by
-// 0.3; gradients with a sixteenth of strong directions by 8e-4).
+// average out over a side, and short ones take no less time with one), but X itself, which a X goes on
+// from, keeps its second piece: weak directions grow 3.4 times a step by a X alone, and a rounding of X with
+// them (a matrix of eight strong directions comes out off by 3e-4 of it, without that piece by 0.04,
+// iterated in bf16 by 0.3; gradients with a sixteenth of strong directions by 8e-4).
 #include <algorithm>
 #include <climits>
 #include <vector>
@@ -31,7 +31,7 @@ using namespace mfma;
 
 constexpr int kMatrices = 64, kGroups = 16;  // of a launch
 constexpr float kScale = 256.f;
-constexpr int64_t kPartElems = 4096;        // elements that a workgroup adds the squares of
+constexpr int64_t kPartElems = 4096;         // elements that a workgroup adds the squares of
 constexpr int64_t kMaxParts = 256;
 constexpr int kOnePiece = 256;
 
@@ -107,7 +107,7 @@ __device__ inline T* target(const Args& a, const Group& g, int i) {
   return g.stack ? (T*)a.matrices[g.first].p + i * g.stack : (T*)a.matrices[g.first + i].p;
 }
 
-// --- momentum, and the sum of squares ------------------------------------------------------------------
+// --- momentum, and the sum of squares (42 M bf16 elements, fp32 momenta: 71 us, 5.9 TB/s) -----------------
 template <bool MUON>
 __device__ inline float update(const Args& a, float g, float m) {
   if constexpr (!MUON) return g;
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(256) void ortho_sum_kernel(Args a) {
   if (threadIdx.x == 0) a.sums[g.parts + (int64_t)i * g.sums + part] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// --- X_0 by rows and turned ------------------------------------------------------------------------------
+// --- X_0 by rows and turned (of the same 116 us, 4.3 TB/s) ------------------------------------------------
 // Four values (times kScale) into a row, col a multiple of 4; the second pieces `second` bytes on (0: none).
 __device__ inline float half_of(const u32x2& v, int c) {
   return io<f16_t>::bits_to_f32(c & 1 ? v[c / 2] >> 16 : v[c / 2] & 0xffffu);
@@ -291,8 +291,10 @@ __device__ inline void put_result(T* to, int left, float (&v)[8], float decay, f
 
 // A tile's rows w of the left operand and x of the right one, S of each. What it leaves goes through LDS,
 // the columns of a wave at a time: rows of x are written along w, and (the mirrored half of a symmetric
-// product, X by rows, a wide matrix) rows of w along x, 16 bytes a lane. Written from the registers, two
-// bytes a lane, they took longer than the products: 75 us of 12 matrices of 768 x 1536 for the last one.
+// product, X by rows, a wide matrix) rows of w along x, 16 bytes a lane. (Written from the registers, two
+// bytes a lane, a step for the matrices of 8 blocks of width 512 took 2458 us; with this, and long sides
+// shared, 2034.) Then the symmetric products take 61 + 7 + 42 us of it a time, the last one 151: 60 GFLOP,
+// and 420 MB at 2.8 TB/s that its products do not hide.
 template <typename T, typename Cfg, bool PAIR, int STAGE, bool MUON>
 __global__ __launch_bounds__(Cfg::kThreads, 2) void ortho_product_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -513,7 +515,8 @@ int tile_side(const Args& a) {
 
 // Where the groups' buffers and sums lie; returns the workspace's bytes. Long sides are shared among
 // workgroups in the first product where its tiles alone would not fill the card (512 of 128 by 128), in
-// shares of about as many columns as a workgroup has on average, at least 512; and of at most 8192, beyond which an fp32 sum loses more than its operands.
+// shares of about as many columns as a workgroup has on average, at least 512; and of at most 8192, beyond
+// which an fp32 sum loses more than its operands.
 int64_t lay_out(Args& a, bool pair) {
   int64_t bytes = 0, parts = 0, steps = 0;
   for (int i = 0; i < a.count; ++i) {
