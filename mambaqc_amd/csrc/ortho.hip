@@ -516,7 +516,8 @@ int tile_side(const Args& a) {
 // Where the groups' buffers and sums lie; returns the workspace's bytes. Long sides are shared among
 // workgroups in the first product where its tiles alone would not fill the card (512 of 128 by 128), in
 // shares of about as many columns as a workgroup has on average, at least 512; and of at most 8192, beyond
-// which an fp32 sum loses more than its operands.
+// which an fp32 sum loses more than its operands. (Up to 2048 columns the launch that joins shares costs
+// more than they save: 12 matrices of 768 by 1536 take 24 us, shared 21 and 12.)
 int64_t lay_out(Args& a, bool pair) {
   int64_t bytes = 0, parts = 0, steps = 0;
   for (int i = 0; i < a.count; ++i) {
@@ -538,7 +539,7 @@ int64_t lay_out(Args& a, bool pair) {
   for (int i = 0; i < a.count; ++i) {
     Group& g = a.groups[i];
     const int64_t have = g.np / 64;
-    const int64_t want = std::max((have + least - 1) / least, (have + 127) / 128);
+    const int64_t want = have <= 32 ? 1 : std::max((have + least - 1) / least, (have + 127) / 128);
     const int64_t each = (have + want - 1) / want;
     g.splits = (int)((have + each - 1) / each);
     g.shares = bytes;
