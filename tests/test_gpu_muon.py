@@ -254,3 +254,38 @@ def test_refusals():
         muon_step_([p.T], [p.T.clone()], [p.T.contiguous()])
     with pytest.raises(RuntimeError, match="ROCm device"):
         muon_step_([p], [p.cpu()], [p.clone()])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(16, 900, 1030), (17, 1030, 770), (300, 5000), (3, 2500, 130)])
+def test_large_tiles_and_shared_sides(dtype, shape):
+    """Last products of 256 tiles of 256 by 256 and more, odd ones; first products shared along the long side."""
+    x = make(shape, dtype)
+    hold("x", orthogonalize(x), iterate(x), REL[dtype])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_muon_step_of_large_tiles_in_a_graph(dtype):
+    """Tall and wide ones beside small ones and a long one; captured as the first such call of a process too."""
+    shapes = [(1000, 900)] * 9 + [(520, 2100)] * 6 + [(64, 40), (70, 4500)]
+    params = [make(s, dtype, seed=i) for i, s in enumerate(shapes)]
+    grads = [make(s, dtype, seed=100 + i) for i, s in enumerate(shapes)]
+    momenta = [torch.zeros(s, device=DEV) for s in shapes]
+    before = [p.clone() for p in params]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        muon_step_(params, grads, momenta, lr=0.5, momentum=0.9, weight_decay=0.1)
+    for rep in range(3):
+        for p, b, m in zip(params, before, momenta):
+            p.copy_(b), m.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [p.clone() for p in params]
+        for p, b, m in zip(params, before, momenta):
+            p.copy_(b), m.zero_()
+        muon_step_(params, grads, momenta, lr=0.5, momentum=0.9, weight_decay=0.1)
+        assert all(torch.equal(u, p) for u, p in zip(got, params))
+    for p, b, g, s in zip(params, before, grads, shapes):
+        # m = 0.1 g, u = 0.9 m + 0.1 g: a multiple of g.
+        step = 0.5 * max(1.0, s[0] / s[1]) ** 0.5 * iterate(g)
+        hold("p", p, b.double() * (1 - 0.5 * 0.1) - step, REL[dtype])
