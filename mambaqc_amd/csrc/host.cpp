@@ -264,7 +264,7 @@ std::optional<std::tuple<Tensor, Tensor>> gate_norm(const Tensor& x, const Tenso
 }
 
 // --- layer norm -----------------------------------------------------------------------------------
-// Operands as the kernels read them, weights in fp32 (kernels/layer_norm.py).
+// Operands as the kernels read them, weights in fp32 (kernels/norm.py).
 struct LayerNorm {
   Tensor x;
   int64_t x_row;
