@@ -20,6 +20,7 @@
 // iterated in bf16 by 0.3; gradients with a sixteenth of strong directions by 8e-4).
 #include <algorithm>
 #include <climits>
+#include <new>
 #include <vector>
 
 #include "mfma_tile.hpp"
@@ -562,6 +563,26 @@ int64_t number(Args& a, const Each& each, int64_t threads) {
   return n * kXCDs;
 }
 
+// Side of a stage's tiles (of the first product those that its shares were laid out for).
+template <int STAGE>
+int stage_side(const Args& a) {
+  return STAGE == ortho::GRAM ? a.side : STAGE == ortho::JOIN ? 64 : tile_side<STAGE>(a);
+}
+template <int STAGE>
+bool stage_fits(Args& a) {
+  const int side = stage_side<STAGE>(a);
+  return (side == 256   ? number(a, ortho::tile_count<STAGE, 256>, 512)
+          : side == 128 ? number(a, ortho::tile_count<STAGE, 128>, 256)
+                        : number(a, ortho::tile_count<STAGE, 64>, 256)) >= 0;
+}
+int64_t init_tiles(const Group& g) { return (int64_t)ortho::ceil_div(g.rows, 64) * ortho::ceil_div(g.cols, 64); }
+// Whether all launches of a call can be made: known before the first, which changes momenta.
+bool fits(Args a) {
+  return number(a, [](const Group& g) { return g.sums; }, 256) >= 0 && number(a, init_tiles, 256) >= 0 &&
+         stage_fits<ortho::GRAM>(a) && stage_fits<ortho::JOIN>(a) && stage_fits<ortho::POLY>(a) &&
+         stage_fits<ortho::LAST>(a);
+}
+
 constexpr int kMaxDevices = 64;
 template <typename T, typename Cfg, bool PAIR, int STAGE, bool MUON>
 int launch_tiles(Args& a, hipStream_t s) {
@@ -587,8 +608,7 @@ int launch_tiles(Args& a, hipStream_t s) {
 }
 template <typename T, bool PAIR, int STAGE, bool MUON>
 int launch_product(Args& a, hipStream_t s) {
-  // (the first product's tiles are those that its shares were laid out for)
-  const int side = STAGE == ortho::GRAM ? a.side : STAGE == ortho::JOIN ? 64 : tile_side<STAGE>(a);
+  const int side = stage_side<STAGE>(a);
   if constexpr (STAGE == ortho::APPLY || STAGE == ortho::LAST)
     if (side == 256) return launch_tiles<T, Tile256, PAIR, STAGE, MUON>(a, s);
   if constexpr (STAGE != ortho::JOIN)
@@ -628,7 +648,7 @@ int run_pieces(Args& a, int steps, char* ws, hipStream_t s) {
   ortho::ortho_sum_kernel<T, MUON><<<dim3((unsigned)n), dim3(256), 0, s>>>(a);
   int st = launch_status();
   if (st != MQC_OK) return st;
-  n = number(a, [](const Group& g) { return ortho::ceil_div(g.rows, 64) * ortho::ceil_div(g.cols, 64); }, 256);
+  n = number(a, init_tiles, 256);
   if (n < 0) return MQC_E_LIMIT;
   ortho::ortho_init_kernel<T, PAIR, MUON><<<dim3((unsigned)n), dim3(256), 0, s>>>(a);
   st = launch_status();
@@ -732,6 +752,7 @@ extern "C" int mqc_orthogonalize(const void* x, void* out, int64_t batch, int64_
   if (!aligned(workspace, 256)) return MQC_E_ALIGN;
   Args k = one_stack(x, out, batch, rows, cols);
   lay_out(k, paired(dtype, rows, cols));
+  if (!fits(k)) return MQC_E_LIMIT;
   k.a = a, k.b = b, k.c = c, k.eps = eps;
   return run<false>(k, dtype, steps, (char*)workspace, (hipStream_t)stream);
 }
@@ -741,7 +762,11 @@ extern "C" int64_t mqc_muon_workspace_bytes(const int64_t* matrices, int64_t cou
   if (st != MQC_OK) return st;
   std::vector<Batch> work;
   std::vector<int> types;
-  batches(matrices, count, 0.f, work, types);
+  try {
+    batches(matrices, count, 0.f, work, types);
+  } catch (const std::bad_alloc&) {
+    return MQC_E_LIMIT;
+  }
   int64_t most = 0;
   for (const Batch& b : work) most = std::max(most, b.bytes);
   return most;
@@ -760,9 +785,15 @@ extern "C" int mqc_muon_step(const int64_t* matrices, int64_t count, float decay
   if (!aligned(workspace, 256)) return MQC_E_ALIGN;
   std::vector<Batch> work;
   std::vector<int> types;
-  batches(matrices, count, rate, work, types);
-  for (const Batch& w : work)
+  try {
+    batches(matrices, count, rate, work, types);
+  } catch (const std::bad_alloc&) {
+    return MQC_E_LIMIT;
+  }
+  for (const Batch& w : work) {
     if (workspace_bytes < w.bytes) return MQC_E_SPACE;
+    if (!fits(w.args)) return MQC_E_LIMIT;
+  }
   const hipStream_t s = (hipStream_t)stream;
   for (size_t i = 0; i < work.size() && st == MQC_OK; ++i) {
     Args& k = work[i].args;

@@ -88,3 +88,7 @@ def test_validation_codes():
     assert lib.mqc_muon_step(None, -1, 1.0, 1.0, 0.9, 1, 5, 1.0, 1.0, 1.0, 0.0, FAKE, 1 << 40, None) == -2
     table = array.array("q", row * 3).tobytes()
     assert lib.mqc_muon_workspace_bytes(table, 3) > lib.mqc_muon_workspace_bytes(table, 1) > 0
+    # Launches of 2^32 threads are refused before the first: nothing of the table is done.
+    big = [4096, 4096, 4096, 32768, 1 << 24, 1]
+    assert f(r=32768, c=1 << 24, dtype=1, ws=1 << 62) == -5
+    assert step([row, big], ws=1 << 62) == -5 and step([big, row], ws=1 << 62) == -5
