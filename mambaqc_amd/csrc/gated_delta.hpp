@@ -214,8 +214,7 @@ __device__ inline Gates chunk_gates(const Args<T>& a, int64_t b, int64_t hv, int
 // ---------------------------------------------------------------------------
 // The products within chunks. A workgroup of four waves takes a chunk of a key head and of the value heads
 // that share it; wave w rows 16 w.., whose gram products stay in its registers. Of 1536 chunks of 128 keys
-// in bf16 49 us (the backward's operands 53), 1.5 TB/s of what it reads and writes: the triangular inverse,
-// whose steps wait for one another.
+// in bf16 49 us (the backward's operands 53): 32 KB read and 84 written of each, 3.6 TB/s.
 // ---------------------------------------------------------------------------
 template <typename T, int KD>
 struct PrepShared {
