@@ -12,8 +12,11 @@
 //   dS = e_63 dS' + Q^T (scale e dO) - K^T (e beta z)
 //   dQ = scale e (S dO^T)^T + (D dP) K with dP = scale dO u^T,  M = -beta_i D (z u^T) below the diagonal,
 //   dK = [M K - e beta (S z^T)^T] + [(D dP)^T Q + M^T K + D_63 (dS' u^T)^T]
-//   dG_i = q_i . dQ_i + k_i . (the first bracket - the second), dG_63 also the second bracket's last part
-//   and e_63 <dS', S>; dg_t is the sum of dG from t to its document's end.
+//   dg_t = sum over j < t <= i of W_ij, with W_ij = (D dP)_ij (q_i . k_j) + M_ij (k_i . k_j),
+//     + sum over i >= t of e_i (scale q_i . (S dO_i) - beta_i k_i . (S z_i))
+//     + sum over j < t of D_63,j k_j . (dS' u_j) + e_63 <dS', S>
+// Every term of dg_t has the factor exp(g_t). (As sums from t on of q_i . dQ_i + k_i . dK_i, signs by bracket,
+// which are the same, terms without it cancel: below g_t = -13 or so nothing but their rounding was left.)
 //
 // Three kinds of kernels. One over all chunks side by side forms the products within them (gram
 // matrices, the triangular inverse) and lays every operand out as the matrix instructions read it. One
@@ -1186,7 +1189,7 @@ __global__ __launch_bounds__(512, 2) void delta_bwd_beside_kernel(Args<T> a) {
 // ---------------------------------------------------------------------------
 // The gradients of q, k, g and beta: a chunk of a value head to a workgroup of four waves, wave w the
 // columns 16 w.. of everything turned (tokens as columns). Operands pass through LDS 32 columns of v_dim
-// at a time, as fragments with their columns in order. 1536 chunks of 128 by 128 in 193 us, 475 MB at
+// at a time, as fragments with their columns in order. 1536 chunks of 128 by 128 in 203 us, 500 MB at
 // 2.5 TB/s: what is loaded is cut into pieces by the lanes that load it, and all waits for that.
 // ---------------------------------------------------------------------------
 // Of wide keys four waves have the same columns and a quarter of k_dim each: with the gradients of q and k
@@ -1206,8 +1209,10 @@ struct GradShared {
     uint16_t tokens[kGradParts<KD> > 1 ? 2 : 1][kGradParts<KD> > 1 ? 4 : 1][3 * kPieces * kFrag];
   };
   double G[kC];
-  float beta[kC], dG[kGradParts<KD>][kC], w[kGradParts<KD>][kC], dbeta[kC], dot[16];
-  int doc[kC], some[4 * kGradParts<KD>];  // (some: whether a wave saw a state that is not zero)
+  float beta[kC], into[kGradParts<KD>][kC], w[kGradParts<KD>][kC], dbeta[kC], dot[16];
+  float across[kGradParts<KD> > 1 ? 2 : 1][4][kC];  // sums of W over j < t <= i, i of a wave
+  floatx4 dots[2][kGradParts<KD> > 1 ? 10 : 1][64];  // of several parts: q's and k's dot products with earlier keys
+  int doc[kC];
 };
 
 // Eight values of row `row`, columns 8 c.., into fragments of N pieces.
@@ -1227,20 +1232,67 @@ __global__ __launch_bounds__(256 * kGradParts<KD>, kGradParts<KD> > 1 ? 4 : 2) v
   const int64_t unit = xcd_order(blockIdx.x, gridDim.x), chunk = unit % a.chunks, bh = unit / a.chunks;
   const int64_t b = bh / a.v_heads, hv = bh % a.v_heads, hk = hv / (a.v_heads / a.k_heads);
   const int64_t t0 = chunk * kC;
-  if (wave == 0) {
-    const Gates x = chunk_gates(a, b, hv, t0);
-    s.G[lane] = x.G;
-    s.beta[lane] = x.beta;
-    s.doc[lane] = x.doc;
-  }
-  __syncthreads();
   // What this thread stages: a row of the states (parts 0 and 1), of u and z (part 2), of dO (part 3).
   const int row = tid >> 2, c8 = tid & 3, token = row & 63;
   const uint32_t at_token = token * a.v_pad + 8 * c8, at_row = row * a.v_pad + 8 * c8;
   const float *resid = a.resid + unit * kC * a.v_pad, *zs = a.z + unit * kC * a.v_pad;
   const float *st = a.states + unit * KD * a.v_pad, *ds = a.dstates + unit * KD * a.v_pad;
   float dot_b = 0.f, dot_s = 0.f;
-  uint32_t bits = 0;  // of the state
+
+  // The wave's column is token `mine`.
+  const int mine = 16 * w + m;
+  const int64_t t = t0 + mine;
+  const bool here = t < a.seq;
+  const T* qrow = a.q + b * a.q_b + (here ? t : a.seq - 1) * a.q_t + hk * a.q_h;
+  const T* krow = a.k + b * a.k_b + (here ? t : a.seq - 1) * a.k_t + hk * a.k_h;
+  const uint16_t* kr = a.keys + ((b * a.k_heads + hk) * a.chunks + chunk) * (3 * kPart);
+  // The dot products of the wave's tokens' q and k with the keys of tokens 16 n.. Where k_dim is a multiple of
+  // four, what lies past it is loaded from within and cut, so that loads are under way together (behind a test
+  // of where the row ends each waits for the one before: 222 us for 205).
+  const auto keys_dots = [&](int n, floatx4& q_dots, floatx4& k_dots) {
+    q_dots = k_dots = (floatx4){};
+    const auto sum = [&](const auto& row_of_q) {
+#pragma unroll
+      for (int i = 0; i < KD / 32; ++i) {
+        float x[8];
+        bf16x8 f[NP], own[NP], kn[NP];
+        row_of_q(i, x);
+        split<NP>(x, f);
+        load_frag(kr + (w * (KD / 32) + i) * NP * kFrag, lane, own);
+        load_frag(kr + (n * (KD / 32) + i) * NP * kFrag, lane, kn);
+        q_dots = mma(kn, f, q_dots);
+        k_dots = mma(kn, own, k_dots);
+      }
+      q_dots = settled(q_dots), k_dots = settled(k_dots);
+    };
+    if (a.k_dim % 4 == 0) {
+      sum([&](int i, float (&x)[8]) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int at = 32 * i + 16 * half + 4 * g;
+          const bool in = here && at < a.k_dim;
+          float v[4];
+          load_part(qrow, in ? at : 0, 4, v);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) x[4 * half + c] = in ? v[c] : 0.f;
+        }
+      });
+    } else sum([&](int i, float (&x)[8]) { load_row8(qrow, i, g, here ? a.k_dim : 0, x); });
+  };
+  if (wave == (H > 1 ? 4 : 0)) {  // (the second part's first wave has no dot products)
+    const Gates x = chunk_gates(a, b, hv, t0);
+    s.G[lane] = x.G;
+    s.beta[lane] = x.beta;
+    s.doc[lane] = x.doc;
+  }
+  if constexpr (H > 1) {  // a part the keys 16 part..
+    if (part <= w) {
+      const int at = w * (w + 1) / 2 + part;
+      floatx4 q_dots, k_dots;
+      keys_dots(part, q_dots, k_dots);
+      s.dots[0][at][lane] = q_dots, s.dots[1][at][lane] = k_dots;
+    }
+  }
 
   // Slot n of the first w + 1: rows of u (tokens 16 n..) against the wave's columns of dO and of z; slot
   // n + 1 of the others: rows of dO and of z against its columns of u. (Of several parts the first takes
@@ -1277,10 +1329,7 @@ __global__ __launch_bounds__(256 * kGradParts<KD>, kGradParts<KD> > 1 ? 4 : 2) v
       load_vec<float, 8>(st + (at_row + v0), x);
       load_vec<float, 8>(ds + (at_row + v0), y);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        dot_s = fmaf(x[i], y[i], dot_s);
-        bits |= __float_as_uint(x[i]);
-      }
+      for (int i = 0; i < 8; ++i) dot_s = fmaf(x[i], y[i], dot_s);
       stage<kPieces>(s.S, row, c8, x);
       stage<kPieces>(s.dS, row, c8, y);
     }
@@ -1323,30 +1372,38 @@ __global__ __launch_bounds__(256 * kGradParts<KD>, kGradParts<KD> > 1 ? 4 : 2) v
     }
   }
 
-  // The wave's column is token `mine`.
-  const int mine = 16 * w + m, doc = s.doc[mine], last = s.doc[kC - 1];
+  const int doc = s.doc[mine], last = s.doc[kC - 1];
   const double Gm = s.G[mine];
   const float bm = s.beta[mine];
   const float e = doc == 0 ? expf((float)Gm) : 0.f;
   const float et = doc == last ? expf((float)(s.G[kC - 1] - Gm)) : 0.f;
-  const int64_t t = t0 + mine;
-  const bool here = t < a.seq;
-  const T* qrow = a.q + b * a.q_b + t * a.q_t + hk * a.q_h;
-  const T* krow = a.k + b * a.k_b + t * a.k_t + hk * a.k_h;
-  float wrote = 0.f;  // k . (dS' u)
+  float wrote = 0.f, into = 0.f;  // k . (dS' u), and what the state's decay up to the token passes on
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     dq[i] = settled(dq[i]), ka[i] = settled(ka[i]), kb[i] = settled(kb[i]);
     const int d = 16 * (part * MT + i) + 4 * g;
-    float kv[4] = {0.f, 0.f, 0.f, 0.f};
-    if (here && d < a.k_dim) load_part(krow, d, a.k_dim - d, kv);
+    float qv[4] = {0.f, 0.f, 0.f, 0.f}, kv[4] = {0.f, 0.f, 0.f, 0.f};
+    if (here && d < a.k_dim) {
+      load_part(qrow, d, a.k_dim - d, qv);
+      load_part(krow, d, a.k_dim - d, kv);
+    }
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       dq[i][r] = doc == 0 ? dq[i][r] * (a.scale * e) : 0.f;
       ka[i][r] = doc == 0 ? ka[i][r] * (-e * bm) : 0.f;
       kb[i][r] = doc == last ? kb[i][r] * et : 0.f;
+      into = fmaf(qv[r], dq[i][r], into);
+      into = fmaf(kv[r], ka[i][r], into);
       wrote = fmaf(kv[r], kb[i][r], wrote);
     }
+  }
+  into += __shfl_xor(into, 16);
+  into += __shfl_xor(into, 32);
+  wrote += __shfl_xor(wrote, 16);
+  wrote += __shfl_xor(wrote, 32);
+  if (g == 0) {
+    s.into[part][mine] = into;
+    s.w[part][mine] = wrote;
   }
   // D dP (turned in the first w + 1 slots), and M.
   if (H == 1 || part < 2) {
@@ -1371,6 +1428,45 @@ __global__ __launch_bounds__(256 * kGradParts<KD>, kGradParts<KD> > 1 ? 4 : 2) v
           p[n][r] = one && (part == 0 || apart) ? p[n][r] * by : 0.f;
         }
       }
+    }
+  }
+  // Sums of W over j < t, and over the wave's i >= t.
+  if (H == 1 || part < 2) {
+    floatx4 W[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      W[n] = (floatx4){};
+      if (n > w) continue;
+      if constexpr (H == 1) {
+        floatx4 q_dots, k_dots;
+        keys_dots(n, q_dots, k_dots);
+        W[n] = p[n] * q_dots + mm[n] * k_dots;
+      } else {
+        W[n] = p[n] * s.dots[part][w * (w + 1) / 2 + n][lane];
+      }
+    }
+    float before = 0.f;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+      const float s0 = W[n][0], s1 = s0 + W[n][1], s2 = s1 + W[n][2];
+      float sum = s2 + W[n][3];
+      float other = __shfl_up(sum, 16);
+      if (g >= 1) sum += other;
+      other = __shfl_up(sum, 32);
+      if (g >= 2) sum += other;
+      other = __shfl_up(sum, 16);
+      const float left = g ? before + other : before;
+      before += __shfl(sum, 48 + m);
+      floatx4 y = {left, left + s0, left + s1, left + s2};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (16 * n + 4 * g + r > mine) y[r] = 0.f;
+        y[r] += lane_xor1(y[r]);
+        y[r] += lane_xor2(y[r]);
+        y[r] += row_rot4(y[r]);
+        y[r] += row_rot8(y[r]);
+      }
+      if (m == 0) *reinterpret_cast<floatx4*>(&s.across[H == 1 ? 0 : part][w][16 * n + 4 * g]) = y;
     }
   }
   const floatx4 none = {};
@@ -1401,8 +1497,7 @@ __global__ __launch_bounds__(256 * kGradParts<KD>, kGradParts<KD> > 1 ? 4 : 2) v
     }
     __syncthreads();
   }
-  const uint16_t* kt = a.keys + ((b * a.k_heads + hk) * a.chunks + chunk) * (3 * kPart) + kPart +
-                       part * MT * 2 * NP * kFrag;
+  const uint16_t* kt = kr + kPart + part * MT * 2 * NP * kFrag;
   const uint16_t* qt = kt + kPart;
 #pragma unroll
   for (int ks = 0; ks < 2; ++ks) {
@@ -1443,20 +1538,15 @@ __global__ __launch_bounds__(256 * kGradParts<KD>, kGradParts<KD> > 1 ? 4 : 2) v
       }
     }
   }
-  float dG = 0.f;
   const bool shared = a.k_heads != a.v_heads;
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
     const int d = 16 * (part * MT + i) + 4 * g;
     dq[i] = settled(dq[i]), ka[i] = settled(ka[i]), kb[i] = settled(kb[i]);
     if (!here || d >= a.k_dim) continue;
-    float qv[4], kv[4], dk[4], dqv[4];
-    load_part(qrow, d, a.k_dim - d, qv);
-    load_part(krow, d, a.k_dim - d, kv);
+    float dk[4], dqv[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      dG = fmaf(qv[r], dq[i][r], dG);
-      dG = fmaf(kv[r], ka[i][r] - kb[i][r], dG);
       dk[r] = ka[i][r] + kb[i][r];
       dqv[r] = dq[i][r];
     }
@@ -1470,48 +1560,39 @@ __global__ __launch_bounds__(256 * kGradParts<KD>, kGradParts<KD> > 1 ? 4 : 2) v
       store_part(a.dk + at, d, a.k_dim - d, dk);
     }
   }
-  dG += __shfl_xor(dG, 16);
-  dG += __shfl_xor(dG, 32);
-  wrote += __shfl_xor(wrote, 16);
-  wrote += __shfl_xor(wrote, 32);
-  if (g == 0) {
-    s.dG[part][mine] = dG;
-    s.w[part][mine] = wrote;
-  }
   dot_b += lane_xor1(dot_b);
   dot_b += lane_xor2(dot_b);
   if (c8 == 0 && part == (H == 1 ? 0 : 2)) s.dbeta[token] = dot_b;
   dot_s = wave_sum_all(dot_s);
-  const bool some = __ballot((bits & 0x7fffffffu) != 0) != 0;
-  if (lane == 0) s.dot[wave] = dot_s, s.some[wave] = some;
+  if (lane == 0) s.dot[wave] = dot_s;
   __syncthreads();
   if (wave == 0) {
     const int d = s.doc[lane];
-    double v = s.dG[0][lane];
-    float ends = s.w[0][lane], all = 0.f;
-    int seen = 0;
+    double v = 0.0, from = 0.0, upto = 0.0;  // W's sums; sums over i >= t, j < t
+    float all = 0.f;
 #pragma unroll
-    for (int n = 1; n < H; ++n) {
-      v += s.dG[n][lane];
-      ends += s.w[n][lane];
+    for (int n = 0; n < H; ++n) {
+      if (d == 0) from += s.into[n][lane];
+      if (d == last) upto += s.w[n][lane];
     }
-    ends = wave_sum_all(ends);  // zero for tokens of other documents than the last
 #pragma unroll
-    for (int n = 0; n < 4 * H; ++n) {
-      all += s.dot[n];
-      seen |= s.some[n];
-    }
-    if (last == 0) ends = fmaf(expf((float)s.G[kC - 1]), all, ends);
-    if (lane == kC - 1) v += ends;
+    for (int n = 0; n < 4 * H; ++n) all += s.dot[n];
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      v += H == 1 ? s.across[0][n][lane] : s.across[0][n][lane] + s.across[H > 1][n][lane];
 #pragma unroll
     for (int n = 1; n < 64; n *= 2) {
-      const double after = __shfl_down(v, n);
-      const int other = __shfl_down(d, n);
-      if (lane + n < 64 && other == d) v += after;
+      const double after = __shfl_down(from, n), before = __shfl_up(upto, n);
+      if (lane + n < 64) from += after;
+      if (lane >= n) upto += before;
     }
+    upto = __shfl_up(upto, 1);
+    if (d == 0) v += from;
+    if (d == last && lane > 0) v += upto;
+    if (last == 0) v += expf((float)s.G[kC - 1]) * all;
+    // Nothing decays into a document's first token.
     const int before = __shfl_up(d, 1);
-    // Nothing decays into a document's first token, nor into one before which the state is zero.
-    if (d != (lane == 0 ? 0 : before) || (lane == 0 && !seen)) v = 0.0;
+    if (d != (lane == 0 ? 0 : before)) v = 0.0;
     const int64_t to = (b * a.seq + t0 + lane) * a.v_heads + hv;
     if (t0 + lane < a.seq) {
       store_any(a.dg, to, a.g_type, (float)v);

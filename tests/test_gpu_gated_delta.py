@@ -484,3 +484,44 @@ def test_what_nothing_decays_into_has_no_gradient(dk):
         ops[2][:, :64] = 0  # nothing is written in the first chunk
     o, h = gated_delta(*ops[:5], return_state=True)
     assert (torch.autograd.grad([o, h], g, [do, dh])[0][:, 64] == 0).all()
+
+
+RATES = (0.5, 5.0, 10.0, 15.0, 30.0, 80.0, 200.0, 1e5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dk,reset", [(24, 0.0), (60, 0.03), (128, 0.0), (128, 0.03)])
+def test_gradient_of_log_decay_of_heads_that_forget_fast(dtype, dk, reset):
+    """Every term of log_decay's gradient has its token's factor exp(log_decay), so a head's gradients are as
+    small as that, and held to a head's own size. (The exponent of a factor is an fp32 number: of the largest
+    one that is not zero, 87, half a step is 2^-18 of the factor.) Where a factor is 0, so is the gradient."""
+    ops, cut, do, dh = make(1, 200, 4, 8, dk, 40, dtype, reset=reset)
+    for head, rate in enumerate(RATES):
+        ops[3][:, :, head] = -rate
+    ref = [x.clone() for x in ops]
+    ref[3] = ops[3].clamp_min(-700.0)  # exp of it is 0 to 64 bits too, and its slope a number
+    want = exact(ref, cut, do, dh)["g"]
+    leaves = [x.detach().requires_grad_() for x in ops]
+    o, h = gated_delta(*leaves[:5], h0=leaves[5], reset=cut, return_state=True)
+    got, = torch.autograd.grad([o, h], leaves[3], [do, dh])
+    for head, rate in enumerate(RATES):
+        hold(rate, got[..., head], want[..., head], GRAD)
+        assert rate < 104 or (got[..., head] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dk", [24, 60, 128])
+def test_gradient_of_log_decay_of_tokens_that_forget(dtype, dk):
+    """Single tokens that forget much or all, among ones that forget little: each held to its own gradient, in
+    terms of the size that its factor gives it."""
+    ops, _, do, dh = make(2, 150, 2, 2, dk, 40, dtype, rate=0.02)
+    for at, rate in ((7, 12.0), (40, 20.0), (64, 16.0), (127, 25.0), (149, 14.0)):
+        ops[3][:, at] = -rate
+    want = exact(ops, None, do, dh)["g"]
+    leaves = [x.detach().requires_grad_() for x in ops]
+    o, h = gated_delta(*leaves[:5], h0=leaves[5], return_state=True)
+    got, = torch.autograd.grad([o, h], leaves[3], [do, dh])
+    # Without its factor a token's gradient is of the size that the other tokens' are.
+    size = want.square().mean().sqrt() * ops[3].double().exp()
+    off = (got.double() - want).abs()
+    assert (off <= 2.0 ** -24 * want.abs() + GRAD * torch.maximum(want.abs(), 8 * size)).all(), (off / size).max()
