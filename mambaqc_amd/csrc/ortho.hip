@@ -204,7 +204,7 @@ __global__ __launch_bounds__(256) void ortho_init_kernel(Args a) {
     tile[r][c] = v;
   }
   __syncthreads();
-  const float norm = (float)total, scale = kScale / (norm < a.eps ? a.eps : norm);
+  const double scale = kScale / (total < a.eps ? (double)a.eps : total);  // (a norm may lie past fp32's ends)
   char* ws = a.ws + g.base + i * g.each;
   const bool tall = g.rows > g.cols;
   // By the rows of what was read, and turned.
@@ -216,10 +216,10 @@ __global__ __launch_bounds__(256) void ortho_init_kernel(Args a) {
   for (int r = threadIdx.x >> 4; r < 64; r += 16) {
     float v[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = tile[r][q + k] * scale;
+    for (int k = 0; k < 4; ++k) v[k] = (float)(tile[r][q + k] * scale);
     if (r0 + r < g.rows) put4<PAIR>(straight + (r0 + r) * sp, c0 + q, v, tall ? second : none);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = tile[q + k][r] * scale;
+    for (int k = 0; k < 4; ++k) v[k] = (float)(tile[q + k][r] * scale);
     if (c0 + r < g.cols) put4<PAIR>(turned + (c0 + r) * tp, r0 + q, v, tall ? none : second);
   }
 }

@@ -289,3 +289,16 @@ def test_muon_step_of_large_tiles_in_a_graph(dtype):
         # m = 0.1 g, u = 0.9 m + 0.1 g: a multiple of g.
         step = 0.5 * max(1.0, s[0] / s[1]) ** 0.5 * iterate(g)
         hold("p", p, b.double() * (1 - 0.5 * 0.1) - step, REL[dtype])
+
+
+@pytest.mark.parametrize("size", [1e-38, 1e-37, 1e36, 1e37])
+@pytest.mark.parametrize("shape", [(40, 90), (90, 40), (300, 280)])
+def test_norms_past_the_ends_of_fp32(size, shape):
+    """Norms that no fp32 number holds, and ones whose inverse is none."""
+    x = make(shape, torch.float32) * size
+    assert x.isfinite().all()
+    hold("x", orthogonalize(x, eps=0.0), iterate(x, eps=0.0), REL[torch.float32])
+    p, m = make(shape, torch.float32), torch.zeros(shape, device=DEV)
+    want, _ = reference(p, x, m, 0.5, 0.0, False, 0.0, eps=0.0)
+    muon_step_([p], [x], [m], lr=0.5, momentum=0.0, nesterov=False, weight_decay=0.0, eps=0.0)
+    hold("p", p, want, REL[torch.float32])
