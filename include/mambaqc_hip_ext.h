@@ -250,9 +250,9 @@ int mqc_layer_norm_bwd(const void* x, int64_t x_row, const float* weight, const 
 
 /* Newton's and Schulz's iteration for each of `batch` matrices [rows, cols], dense, x to out (which may be x):
  *   X = x / max(|x|_F, eps);  `steps` times  A = X X^T,  X = a X + (b A + c A^2) X
- * (on the shorter side). Singular values of X and of A have to stay below 64 on the way. bf16 matrices pass
- * through products of fp16 operands, fp32 and fp16 ones through pairs of them (2^-22 of a value). steps 1 to
- * 100; MQC_E_LIMIT beyond 65535 matrices, a shorter side of 32768, a longer one of 2^24 and launches of 2^32
+ * (on the shorter side). Elements of X, of A and of b A + c A^2 have to stay below 255 on the way: they are
+ * held in fp16 times 2^8. bf16 matrices pass through products of fp16 operands, fp32 and fp16 ones through
+ * pairs of them (2^-22 of a value). steps 1 to 100; MQC_E_LIMIT beyond 65535 matrices, a shorter side of 32768, a longer one of 2^24 and launches of 2^32
  * threads. workspace (256-byte aligned) of mqc_orthogonalize_workspace_bytes.
  *
  * mqc_muon_step: for each of `count` matrices, rows of six values p, grad, m, rows, cols, dtype (pointers as

@@ -31,7 +31,7 @@ namespace ortho {
 using namespace mfma;
 
 constexpr int kMatrices = 64, kGroups = 16;  // of a launch
-constexpr float kScale = 256.f;
+constexpr float kScale = 256.f;              // (an fp16 number ends at 65504: values have to stay below 255)
 constexpr int64_t kPartElems = 4096;         // elements that a workgroup adds the squares of
 constexpr int64_t kMaxParts = 256;
 constexpr int kOnePiece = 256;

@@ -318,7 +318,8 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=COEFFICIENTS,
                   eps: float = 1e-7) -> torch.Tensor:
     """x [..., rows, cols] (fp32, bf16 or fp16) after `steps` of Newton's and Schulz's iteration, in its
     dtype: each matrix over max(its 2-norm, eps), then X <- a X + (b A + c A^2) X with A = X X^T, which
-    brings its singular values near 1. The coefficients have to keep them below 64 on the way. fp32 and
+    brings its singular values near 1. The coefficients have to keep the elements of X, of A and of b A + c A^2
+    below 255 on the way (their singular values below it is enough): beyond, results are not finite. fp32 and
     fp16 matrices are iterated at fp32's accuracy, bf16 ones with 11-bit operands (off by an eighth of what
     the matrix' own 8 bits do). No autograd."""
     how = _iteration("orthogonalize", steps, coefficients, eps)

@@ -302,3 +302,20 @@ def test_norms_past_the_ends_of_fp32(size, shape):
     want, _ = reference(p, x, m, 0.5, 0.0, False, 0.0, eps=0.0)
     muon_step_([p], [x], [m], lr=0.5, momentum=0.0, nesterov=False, weight_decay=0.0, eps=0.0)
     hold("p", p, want, REL[torch.float32])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1, 1), (20, 33), (300, 280)])
+def test_values_just_below_what_the_iteration_holds(dtype, shape):
+    """Elements of X, A and b A + c A^2 have to be below 255. One direction, whose singular value goes 1 -> 15.9 ->
+    52.6, with A = 252.8 in the second step; and one with b A + c A^2 = 253 and X = 254."""
+    x = make((shape[0], 1), torch.float32) @ make((1, shape[1]), torch.float32, seed=5)
+    x = (x / x.abs().max()).to(dtype)
+    if dtype != torch.float32 and shape != (1, 1):  # (rounded, it has more directions than one)
+        x = torch.zeros_like(x)
+        x[3, 5] = -1.0
+    for coefficients in ((15.95, -0.05, 0.0), (1.0, 13.0, 240.0)):
+        steps = 1 if coefficients[0] == 1.0 else 2
+        want = iterate(x, steps, coefficients)
+        assert want.isfinite().all()
+        hold(coefficients, orthogonalize(x, steps=steps, coefficients=coefficients), want, REL[dtype])
