@@ -251,14 +251,16 @@ int mqc_layer_norm_bwd(const void* x, int64_t x_row, const float* weight, const 
 /* Newton's and Schulz's iteration for each of `batch` matrices [rows, cols], dense, x to out (which may be x):
  *   X = x / max(|x|_F, eps);  `steps` times  A = X X^T,  X = a X + (b A + c A^2) X
  * (on the shorter side). Elements of X, of A and of b A + c A^2 have to stay below 255 on the way: they are
- * held in fp16 times 2^8. bf16 matrices pass through products of fp16 operands, fp32 and fp16 ones through
- * pairs of them (2^-22 of a value). steps 1 to 100; MQC_E_LIMIT beyond 65535 matrices, a shorter side of 32768, a longer one of 2^24 and launches of 2^32
+ * held in fp16 times 2^8. Matrices pass through products of pairs of fp16 operands (2^-22 of a value); bf16 ones
+ * with a shorter side of 256 or more of single ones (2^-12), unless dtype is MQC_BF16 | MQC_ORTHO_PAIRS (allowed
+ * with the other types, whose matrices are in pairs without it). steps 1 to 100; MQC_E_LIMIT beyond 65535 matrices, a shorter side of 32768, a longer one of 2^24 and launches of 2^32
  * threads. workspace (256-byte aligned) of mqc_orthogonalize_workspace_bytes.
  *
- * mqc_muon_step: for each of `count` matrices, rows of six values p, grad, m, rows, cols, dtype (pointers as
- * integers, dense, aligned to their elements; m fp32; read before the call returns):
+ * mqc_muon_step: for each of `count` matrices, rows of six values p, grad, m, rows, cols, dtype (as above;
+ * pointers as integers, dense, aligned to their elements; m fp32; read before the call returns):
  *   m = momentum m + (1 - momentum) grad,  u = momentum m + (1 - momentum) grad (nesterov) or m
  *   p = p decay - rate sqrt(max(1, rows / cols)) X  with X from u as above */
+#define MQC_ORTHO_PAIRS 16
 int64_t mqc_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int dtype);
 int mqc_orthogonalize(const void* x, void* out, int64_t batch, int64_t rows, int64_t cols, int steps,
                       float a, float b, float c, float eps, int dtype, void* workspace,

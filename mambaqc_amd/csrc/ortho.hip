@@ -12,12 +12,15 @@
 // mirrors. Every matrix of a call is in the same launches, whatever its shape.
 //
 // Operands are fp16 times 2^8 (X, A and B have values up to about 3, and most near n^-1/2), accumulators
-// fp32. For matrices in fp32 and fp16 a value is two fp16 pieces, held to 2^-23 of itself or 2^-33, and a
-// product three: off by 2e-6. For those in bf16 it is one (of shorter sides from kOnePiece on: roundings
-// average out over a side, and short ones take no less time with one), but X itself, which a X goes on
-// from, keeps its second piece: weak directions grow 3.4 times a step by a X alone, and a rounding of X with
-// them (a matrix of eight strong directions comes out off by 3e-4 of it, without that piece by 0.04,
-// iterated in bf16 by 0.3; gradients with a sixteenth of strong directions by 8e-4).
+// fp32. A value is two fp16 pieces, held to 2^-23 of itself or 2^-33, and a product three: off by 2e-6 at
+// sides of 1024, 4.6e-6 at 12000 (a product of fp32 operands by 3e-6 and 7e-6). Matrices in bf16 may have one
+// piece, where the caller leaves them that (from shorter sides of kOnePiece on: roundings average out over a
+// side, and short ones take no less time with one): off by 1e-3 where bf16's own rounding is 1.7e-3, in 443 us
+// for 744 to 805 (12 matrices of 1536 by 768), 1460 for 2290 to 2390 (the step of 8 blocks of width 512) or 1934
+// for 4063 (8 of 2048 by 2048). X itself, which a X goes on from, keeps its second piece then too: weak
+// directions grow 3.4 times a step by a X alone, and a rounding of X with them (a matrix of eight strong
+// directions comes out off by 3e-4 of it, without that piece by 0.04, iterated in bf16 by 0.3; gradients with a
+// sixteenth of strong directions by 8e-4).
 #include <algorithm>
 #include <climits>
 #include <new>
@@ -150,7 +153,7 @@ __global__ __launch_bounds__(256) void ortho_sum_kernel(Args a) {
   if (threadIdx.x == 0) a.sums[g.parts + (int64_t)i * g.sums + part] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// --- X_0 by rows and turned (of the same 116 us, 4.3 TB/s) ------------------------------------------------
+// --- X_0 by rows and turned (of the same in pairs 151 us, 590 MB at 3.9 TB/s) ----------------------------
 // Four values (times kScale) into a row, col a multiple of 4; the second pieces `second` bytes on (0: none).
 __device__ inline float half_of(const u32x2& v, int c) {
   return io<f16_t>::bits_to_f32(c & 1 ? v[c / 2] >> 16 : v[c / 2] & 0xffffu);
@@ -293,9 +296,9 @@ __device__ inline void put_result(T* to, int left, float (&v)[8], float decay, f
 // A tile's rows w of the left operand and x of the right one, S of each. What it leaves goes through LDS,
 // the columns of a wave at a time: rows of x are written along w, and (the mirrored half of a symmetric
 // product, X by rows, a wide matrix) rows of w along x, 16 bytes a lane. (Written from the registers, two
-// bytes a lane, a step for the matrices of 8 blocks of width 512 took 2458 us; with this, and long sides
-// shared, 2034.) Then the symmetric products take 61 + 7 + 42 us of it a time, the last one 151: 60 GFLOP,
-// and 420 MB at 2.8 TB/s that its products do not hide.
+// bytes a lane, a step for the matrices of 8 blocks of width 512 took 2458 us in single pieces; with this,
+// and long sides shared, 2034.) In pairs the symmetric products take 116 + 7 + 83 us of it a time, the last one
+// 231: 60 GFLOP in three products, 0.78 PFLOP/s.
 template <typename T, typename Cfg, bool PAIR, int STAGE, bool MUON>
 __global__ __launch_bounds__(Cfg::kThreads, 2) void ortho_product_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -505,9 +508,9 @@ int64_t total(const Args& a, const Count& count) {
   return n;
 }
 // The side of a launch's tiles. The last product's are of 256 rows by 256 where they fill the card (half the
-// bytes to LDS: with 8 bf16 matrices of 2048 x 2048 a call takes 1930 us for 2074 at 128; with two, of 128
-// such tiles, 772 for 653), the symmetric ones, of fewer and with half a tile lost on the diagonal, of 128
-// (all at 256: 2136); where fewer than 128 of these are left, of 64.
+// bytes to LDS: with 8 matrices of 2048 x 2048 a call takes 4063 us in pairs for 4267 at 128, in single pieces
+// 1934 for 2088; with two, of 128 such tiles, in single pieces 772 for 653), the symmetric ones, of fewer and
+// with half a tile lost on the diagonal, of 128 (all at 256: 2136); where fewer than 128 of these are left, of 64.
 template <int STAGE>
 int tile_side(const Args& a) {
   if ((STAGE == ortho::APPLY || STAGE == ortho::LAST) && total(a, ortho::tile_count<STAGE, 256>) >= 256) return 256;
@@ -635,7 +638,12 @@ int iterate(Args& a, int steps, hipStream_t s) {
   return st;
 }
 
-bool paired(int dtype, int64_t rows, int64_t cols) {
+// A dtype of the C interface: the type, and whether bf16 matrices of any size are iterated in pairs.
+int type_of(int64_t dtype) {
+  const int64_t type = dtype & ~(int64_t)MQC_ORTHO_PAIRS;
+  return type == MQC_F32 || type == MQC_BF16 || type == MQC_F16 ? (int)type : -1;
+}
+bool paired(int64_t dtype, int64_t rows, int64_t cols) {
   return dtype != MQC_BF16 || std::min(rows, cols) < ortho::kOnePiece;
 }
 
@@ -658,8 +666,8 @@ int run_pieces(Args& a, int steps, char* ws, hipStream_t s) {
 template <bool MUON>
 int run(Args& a, int dtype, int steps, char* ws, hipStream_t s) {
   const bool pair = paired(dtype, a.groups[0].rows, a.groups[0].cols);
-  if (dtype == MQC_F32) return run_pieces<float, true, MUON>(a, steps, ws, s);
-  if (dtype == MQC_F16) return run_pieces<f16_t, true, MUON>(a, steps, ws, s);
+  if (type_of(dtype) == MQC_F32) return run_pieces<float, true, MUON>(a, steps, ws, s);
+  if (type_of(dtype) == MQC_F16) return run_pieces<f16_t, true, MUON>(a, steps, ws, s);
   return pair ? run_pieces<bf16_t, true, MUON>(a, steps, ws, s) : run_pieces<bf16_t, false, MUON>(a, steps, ws, s);
 }
 
@@ -674,7 +682,7 @@ void batches(const int64_t* rows, int64_t count, float rate, std::vector<Batch>&
     const bool pair = kind < 3;
     std::vector<int64_t> order;
     for (int64_t i = 0; i < count; ++i)
-      if (rows[6 * i + 5] == dtype && paired(dtype, rows[6 * i + 3], rows[6 * i + 4]) == pair)
+      if (type_of(rows[6 * i + 5]) == dtype && paired(rows[6 * i + 5], rows[6 * i + 3], rows[6 * i + 4]) == pair)
         order.push_back(i);
     std::stable_sort(order.begin(), order.end(), [&](int64_t x, int64_t y) {
       const int64_t *u = rows + 6 * x, *v = rows + 6 * y;
@@ -700,7 +708,7 @@ void batches(const int64_t* rows, int64_t count, float rate, std::vector<Batch>&
       }
       b.bytes = lay_out(b.args, pair);
       out.push_back(b);
-      types.push_back(dtype);
+      types.push_back(pair ? dtype | MQC_ORTHO_PAIRS : dtype);
     }
   }
 }
@@ -710,7 +718,7 @@ int table(const int64_t* rows, int64_t count) {
   if (count > 0 && !rows) return MQC_E_NULL;
   for (int64_t i = 0; i < count; ++i) {
     const int64_t* r = rows + 6 * i;
-    if (r[5] != MQC_F32 && r[5] != MQC_BF16 && r[5] != MQC_F16) return MQC_E_DTYPE;
+    if (type_of(r[5]) < 0) return MQC_E_DTYPE;
     const int st = shape(r[3], r[4]);
     if (st != MQC_OK) return st;
   }
@@ -733,7 +741,7 @@ extern "C" int64_t mqc_orthogonalize_workspace_bytes(int64_t batch, int64_t rows
   if (batch < 0) return MQC_E_SHAPE;
   const int st = shape(rows, cols);
   if (st != MQC_OK) return st;
-  if (dtype != MQC_F32 && dtype != MQC_BF16 && dtype != MQC_F16) return MQC_E_DTYPE;
+  if (type_of(dtype) < 0) return MQC_E_DTYPE;
   if (batch > 65535) return MQC_E_LIMIT;
   Args a = one_stack(nullptr, nullptr, batch, rows, cols);
   return lay_out(a, paired(dtype, rows, cols));

@@ -295,6 +295,7 @@ class AdamW(torch.optim.Optimizer):
 # --- orthogonalised updates of matrices ------------------------------------------------------------
 
 COEFFICIENTS = (3.4445, -4.775, 2.0315)  # of Muon: a steep start, and an end between 0.7 and 1.2
+_PAIRS = 16  # MQC_ORTHO_PAIRS
 
 
 def _iteration(name, steps, coefficients, eps):
@@ -307,6 +308,10 @@ def _iteration(name, steps, coefficients, eps):
     return (steps, *map(float, coefficients), eps)
 
 
+def _code(x, fast_bf16):
+    return nat.dtype_code(x) | (0 if fast_bf16 else _PAIRS)
+
+
 def _workspace(nbytes, name, like):
     if nbytes < 0:
         nat.check(nbytes, name)
@@ -315,17 +320,18 @@ def _workspace(nbytes, name, like):
 
 @torch.no_grad()
 def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=COEFFICIENTS,
-                  eps: float = 1e-7) -> torch.Tensor:
+                  eps: float = 1e-7, fast_bf16: bool = False) -> torch.Tensor:
     """x [..., rows, cols] (fp32, bf16 or fp16) after `steps` of Newton's and Schulz's iteration, in its
     dtype: each matrix over max(its 2-norm, eps), then X <- a X + (b A + c A^2) X with A = X X^T, which
     brings its singular values near 1. The coefficients have to keep the elements of X, of A and of b A + c A^2
-    below 255 on the way (their singular values below it is enough): beyond, results are not finite. fp32 and
-    fp16 matrices are iterated at fp32's accuracy, bf16 ones with 11-bit operands (off by an eighth of what
-    the matrix' own 8 bits do). No autograd."""
+    below 255 on the way (their singular values below it is enough): beyond, results are not finite.
+    Everything is iterated at fp32's accuracy and rounded once. fast_bf16: bf16 matrices with a shorter side of
+    256 or more with 11-bit operands instead, in half to two thirds of the time, off by 1e-3 (the type's own
+    rounding: 1.7e-3). No autograd."""
     how = _iteration("orthogonalize", steps, coefficients, eps)
     if x.dim() < 2:
         raise ValueError(f"orthogonalize: x is [..., rows, cols], got {tuple(x.shape)}")
-    dtype = nat.dtype_code(x)
+    dtype = _code(x, fast_bf16)
     nat.require_device("orthogonalize", x)
     x = x.detach().contiguous().resolve_neg()
     out = torch.empty_like(x)
@@ -340,7 +346,7 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=COEFFICIENTS,
     return out
 
 
-def _muon_rows(name, params, grads, momenta):
+def _muon_rows(name, params, grads, momenta, fast_bf16=False):
     """The rows that mqc_muon_step reads."""
     _check_lengths(name, params, grads, momenta)
     for p in params:
@@ -354,20 +360,20 @@ def _muon_rows(name, params, grads, momenta):
     spans = sorted((t.data_ptr(), t.data_ptr() + t.nbytes) for t in written)
     if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
         raise ValueError(f"{name}: a parameter is there twice, or two of them share memory")
-    return [(p.data_ptr(), g.data_ptr(), m.data_ptr(), *p.shape, nat.dtype_code(p))
+    return [(p.data_ptr(), g.data_ptr(), m.data_ptr(), *p.shape, _code(p, fast_bf16))
             for p, g, m in zip(params, grads, momenta) if p.numel()]
 
 
 @torch.no_grad()
 def muon_step_(params, grads, momenta, *, lr: float = 1e-3, momentum: float = 0.95, nesterov: bool = True,
                weight_decay: float = 0.1, steps: int = 5, coefficients=COEFFICIENTS,
-               eps: float = 1e-7) -> None:
+               eps: float = 1e-7, fast_bf16: bool = False) -> None:
     """One Muon step in place over lists of matrices: contiguous parameters and gradients of one dtype each
     (fp32, bf16 or fp16), no two parameters in the same memory, fp32 momenta of their sizes. The iteration
-    is orthogonalize's."""
+    (and fast_bf16) is orthogonalize's."""
     params, grads, momenta = list(params), list(grads), list(momenta)
     how = _iteration("muon_step_", steps, coefficients, eps)
-    rows = _muon_rows("muon_step_", params, grads, momenta)
+    rows = _muon_rows("muon_step_", params, grads, momenta, fast_bf16)
     _launch_muon(rows, (params, momenta), lr, momentum, nesterov, weight_decay, how)
 
 
@@ -386,11 +392,11 @@ def _launch_muon(rows, changed, lr, momentum, nesterov, weight_decay, how):
 
 class Muon(torch.optim.Optimizer):
     """Muon over the kernels of this module, for parameters that are matrices (embeddings, heads, norms and
-    biases belong to an AdamW beside it). Momenta are fp32."""
+    biases belong to an AdamW beside it). Momenta are fp32. fast_bf16: as orthogonalize's."""
 
     def __init__(self, params, lr: float = 1e-3, momentum: float = 0.95, nesterov: bool = True,
                  weight_decay: float = 0.1, steps: int = 5, coefficients=COEFFICIENTS,
-                 eps: float = 1e-7):
+                 eps: float = 1e-7, fast_bf16: bool = False):
         if lr < 0 or weight_decay < 0:
             raise ValueError(f"Muon: lr {lr} and weight_decay {weight_decay} are not negative")
         if not 0 <= momentum < 1:
@@ -398,7 +404,13 @@ class Muon(torch.optim.Optimizer):
         _iteration("Muon", steps, coefficients, eps)
         super().__init__(params, {"lr": lr, "momentum": momentum, "nesterov": nesterov,
                                   "weight_decay": weight_decay, "steps": steps,
-                                  "coefficients": tuple(coefficients), "eps": eps})
+                                  "coefficients": tuple(coefficients), "eps": eps,
+                                  "fast_bf16": fast_bf16})
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for group in self.param_groups:  # (saved before there was one)
+            group.setdefault("fast_bf16", False)
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
@@ -435,8 +447,9 @@ class Muon(torch.optim.Optimizer):
         for group, entries in work:
             params, grads, momenta = map(list, zip(*entries))
             how = _iteration("Muon", group["steps"], group["coefficients"], group["eps"])
-            _launch_muon(_muon_rows("Muon", params, grads, momenta), (params, momenta), group["lr"],
-                         group["momentum"], group["nesterov"], group["weight_decay"], how)
+            rows = _muon_rows("Muon", params, grads, momenta, group["fast_bf16"])
+            _launch_muon(rows, (params, momenta), group["lr"], group["momentum"], group["nesterov"],
+                         group["weight_decay"], how)
         return loss
 
     def load_state_dict(self, state_dict):

@@ -319,3 +319,90 @@ def test_values_just_below_what_the_iteration_holds(dtype, shape):
         want = iterate(x, steps, coefficients)
         assert want.isfinite().all()
         hold(coefficients, orthogonalize(x, steps=steps, coefficients=coefficients), want, REL[dtype])
+
+
+def rounded_once(what, got, want, rel):
+    """Each element is want's rounding, but for an error before it of rel as a 2-norm, of which one of up to a
+    million elements has eight times the root mean square at most."""
+    off, rms = (got.double() - want).abs(), want.square().mean().sqrt()
+    bad = ~(off <= torch.finfo(got.dtype).eps / 2 * want.abs() + 8 * rel * rms)
+    assert not bad.any(), (what, int(bad.sum()), (off / rms)[bad][:4], (want / rms)[bad][:4])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(300, 280), (2, 515, 1000), (700, 260), (256, 256), (40, 600)])
+def test_rounded_once(dtype, shape):
+    """16-bit matrices too are iterated at fp32's accuracy: their only rounding to 16 bits is the last."""
+    x = make(shape, dtype)
+    rounded_once("x", orthogonalize(x), iterate(x), 2.0 ** -18)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_muon_step_rounds_once(dtype):
+    shapes = [(300, 280), (256, 512), (40, 30), (515, 300)]
+    params = [0.02 * make(s, dtype, seed=i) for i, s in enumerate(shapes)]
+    grads = [make(s, dtype, seed=100 + i) for i, s in enumerate(shapes)]
+    momenta = [make(s, torch.float32, seed=200 + i) for i, s in enumerate(shapes)]
+    want = [reference(p, g, m, 0.02, 0.95, True, 0.1) for p, g, m in zip(params, grads, momenta)]
+    opt = Muon([torch.nn.Parameter(p.clone()) for p in params], lr=0.02)
+    muon_step_(params, grads, momenta, lr=0.02)
+    for i, (p, (w, _)) in enumerate(zip(params, want)):
+        rounded_once(i, p, w, 2.0 ** -18)
+    for p, g in zip(opt.param_groups[0]["params"], grads):
+        before, p.grad = p.detach().clone(), g
+        opt.step()
+        rounded_once("opt", p.detach(), reference(before, g, 0 * g, 0.02, 0.95, True, 0.1)[0], 2.0 ** -18)
+        p.grad = None
+
+
+@pytest.mark.parametrize("kind", ["normal", "weak"])
+@pytest.mark.parametrize("shape", [(300, 280), (5, 600, 300), (256, 2100), (900, 1030)])
+def test_fast_bf16(shape, kind):
+    """Operands of 11 bits (the tolerance above)."""
+    x = make(shape, torch.bfloat16, kind=kind)
+    y = orthogonalize(x, fast_bf16=True)
+    rel = 2.0 ** -9 + (2 * 377 * 2.0 ** -23 if kind == "weak" else 0)
+    hold("x", y, iterate(x), rel)
+    assert not torch.equal(y, orthogonalize(x))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(300, 280), (255, 400), (30, 20)])
+def test_fast_bf16_leaves_others_as_they_are(dtype, shape):
+    x = make(shape, dtype)
+    same = torch.equal(orthogonalize(x, fast_bf16=True), orthogonalize(x))
+    assert same == (dtype != torch.bfloat16 or min(shape) < 256)
+
+
+def test_fast_bf16_steps():
+    """In a list beside other types and sizes, in an optimizer's group and in a graph."""
+    shapes = [(300, 280), (64, 40), (300, 280), (280, 512), (300, 280)]
+    types = [torch.bfloat16, torch.bfloat16, torch.float32, torch.bfloat16, torch.float16]
+    params = [0.02 * make(s, t, seed=i) for i, (s, t) in enumerate(zip(shapes, types))]
+    grads = [make(s, t, seed=100 + i) for i, (s, t) in enumerate(zip(shapes, types))]
+    momenta = [torch.zeros(s, device=DEV) for s in shapes]
+    copy_of = lambda ts: [t.clone() for t in ts]
+    exact, fast, graphed = copy_of(params), copy_of(params), copy_of(params)
+    muon_step_(exact, grads, copy_of(momenta), lr=0.02)
+    muon_step_(fast, grads, copy_of(momenta), lr=0.02, fast_bf16=True)
+    for i, (p, e, f, g) in enumerate(zip(params, exact, fast, grads)):
+        big = types[i] == torch.bfloat16 and min(shapes[i]) >= 256
+        assert torch.equal(e, f) != big
+        want, _ = reference(p, g, 0 * g.double(), 0.02, 0.95, True, 0.1)
+        hold(i, f, want, 2.0 ** -9 if big else 2.0 ** -18)
+    weights = [torch.nn.Parameter(p.clone()) for p in params]
+    opt = Muon([{"params": weights[:3], "fast_bf16": True}, {"params": weights[3:]}], lr=0.02)
+    for w, g in zip(weights, grads):
+        w.grad = g
+    opt.step()
+    for i, w in enumerate(weights):
+        assert torch.equal(w.detach(), fast[i] if i < 3 else exact[i])
+    kept, graph = copy_of(momenta), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        muon_step_(graphed, grads, kept, lr=0.02, fast_bf16=True)
+    for _ in range(3):
+        for a, b, m in zip(graphed, params, kept):
+            a.copy_(b), m.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, f) for a, f in zip(graphed, fast))

@@ -92,3 +92,26 @@ def test_validation_codes():
     big = [4096, 4096, 4096, 32768, 1 << 24, 1]
     assert f(r=32768, c=1 << 24, dtype=1, ws=1 << 62) == -5
     assert step([row, big], ws=1 << 62) == -5 and step([big, row], ws=1 << 62) == -5
+
+
+def test_pairs_for_every_type():
+    """The C interface's choice for bf16 matrices: as much room as fp32's take; none for the other types."""
+    size = nat.load().mqc_orthogonalize_workspace_bytes
+    assert size(1, 512, 300, 17) == size(1, 512, 300, 0) == size(1, 512, 300, 16) == size(1, 512, 300, 18)
+    assert size(1, 512, 300, 1) < size(1, 512, 300, 17) and size(1, 64, 64, 1) == size(1, 64, 64, 17)
+    for bad in (-1, 3, 15, 19, 32, 33):
+        assert size(1, 512, 300, bad) == -3
+    room = nat.load().mqc_muon_workspace_bytes
+    table = lambda dtype: array.array("q", [4096, 4096, 4096, 512, 300, dtype]).tobytes()
+    assert room(table(1), 1) < room(table(17), 1) == room(table(0), 1) and room(table(19), 1) == -3
+    both = array.array("q", [4096, 4096, 4096, 512, 300, 1, 4096, 4096, 4096, 512, 300, 17]).tobytes()
+    assert room(both, 2) == room(table(17), 1)
+
+
+def test_groups_saved_without_the_choice():
+    p = torch.nn.Parameter(torch.zeros(2, 3))
+    opt = Muon([p], fast_bf16=True)
+    saved = opt.state_dict()
+    assert saved["param_groups"][0].pop("fast_bf16") is True
+    opt.load_state_dict(saved)
+    assert opt.param_groups[0]["fast_bf16"] is False
