@@ -406,3 +406,21 @@ def test_fast_bf16_steps():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, f) for a, f in zip(graphed, fast))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(2048, 2048), (2, 2100, 3000), (2500, 2200)])
+def test_long_short_sides(dtype, shape):
+    x = make(shape, dtype)
+    hold("x", orthogonalize(x), iterate(x), REL[dtype])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_short_sides_past_8192(dtype):
+    """All three products sum over n = 8500 elements, for which the fp32 accumulators count too: three roundings
+    per 32 elements, each 2^-24 / sqrt(3) (as squares) of a partial sum that is 1 / sqrt(2) of the whole one on
+    the average, (3 n / 32)^1/2 2^-24 / sqrt(6) = 2^-20.5 a product beside the 2^-21 above. Of fifteen products,
+    twice that: 2^-17.2."""
+    x = make((8500, 8400), dtype)
+    rel = 2 * 15 ** 0.5 * (2.0 ** -42 + 3 * 8500 / 32 * 2.0 ** -48 / 6) ** 0.5
+    hold("x", orthogonalize(x), iterate(x), rel)
