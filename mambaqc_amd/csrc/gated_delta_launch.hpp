@@ -10,11 +10,20 @@ namespace delta {
   if (a.k_dim <= 64) return F(64);  \
   return F(128);
 
-// Columns of the state to a workgroup: 16 as long as the card has room for more workgroups.
+// Columns of the state to a workgroup: 16 as long as the card has room for more workgroups, which is one to a CU
+// (of eight waves, or of four for fp32's 128 keys, whose operands leave no registers for it), and two where the
+// registers of two fit. 384 walks of 16 columns over 16 chunks, forward and back, us, by 16 and by 32 columns:
+//   bf16, 128 keys 73 + 72, 78 + 82;  64 keys 52 + 55, 66 + 66;  32 keys 47 + 52, 64 + 63
+//   fp16, 128 keys 113 + 119, 90 + 99;  64 keys 66 + 61, 72 + 69;  32 keys 49 + 52, 65 + 65
+//   fp32, 128 keys 139 + 134, 109 + 110;  64 keys 92 + 102, 75 + 82;  32 keys 79 + 87, 69 + 70
+// (256 of them: bf16, 128 keys 40 + 38, fp32 68 + 82; 1024: 182 + 182 and 255 + 266.)
+template <typename T, int KD>
+constexpr bool kTwoToACu = kIn<T> == 1 || (kIn<T> == 2 && KD < 128);
 template <typename T, int KD, bool BWD>
 int launch_walk(const Args<T>& a, hipStream_t s) {
   const int64_t tiles = a.v_pad / 16, heads = a.batch * a.v_heads;
-  if constexpr (kIn<T> < 3 || KD < 128) {  // (fp32's operands of 128 keys leave no registers for it)
+  constexpr bool kBeside = kIn<T> < 3 || KD < 128;
+  if constexpr (kBeside) {
     if (heads * tiles <= 256) {
       const dim3 grid((unsigned)(heads * tiles));
       if constexpr (BWD) delta_bwd_beside_kernel<T, KD><<<grid, dim3(512), 0, s>>>(a);
@@ -22,15 +31,17 @@ int launch_walk(const Args<T>& a, hipStream_t s) {
       return launch_status();
     }
   }
-  if (heads * tiles <= 512) {
-    const dim3 grid((unsigned)(heads * tiles));
-    if constexpr (BWD) delta_bwd_kernel<T, KD, 1><<<grid, dim3(256), 0, s>>>(a);
-    else delta_fwd_kernel<T, KD, 1><<<grid, dim3(256), 0, s>>>(a);
-  } else {
-    const dim3 grid((unsigned)(heads * (tiles / 2)));
-    if constexpr (BWD) delta_bwd_kernel<T, KD, 2><<<grid, dim3(256), 0, s>>>(a);
-    else delta_fwd_kernel<T, KD, 2><<<grid, dim3(256), 0, s>>>(a);
+  if constexpr (!kBeside || kTwoToACu<T, KD>) {
+    if (heads * tiles <= (kTwoToACu<T, KD> ? 512 : 256)) {
+      const dim3 grid((unsigned)(heads * tiles));
+      if constexpr (BWD) delta_bwd_kernel<T, KD, 1><<<grid, dim3(256), 0, s>>>(a);
+      else delta_fwd_kernel<T, KD, 1><<<grid, dim3(256), 0, s>>>(a);
+      return launch_status();
+    }
   }
+  const dim3 grid((unsigned)(heads * (tiles / 2)));
+  if constexpr (BWD) delta_bwd_kernel<T, KD, 2><<<grid, dim3(256), 0, s>>>(a);
+  else delta_fwd_kernel<T, KD, 2><<<grid, dim3(256), 0, s>>>(a);
   return launch_status();
 }
 
