@@ -10,6 +10,8 @@ import torch.nn as nn
 
 from .. import _native as nat
 
+MAX_WIDTH = 8192  # elements of a row: sixteen in the registers of each of a workgroup's 512 lanes
+
 
 def _check(x, weight, bias):
     if x.dim() < 1:
@@ -42,14 +44,16 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None, bias: torch.
 
 
 class LayerNorm(nn.LayerNorm):
-    """nn.LayerNorm over the last axis on the kernel (same parameters and state dict). The output is in
-    the input's dtype, under autocast too."""
+    """nn.LayerNorm over the last axis, of at most 8192 elements, on the kernel (same parameters and state
+    dict). The output is in the input's dtype, under autocast too."""
 
     def __init__(self, normalized_shape, eps: float = 1e-5, elementwise_affine: bool = True,
                  bias: bool = True, device=None, dtype=None):
         super().__init__(normalized_shape, eps, elementwise_affine, bias, device, dtype)
         if len(self.normalized_shape) != 1:
             raise ValueError(f"LayerNorm: normalises over the last axis, got {self.normalized_shape}")
+        if self.normalized_shape[0] > MAX_WIDTH:
+            raise ValueError(f"LayerNorm: rows have at most {MAX_WIDTH} elements, got {self.normalized_shape[0]}")
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.dim() < 1 or x.shape[-1] != self.normalized_shape[0]:

@@ -62,3 +62,12 @@ def test_fake_kernels():
         x = torch.empty(2, 7, 6, device="cuda", dtype=torch.bfloat16)
         y, stats = torch.ops.mambaqc.layer_norm(x, torch.empty(6, device="cuda"))
         assert y.shape == x.shape and y.dtype == x.dtype and stats.shape == (14, 2)
+
+
+def test_too_wide_a_module_is_refused_as_it_is_made():
+    from mambaqc_amd.kernels.norm import MAX_WIDTH
+
+    assert MAX_WIDTH == nat.load().mqc_layer_norm_max_width()
+    assert LayerNorm(MAX_WIDTH).normalized_shape == (MAX_WIDTH,)
+    with pytest.raises(ValueError, match="at most 8192"):
+        LayerNorm(MAX_WIDTH + 1)
