@@ -26,6 +26,7 @@ matrices of a type go through the same launches, up to 64 of 16 shapes at a time
 from __future__ import annotations
 
 import array
+import bisect
 import collections
 import itertools
 import math
@@ -360,6 +361,11 @@ def _muon_rows(name, params, grads, momenta, fast_bf16=False):
     spans = sorted((t.data_ptr(), t.data_ptr() + t.nbytes) for t in written)
     if any(b[0] < a[1] for a, b in zip(spans, spans[1:])):
         raise ValueError(f"{name}: a parameter is there twice, or two of them share memory")
+    starts = [start for start, _ in spans]
+    for p, g in zip(params, grads):  # (momenta are written before gradients are read again)
+        last = bisect.bisect_left(starts, g.data_ptr() + g.nbytes) - 1
+        if g.numel() and g.data_ptr() != p.data_ptr() and last >= 0 and spans[last][1] > g.data_ptr():
+            raise ValueError(f"{name}: a gradient shares memory with a momentum or another parameter")
     return [(p.data_ptr(), g.data_ptr(), m.data_ptr(), *p.shape, _code(p, fast_bf16))
             for p, g, m in zip(params, grads, momenta) if p.numel()]
 
@@ -369,8 +375,8 @@ def muon_step_(params, grads, momenta, *, lr: float = 1e-3, momentum: float = 0.
                weight_decay: float = 0.1, steps: int = 5, coefficients=COEFFICIENTS,
                eps: float = 1e-7, fast_bf16: bool = False) -> None:
     """One Muon step in place over lists of matrices: contiguous parameters and gradients of one dtype each
-    (fp32, bf16 or fp16), no two parameters in the same memory, fp32 momenta of their sizes. The iteration
-    (and fast_bf16) is orthogonalize's."""
+    (fp32, bf16 or fp16), fp32 momenta of their sizes, no two parameters in the same memory and no gradient in
+    a momentum's. The iteration (and fast_bf16) is orthogonalize's."""
     params, grads, momenta = list(params), list(grads), list(momenta)
     how = _iteration("muon_step_", steps, coefficients, eps)
     rows = _muon_rows("muon_step_", params, grads, momenta, fast_bf16)

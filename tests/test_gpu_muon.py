@@ -442,3 +442,20 @@ def test_steps_go_downhill(dtype):
         loss.backward()
         opt.step()
     assert all(b < a for a, b in zip(losses, losses[1:])), losses
+
+
+def test_gradients_in_the_momenta_are_refused():
+    """They are read again after the momenta are written. (A parameter may be its own gradient.)"""
+    p, g = make((40, 30), torch.float32), make((40, 30), torch.float32, seed=1)
+    with pytest.raises(ValueError, match="shares memory"):
+        muon_step_([p], [g], [g])
+    wide = torch.cat([g, g])
+    with pytest.raises(ValueError, match="shares memory"):
+        muon_step_([p], [wide[:40]], [wide[39:79]])
+    q = make((40, 30), torch.float32, seed=2)
+    with pytest.raises(ValueError, match="shares memory"):
+        muon_step_([p, q], [q, g], [torch.zeros_like(p), torch.zeros_like(p)])
+    want, _ = reference(p, p.clone(), torch.zeros_like(p), 0.02, 0.95, True, 0.1)
+    muon_step_([p], [p], [torch.zeros_like(p)], lr=0.02)
+    hold("p", p, want, REL[torch.float32])
+    muon_step_([p, q], [g, g], [torch.zeros_like(p), torch.zeros_like(p)])  # read twice, written nowhere
