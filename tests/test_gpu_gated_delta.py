@@ -490,7 +490,7 @@ RATES = (0.5, 5.0, 10.0, 15.0, 30.0, 80.0, 200.0, 1e5)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("dk,reset", [(24, 0.0), (60, 0.03), (128, 0.0), (128, 0.03)])
+@pytest.mark.parametrize("dk,reset", [(24, 0.0), (60, 0.03), (101, 0.02), (128, 0.0), (128, 0.03)])
 def test_gradient_of_log_decay_of_heads_that_forget_fast(dtype, dk, reset):
     """Every term of log_decay's gradient has its token's factor exp(log_decay), so a head's gradients are as
     small as that, and held to a head's own size. (The exponent of a factor is an fp32 number: of the largest
