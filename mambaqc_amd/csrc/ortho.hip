@@ -22,6 +22,7 @@
 // directions comes out off by 3e-4 of it, without that piece by 0.04, iterated in bf16 by 0.3; gradients with a
 // sixteenth of strong directions by 8e-4).
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <new>
 #include <vector>
@@ -596,7 +597,7 @@ int launch_tiles(Args& a, hipStream_t s) {
   if (n == 0) return MQC_OK;
   const auto kernel = ortho::ortho_product_kernel<T, Cfg, PAIR, STAGE, MUON>;
   if (ortho::kLdsBytes<Cfg> > 65536) {  // has to be asked for, once on each device
-    static bool done[kMaxDevices] = {};
+    static std::atomic<bool> done[kMaxDevices];
     int device = -1;
     hipError_t e = hipGetDevice(&device);
     if (e != hipSuccess) return (int)e;

@@ -321,6 +321,42 @@ def test_values_just_below_what_the_iteration_holds(dtype, shape):
         hold(coefficients, orthogonalize(x, steps=steps, coefficients=coefficients), want, REL[dtype])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(2048, 2048), (2, 2100, 3000), (2500, 2200)])
+def test_long_short_sides(dtype, shape):
+    x = make(shape, dtype)
+    hold("x", orthogonalize(x), iterate(x), REL[dtype])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_short_sides_past_8192(dtype):
+    """All three products sum over n = 8500 elements, for which the fp32 accumulators count too: three roundings
+    per 32 elements, each 2^-24 / sqrt(3) (as squares) of a partial sum that is 1 / sqrt(2) of the whole one on
+    the average, (3 n / 32)^1/2 2^-24 / sqrt(6) = 2^-20.5 a product beside the 2^-21 above. Of fifteen products,
+    twice that: 2^-17.2."""
+    x = make((8500, 8400), dtype)
+    rel = 2 * 15 ** 0.5 * (2.0 ** -42 + 3 * 8500 / 32 * 2.0 ** -48 / 6) ** 0.5
+    hold("x", orthogonalize(x), iterate(x), rel)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_steps_go_downhill(dtype):
+    """Of |w - target|^2 / 2 the update X of the gradient has <X, gradient> above 0.6 of its singular values'
+    sum (the iteration ends between 0.68 and 1.21): with steps of at most a tenth of the least singular value
+    of w - target the loss falls in each."""
+    target = torch.eye(30, 40, device=DEV) * 3
+    w = torch.nn.Parameter(torch.zeros(30, 40, device=DEV, dtype=dtype))
+    opt = Muon([w], lr=0.1, momentum=0.0, weight_decay=0.0)
+    losses = []
+    for _ in range(6):
+        loss = (w.float() - target).square().sum() / 2
+        losses.append(loss.item())
+        opt.zero_grad()
+        loss.backward()
+        opt.step()
+    assert all(b < a for a, b in zip(losses, losses[1:])), losses
+
+
 def rounded_once(what, got, want, rel):
     """Each element is want's rounding, but for an error before it of rel as a 2-norm, of which one of up to a
     million elements has eight times the root mean square at most."""
@@ -408,42 +444,6 @@ def test_fast_bf16_steps():
         assert all(torch.equal(a, f) for a, f in zip(graphed, fast))
 
 
-@pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("shape", [(2048, 2048), (2, 2100, 3000), (2500, 2200)])
-def test_long_short_sides(dtype, shape):
-    x = make(shape, dtype)
-    hold("x", orthogonalize(x), iterate(x), REL[dtype])
-
-
-@pytest.mark.parametrize("dtype", TYPES)
-def test_short_sides_past_8192(dtype):
-    """All three products sum over n = 8500 elements, for which the fp32 accumulators count too: three roundings
-    per 32 elements, each 2^-24 / sqrt(3) (as squares) of a partial sum that is 1 / sqrt(2) of the whole one on
-    the average, (3 n / 32)^1/2 2^-24 / sqrt(6) = 2^-20.5 a product beside the 2^-21 above. Of fifteen products,
-    twice that: 2^-17.2."""
-    x = make((8500, 8400), dtype)
-    rel = 2 * 15 ** 0.5 * (2.0 ** -42 + 3 * 8500 / 32 * 2.0 ** -48 / 6) ** 0.5
-    hold("x", orthogonalize(x), iterate(x), rel)
-
-
-@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_steps_go_downhill(dtype):
-    """Of |w - target|^2 / 2 the update X of the gradient has <X, gradient> above 0.6 of its singular values'
-    sum (the iteration ends between 0.68 and 1.21): with steps of at most a tenth of the least singular value
-    of w - target the loss falls in each."""
-    target = torch.eye(30, 40, device=DEV) * 3
-    w = torch.nn.Parameter(torch.zeros(30, 40, device=DEV, dtype=dtype))
-    opt = Muon([w], lr=0.1, momentum=0.0, weight_decay=0.0)
-    losses = []
-    for _ in range(6):
-        loss = (w.float() - target).square().sum() / 2
-        losses.append(loss.item())
-        opt.zero_grad()
-        loss.backward()
-        opt.step()
-    assert all(b < a for a, b in zip(losses, losses[1:])), losses
-
-
 def test_gradients_in_the_momenta_are_refused():
     """They are read again after the momenta are written. (A parameter may be its own gradient.)"""
     p, g = make((40, 30), torch.float32), make((40, 30), torch.float32, seed=1)
@@ -459,3 +459,27 @@ def test_gradients_in_the_momenta_are_refused():
     muon_step_([p], [p], [torch.zeros_like(p)], lr=0.02)
     hold("p", p, want, REL[torch.float32])
     muon_step_([p, q], [g, g], [torch.zeros_like(p), torch.zeros_like(p)])  # read twice, written nowhere
+
+
+def test_calls_from_several_threads():
+    """Calls at once, on streams of their own."""
+    import threading
+
+    x = [make((6, 900, 1030), t) for t in TYPES] + [make((3, 70, 90), torch.float32)]
+    want = [orthogonalize(v) for v in x]
+    torch.cuda.synchronize()
+    got = [None] * len(x)
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(3):
+                got[i] = orthogonalize(x[i])
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(x))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for u, v in zip(got, want):
+        assert torch.equal(u, v)
